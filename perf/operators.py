@@ -91,7 +91,7 @@ def lengths(case):
 # ------------------------------------------------------------------------------------------ inputs
 def needed(amax):
     """The smallest power of two that brings ``amax`` down to 127."""
-    m, e = torch.frexp(amax.double() / 127)
+    m, e = torch.frexp(amax.double().clamp_min(FLOOR) / 127)
     return torch.ldexp(torch.ones_like(m), torch.where(m == 0.5, e - 1, e)).clamp_min(FLOOR).float()
 
 
