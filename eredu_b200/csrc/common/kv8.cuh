@@ -1,0 +1,43 @@
+// Blocks of a cache held in 8 bits: the 16 rows of one key / value head in a page, int8 codes [16, D] and one scale, a power of two.
+// value = code * scale; code = round(x / scale), ties to even; the scale is the smallest that keeps |code| <= 127, at least 2^-100.
+// A power of two: products and quotients by it are exact, and a block whose scale was raised several times (each time at least twofold) is off
+// by less than one step of the last scale in all, where scales of any value would add up half a step for every time.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace eredu {
+
+constexpr int kKv8Page = 16;
+constexpr float kKv8Floor = 7.888609052210118e-31f;   // 2^-100
+
+// Scale that the largest magnitude `amax` needs; not a number where amax is none (or infinite).
+__device__ __forceinline__ float kv8_needed(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  // amax = f 2^e, 1 <= f < 2, and 127 = 1.984375 * 2^6
+  const int e = static_cast<int>(u >> 23) - 6 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  return e < 27 ? kKv8Floor : __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+// 1 / scale of a power of two (not a number stays none).
+__device__ __forceinline__ float kv8_inverse(float scale) {
+  const uint32_t u = __float_as_uint(scale);
+  return u >= 0x7f800000u ? scale : __uint_as_float(0x7f000000u - u);
+}
+__device__ __forceinline__ uint32_t kv8_pack(float a, float b, float c, float d) {
+  const int i = __float2int_rn(a), j = __float2int_rn(b), k = __float2int_rn(c), l = __float2int_rn(d);
+  return (i & 0xff) | (j & 0xff) << 8 | (k & 0xff) << 16 | static_cast<uint32_t>(l) << 24;
+}
+__device__ __forceinline__ float kv8_code(uint32_t word, int i) { return static_cast<float>(static_cast<int8_t>(word >> (8 * i))); }
+
+// Two bytes of `biased` (codes + 128) as exact halves: 0x6400 | u is 1024 + u. `pick` = 0x4140 for the lower two, 0x4342 for the upper.
+template <uint32_t PICK>
+__device__ __forceinline__ uint32_t kv8_halves(uint32_t biased) {
+  uint32_t h = __byte_perm(biased, 0x64646464u, PICK);
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0x64806480u));   // 1024 + 128
+  return h;
+}
+
+}  // namespace eredu

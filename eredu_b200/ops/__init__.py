@@ -2,6 +2,7 @@
 from .core import (CLUSTER_SPLITS, KERNEL_HEAD_DIMS, PAGE, XIELU, attention_decode, attention_decode_rope, attention_prefill, attention_ref, branch_norm, branch_norm_ref, decode_scratch, decode_splits, embedding,
                    embedding_stream, gated_linear, gated_linear_ref, linear, linear_ref, qkv_prepare, qkv_prepare_ref, residual_norm,
                    residual_norm_ref, rms_residual, rms_residual_ref, rmsnorm, rmsnorm_ref, rope_kv, rope_kv_ref, silu_mul)
+from .kv8 import KV8_HEAD_DIMS, Pages8, copy_pages, page_values, store_kv
 from .sampling import (SamplingParams, pack_allow_mask, pack_rows, philox_uniform, process_logits_ref, rows_to_tensor,
                        sample, sample_ref, spec_verify, verify_ref)
 from .conv import (ConvChannels, ConvHeads, StreamConv, conv_project, conv_project_ref, short_conv, short_conv_ref, stream_conv,

@@ -18,6 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import native
+from .kv8 import Pages8, attention_decode8, check_attention8, decode_splits8, gather_values, rope_kv8, store_kv
 from .native import check, lib, ptr, status_word, stream_ptr
 
 PAGE = 16
@@ -466,7 +467,7 @@ def rope_kv_ref(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, he
         if w is None:
             return t
         y = t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + norm_eps) * (w.float() + norm_w_off)
-        return y.to(qkv.dtype).float()
+        return y if isinstance(k_cache, Pages8) else y.to(qkv.dtype).float()
 
     q, k = hnorm(q, q_norm_w), hnorm(k, k_norm_w)
     if positions.dim() == 2:
@@ -490,6 +491,9 @@ def rope_kv_ref(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, he
         return torch.cat((out, tp), dim=-1)
 
     q, k = rotate(q), rotate(k)
+    if isinstance(k_cache, Pages8):
+        store_kv(k, v, slots, k_cache, v_cache)
+        return q.to(qkv.dtype).contiguous()
     ok = slots >= 0
     page, off = (slots[ok] // PAGE), (slots[ok] % PAGE)
     k_cache[page, :, off] = k[ok].to(k_cache.dtype)
@@ -500,7 +504,11 @@ def rope_kv_ref(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, he
 def rope_kv(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot=None, interleaved=False,
             attn_factor=1.0, q_norm_w=None, k_norm_w=None, norm_eps=1e-6, norm_w_off=0.0, q_out=None, mrope_section=None):
     """Per-head q/k norm (optional) + RoPE on q and k, K/V scattered into their cache pages. Returns q [M,n_q,D].
-    Three-axis positions ([3, M], prompts with images) take the tensor-operation path on either device."""
+    Three-axis positions ([3, M], prompts with images) take the tensor-operation path on either device.
+    Caches of :class:`Pages8` are written as :mod:`.kv8` says."""
+    if isinstance(k_cache, Pages8) and qkv.is_cuda and positions.dim() == 1:
+        return rope_kv8(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot or head_dim, interleaved, attn_factor, q_norm_w,
+                        k_norm_w, norm_eps, norm_w_off, q_out)
     if not qkv.is_cuda or head_dim not in KERNEL_HEAD_DIMS or positions.dim() == 2:
         return rope_kv_ref(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, interleaved,
                            attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, mrope_section)
@@ -524,7 +532,8 @@ KERNEL_HEAD_DIMS = (64, 128)
 # ------------------------------------------------------------------------------------------ attention
 def _gather_kv(cache, block_table_row, kv_len):
     n_pages = (kv_len + PAGE - 1) // PAGE
-    pages = cache[block_table_row[:n_pages].long()]  # [n_pages, n_kv, 16, D]
+    which = block_table_row[:n_pages].long()
+    pages = cache.values(which) if isinstance(cache, Pages8) else cache[which]  # [n_pages, n_kv, 16, D]
     return pages.permute(1, 0, 2, 3).reshape(cache.shape[1], n_pages * PAGE, cache.shape[3])[:, :kv_len]
 
 
@@ -561,6 +570,8 @@ def attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, scale, win
             p = torch.softmax(s, dim=-1)[..., :-1]
         else:
             p = torch.softmax(s, dim=-1)
+        if isinstance(k_cache, Pages8):
+            p = p.masked_fill(~mask.any(-1)[None, :, None], 0.0)     # a row that sees nothing is zero, as in the kernels
         out[start:start + ql] = torch.einsum("hqk,hkd->hqd", p, v).permute(1, 0, 2).to(q.dtype)
         start += ql
     return out
@@ -597,7 +608,11 @@ def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_le
                       out=None, chunk=0, max_kv_len=0):
     """``window`` > 0: a query at position p sees keys in (p - window, p]; ``chunk`` > 0: the keys of its own chunk of
     positions. ``max_kv_len``: the largest of ``seq_lens`` where the host knows it (it chooses how the work is split, never what is
-    computed; 0: unknown). Key and value widths are those of the caches. Returns [total_q, n_q, value width]."""
+    computed; 0: unknown). Key and value widths are those of the caches. Returns [total_q, n_q, value width].
+    Caches of :class:`Pages8`: the pages that some query sees are brought to bf16 first - once for all query tiles and heads that read them -, in memory
+    that the call allocates (``max_kv_len`` bounds it, and then has to be that of the longest sequence at least)."""
+    if isinstance(k_cache, Pages8) and q.is_cuda:
+        return _attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
         if not _tensor_core_dims(q, k_cache, v_cache):
             return _attention_simt(q, k_cache, v_cache, block_table, seq_lens, cu_q, 0, max_q_len, scale, window, chunk, sinks)
@@ -628,6 +643,16 @@ def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_le
     return out
 
 
+def _attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len):
+    check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q)
+    if out is None:
+        out = torch.empty_like(q)
+    if q.shape[0] == 0 or seq_lens.shape[0] == 0:
+        return out
+    k, v, table = gather_values(k_cache, v_cache, block_table, seq_lens, cu_q, max_kv_len, window, chunk)
+    return attention_prefill(q, k, v, table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len)
+
+
 import os as _os
 
 _SPLIT_WAVES = int(_os.environ.get("EREDU_DECODE_SPLIT_WAVES", "2"))   # CTAs per SM the split-KV grid aims for
@@ -637,13 +662,16 @@ CLUSTER_SPLITS = 8      # splits the decode kernel combines through distributed 
 FUSED_ROPE_MAX_NEW = 8  # new tokens per sequence the fused RoPE + append decode path takes
 
 
-def decode_splits(batch, n_kv, max_kv_len, sm_count=148, rows=0, head_dim=128):
+def decode_splits(batch, n_kv, max_kv_len, sm_count=148, rows=0, head_dim=128, bits=16):
     """Split-KV factor: enough CTAs to fill the GPU once (a second wave costs more than it returns: the CTAs of the
     following kernel are already resident under programmatic dependent launch), at least 8 pages per split.
     ``rows``: query rows that share a key / value head where the caller knows that the plain kernel takes them (head sizes 64 and 128, at
     most 16 rows), else 0. Its CTAs of eight warps run one to an SM, and as many splits as that allows are the best there are in contexts of
     some length (us with the splits of either rule: one sequence of 4096, 32 heads over 8, 13.8 with 32 and 10.2 with 8; eight of 1024, 64 heads
-    over 8, 15.2 with 4 and 13.3 with 2; 32 of 1024, 32 heads over 4, 21.6 with 2 and 16.9 with 1). How long: see _one_round_pays."""
+    over 8, 15.2 with 4 and 13.3 with 2; 32 of 1024, 32 heads over 4, 21.6 with 2 and 16.9 with 1). How long: see _one_round_pays.
+    ``bits`` = 8: for caches of :class:`Pages8`, which have a kernel and a rule of their own."""
+    if bits == 8:
+        return decode_splits8(batch, n_kv, max_kv_len, sm_count, rows)
     ctas = max(1, batch * n_kv)
     pages = max(1, (max_kv_len + PAGE - 1) // PAGE)
     want = max(1, (_SPLIT_WAVES * sm_count) // ctas)
@@ -679,7 +707,9 @@ def _one_round_pays(ctas, pages, one_round, splits, sm_count, head_dim):
 def attention_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits=1, window=0, sinks=None,
                      scratch=None, out=None, chunk=0):
     """q: [B * q_per_seq, n_q, D]; ``window`` / ``chunk`` as in :func:`attention_prefill`. ``scratch`` = (part_o, part_ml, counters) from :func:`decode_scratch` when
-    splits > 1 (fp32 partials and zeroed int32 arrival tickets)."""
+    splits > 1 (fp32 partials and zeroed int32 arrival tickets). Caches of :class:`Pages8` need no ``scratch``; a query that sees no key gives zeros."""
+    if isinstance(k_cache, Pages8) and q.is_cuda:
+        return attention_decode8(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
         if not _tensor_core_dims(q, k_cache, v_cache) or q.shape[1] // k_cache.shape[1] > 32:
             return _attention_simt(q, k_cache, v_cache, block_table, seq_lens, None, q_per_seq, q_per_seq, scale, window, chunk,
@@ -719,6 +749,11 @@ def attention_decode_rope(qkv, k_cache, v_cache, block_table, seq_lens, q_per_se
     ``settled``: the kernel enqueued just before this call writes ``qkv`` only, not the pages, ``block_table``, ``seq_lens``, ``positions``, ``slots``
     or ``inv_freq`` (the projection of a decode step); these are then read ahead of the stream dependency on it."""
     value_dim = value_dim or head_dim
+    if isinstance(k_cache, Pages8):
+        if norm_whole or value_norm or not append or value_dim != head_dim:
+            raise NotImplementedError("8-bit pages: norms per head, values as wide as keys, and rows that are appended")
+        q = rope_kv(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off)
+        return attention_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, chunk=chunk)
     if norm_whole or value_norm or not append or value_dim != head_dim or chunk:
         whole = (qkv.is_cuda and qkv.dtype == torch.bfloat16 and _tma_rows(qkv) and head_dim % 8 == 0 and value_dim % 8 == 0
                  and max(head_dim, value_dim) <= 128 and n_q // n_kv <= 32 and q_per_seq <= FUSED_ROPE_MAX_NEW

@@ -1,0 +1,323 @@
+"""Keys and values held in 8 bits.
+
+The cache of a layer is a pair of :class:`Pages8` in place of two bf16 tensors; :func:`rope_kv`, :func:`attention_prefill`,
+:func:`attention_decode`, :func:`attention_decode_rope` and :func:`attention_ref` of :mod:`.core` take either.
+
+A block is the 16 rows of one key / value head in a page: int8 codes in [-127, 127] and one fp32 scale, a power of two, value = code * scale.
+``code = round(x / scale)`` (ties to even) with the smallest scale that keeps all codes in range, 2^-100 at least: a value is off by at most
+half a scale, between 1/254 and 1/127 of the block's largest magnitude.
+Rows are written in the order of their tokens. A row at offset 0 opens its block and sets the scale; rows behind others keep the scale or,
+where one of them needs a larger one, raise it, and the codes in front are rounded again (at least twofold each time, so that all roundings of a value
+together stay below one scale). What lies behind the last row written is left from earlier use and means nothing. A row with an infinity or a NaN
+makes the scale, and with it the whole block, no number until the block is opened again.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import native
+from .native import check, lib, ptr, status_word, stream_ptr
+
+PAGE = 16
+FLOOR = 2.0 ** -100          # smallest scale
+KV8_HEAD_DIMS = (64, 128)    # head sizes of the kernels
+
+P, I, F = native.P, native.I, native.F
+native.register("eredu_kv8_store", I, [P] * 13 + [I] * 10 + [F] * 3 + [P] * 2)
+native.register("eredu_kv8_values", I, [P] * 10 + [I] * 8 + [P] * 2)
+native.register("eredu_attn_kv8_decode", I, [P] * 11 + [I] * 10 + [F] + [P] * 2)
+native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
+
+
+class Pages8(NamedTuple):
+    """``codes`` [pages, heads, 16, head size] int8 and ``scales`` [pages, heads] fp32 of the keys or of the values of a layer."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.codes.is_cuda
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def values(self, pages=None) -> torch.Tensor:
+        """fp32 values of ``pages`` (all by default), by tensor operations; :func:`page_values` is the kernel."""
+        codes, scales = (self.codes, self.scales) if pages is None else (self.codes[pages], self.scales[pages])
+        return codes.float() * scales[..., None, None]
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, head_dim: int, device, layers: int = 0) -> "Pages8":
+        """Zeroed blocks; with ``layers``, [layers, pages, ...]."""
+        lead = (layers, pages, heads) if layers else (pages, heads)
+        return cls(torch.zeros((*lead, PAGE, head_dim), dtype=torch.int8, device=device), torch.full(lead, FLOOR, dtype=torch.float32, device=device))
+
+
+def check_pages8(k: Pages8, v: Pages8, n_kv: int, head_dim: int) -> None:
+    for name, t in (("keys", k), ("values", v)):
+        if not isinstance(t, Pages8):
+            raise TypeError(f"{name}: a pair of Pages8 is expected, both or neither")
+        if t.codes.dtype != torch.int8 or t.scales.dtype != torch.float32 or tuple(t.codes.shape[1:]) != (n_kv, PAGE, head_dim) \
+                or t.scales.shape != t.codes.shape[:2]:
+            raise ValueError(f"{name}: codes {tuple(t.codes.shape)} {t.codes.dtype} with scales {tuple(t.scales.shape)} {t.scales.dtype} are no pages of "
+                             f"{n_kv} heads of {head_dim}")
+        if not t.codes.is_contiguous() or not t.scales.is_contiguous() or t.scales.device != t.codes.device:
+            raise ValueError(f"{name}: codes and scales have to be contiguous and on one device")
+    if k.codes.shape[0] != v.codes.shape[0] or k.device != v.device:
+        raise ValueError("keys and values have to have the same pages")
+    if k.is_cuda and head_dim not in KV8_HEAD_DIMS:
+        raise NotImplementedError(f"the kernels of 8-bit pages are built for head sizes {KV8_HEAD_DIMS}, not {head_dim}")
+
+
+def _on(device, **tensors) -> None:
+    for name, (t, dtype) in tensors.items():
+        if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.device != device):
+            raise ValueError(f"{name}: a contiguous {dtype} tensor on {device} is expected, not {t.dtype} on {t.device}")
+
+
+# ------------------------------------------------------------------------------------------ writing
+def needed_scale(amax: torch.Tensor) -> torch.Tensor:
+    """The smallest power of two that brings ``amax`` down to 127 (at least :data:`FLOOR`); no number for what is none."""
+    m, e = torch.frexp(amax.double().clamp_min(FLOOR) / 127)
+    s = torch.ldexp(torch.ones_like(m), torch.where(m == 0.5, e - 1, e)).clamp_min(FLOOR)
+    return torch.where(torch.isfinite(amax), s, torch.full_like(s, float("nan"))).float()
+
+
+def store_rows_ref(x, slots, pages: Pages8) -> None:
+    """Rows ``x`` [M, heads, head size] into their blocks, run by run (rows that follow one another in a page)."""
+    at, i = slots.tolist(), 0
+    while i < len(at):
+        n = 1
+        if at[i] >= 0:
+            page, first = divmod(at[i], PAGE)
+            if page >= pages.shape[0]:
+                raise IndexError(f"slot {at[i]} lies behind the last of {pages.shape[0]} pages")
+            while i + n < len(at) and first + n < PAGE and at[i + n] == at[i] + n:
+                n += 1
+            rows = x[i:i + n].float().transpose(0, 1)                          # [heads, n, head size]
+            before = pages.scales[page]
+            scale = needed_scale(rows.abs().amax((1, 2)))
+            if first:
+                scale = torch.maximum(scale, before)                           # (keeps what is no number)
+                front = pages.codes[page, :, :first].float() * (before / scale)[:, None, None]
+                pages.codes[page, :, :first] = torch.nan_to_num(front.round()).to(torch.int8)
+            pages.scales[page] = scale
+            pages.codes[page, :, first:first + n] = torch.nan_to_num((rows / scale[:, None, None]).round()).to(torch.int8)
+        i += n
+
+
+def _store(q, k, v, slots, k_cache, v_cache, q_out, positions, inv_freq, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
+           norm_eps, norm_w_off, ld):
+    dev = k_cache.device
+    code = lib().eredu_kv8_store(q, k, v, ptr(q_out), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), ptr(positions),
+                                 ptr(slots), ptr(inv_freq), ptr(q_norm_w), ptr(k_norm_w), slots.shape[0], ld[0], ld[1], ld[2], n_q, n_kv, head_dim, rot,
+                                 1 if interleaved else 0, k_cache.codes.shape[0], attn_factor, norm_eps, norm_w_off, ptr(status_word(dev)), stream_ptr(dev))
+    check(code, "eredu_kv8_store")
+
+
+def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
+    """Keys and values [M, heads, head size] (as they are: rotated where the model rotates them) into the blocks of ``slots`` [M] int64 (page * 16 +
+    offset; negative: not stored). The rows of a page follow one another in the order of their offsets, and a page occurs once in a call."""
+    if k.shape != v.shape or k.dim() != 3 or slots.shape != k.shape[:1]:
+        raise ValueError(f"keys {tuple(k.shape)}, values {tuple(v.shape)} and slots {tuple(slots.shape)} do not go together")
+    n_kv, head_dim = k.shape[1:]
+    check_pages8(k_cache, v_cache, n_kv, head_dim)
+    if not k_cache.is_cuda:
+        store_rows_ref(k, slots, k_cache)
+        store_rows_ref(v, slots, v_cache)
+        return
+    _on(k_cache.device, slots=(slots, torch.int64))
+    k, v = (t if t.dtype == torch.bfloat16 and t.stride()[1:] == (head_dim, 1) and t.stride(0) % 4 == 0 and t.data_ptr() % 8 == 0
+            else t.to(torch.bfloat16).contiguous() for t in (k, v))
+    _store(None, k.data_ptr(), v.data_ptr(), slots, k_cache, v_cache, None, None, None, 0, n_kv, head_dim, 0, False, 1.0, None, None, 0.0, 0.0,
+           (0, k.stride(0), v.stride(0)))
+
+
+def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
+             norm_eps, norm_w_off, q_out):
+    """The form of :func:`.core.rope_kv` for 8-bit pages on a GPU. Norm and rotation run in 32 bits throughout; a key is rounded once, to its code."""
+    check_pages8(k_cache, v_cache, n_kv, head_dim)
+    dev, M = k_cache.device, qkv.shape[0]
+    if qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.stride(0) % 4 or qkv.data_ptr() % 8 \
+            or qkv.shape[1] < (n_q + 2 * n_kv) * head_dim or n_q % n_kv:
+        raise ValueError(f"qkv: bf16 rows of {n_q} + 2 * {n_kv} heads of {head_dim}, 8-byte aligned, on {dev} are expected")
+    if rot % 8 or rot > head_dim or inv_freq.numel() != rot // 2:
+        raise ValueError(f"{rot} rotated dims with {inv_freq.numel()} frequencies: a multiple of 8 up to the head size, and half as many frequencies")
+    if positions.shape != (M,) or slots.shape != (M,):
+        raise ValueError("one position and one slot per row are expected")
+    _on(dev, positions=(positions, torch.int32), slots=(slots, torch.int64), inv_freq=(inv_freq, torch.float32), q_norm_w=(q_norm_w, torch.float32),
+        k_norm_w=(k_norm_w, torch.float32))
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and w.numel() != head_dim:
+            raise ValueError(f"a norm has {w.numel()} weights for heads of {head_dim}")
+    if q_out is None:
+        q_out = torch.empty((M, n_q, head_dim), dtype=qkv.dtype, device=dev)
+    else:
+        _on(dev, q_out=(q_out, qkv.dtype))
+        if q_out.numel() != M * n_q * head_dim:
+            raise ValueError(f"q_out has {q_out.numel()} elements for {M} rows of {n_q} heads of {head_dim}")
+    ld, at = qkv.stride(0), qkv.data_ptr()
+    _store(at, at + 2 * n_q * head_dim, at + 2 * (n_q + n_kv) * head_dim, slots, k_cache, v_cache, q_out, positions, inv_freq, n_q, n_kv, head_dim, rot,
+           interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, (ld, ld, ld))
+    return q_out
+
+
+# ------------------------------------------------------------------------------------------ reading
+def page_values(k_cache: Pages8, v_cache: Pages8, pages):
+    """Keys and values of ``pages`` [n] int32 as bf16 [n, heads, 16, head size] each (exact: a code has seven bits)."""
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("keys and values have to have the same pages")
+    check_pages8(k_cache, v_cache, *k_cache.shape[1::2])
+    if not k_cache.is_cuda:
+        return tuple(t.values(pages.long()).to(torch.bfloat16) for t in (k_cache, v_cache))
+    dev, (num, n_kv, _, dim) = k_cache.device, k_cache.shape
+    _on(dev, pages=(pages, torch.int32))
+    n = pages.shape[0]
+    out = torch.empty((2, n, n_kv, PAGE, dim), dtype=torch.bfloat16, device=dev)
+    if n:
+        half = out.data_ptr()
+        code = lib().eredu_kv8_values(ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), half, half + out.nbytes // 2,
+                                      ptr(pages), None, None, None, 1, n, n, n_kv, dim, num, 0, 0, ptr(status_word(dev)), stream_ptr(dev))
+        check(code, "eredu_kv8_values")
+    return out[0], out[1]
+
+
+def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q=None):
+    n_q, dim = q.shape[1:]
+    check_pages8(k_cache, v_cache, k_cache.shape[1], dim)
+    if n_q % k_cache.shape[1]:
+        raise ValueError(f"{n_q} query heads do not share {k_cache.shape[1]} key / value heads evenly")
+    dev = k_cache.device
+    if q.dtype != torch.bfloat16:
+        raise ValueError(f"queries over 8-bit pages are bf16 on a GPU, not {q.dtype}")
+    _on(dev, q=(q, torch.bfloat16), seq_lens=(seq_lens, torch.int32), sinks=(sinks, torch.float32), out=(out, q.dtype))
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0] \
+            or block_table.device != dev:
+        raise ValueError("block_table: int32 rows, one per sequence")
+    _on(dev, cu_q=(cu_q, torch.int32))
+    if cu_q is not None and cu_q.shape[0] != seq_lens.shape[0] + 1:
+        raise ValueError(f"{cu_q.shape[0]} query offsets for {seq_lens.shape[0]} sequences")
+    if sinks is not None and sinks.numel() != n_q:
+        raise ValueError(f"{sinks.numel()} sinks for {n_q} query heads")
+    if out is not None and out.shape != q.shape:
+        raise ValueError(f"out {tuple(out.shape)} for queries {tuple(q.shape)}")
+
+
+def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk):
+    """The form of :func:`.core.attention_decode` for 8-bit pages on a GPU. More splits than a cluster holds leave partial sums in memory that the
+    call allocates; a second kernel adds them up."""
+    check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out)
+    dev, B = q.device, seq_lens.shape[0]
+    n_q, dim = q.shape[1:]
+    n_kv = k_cache.codes.shape[1]
+    if q.shape[0] != B * q_per_seq:
+        raise ValueError(f"{q.shape[0]} query rows for {B} sequences of {q_per_seq}")
+    if out is None:
+        out = torch.empty_like(q)
+    part_o = part_ml = None
+    if splits > 8:
+        rows = q_per_seq * (n_q // n_kv)
+        tile = 8 if rows <= 8 else 16
+        elements = B * n_kv * -(-rows // tile) * tile * splits
+        part = torch.empty(elements * (dim + 4), dtype=torch.float32, device=dev)
+        part_o = part.data_ptr()
+        part_ml = part_o + elements * dim * 4
+    code = lib().eredu_attn_kv8_decode(q.data_ptr(), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
+                                       block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, B, q_per_seq, block_table.stride(0),
+                                       k_cache.codes.shape[0], n_q, n_kv, dim, splits, int(window), int(chunk), scale, ptr(status_word(dev)), stream_ptr(dev))
+    check(code, "eredu_attn_kv8_decode")
+    return out
+
+
+def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
+    """Split factor of the decode kernel for 8-bit pages: CTAs of eight warps, two to an SM where a key / value head has up to eight query rows,
+    one where it has more; a page per warp and split at least."""
+    tile = 8 if rows <= 8 else 16
+    ctas = max(1, batch * n_kv * -(-max(rows, 1) // tile))
+    pages = max(1, -(-max_kv_len // PAGE))
+    want = sm_count * (2 if tile == 8 else 1) // ctas
+    splits = max(1, min(want, pages // 8, 64))
+    return 8 if 8 < splits < 16 and pages <= 1024 else splits
+
+
+def gather_values(k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_kv_len, window, chunk):
+    """The pages that some query sees, as bf16 pages of their own, and the block table that finds them: (keys, values, table). Entries of the
+    table that nobody sees point behind the last page, where the tensor maps of prefill attention read zeros; rows of eight pages, a key tile."""
+    dev, B = k_cache.device, seq_lens.shape[0]
+    num, n_kv, _, dim = k_cache.shape
+    wide = block_table.shape[1]
+    if max_kv_len > 0:
+        wide = min(wide, -(-max_kv_len // PAGE))
+    wide = -(-wide // 8) * 8
+    out = torch.empty((2, B * wide, n_kv, PAGE, dim), dtype=torch.bfloat16, device=dev)
+    table = torch.empty((B, wide), dtype=torch.int32, device=dev)
+    code = lib().eredu_kv8_values(ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
+                                  out.data_ptr() + out.nbytes // 2, ptr(block_table), ptr(seq_lens), ptr(cu_q), ptr(table), B, block_table.stride(0), wide,
+                                  n_kv, dim, num, int(window), int(chunk), ptr(status_word(dev)), stream_ptr(dev))
+    check(code, "eredu_kv8_values")
+    return out[0], out[1], table
+
+
+# ------------------------------------------------------------------------------------------ moving
+def _page_list(pages, device):
+    t = pages if torch.is_tensor(pages) else torch.as_tensor(list(pages), dtype=torch.int32)
+    if t.is_cuda:
+        return t
+    return t.to(torch.int32).pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t.to(torch.int32)
+
+
+def copy_pages(pools, src, dst) -> None:
+    """Page ``src[i]`` to page ``dst[i]`` in every layer of every tensor of ``pools``, in one launch (for eight tensors). ``pools``: tensors
+    [layers, pages, ...] with pages that are contiguous. ``src``, ``dst``: page numbers on the host, which are checked (in range, no destination twice, none
+    that is a source as well), or int32 tensors on the pools' device, for which that is the caller's part (pages out of range are not copied, and reported)."""
+    pools = [t for t in pools]
+    if not pools:
+        return
+    dev, num = pools[0].device, pools[0].shape[1]
+    for t in pools:
+        if t.device != dev or t.dim() < 2 or t.shape[1] != num:
+            raise ValueError("the pools have to have the same pages, on one device")
+        if not t[0].is_contiguous() if t.shape[0] else False:
+            raise ValueError("the pages of a layer have to be contiguous")
+        if (t[0, 0].numel() if t.shape[0] and num else 0) * t.element_size() % 4 or t.data_ptr() % 4:
+            raise ValueError("pages have to be whole words")
+    on_host = [x for x in (src, dst) if not (torch.is_tensor(x) and x.is_cuda)]
+    if len(on_host) == 2:
+        a, b = ([int(i) for i in (x.tolist() if torch.is_tensor(x) else x)] for x in (src, dst))
+        if len(a) != len(b):
+            raise ValueError(f"{len(a)} sources for {len(b)} destinations")
+        if any(not 0 <= i < num for i in a + b):
+            raise IndexError(f"a page is not one of {num}")
+        if len(set(b)) != len(b) or set(a) & set(b):
+            raise ValueError("a page is the destination of two copies, or a destination and a source")
+        if not a:
+            return
+        src, dst = a, b
+    elif on_host:
+        raise ValueError("sources and destinations are either both on the host or both on the device")
+    elif src.shape != dst.shape or src.dim() != 1 or any(t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev for t in (src, dst)):
+        raise ValueError(f"src, dst: int32 vectors of one length on {dev}")
+    if dev.type != "cuda":
+        for t in pools:
+            t[:, list(dst)] = t[:, list(src)]
+        return
+    if on_host:
+        both = _page_list(src + dst, dev)
+        src, dst = both[:len(src)], both[len(src):]
+    if src.shape[0] == 0:
+        return
+    import ctypes
+
+    for i in range(0, len(pools), 8):
+        part = [t for t in pools[i:i + 8] if t.shape[0]]
+        words = [w for t in part for w in (t.data_ptr(), t.stride(0) * t.element_size(), t[0, 0].numel() * t.element_size(), t.shape[0])]
+        code = lib().eredu_copy_pages((ctypes.c_longlong * len(words))(*words), len(part), src.data_ptr(), dst.data_ptr(), src.shape[0], num,
+                                      ptr(status_word(dev)), stream_ptr(dev))
+        check(code, "eredu_copy_pages")
