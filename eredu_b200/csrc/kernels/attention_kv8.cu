@@ -2,28 +2,32 @@
 //
 //   s_j = (q . c_j) scale ks,   o = sum_j 2^(s_j log2 e - m) vs c'_j / sum_j 2^(s_j log2 e - m)     (ks, vs: scales of token j's blocks)
 //
-// Bound by memory: every cached token is read once per key / value head, 2 D bytes. A warp walks pages of its own; codes go from
-// memory straight into the registers that mma.sync m16n8k16 takes, without shared memory:
-//   scores  S^T[16 tokens, 8 query rows] = K[16, D] Q^T: the page is the A operand. The sum over D may run in any order, so a lane takes 16
-//           neighbouring bytes of two token rows and the query fragment is laid out to match.
-//   output  O^T[D, 8 rows] = V^T[D, 16] P^T: a lane takes 16 neighbouring bytes (8 where D = 64) of four token rows and pairs tokens by byte
+// Bound by memory where contexts are long: every cached token is read once per key / value head, 2 D bytes. A warp walks pairs of pages of its own,
+// and every lane brings the bytes that it is going to need into a ring of its own in shared memory (cp.async; nothing is exchanged, so no
+// barrier and no bank conflicts): a pair is on its way while another is worked on. From there they go into the registers of mma.sync:
+//   scores  S^T[16 tokens, 8 query rows] = K[16, D] Q^T as integers (m16n8k32): the codes are the A operand as they are. A query row is rounded to 16 bits,
+//           with a power of two that brings its largest magnitude to 2^14 (a bf16 query keeps all its bits down to 2^-7 of that), and taken as a signed upper and
+//           an unsigned lower byte. The sum over D may run in any order, so a lane takes 16 neighbouring bytes of two token rows.
+//   output  O^T[D, 8 rows] = V^T[D, 16] P^T in f16 (m16n8k16): a lane takes 16 neighbouring bytes (8 where D = 64) of four token rows and pairs tokens by byte
 //           permutation; which accumulator row is which value channel is settled when they are written out. P^T comes from S^T by movmatrix.
 // The 8 query rows of a tile are the query heads that share the key / value head, times the new tokens; two tiles side by side above 8.
-// Codes are exact as f16, and so are queries scaled by a power of two per row (to a largest magnitude of 2^14: what f16 drops is below 2^-38 of that).
-// Probabilities are rounded to f16 (11 bits). The page's value scale goes into their exponent, with a running maximum of its own (m2, of s_j + log2 vs): the largest
-// contribution to the output is near 1 whatever the scales are. The maxima are raised only where a score passes one by more than 2^8.
+// Probabilities are rounded to f16 (11 bits; codes are exact in it). The page's value scale goes into their exponent, with a running maximum of its own (m2, of
+// s_j + log2 vs): the largest contribution to the output is near 1 whatever the scales are. The maxima are raised only where a score passes one by more than 2^8.
+// 64 sequences of 4096 to 8192 tokens, 32 heads of 128 over 8: registers straight from memory, one page at a time, scores in f16 178 us; through the ring 174.
 #include <cuda_bf16.h>
 
 #include "../common/kv8.cuh"
 #include "../common/launch.h"
 #include "../common/launch_count.h"
+#include "../common/mma.cuh"
 #include "../common/ptx.cuh"
 #include "../common/trace.cuh"
 
 namespace eredu {
 
 struct AttnKv8Params {
-  const __nv_bfloat16* q;          // [B * q_per_seq, n_q, D]
+  const __nv_bfloat16* q;          // [B * q_per_seq, n_q, D], or
+  const float* q32;                // the same in 32 bits
   const int8_t *k_codes, *v_codes; // [pages, n_kv, 16, D]
   const float *k_scales, *v_scales;
   __nv_bfloat16* out;              // [B * q_per_seq, n_q, D]
@@ -36,18 +40,33 @@ struct AttnKv8Params {
   float scale_log2;
   int* status;
 };
-constexpr int kKv8Warps = 8;
+constexpr int kKv8Warps = 4;         // three CTAs of four warps to an SM: four pages a warp fill shared memory
+constexpr int kKv8Threads = 32 * kKv8Warps;
 constexpr int kKv8Cluster = 8;      // splits that meet in a cluster
 constexpr float kKv8Slack = 8.f;    // log2 units by which a score may pass the maximum in use
 constexpr float kLowest = -3.402823466e38f;
+// Integer sums start at the bits of 1.5 * 2^23: as floats they are that plus the sum, which stays below 2^22 (128 * 127 * 255).
+constexpr int kMagicBits = 0x4b400000;
+constexpr float kMagic = 12582912.f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Codes times the upper (signed) and the lower (unsigned) byte of queries.
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
   return v;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -55,16 +74,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Codes of the cache; a step reads each of them once.
-__device__ __forceinline__ uint4 ld_codes16(const int8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 ld_codes8(const int8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ void copy16(uint32_t smem, const int8_t* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(from) : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
@@ -92,15 +103,32 @@ __device__ __forceinline__ float kv8_finish(float o, const Kv8Row& r, const floa
   return l == 0.f || r.l == 0.f ? 0.f : o / l * ex2_approx(r.m2 - m);
 }
 
+__device__ __forceinline__ float exp2_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }   // -126 <= e <= 127
+// The exchange of 16-byte pieces in row r of a page of 128-byte rows.
+__device__ __forceinline__ int swap128(int r) { return (r & 6) ^ (r & 1) << 2; }
+// Eight values of a query row times two powers of two, rounded to 16 bits: their upper bytes and their lower bytes.
+__device__ __forceinline__ uint4 query_bytes(const float (&x)[8], float up, float more) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = static_cast<uint32_t>(min(__float2int_rn(x[i] * up * more), 32767));
+  auto pick = [&](int i, uint32_t sel) { return __byte_perm(__byte_perm(w[i], w[i + 1], sel), __byte_perm(w[i + 2], w[i + 3], sel), 0x5410); };
+  return make_uint4(pick(0, 0x0051), pick(4, 0x0051), pick(0, 0x0040), pick(4, 0x0040));
+}
+
 // grid (splits, n_kv * tiles, B)
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kernel(AttnKv8Params p) {
+__global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params p) {
   constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16, VW = D / 32;   // KC: 16-byte pieces of a token row per lane; VW: value words per token and lane
-  extern __shared__ float smem[];
-  float* o_warp = smem;                                  // [warps][ROWS][D]
+  constexpr int PAGE_BYTES = 2 * kKv8Page * D;
+  extern __shared__ __align__(16) uint8_t smem[];
+  // queries as bytes [NT][2 KC][32 lanes], then the rings [warps][2 pairs][2 pages]; behind the last page, what the warps have gathered takes their place
+  uint4* q_s = reinterpret_cast<uint4*>(smem);
+  uint8_t* rings = smem + NT * 2 * KC * 512;
+  float* o_warp = reinterpret_cast<float*>(rings);       // [warps][ROWS][D]
   float* o_s = o_warp + kKv8Warps * ROWS * D;            // [ROWS][D]
   Kv8Row* row_warp = reinterpret_cast<Kv8Row*>(o_s + ROWS * D);   // [warps][ROWS]
   Kv8Row* row_s = row_warp + kKv8Warps * ROWS;           // [ROWS]
+  __shared__ float back_s[ROWS];
   pdl_launch_early();
   trace_mark(kTraceAttnDecode, kTraceStart);
   pdl_wait();
@@ -114,150 +142,178 @@ __global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kern
   const int page_lo = kv8_lowest_key(p, pos_first) / kKv8Page, page_hi = min(pos_last / kKv8Page + (pos_last >= 0), p.max_pages);
   const int per = max(0, page_hi - page_lo + p.splits - 1) / p.splits;
   const int page0 = page_lo + split * per, page1 = min(page_hi, page0 + per);
-  const int mask_hi = pos_first, mask_lo = kv8_lowest_key(p, pos_last);   // pages inside need no mask
+  const int last_key = page1 * kKv8Page - 1;                                                  // of this split
+  const int mask_hi = min(pos_first, last_key), mask_lo = kv8_lowest_key(p, pos_last);        // pages inside need no mask
 
-  // ---- the query rows: f16 fragments, and what takes a score back to log2 units
-  uint32_t qf[NT][STEPS][2];
-  float back[NT][2];                                    // of the lane's columns 2t, 2t + 1
-  int pos[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + nt * 8 + g;
-    const bool in = nt * 8 + g < rows;
-    const __nv_bfloat16* src = p.q + (static_cast<size_t>(b * p.q_per_seq + (in ? r / group : 0)) * p.n_q + kvh * group + (in ? r % group : 0)) * D;
-    uint4 raw[KC][2];
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < KC; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        raw[j][h] = in ? *reinterpret_cast<const uint4*>(src + 64 * j + 16 * t + 8 * h) : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {raw[j][h].x, raw[j][h].y, raw[j][h].z, raw[j][h].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-      }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = top >= 0x7f80u || top < 0x0080u ? 0 : max(-110, min(110, 141 - static_cast<int>(top >> 7)));   // 2^e brings the largest to 2^14
-    const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-    for (int j = 0; j < KC; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t w[4] = {raw[j][h].x, raw[j][h].y, raw[j][h].z, raw[j][h].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qf[nt][4 * j + 2 * h + (i >> 1)][i & 1] = pack_f16x2(bf16_lo(w[i]) * up, bf16_hi(w[i]) * up);
-      }
-    const float mine = p.scale_log2 * down;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      back[nt][c] = __shfl_sync(0xffffffffu, mine, (2 * t + c) * 4);
-      pos[nt][c] = pos_new + (r0 + min(nt * 8 + 2 * t + c, rows - 1)) / group;
-    }
-  }
-
-  float o[NT][STEPS][4], m[NT][2], m2[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-    m[nt][0] = m[nt][1] = m2[nt][0] = m2[nt][1] = kLowest;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-
-  // ---- pages warp, warp + 8, ... of the split. Lane i holds page id and scales of the i-th of 32 turns.
+  // ---- pairs warp, warp + 6, ... of the split. Lanes 2 i and 2 i + 1 hold page ids and scales of the i-th of 16 turns; those of the 16 before stay at hand.
   const int* table = p.block_table + static_cast<size_t>(b) * p.max_pages;
-  const int turns = page1 > page0 + warp ? (page1 - page0 - warp + kKv8Warps - 1) / kKv8Warps : 0;
+  const int turns = page1 > page0 + 2 * warp ? (page1 - page0 - 2 * warp + 2 * kKv8Warps - 1) / (2 * kKv8Warps) : 0;
   int ids = 0;
-  float ks = 0.f, ev = 0.f;
+  float ks = 0.f, ev = 0.f, ks_before = 0.f, ev_before = 0.f;
   auto look_up = [&](int turn) {
-    const int pg = page0 + warp + kKv8Warps * (turn + lane);
+    const int pg = page0 + 2 * (warp + kKv8Warps * (turn + (lane >> 1))) + (lane & 1);
     ids = pg < page1 ? table[pg] : 0;
     if (ids < 0 || ids >= p.num_pages) {
       report_status(p.status, kStatusBadArgument);
       ids = 0;
     }
     const size_t cell = static_cast<size_t>(ids) * p.n_kv + kvh;
+    ks_before = ks;
+    ev_before = ev;
     ks = p.k_scales[cell];
     ev = log2f(p.v_scales[cell]);
   };
-  uint4 kr[2][KC];
-  uint32_t vr[4][VW];
-  float ks_next = 0.f, ev_next = 0.f;
-  auto fetch_k = [&](int turn) {
-    const int id = __shfl_sync(0xffffffffu, ids, turn & 31);
-    const int8_t* at = p.k_codes + (static_cast<size_t>(id) * p.n_kv + kvh) * (kKv8Page * D) + g * D + 16 * t;
+  // A page comes in as it lies in memory, 512 bytes at a time; 16-byte pieces change places within 128 bytes so that eight lanes that read side by
+  // side, two token rows for scores and four for the output, meet all banks.
+  const uint8_t* mine = rings + warp * (4 * PAGE_BYTES);
+  const int k_at = D == 128 ? g * 128 + (t ^ swap128(g)) * 16 : (g >> 1) * 128 + (((g & 1) << 2 | t) ^ (g & 6)) * 16;
+  const int v_at = D == 128 ? 2 * t * 128 + (g ^ swap128(2 * t)) * 16 : t * 128 + ((g >> 1) ^ 2 * t) * 16 + (g & 1) * 8;
+  const int in_at = D == 128 ? (lane >> 3) * 128 + ((lane & 7) ^ swap128(lane >> 3)) * 16 : (lane >> 3) * 128 + ((lane & 7) ^ 2 * (lane >> 3)) * 16;
+  const uint32_t ring = smem_u32(mine);
+  auto fetch = [&](int turn) {
+    if ((turn & 15) == 0) look_up(turn);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int u = 0; u < 2; ++u) {
+      const int id = __shfl_sync(0xffffffffu, ids, 2 * (turn & 15) + u);
+      const size_t cell = (static_cast<size_t>(id) * p.n_kv + kvh) * (kKv8Page * D) + lane * 16;
+      const uint32_t to = ring + ((turn & 1) * 2 + u) * PAGE_BYTES;
 #pragma unroll
-      for (int j = 0; j < KC; ++j) kr[h][j] = ld_codes16(at + h * 8 * D + 64 * j);
+      for (int i = 0; i < D / 32; ++i) {
+        const int at = i * 512 + (D == 128 && (i & 1) ? in_at ^ 64 : in_at);
+        copy16(to + at, p.k_codes + cell + i * 512);
+        copy16(to + PAGE_BYTES / 2 + at, p.v_codes + cell + i * 512);
+      }
+    }
   };
-  auto fetch_v = [&](int turn) {
-    const int id = __shfl_sync(0xffffffffu, ids, turn & 31);
-    const int8_t* at = p.v_codes + (static_cast<size_t>(id) * p.n_kv + kvh) * (kKv8Page * D) + 2 * t * D + g * (D / 8);
+  if (turns > 0) fetch(0);
+  cp_async_commit();
+  if (turns > 1) fetch(1);
+  cp_async_commit();
+
+  // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
+  for (int nt = warp; nt < NT; nt += kKv8Warps) {
+    const int r = r0 + nt * 8 + g;
+    const bool in = nt * 8 + g < rows;
+    const size_t at = (static_cast<size_t>(b * p.q_per_seq + (in ? r / group : 0)) * p.n_q + kvh * group + (in ? r % group : 0)) * D + 16 * t;
+    float x[2 * KC][8];
+    float top = 0.f;
+    bool fine = true;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-      const int8_t* row = at + ((i >> 1) * 8 + (i & 1)) * D;
-      if (VW == 4) {
-        const uint4 u = ld_codes16(row);
-        vr[i][0] = u.x; vr[i][1] = u.y; vr[i][VW - 2] = u.z; vr[i][VW - 1] = u.w;
+    for (int j = 0; j < 2 * KC; ++j) {
+      const size_t from = at + 64 * (j >> 1) + 8 * (j & 1);
+      if (p.q32 != nullptr) {
+        const float4 u = *reinterpret_cast<const float4*>(p.q32 + from), w = *reinterpret_cast<const float4*>(p.q32 + from + 4);
+        x[j][0] = u.x; x[j][1] = u.y; x[j][2] = u.z; x[j][3] = u.w;
+        x[j][4] = w.x; x[j][5] = w.y; x[j][6] = w.z; x[j][7] = w.w;
       } else {
-        const uint2 u = ld_codes8(row);
-        vr[i][0] = u.x; vr[i][1] = u.y;
+        const uint4 u = *reinterpret_cast<const uint4*>(p.q + from);
+        x[j][0] = bf16_lo(u.x); x[j][1] = bf16_hi(u.x); x[j][2] = bf16_lo(u.y); x[j][3] = bf16_hi(u.y);
+        x[j][4] = bf16_lo(u.z); x[j][5] = bf16_hi(u.z); x[j][6] = bf16_lo(u.w); x[j][7] = bf16_hi(u.w);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!in) x[j][i] = 0.f;
+        top = fmaxf(top, fabsf(x[j][i]));
+        fine = fine && fabsf(x[j][i]) < INFINITY;
       }
     }
-    ks_next = __shfl_sync(0xffffffffu, ks, turn & 31);
-    ev_next = __shfl_sync(0xffffffffu, ev, turn & 31);
-  };
-  if (turns > 0) {
-    look_up(0);
-    fetch_k(0);
-    fetch_v(0);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t four = __ballot_sync(0xffffffffu, fine) >> (4 * g) & 15u;
+    const int e = static_cast<int>(__float_as_uint(top) >> 23);                  // 2^(e - 127) <= top
+    const int up = four != 15u || e == 0 ? 0 : 141 - e, half = up / 2;           // 2^up brings the largest to 2^14
+#pragma unroll
+    for (int j = 0; j < 2 * KC; ++j) q_s[(nt * 2 * KC + j) * 32 + lane] = query_bytes(x[j], exp2_of(half), exp2_of(up - half));
+    if (t == 0) back_s[nt * 8 + g] = four == 15u ? p.scale_log2 * exp2_of(-half) * exp2_of(half - up) : __uint_as_float(0x7fc00000u);
   }
+  __syncthreads();
+  float back[NT][2];                                    // of the lane's columns 2t, 2t + 1
+  int pos[NT][2];
+  float o[NT][STEPS][4], m[NT][2], m2[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      back[nt][c] = back_s[nt * 8 + 2 * t + c];
+      pos[nt][c] = pos_new + (r0 + min(nt * 8 + 2 * t + c, rows - 1)) / group;
+      m[nt][c] = m2[nt][c] = kLowest;
+      l[nt][c] = 0.f;
+    }
+  }
+
   for (int turn = 0; turn < turns; ++turn) {
-    const int tok = (page0 + warp + kKv8Warps * turn) * kKv8Page;
-    float s[NT][4];
+    const int tok = (page0 + 2 * (warp + kKv8Warps * turn)) * kKv8Page;
+    cp_async_wait<1>();
+    __syncwarp();
+    const uint8_t* from = mine + (turn & 1) * 2 * PAGE_BYTES;
+    // scales of this turn: its 16 may have been followed by the next ones already
+    const bool before = (turn >> 4) != (min(turn + 1, turns - 1) >> 4);
+    float s[2][NT][4], ev_now[2];
+    {
+      int hi[2][NT][4], lo[2][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int j = 0; j < KC; ++j) {
-      const uint32_t lo[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w}, hi[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t x = lo[w] ^ 0x80808080u, y = hi[w] ^ 0x80808080u;
-        const uint32_t a0 = kv8_halves<0x4140>(x), a1 = kv8_halves<0x4140>(y), a2 = kv8_halves<0x4342>(x), a3 = kv8_halves<0x4342>(y);
+          for (int c = 0; c < 4; ++c) hi[u][nt][c] = lo[u][nt][c] = kMagicBits;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qf[nt][4 * j + w][0], qf[nt][4 * j + w][1]);
+      for (int j = 0; j < KC; ++j) {
+        uint4 a[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          a[u][0] = *reinterpret_cast<const uint4*>(from + u * PAGE_BYTES + (k_at ^ (64 * j)));
+          a[u][1] = *reinterpret_cast<const uint4*>(from + u * PAGE_BYTES + 8 * D + (k_at ^ (64 * j)));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 q = q_s[(nt * 2 * KC + 2 * j + h) * 32 + lane];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t a0 = h == 0 ? a[u][0].x : a[u][0].z, a1 = h == 0 ? a[u][1].x : a[u][1].z;
+              const uint32_t a2 = h == 0 ? a[u][0].y : a[u][0].w, a3 = h == 0 ? a[u][1].y : a[u][1].w;
+              mma_s8(hi[u][nt], a0, a1, a2, a3, q.x, q.y);
+              mma_u8(lo[u][nt], a0, a1, a2, a3, q.z, q.w);
+            }
+          }
+      }
+      // ---- scores in log2 units
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = 2 * (turn & 15) + u;
+        const float ks_now = __shfl_sync(0xffffffffu, before ? ks_before : ks, at);
+        ev_now[u] = __shfl_sync(0xffffffffu, before ? ev_before : ev, at);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f0 = back[nt][0] * ks_now, f1 = back[nt][1] * ks_now;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[u][nt][c] = fmaf(__int_as_float(hi[u][nt][c]) - kMagic, 256.f, __int_as_float(lo[u][nt][c]) - kMagic) * (c & 1 ? f1 : f0);
+        }
       }
     }
-    const float ks_now = ks_next, ev_now = ev_next;
-    const bool more = turn + 1 < turns;
-    if (more) {
-      if (((turn + 1) & 31) == 0) look_up(turn + 1);
-      fetch_k(turn + 1);
+    const bool edge = tok + 2 * kKv8Page - 1 > mask_hi || tok < mask_lo;
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = tok + u * kKv8Page + g + (c >> 1) * 8, at = pos[nt][c & 1];
+            if (key > min(at, last_key) || key < kv8_lowest_key(p, at)) s[u][nt][c] = -INFINITY;
+          }
     }
-    // ---- scores in log2 units, masks, maxima
     bool passes = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[nt][c] *= back[nt][c & 1] * ks_now;
-    }
-    if (tok + kKv8Page - 1 > mask_hi || tok < mask_lo) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int key = tok + g + (c >> 1) * 8, at = pos[nt][c & 1];
-          if (key > at || key < kv8_lowest_key(p, at)) s[nt][c] = -INFINITY;
-        }
-    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float top = fmaxf(s[nt][c], s[nt][c + 2]);
-        passes |= top > m[nt][c] + kKv8Slack || top + ev_now > m2[nt][c] + kKv8Slack;
+        const float t0 = fmaxf(s[0][nt][c], s[0][nt][c + 2]), t1 = fmaxf(s[1][nt][c], s[1][nt][c + 2]);
+        passes |= fmaxf(t0, t1) > m[nt][c] + kKv8Slack || fmaxf(t0 + ev_now[0], t1 + ev_now[1]) > m2[nt][c] + kKv8Slack;
       }
     if (__any_sync(0xffffffffu, passes)) {
 #pragma unroll
@@ -265,10 +321,13 @@ __global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kern
         float down[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float top = fmaxf(s[nt][c], s[nt][c + 2]);
+          const float t0 = fmaxf(s[0][nt][c], s[0][nt][c + 2]), t1 = fmaxf(s[1][nt][c], s[1][nt][c + 2]);
+          float up = fmaxf(m[nt][c], fmaxf(t0, t1)), up2 = fmaxf(m2[nt][c], fmaxf(t0 + ev_now[0], t1 + ev_now[1]));
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const float up = fmaxf(m[nt][c], top), up2 = fmaxf(m2[nt][c], top + ev_now);
+          for (int x = 4; x < 32; x <<= 1) {
+            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, x));
+            up2 = fmaxf(up2, __shfl_xor_sync(0xffffffffu, up2, x));
+          }
           l[nt][c] *= ex2_approx(m[nt][c] - up);
           down[c] = ex2_approx(m2[nt][c] - up2);
           m[nt][c] = up;
@@ -283,36 +342,61 @@ __global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kern
         }
       }
     }
-    uint32_t pf[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        l[nt][c & 1] += ex2_approx(s[nt][c] - m[nt][c & 1]);
-        // a masked place is zero whatever the scale of its block is
-        w[c] = s[nt][c] == -INFINITY ? 0.f : ex2_approx(s[nt][c] + ev_now - m2[nt][c & 1]);
-      }
-      pf[nt][0] = transposed(pack_f16x2(w[0], w[1]));
-      pf[nt][1] = transposed(pack_f16x2(w[2], w[3]));
-    }
-    // ---- output
-#pragma unroll
-    for (int w = 0; w < VW; ++w) {
-      const uint32_t a = vr[0][w] ^ 0x80808080u, bb = vr[1][w] ^ 0x80808080u, c = vr[2][w] ^ 0x80808080u, d = vr[3][w] ^ 0x80808080u;
-      const uint32_t x0 = __byte_perm(a, bb, 0x5140), x1 = __byte_perm(a, bb, 0x7362), y0 = __byte_perm(c, d, 0x5140), y1 = __byte_perm(c, d, 0x7362);
-      const uint32_t e0 = kv8_halves<0x4140>(x0), e1 = kv8_halves<0x4342>(x0), e2 = kv8_halves<0x4140>(y0), e3 = kv8_halves<0x4342>(y0);
-      const uint32_t f0 = kv8_halves<0x4140>(x1), f1 = kv8_halves<0x4342>(x1), f2 = kv8_halves<0x4140>(y1), f3 = kv8_halves<0x4342>(y1);
+    for (int u = 0; u < 2; ++u) {
+      uint32_t pf[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mma_f16(o[nt][2 * w], e0, e1, e2, e3, pf[nt][0], pf[nt][1]);
-        mma_f16(o[nt][2 * w + 1], f0, f1, f2, f3, pf[nt][0], pf[nt][1]);
+        float w[4];
+        // from a probability to what it weighs in the output. (Value scales that are further apart than this has room for, over 2^126, lose the smaller ones.)
+        const float f0 = ex2_approx(fminf(ev_now[u] + m[nt][0] - m2[nt][0], 126.f)), f1 = ex2_approx(fminf(ev_now[u] + m[nt][1] - m2[nt][1], 126.f));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float e = ex2_approx(s[u][nt][c] - m[nt][c & 1]);
+          l[nt][c & 1] += e;
+          w[c] = e * (c & 1 ? f1 : f0);
+        }
+        if (edge) {   // a masked place is zero whatever the scale of its block is
+#pragma unroll
+          for (int c = 0; c < 4; ++c) w[c] = s[u][nt][c] == -INFINITY ? 0.f : w[c];
+        }
+        pf[nt][0] = transposed(pack_f16x2(w[0], w[1]));
+        pf[nt][1] = transposed(pack_f16x2(w[2], w[3]));
+      }
+      // ---- output
+      uint32_t vr[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* row = from + u * PAGE_BYTES + PAGE_BYTES / 2 + (i >> 1) * 8 * D + (i & 1 ? (v_at ^ 64) + (D == 128 ? 128 : 0) : v_at);
+        if (VW == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(row);
+          vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(row);
+          vr[i][0] = x.x; vr[i][1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t a = vr[0][w] ^ 0x80808080u, bb = vr[1][w] ^ 0x80808080u, c = vr[2][w] ^ 0x80808080u, d = vr[3][w] ^ 0x80808080u;
+        const uint32_t x0 = __byte_perm(a, bb, 0x5140), x1 = __byte_perm(a, bb, 0x7362), y0 = __byte_perm(c, d, 0x5140), y1 = __byte_perm(c, d, 0x7362);
+        const uint32_t e0 = kv8_halves<0x4140>(x0), e1 = kv8_halves<0x4342>(x0), e2 = kv8_halves<0x4140>(y0), e3 = kv8_halves<0x4342>(y0);
+        const uint32_t f0 = kv8_halves<0x4140>(x1), f1 = kv8_halves<0x4342>(x1), f2 = kv8_halves<0x4140>(y1), f3 = kv8_halves<0x4342>(y1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_f16(o[nt][2 * w], e0, e1, e2, e3, pf[nt][0], pf[nt][1]);
+          mma_f16(o[nt][2 * w + 1], f0, f1, f2, f3, pf[nt][0], pf[nt][1]);
+        }
       }
     }
-    if (more) fetch_v(turn + 1);
+    __syncwarp();
+    if (turn + 2 < turns) fetch(turn + 2);
+    cp_async_commit();
   }
 
   // ---- the warps of the CTA together
+  cp_async_wait<0>();
+  __syncthreads();
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -339,7 +423,7 @@ __global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kern
   __syncthreads();
   const bool alone = p.splits == 1, cluster = p.splits > 1 && p.splits <= kKv8Cluster;
   const size_t part = ((static_cast<size_t>(b) * p.n_kv * p.tiles + blockIdx.y) * p.splits + split) * ROWS;
-  for (int i = threadIdx.x; i < rows * D; i += 32 * kKv8Warps) {
+  for (int i = threadIdx.x; i < rows * D; i += kKv8Threads) {
     const int row = i / D, d = i % D;
     const Kv8Row r = row_s[row];
     float sum = 0.f;
@@ -360,7 +444,7 @@ __global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kern
   // ---- the splits: every CTA of the cluster finishes some of the values
   cluster_arrive_release();
   cluster_wait_acquire();
-  for (int i = split * 32 * kKv8Warps + threadIdx.x; i < rows * D; i += p.splits * 32 * kKv8Warps) {
+  for (int i = split * kKv8Threads + threadIdx.x; i < rows * D; i += p.splits * kKv8Threads) {
     const int row = i / D;
     Kv8Row part_row[kKv8Cluster], r = {kLowest, 0.f, kLowest};
 #pragma unroll
@@ -386,47 +470,81 @@ __global__ void __launch_bounds__(32 * kKv8Warps, NT == 1 ? 2 : 1) attn_kv8_kern
   cluster_wait_acquire();
 }
 
-// More splits than a cluster holds: a warp per query row. grid (rows, n_kv, B), 32 threads
+// More splits than a cluster holds: eight warps per query row, each of them some of the splits. grid (rows, n_kv, B)
+constexpr int kCombineWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(32) attn_kv8_combine_kernel(AttnKv8Params p, int tile_rows) {
+__global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(AttnKv8Params p, int tile_rows) {
   constexpr int PER = D / 32;
+  __shared__ Kv8Row row_s[kCombineWarps];
+  __shared__ float sum_s[kCombineWarps][D];
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.z, kvh = blockIdx.y, at = blockIdx.x, lane = threadIdx.x, group = p.n_q / p.n_kv;
+  const int b = blockIdx.z, kvh = blockIdx.y, at = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.n_q / p.n_kv;
   const int tile = at / tile_rows, row = at % tile_rows;
   const size_t first = ((static_cast<size_t>(b) * p.n_kv + kvh) * p.tiles + tile) * p.splits * tile_rows + row;
   Kv8Row r = {kLowest, 0.f, kLowest};
-  for (int s = lane; s < p.splits; s += 32) {
-    const float* ml = p.part_ml + (first + static_cast<size_t>(s) * tile_rows) * 4;
-    r.m = fmaxf(r.m, ml[0]);
-    r.m2 = fmaxf(r.m2, ml[2]);
-  }
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) {
-    r.m = fmaxf(r.m, __shfl_xor_sync(0xffffffffu, r.m, x));
-    r.m2 = fmaxf(r.m2, __shfl_xor_sync(0xffffffffu, r.m2, x));
-  }
   float sum[PER] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const size_t i = first + static_cast<size_t>(s) * tile_rows;
-    const float4 ml = *reinterpret_cast<const float4*>(p.part_ml + i * 4);
-    r.l += ml.y * ex2_approx(ml.x - r.m);
-    const float w = ex2_approx(ml.z - r.m2);
+  // up to eight splits a warp at once, so that their loads are on the way together
+  for (int s0 = warp; s0 < p.splits; s0 += 8 * kCombineWarps) {
+    float4 ml[8];
+    float part[8][PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) sum[j] += p.part_o[i * D + lane + 32 * j] * w;
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i * kCombineWarps;
+      const size_t from = first + static_cast<size_t>(min(s, p.splits - 1)) * tile_rows;
+      ml[i] = s < p.splits ? *reinterpret_cast<const float4*>(p.part_ml + from * 4) : make_float4(kLowest, 0.f, kLowest, 0.f);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) part[i][j] = s < p.splits ? p.part_o[from * D + lane + 32 * j] : 0.f;
+    }
+    float m = r.m, m2 = r.m2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m = fmaxf(m, ml[i].x);
+      m2 = fmaxf(m2, ml[i].z);
+    }
+    r.l *= ex2_approx(r.m - m);
+    const float down = ex2_approx(r.m2 - m2);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum[j] *= down;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      r.l += ml[i].y * ex2_approx(ml[i].x - m);
+      const float w = ex2_approx(ml[i].z - m2);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) sum[j] += part[i][j] * w;
+    }
+    r.m = m;
+    r.m2 = m2;
+  }
+  if (lane == 0) row_s[warp] = r;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) sum_s[warp][lane + 32 * j] = sum[j];
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  r = Kv8Row{kLowest, 0.f, kLowest};
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) {
+    r.m = fmaxf(r.m, row_s[w].m);
+    r.m2 = fmaxf(r.m2, row_s[w].m2);
+  }
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) {
+    r.l += row_s[w].l * ex2_approx(row_s[w].m - r.m);
+    all += sum_s[w][threadIdx.x] * ex2_approx(row_s[w].m2 - r.m2);
   }
   const int head = kvh * group + at % group;
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-    p.out[(static_cast<size_t>(b * p.q_per_seq + at / group) * p.n_q + head) * D + lane + 32 * j] =
-        __float2bfloat16(kv8_finish(sum[j], r, p.sinks == nullptr ? nullptr : p.sinks + head));
+  p.out[(static_cast<size_t>(b * p.q_per_seq + at / group) * p.n_q + head) * D + threadIdx.x] =
+      __float2bfloat16(kv8_finish(all, r, p.sinks == nullptr ? nullptr : p.sinks + head));
 }
 
 template <int D, int NT>
 static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream_t stream) {
   constexpr int ROWS = 8 * NT;
-  const size_t smem = static_cast<size_t>(kKv8Warps + 1) * ROWS * (D * sizeof(float) + sizeof(Kv8Row));
+  constexpr size_t rings = static_cast<size_t>(kKv8Warps) * 4 * 2 * kKv8Page * D;
+  constexpr size_t gathered = static_cast<size_t>(kKv8Warps + 1) * ROWS * (D * sizeof(float) + sizeof(Kv8Row));
+  constexpr size_t smem = NT * (D / 32) * 512 + (rings > gathered ? rings : gathered);
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -438,7 +556,7 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.splits, p.n_kv * p.tiles, batch);
-  cfg.blockDim = dim3(32 * kKv8Warps);
+  cfg.blockDim = dim3(kKv8Threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -459,7 +577,7 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream
   cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv8_kernel<D, NT>, p);
   eredu_count_launches(1);
   if (e == cudaSuccess && p.splits > kKv8Cluster) {
-    e = launch_pdl(attn_kv8_combine_kernel<D>, dim3(p.q_per_seq * (p.n_q / p.n_kv), p.n_kv, batch), dim3(32), 0, stream, p, ROWS);
+    e = launch_pdl(attn_kv8_combine_kernel<D>, dim3(p.q_per_seq * (p.n_q / p.n_kv), p.n_kv, batch), dim3(32 * kCombineWarps), 0, stream, p, ROWS);
     eredu_count_launches(1);
   }
   return e;
@@ -484,6 +602,7 @@ extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const v
     return -2;
   AttnKv8Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q32 = nullptr;
   p.k_codes = static_cast<const int8_t*>(k_codes);
   p.v_codes = static_cast<const int8_t*>(v_codes);
   p.k_scales = k_scales;
