@@ -34,9 +34,10 @@ struct AttnKv8Params {
   const int* block_table;          // [B, max_pages]
   const int* seq_lens;             // [B], new tokens included
   const float* sinks;              // optional [n_q]
-  float* part_o;                   // more splits than a cluster holds: [B, n_kv, tiles, splits, rows of a tile, D]
-  float* part_ml;                  //                                   [B, n_kv, tiles, splits, rows of a tile, 4]
-  int max_pages, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
+  float* part_o;                   // even shares: [CTAs, 2, rows of a tile, D]
+  float* part_ml;                  //              [CTAs, 2, rows of a tile, 4]
+  int4* joins;                     //              [CTAs]: what of the CTA's first part is to be added up, see attn_kv8_combine_kernel
+  int batch, max_pages, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
   float scale_log2;
   int* status;
 };
@@ -87,6 +88,56 @@ __device__ __forceinline__ int kv8_lowest_key(const AttnKv8Params& p, int pos) {
   return p.chunk > 0 && pos > 0 ? pos - pos % p.chunk : 0;
 }
 
+// Pages of a sequence that one of its queries sees: [first, end).
+struct Kv8Pages {
+  int first, end;
+};
+__device__ __forceinline__ Kv8Pages kv8_pages(const AttnKv8Params& p, int kv_len) {
+  const int last = min((kv_len + kKv8Page - 1) / kKv8Page, p.max_pages);
+  return Kv8Pages{min(kv8_lowest_key(p, kv_len - p.q_per_seq) / kKv8Page, last), last};
+}
+// Even shares: the pairs of pages of all sequences, heads and tiles of rows in one line, of which every CTA takes as many. A sequence has one pair at
+// least, so that somebody writes its rows.
+__device__ __forceinline__ int kv8_pairs(const AttnKv8Params& p, int b) {
+  const Kv8Pages r = kv8_pages(p, p.seq_lens[b]);
+  return max(1, (r.end - r.first + 1) / 2);
+}
+constexpr int kKv8LeastPairs = 4;   // of a CTA: one per warp
+struct Kv8Place {
+  int total, share;      // pairs in all, pairs of a CTA
+  int b, begin, pairs;   // sequence in which pair `at` lies, where its pairs begin, and how many a head and tile of it has
+};
+// Place of pair share * i, by one warp; b = -1 behind the last.
+__device__ __forceinline__ Kv8Place kv8_place(const AttnKv8Params& p, int i, int ctas, int lane) {
+  const int heads = p.n_kv * p.tiles;
+  Kv8Place r = {0, 0, -1, 0, 0};
+  int pairs = lane < p.batch ? kv8_pairs(p, lane) : 0;
+  r.total = __reduce_add_sync(0xffffffffu, pairs);
+  for (int base = 32; base < p.batch; base += 32) r.total += __reduce_add_sync(0xffffffffu, base + lane < p.batch ? kv8_pairs(p, base + lane) : 0);
+  r.total *= heads;
+  r.share = max(kKv8LeastPairs, (r.total + ctas - 1) / ctas);
+  const int at = r.share * i;
+  if (at >= r.total) return r;
+  for (int base = 0;; base += 32) {
+    if (base > 0) pairs = base + lane < p.batch ? kv8_pairs(p, base + lane) : 0;
+    int end = pairs;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, end, x);
+      if (lane >= x) end += o;
+    }
+    const uint32_t behind = __ballot_sync(0xffffffffu, r.begin + end * heads > at);
+    if (behind != 0) {   // at < total: it comes
+      const int l = __ffs(behind) - 1;
+      r.b = base + l;
+      r.pairs = __shfl_sync(0xffffffffu, pairs, l);
+      r.begin += __shfl_sync(0xffffffffu, end - pairs, l) * heads;
+      return r;
+    }
+    r.begin += __shfl_sync(0xffffffffu, end, 31) * heads;
+  }
+}
+
 // What a row has gathered: maximum and sum of the scores, maximum the output is relative to.
 struct Kv8Row {
   float m, l, m2;
@@ -115,8 +166,10 @@ __device__ __forceinline__ uint4 query_bytes(const float (&x)[8], float up, floa
   return make_uint4(pick(0, 0x0051), pick(4, 0x0051), pick(0, 0x0040), pick(4, 0x0040));
 }
 
-// grid (splits, n_kv * tiles, B)
-template <int D, int NT>
+// grid (splits, n_kv * tiles, B): the splits of a sequence and head form a cluster and meet in its shared memory.
+// EVEN: grid (CTAs): even shares of all pairs, so that long and short sequences, and few and many, fill the SMs alike. What a CTA has of a sequence and head
+// that others have a part of as well goes to memory, and attn_kv8_combine_kernel adds it up.
+template <int D, int NT, bool EVEN>
 __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params p) {
   constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16, VW = D / 32;   // KC: 16-byte pieces of a token row per lane; VW: value words per token and lane
   constexpr int PAGE_BYTES = 2 * kKv8Page * D;
@@ -134,18 +187,46 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   pdl_wait();
   trace_mark(kTraceAttnDecode, kTraceAfterWait);
   pdl_launch_dependents();
-  const int b = blockIdx.z, kvh = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles, split = blockIdx.x;
   const int warp = static_cast<int>(warp_uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int group = p.n_q / p.n_kv, rows_all = p.q_per_seq * group, r0 = tile * ROWS, rows = min(ROWS, rows_all - r0);
+  const int group = p.n_q / p.n_kv, rows_all = p.q_per_seq * group;
+  // the CTA's share: pairs [at, end) of the line; or one split
+  Kv8Place place = {};
+  int at = 0, end = 0, slot = 0;
+  if (EVEN) {
+    place = kv8_place(p, blockIdx.x, gridDim.x, lane);
+    at = place.share * blockIdx.x;
+    if (threadIdx.x == 0) {
+      const int head_tile = place.b < 0 ? 0 : (at - place.begin) / place.pairs, begin = place.begin + head_tile * place.pairs;
+      // of the CTAs that have a part of these rows, the second one stands for all: it begins behind their first pair, and the CTA in front does not
+      const bool second = place.b >= 0 && at > begin && at - place.share <= begin;
+      p.joins[blockIdx.x] = second ? make_int4((begin + place.pairs - 1) / place.share - blockIdx.x + 2, place.b, head_tile, at - place.share == begin) : make_int4(0, 0, 0, 0);
+    }
+    if (place.b < 0) return;
+    end = min(place.total, at + place.share);
+  }
+  do {
+  const int b = EVEN ? place.b : blockIdx.z, head_tile = EVEN ? (at - place.begin) / place.pairs : blockIdx.y, split = EVEN ? 0 : blockIdx.x;
+  const int kvh = head_tile / p.tiles, r0 = head_tile % p.tiles * ROWS, rows = min(ROWS, rows_all - r0);
   const int kv_len = p.seq_lens[b], pos_new = kv_len - p.q_per_seq;
   const int pos_first = pos_new + r0 / group, pos_last = pos_new + (r0 + rows - 1) / group;   // positions of the tile's first and last row
-  const int page_lo = kv8_lowest_key(p, pos_first) / kKv8Page, page_hi = min(pos_last / kKv8Page + (pos_last >= 0), p.max_pages);
-  const int per = max(0, page_hi - page_lo + p.splits - 1) / p.splits;
-  const int page0 = page_lo + split * per, page1 = min(page_hi, page0 + per);
-  const int last_key = page1 * kKv8Page - 1;                                                  // of this split
+  const Kv8Pages pages = kv8_pages(p, kv_len);
+  int page0, page1;
+  bool whole = p.splits == 1;                                                                 // nobody else has a part of these rows
+  if (EVEN) {
+    const int first = (at - place.begin) % place.pairs, n = min(end - at, place.pairs - first);
+    whole = n == place.pairs;
+    at += n;
+    page0 = pages.first + 2 * first;
+    page1 = min(pages.end, page0 + 2 * n);
+  } else {
+    const int per = (pages.end - pages.first + p.splits - 1) / p.splits;
+    page0 = pages.first + split * per;
+    page1 = min(pages.end, page0 + per);
+  }
+  const int last_key = page1 * kKv8Page - 1;                                                  // of this part
   const int mask_hi = min(pos_first, last_key), mask_lo = kv8_lowest_key(p, pos_last);        // pages inside need no mask
 
-  // ---- pairs warp, warp + 6, ... of the split. Lanes 2 i and 2 i + 1 hold page ids and scales of the i-th of 16 turns; those of the 16 before stay at hand.
+  // ---- pairs warp, warp + 4, ... of the part. Lanes 2 i and 2 i + 1 hold page ids and scales of the i-th of 16 turns; those of the 16 before stay at hand.
   const int* table = p.block_table + static_cast<size_t>(b) * p.max_pages;
   const int turns = page1 > page0 + 2 * warp ? (page1 - page0 - 2 * warp + 2 * kKv8Warps - 1) / (2 * kKv8Warps) : 0;
   int ids = 0;
@@ -421,26 +502,34 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     row_s[threadIdx.x] = r;
   }
   __syncthreads();
-  const bool alone = p.splits == 1, cluster = p.splits > 1 && p.splits <= kKv8Cluster;
-  const size_t part = ((static_cast<size_t>(b) * p.n_kv * p.tiles + blockIdx.y) * p.splits + split) * ROWS;
+  const size_t part = (static_cast<size_t>(blockIdx.x) * 2 + slot) * ROWS;
   for (int i = threadIdx.x; i < rows * D; i += kKv8Threads) {
     const int row = i / D, d = i % D;
     const Kv8Row r = row_s[row];
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kKv8Warps; ++w) sum += o_warp[(w * ROWS + row) * D + d] * ex2_approx(row_warp[w * ROWS + row].m2 - r.m2);
-    if (alone) {
-      const int at = r0 + row, head = kvh * group + at % group;
-      p.out[(static_cast<size_t>(b * p.q_per_seq + at / group) * p.n_q + head) * D + d] =
+    if (whole) {
+      const int n = r0 + row, head = kvh * group + n % group;
+      p.out[(static_cast<size_t>(b * p.q_per_seq + n / group) * p.n_q + head) * D + d] =
           __float2bfloat16(kv8_finish(sum, r, p.sinks == nullptr ? nullptr : p.sinks + head));
-    } else if (cluster) {
+    } else if (!EVEN) {
       o_s[i] = sum;
     } else {
       p.part_o[part * D + i] = sum;
       if (d == 0) *reinterpret_cast<float4*>(p.part_ml + (part + row) * 4) = make_float4(r.m, r.l, r.m2, 0.f);
     }
   }
-  if (!cluster) return;
+  if (EVEN) {
+    slot = 1;
+    if (at < end && at == place.begin + place.pairs * p.n_kv * p.tiles) {
+      place.begin = at;
+      place.pairs = kv8_pairs(p, ++place.b);
+    }
+    __syncthreads();   // shared memory is free again
+    continue;
+  }
+  if (whole) return;
   // ---- the splits: every CTA of the cluster finishes some of the values
   cluster_arrive_release();
   cluster_wait_acquire();
@@ -462,40 +551,45 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       r.l += part_row[s].l * ex2_approx(part_row[s].m - r.m);
       sum += ld_cluster_f32(mapa_shared(smem_u32(o_s + i), s)) * ex2_approx(part_row[s].m2 - r.m2);
     }
-    const int at = r0 + row, head = kvh * group + at % group;
-    p.out[(static_cast<size_t>(b * p.q_per_seq + at / group) * p.n_q + head) * D + i % D] =
+    const int n = r0 + row, head = kvh * group + n % group;
+    p.out[(static_cast<size_t>(b * p.q_per_seq + n / group) * p.n_q + head) * D + i % D] =
         __float2bfloat16(kv8_finish(sum, r, p.sinks == nullptr ? nullptr : p.sinks + head));
   }
   cluster_arrive_release();   // nobody leaves while its shared memory is read
   cluster_wait_acquire();
+  } while (EVEN && at < end);
 }
 
-// More splits than a cluster holds: eight warps per query row, each of them some of the splits. grid (rows, n_kv, B)
-constexpr int kCombineWarps = 8;
-template <int D>
-__global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(AttnKv8Params p, int tile_rows) {
-  constexpr int PER = D / 32;
+// Rows of a sequence and head of which several CTAs have a part. grid (CTAs, rows of a tile): joins[i] = {parts, sequence, head and tile, whether the first
+// part, that of CTA i - 1, is also the first of that CTA}, no parts where there is nothing to add up. Four warps take some parts each.
+constexpr int kCombineWarps = 4;
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(AttnKv8Params p) {
+  constexpr int PER = D / 32, ROWS = 8 * NT;
   __shared__ Kv8Row row_s[kCombineWarps];
   __shared__ float sum_s[kCombineWarps][D];
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.z, kvh = blockIdx.y, at = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.n_q / p.n_kv;
-  const int tile = at / tile_rows, row = at % tile_rows;
-  const size_t first = ((static_cast<size_t>(b) * p.n_kv + kvh) * p.tiles + tile) * p.splits * tile_rows + row;
+  const int4 join = p.joins[blockIdx.x];
+  const int parts = join.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.n_q / p.n_kv;
+  const int kvh = join.z / p.tiles, n = join.z % p.tiles * ROWS + row, c0 = blockIdx.x - 1;
+  if (parts == 0 || n >= p.q_per_seq * group) return;
+  // the first of the CTAs has it as its last part, the others as their first
+  auto place_of = [&](int s) { return (static_cast<size_t>(c0 + s) * 2 + (s == 0 && join.w == 0 ? 1 : 0)) * ROWS + row; };
   Kv8Row r = {kLowest, 0.f, kLowest};
   float sum[PER] = {};
   // up to eight splits a warp at once, so that their loads are on the way together
-  for (int s0 = warp; s0 < p.splits; s0 += 8 * kCombineWarps) {
+  for (int s0 = warp; s0 < parts; s0 += 8 * kCombineWarps) {
     float4 ml[8];
     float part[8][PER];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int s = s0 + i * kCombineWarps;
-      const size_t from = first + static_cast<size_t>(min(s, p.splits - 1)) * tile_rows;
-      ml[i] = s < p.splits ? *reinterpret_cast<const float4*>(p.part_ml + from * 4) : make_float4(kLowest, 0.f, kLowest, 0.f);
+      const size_t from = place_of(min(s, parts - 1));
+      ml[i] = s < parts ? *reinterpret_cast<const float4*>(p.part_ml + from * 4) : make_float4(kLowest, 0.f, kLowest, 0.f);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) part[i][j] = s < p.splits ? p.part_o[from * D + lane + 32 * j] : 0.f;
+      for (int j = 0; j < PER; ++j) part[i][j] = s < parts ? p.part_o[from * D + lane + 32 * j] : 0.f;
     }
     float m = r.m, m2 = r.m2;
 #pragma unroll
@@ -521,7 +615,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(At
 #pragma unroll
   for (int j = 0; j < PER; ++j) sum_s[warp][lane + 32 * j] = sum[j];
   __syncthreads();
-  if (threadIdx.x >= D) return;
+  if (threadIdx.x >= D) return;   // (D is at most the number of threads)
   r = Kv8Row{kLowest, 0.f, kLowest};
 #pragma unroll
   for (int w = 0; w < kCombineWarps; ++w) {
@@ -534,13 +628,13 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(At
     r.l += row_s[w].l * ex2_approx(row_s[w].m - r.m);
     all += sum_s[w][threadIdx.x] * ex2_approx(row_s[w].m2 - r.m2);
   }
-  const int head = kvh * group + at % group;
-  p.out[(static_cast<size_t>(b * p.q_per_seq + at / group) * p.n_q + head) * D + threadIdx.x] =
+  const int head = kvh * group + n % group;
+  p.out[(static_cast<size_t>(join.y * p.q_per_seq + n / group) * p.n_q + head) * D + threadIdx.x] =
       __float2bfloat16(kv8_finish(all, r, p.sinks == nullptr ? nullptr : p.sinks + head));
 }
 
-template <int D, int NT>
-static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream_t stream) {
+template <int D, int NT, bool EVEN>
+static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int ctas, cudaStream_t stream) {
   constexpr int ROWS = 8 * NT;
   constexpr size_t rings = static_cast<size_t>(kKv8Warps) * 4 * 2 * kKv8Page * D;
   constexpr size_t gathered = static_cast<size_t>(kKv8Warps + 1) * ROWS * (D * sizeof(float) + sizeof(Kv8Row));
@@ -550,18 +644,18 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<D, NT, EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.splits, p.n_kv * p.tiles, batch);
+  cfg.gridDim = EVEN ? dim3(ctas) : dim3(p.splits, p.n_kv * p.tiles, p.batch);
   cfg.blockDim = dim3(kKv8Threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (p.splits > 1 && p.splits <= kKv8Cluster) {
+  if (!EVEN && p.splits > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = p.splits;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
@@ -574,10 +668,10 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int batch, cudaStream
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv8_kernel<D, NT>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv8_kernel<D, NT, EVEN>, p);
   eredu_count_launches(1);
-  if (e == cudaSuccess && p.splits > kKv8Cluster) {
-    e = launch_pdl(attn_kv8_combine_kernel<D>, dim3(p.q_per_seq * (p.n_q / p.n_kv), p.n_kv, batch), dim3(32 * kCombineWarps), 0, stream, p, ROWS);
+  if (EVEN && e == cudaSuccess) {
+    e = launch_pdl(attn_kv8_combine_kernel<D, NT>, dim3(ctas, p.tiles == 1 ? p.q_per_seq * (p.n_q / p.n_kv) : ROWS), dim3(32 * kCombineWarps), 0, stream, p);
     eredu_count_launches(1);
   }
   return e;
@@ -592,13 +686,14 @@ EREDU_TRACE_INSTALLER(attention_kv8)
 // Query rows of one key / value head that a CTA takes at once; beyond 16, a tile more of them reads the pages again.
 static int kv8_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
 
+// splits 1 to 8: CTAs of a sequence and head. 0: even shares for `ctas` CTAs, with scratch for 2 * ctas tiles of 8 rows (16 where a head has more than 8).
 extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
-                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, int batch,
-                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int D, int splits, int window, int chunk, float scale,
-                                     int* status, cudaStream_t stream) {
+                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
+                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int D, int splits, int ctas, int window, int chunk,
+                                     float scale, int* status, cudaStream_t stream) {
   if (batch <= 0) return 0;
-  if ((D != 64 && D != 128) || n_kv <= 0 || n_q % n_kv != 0 || n_q <= 0 || q_per_seq <= 0 || splits <= 0 || max_pages <= 0 || num_pages <= 0 ||
-      window < 0 || chunk < 0 || batch > 65535 || (splits > kKv8Cluster && (part_o == nullptr || part_ml == nullptr)))
+  if ((D != 64 && D != 128) || n_kv <= 0 || n_q % n_kv != 0 || n_q <= 0 || q_per_seq <= 0 || splits < 0 || splits > kKv8Cluster || max_pages <= 0 ||
+      num_pages <= 0 || window < 0 || chunk < 0)
     return -2;
   AttnKv8Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -613,6 +708,8 @@ extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const v
   p.sinks = sinks;
   p.part_o = part_o;
   p.part_ml = part_ml;
+  p.joins = static_cast<int4*>(joins);
+  p.batch = batch;
   p.max_pages = max_pages;
   p.num_pages = num_pages;
   p.n_q = n_q;
@@ -625,9 +722,14 @@ extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const v
   p.chunk = chunk;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status;
-  if (static_cast<long long>(n_kv) * p.tiles > 65535) return -2;
+  const long long line = static_cast<long long>(batch) * n_kv * p.tiles * (max_pages / 2 + 1);
+  if (splits == 0 ? ctas <= 0 || part_o == nullptr || part_ml == nullptr || joins == nullptr || line > (1LL << 30) : batch > 65535 || static_cast<long long>(n_kv) * p.tiles > 65535) return -2;
   cudaError_t e;
-  if (D == 128) e = tile == 8 ? launch_attn_kv8<128, 1>(p, batch, stream) : launch_attn_kv8<128, 2>(p, batch, stream);
-  else e = tile == 8 ? launch_attn_kv8<64, 1>(p, batch, stream) : launch_attn_kv8<64, 2>(p, batch, stream);
+#define ER_KV8(D_, NT_) e = splits == 0 ? launch_attn_kv8<D_, NT_, true>(p, ctas, stream) : launch_attn_kv8<D_, NT_, false>(p, ctas, stream)
+  if (D == 128 && tile == 8) ER_KV8(128, 1);
+  else if (D == 128) ER_KV8(128, 2);
+  else if (tile == 8) ER_KV8(64, 1);
+  else ER_KV8(64, 2);
+#undef ER_KV8
   return static_cast<int>(e);
 }

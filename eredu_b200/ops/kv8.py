@@ -23,11 +23,23 @@ from .native import check, lib, ptr, status_word, stream_ptr
 PAGE = 16
 FLOOR = 2.0 ** -100          # smallest scale
 KV8_HEAD_DIMS = (64, 128)    # head sizes of the kernels
+CLUSTER = 8                  # splits of a sequence and head that meet in a cluster
+EVEN_CTAS = 3                # CTAs to an SM that take even shares of all pages
+
+_sms: dict = {}
+
+
+def _sm_count(device) -> int:
+    n = _sms.get(device)
+    if n is None:
+        n = _sms[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
+
 
 P, I, F = native.P, native.I, native.F
 native.register("eredu_kv8_store", I, [P] * 13 + [I] * 10 + [F] * 3 + [P] * 2)
 native.register("eredu_kv8_values", I, [P] * 10 + [I] * 8 + [P] * 2)
-native.register("eredu_attn_kv8_decode", I, [P] * 11 + [I] * 10 + [F] + [P] * 2)
+native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 11 + [F] + [P] * 2)
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 
@@ -211,8 +223,9 @@ def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_
 
 
 def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk):
-    """The form of :func:`.core.attention_decode` for 8-bit pages on a GPU. More splits than a cluster holds leave partial sums in memory that the
-    call allocates; a second kernel adds them up."""
+    """The form of :func:`.core.attention_decode` for 8-bit pages on a GPU. ``splits`` from 1 to 8: CTAs for a sequence and head, which meet in a cluster;
+    any other number: even shares of all pages whatever the sequences' lengths are, partial sums in memory that the call allocates, and a second kernel
+    that adds them up."""
     check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out)
     dev, B = q.device, seq_lens.shape[0]
     n_q, dim = q.shape[1:]
@@ -221,30 +234,30 @@ def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
         raise ValueError(f"{q.shape[0]} query rows for {B} sequences of {q_per_seq}")
     if out is None:
         out = torch.empty_like(q)
-    part_o = part_ml = None
-    if splits > 8:
-        rows = q_per_seq * (n_q // n_kv)
-        tile = 8 if rows <= 8 else 16
-        elements = B * n_kv * -(-rows // tile) * tile * splits
-        part = torch.empty(elements * (dim + 4), dtype=torch.float32, device=dev)
+    part_o = part_ml = joins = None
+    ctas = 0
+    if splits > CLUSTER or splits < 1:
+        splits, ctas = 0, EVEN_CTAS * _sm_count(dev)
+        rows = 2 * ctas * (8 if q_per_seq * (n_q // n_kv) <= 8 else 16)
+        part = torch.empty(rows * (dim + 4) + 4 * ctas, dtype=torch.float32, device=dev)
         part_o = part.data_ptr()
-        part_ml = part_o + elements * dim * 4
+        part_ml = part_o + rows * dim * 4
+        joins = part_ml + rows * 16
     code = lib().eredu_attn_kv8_decode(q.data_ptr(), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
-                                       block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, B, q_per_seq, block_table.stride(0),
-                                       k_cache.codes.shape[0], n_q, n_kv, dim, splits, int(window), int(chunk), scale, ptr(status_word(dev)), stream_ptr(dev))
+                                       block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins, B, q_per_seq, block_table.stride(0),
+                                       k_cache.codes.shape[0], n_q, n_kv, dim, splits, ctas, int(window), int(chunk), scale, ptr(status_word(dev)), stream_ptr(dev))
     check(code, "eredu_attn_kv8_decode")
     return out
 
 
 def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
-    """Split factor of the decode kernel for 8-bit pages: CTAs of eight warps, two to an SM where a key / value head has up to eight query rows,
-    one where it has more; a page per warp and split at least."""
+    """Split factor of the decode kernel for 8-bit pages: 1 to 8 CTAs for a sequence and head, or 0 for even shares."""
     tile = 8 if rows <= 8 else 16
-    ctas = max(1, batch * n_kv * -(-max(rows, 1) // tile))
-    pages = max(1, -(-max_kv_len // PAGE))
-    want = sm_count * (2 if tile == 8 else 1) // ctas
-    splits = max(1, min(want, pages // 8, 64))
-    return 8 if 8 < splits < 16 and pages <= 1024 else splits
+    heads = max(1, batch * n_kv * -(-max(rows, 1) // tile))
+    pairs = max(1, -(-max_kv_len // (2 * PAGE)))
+    if heads * pairs >= 8 * EVEN_CTAS * sm_count:
+        return 0
+    return max(1, min(EVEN_CTAS * sm_count // heads, pairs // 4, CLUSTER))
 
 
 def gather_values(k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_kv_len, window, chunk):
