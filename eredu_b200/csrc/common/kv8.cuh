@@ -32,11 +32,11 @@ __device__ __forceinline__ uint32_t kv8_pack(float a, float b, float c, float d)
 }
 __device__ __forceinline__ float kv8_code(uint32_t word, int i) { return static_cast<float>(static_cast<int8_t>(word >> (8 * i))); }
 
-// Two bytes of `biased` (codes + 128) as exact halves: 0x6400 | u is 1024 + u. `pick` = 0x4140 for the lower two, 0x4342 for the upper.
-template <uint32_t PICK>
-__device__ __forceinline__ uint32_t kv8_halves(uint32_t biased) {
-  uint32_t h = __byte_perm(biased, 0x64646464u, PICK);
-  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0x64806480u));   // 1024 + 128
+// The lower (UPPER: the upper) bytes of both halves of a word as exact f16: 0x6400 | c + 128 is 1152 + c.
+template <bool UPPER>
+__device__ __forceinline__ uint32_t kv8_parted(uint32_t word) {
+  uint32_t h = ((UPPER ? word >> 8 : word) & 0x00ff00ffu) ^ 0x64806480u;
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0x64806480u));
   return h;
 }
 

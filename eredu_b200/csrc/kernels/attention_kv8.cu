@@ -2,18 +2,16 @@
 //
 //   s_j = (q . c_j) scale ks,   o = sum_j 2^(s_j log2 e - m) vs c'_j / sum_j 2^(s_j log2 e - m)     (ks, vs: scales of token j's blocks)
 //
-// Bound by memory where contexts are long: every cached token is read once per key / value head, 2 D bytes. A warp walks pairs of pages of its own,
-// and every lane brings the bytes that it is going to need into a ring of its own in shared memory (cp.async; nothing is exchanged, so no
-// barrier and no bank conflicts): a pair is on its way while another is worked on. From there they go into the registers of mma.sync:
+// Bound by memory where contexts are long: every cached token is read once per key / value head, 2 D bytes. A warp walks pairs of pages of its own, which
+// come into its ring in shared memory by cp.async, one pair on its way while another is worked on, and go from there into the registers of mma.sync by ldmatrix:
 //   scores  S^T[16 tokens, 8 query rows] = K[16, D] Q^T as integers (m16n8k32): the codes are the A operand as they are. A query row is rounded to 16 bits,
 //           with a power of two that brings its largest magnitude to 2^14 (a bf16 query keeps all its bits down to 2^-7 of that), and taken as a signed upper and
-//           an unsigned lower byte. The sum over D may run in any order, so a lane takes 16 neighbouring bytes of two token rows.
-//   output  O^T[D, 8 rows] = V^T[D, 16] P^T in f16 (m16n8k16): a lane takes 16 neighbouring bytes (8 where D = 64) of four token rows and pairs tokens by byte
-//           permutation; which accumulator row is which value channel is settled when they are written out. P^T comes from S^T by movmatrix.
+//           an unsigned lower byte.
+//   output  O^T[D, 8 rows] = V^T[D, 16] P^T in f16 (m16n8k16): ldmatrix transposes pairs of channels; the two bytes of a pair are parted into an upper
+//           and a lower accumulator row. P^T comes from S^T by movmatrix.
 // The 8 query rows of a tile are the query heads that share the key / value head, times the new tokens; two tiles side by side above 8.
-// Probabilities are rounded to f16 (11 bits; codes are exact in it). The page's value scale goes into their exponent, with a running maximum of its own (m2, of
-// s_j + log2 vs): the largest contribution to the output is near 1 whatever the scales are. The maxima are raised only where a score passes one by more than 2^8.
-// 64 sequences of 4096 to 8192 tokens, 32 heads of 128 over 8: registers straight from memory, one page at a time, scores in f16 178 us; through the ring 174.
+// Probabilities are rounded to f16 (11 bits; codes are exact in it). The page's value scale goes into what a probability weighs, relative to a running maximum of its
+// own (m2, of s_j + log2 vs): the largest contribution to the output is near 1 whatever the scales are. The maxima are raised only where a score passes one by far.
 #include <cuda_bf16.h>
 
 #include "../common/kv8.cuh"
@@ -44,7 +42,8 @@ struct AttnKv8Params {
 constexpr int kKv8Warps = 4;         // three CTAs of four warps to an SM: four pages a warp fill shared memory
 constexpr int kKv8Threads = 32 * kKv8Warps;
 constexpr int kKv8Cluster = 8;      // splits that meet in a cluster
-constexpr float kKv8Slack = 8.f;    // log2 units by which a score may pass the maximum in use
+// log2 units by which a score may pass the maximum in use, and a probability's weight the probability: what they give together, 2^14, f16 holds.
+constexpr float kKv8Slack = 6.f, kKv8Weight = 8.f;
 constexpr float kLowest = -3.402823466e38f;
 // Integer sums start at the bits of 1.5 * 2^23: as floats they are that plus the sum, which stays below 2^22 (128 * 127 * 255).
 constexpr int kMagicBits = 0x4b400000;
@@ -55,16 +54,21 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Codes times the upper (signed) and the lower (unsigned) byte of queries.
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// Codes times the upper (signed) and the lower (unsigned) byte of queries. d = a b + c.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
-__device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
@@ -155,8 +159,12 @@ __device__ __forceinline__ float kv8_finish(float o, const Kv8Row& r, const floa
 }
 
 __device__ __forceinline__ float exp2_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }   // -126 <= e <= 127
-// The exchange of 16-byte pieces in row r of a page of 128-byte rows.
-__device__ __forceinline__ int swap128(int r) { return (r & 6) ^ (r & 1) << 2; }
+// Where 16-byte piece c of token row r lies in a page's half of a ring slot: pieces change places within 128 bytes, so that the eight rows of an 8 x 8 matrix
+// that ldmatrix reads meet all banks.
+template <int D>
+__device__ __forceinline__ int kv8_piece(int r, int c) {
+  return D == 128 ? r * 128 + (c ^ (r & 7)) * 16 : (r >> 1) * 128 + (((r & 1) << 2 | c) ^ (r >> 1 & 3)) * 16;
+}
 // Eight values of a query row times two powers of two, rounded to 16 bits: their upper bytes and their lower bytes.
 __device__ __forceinline__ uint4 query_bytes(const float (&x)[8], float up, float more) {
   uint32_t w[8];
@@ -171,7 +179,7 @@ __device__ __forceinline__ uint4 query_bytes(const float (&x)[8], float up, floa
 // that others have a part of as well goes to memory, and attn_kv8_combine_kernel adds it up.
 template <int D, int NT, bool EVEN>
 __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params p) {
-  constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16, VW = D / 32;   // KC: 16-byte pieces of a token row per lane; VW: value words per token and lane
+  constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16;
   constexpr int PAGE_BYTES = 2 * kKv8Page * D;
   extern __shared__ __align__(16) uint8_t smem[];
   // queries as bytes [NT][2 KC][32 lanes], then the rings [warps][2 pairs][2 pages]; behind the last page, what the warps have gathered takes their place
@@ -242,14 +250,13 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     ks_before = ks;
     ev_before = ev;
     ks = p.k_scales[cell];
-    ev = log2f(p.v_scales[cell]);
+    ev = p.v_scales[cell];
   };
-  // A page comes in as it lies in memory, 512 bytes at a time; 16-byte pieces change places within 128 bytes so that eight lanes that read side by
-  // side, two token rows for scores and four for the output, meet all banks.
+  // A page comes in as it lies in memory, 512 bytes at a time. ldmatrix: lane i names row i & 7 of matrix i >> 3; the four are tokens 0 to 7 and 8 to 15 of one
+  // piece, then of the next.
   const uint8_t* mine = rings + warp * (4 * PAGE_BYTES);
-  const int k_at = D == 128 ? g * 128 + (t ^ swap128(g)) * 16 : (g >> 1) * 128 + (((g & 1) << 2 | t) ^ (g & 6)) * 16;
-  const int v_at = D == 128 ? 2 * t * 128 + (g ^ swap128(2 * t)) * 16 : t * 128 + ((g >> 1) ^ 2 * t) * 16 + (g & 1) * 8;
-  const int in_at = D == 128 ? (lane >> 3) * 128 + ((lane & 7) ^ swap128(lane >> 3)) * 16 : (lane >> 3) * 128 + ((lane & 7) ^ 2 * (lane >> 3)) * 16;
+  const int in_at = kv8_piece<D>(lane / (D / 16), lane % (D / 16));
+  const int out_at = kv8_piece<D>(lane & 15, lane >> 4);
   const uint32_t ring = smem_u32(mine);
   auto fetch = [&](int turn) {
     if ((turn & 15) == 0) look_up(turn);
@@ -260,7 +267,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       const uint32_t to = ring + ((turn & 1) * 2 + u) * PAGE_BYTES;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        const int at = i * 512 + (D == 128 && (i & 1) ? in_at ^ 64 : in_at);
+        const int at = i * 512 + (D == 128 && (i & 1) ? in_at ^ 64 : in_at);   // rows 4 i and on, of which every second four have bit 2
         copy16(to + at, p.k_codes + cell + i * 512);
         copy16(to + PAGE_BYTES / 2 + at, p.v_codes + cell + i * 512);
       }
@@ -275,21 +282,22 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   for (int nt = warp; nt < NT; nt += kKv8Warps) {
     const int r = r0 + nt * 8 + g;
     const bool in = nt * 8 + g < rows;
-    const size_t at = (static_cast<size_t>(b * p.q_per_seq + (in ? r / group : 0)) * p.n_q + kvh * group + (in ? r % group : 0)) * D + 16 * t;
-    float x[2 * KC][8];
+    const size_t at = (static_cast<size_t>(b * p.q_per_seq + (in ? r / group : 0)) * p.n_q + kvh * group + (in ? r % group : 0)) * D + 4 * t;
+    float x[2 * KC][8];                           // channels 32 j + 4 t and three more, and 16 further on
     float top = 0.f;
     bool fine = true;
 #pragma unroll
     for (int j = 0; j < 2 * KC; ++j) {
-      const size_t from = at + 64 * (j >> 1) + 8 * (j & 1);
-      if (p.q32 != nullptr) {
-        const float4 u = *reinterpret_cast<const float4*>(p.q32 + from), w = *reinterpret_cast<const float4*>(p.q32 + from + 4);
-        x[j][0] = u.x; x[j][1] = u.y; x[j][2] = u.z; x[j][3] = u.w;
-        x[j][4] = w.x; x[j][5] = w.y; x[j][6] = w.z; x[j][7] = w.w;
-      } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p.q + from);
-        x[j][0] = bf16_lo(u.x); x[j][1] = bf16_hi(u.x); x[j][2] = bf16_lo(u.y); x[j][3] = bf16_hi(u.y);
-        x[j][4] = bf16_lo(u.z); x[j][5] = bf16_hi(u.z); x[j][6] = bf16_lo(u.w); x[j][7] = bf16_hi(u.w);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const size_t from = at + 32 * j + 16 * h;
+        if (p.q32 != nullptr) {
+          const float4 u = *reinterpret_cast<const float4*>(p.q32 + from);
+          x[j][4 * h] = u.x; x[j][4 * h + 1] = u.y; x[j][4 * h + 2] = u.z; x[j][4 * h + 3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(p.q + from);
+          x[j][4 * h] = bf16_lo(u.x); x[j][4 * h + 1] = bf16_hi(u.x); x[j][4 * h + 2] = bf16_lo(u.y); x[j][4 * h + 3] = bf16_hi(u.y);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -328,51 +336,44 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const int tok = (page0 + 2 * (warp + kKv8Warps * turn)) * kKv8Page;
     cp_async_wait<1>();
     __syncwarp();
-    const uint8_t* from = mine + (turn & 1) * 2 * PAGE_BYTES;
+    const uint32_t from = ring + (turn & 1) * 2 * PAGE_BYTES;
     // scales of this turn: its 16 may have been followed by the next ones already
     const bool before = (turn >> 4) != (min(turn + 1, turns - 1) >> 4);
     float s[2][NT][4], ev_now[2];
     {
       int hi[2][NT][4], lo[2][NT][4];
+      const int magic[4] = {kMagicBits, kMagicBits, kMagicBits, kMagicBits};
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int j = 0; j < 2 * KC; ++j) {          // 32 channels at a time
+        uint32_t a[2][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < 2; ++u) ldsm_x4(from + u * PAGE_BYTES + (out_at ^ (32 * j)), a[u][0], a[u][1], a[u][2], a[u][3]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) hi[u][nt][c] = lo[u][nt][c] = kMagicBits;
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 q = q_s[(nt * 2 * KC + j) * 32 + lane];
 #pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        uint4 a[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          a[u][0] = *reinterpret_cast<const uint4*>(from + u * PAGE_BYTES + (k_at ^ (64 * j)));
-          a[u][1] = *reinterpret_cast<const uint4*>(from + u * PAGE_BYTES + 8 * D + (k_at ^ (64 * j)));
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 q = q_s[(nt * 2 * KC + 2 * j + h) * 32 + lane];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint32_t a0 = h == 0 ? a[u][0].x : a[u][0].z, a1 = h == 0 ? a[u][1].x : a[u][1].z;
-              const uint32_t a2 = h == 0 ? a[u][0].y : a[u][0].w, a3 = h == 0 ? a[u][1].y : a[u][1].w;
-              mma_s8(hi[u][nt], a0, a1, a2, a3, q.x, q.y);
-              mma_u8(lo[u][nt], a0, a1, a2, a3, q.z, q.w);
+          for (int u = 0; u < 2; ++u) {
+            if (j == 0) {
+              mma_s8(hi[u][nt], a[u], q.x, q.y, magic);
+              mma_u8(lo[u][nt], a[u], q.z, q.w, magic);
+            } else {
+              mma_s8(hi[u][nt], a[u], q.x, q.y, hi[u][nt]);
+              mma_u8(lo[u][nt], a[u], q.z, q.w, lo[u][nt]);
             }
           }
+        }
       }
       // ---- scores in log2 units
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int at = 2 * (turn & 15) + u;
         const float ks_now = __shfl_sync(0xffffffffu, before ? ks_before : ks, at);
-        ev_now[u] = __shfl_sync(0xffffffffu, before ? ev_before : ev, at);
+        ev_now[u] = lg2_approx(__shfl_sync(0xffffffffu, before ? ev_before : ev, at));   // (exact for powers of two)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float f0 = back[nt][0] * ks_now, f1 = back[nt][1] * ks_now;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[u][nt][c] = fmaf(__int_as_float(hi[u][nt][c]) - kMagic, 256.f, __int_as_float(lo[u][nt][c]) - kMagic) * (c & 1 ? f1 : f0);
+          for (int c = 0; c < 4; ++c) s[u][nt][c] = (fmaf(__int_as_float(hi[u][nt][c]), 256.f, -257.f * kMagic) + __int_as_float(lo[u][nt][c])) * (c & 1 ? f1 : f0);
         }
       }
     }
@@ -388,15 +389,26 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
             if (key > min(at, last_key) || key < kv8_lowest_key(p, at)) s[u][nt][c] = -INFINITY;
           }
     }
-    bool passes = false;
+    // ---- d: score against the maximum in use. f: what a probability weighs in the output, against m2
+    float d[2][NT][4], f[2][NT][2];
+    auto relate = [&]() {
+      bool passes = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float t0 = fmaxf(s[0][nt][c], s[0][nt][c + 2]), t1 = fmaxf(s[1][nt][c], s[1][nt][c + 2]);
-        passes |= fmaxf(t0, t1) > m[nt][c] + kKv8Slack || fmaxf(t0 + ev_now[0], t1 + ev_now[1]) > m2[nt][c] + kKv8Slack;
-      }
-    if (__any_sync(0xffffffffu, passes)) {
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            d[u][nt][c] = s[u][nt][c] - m[nt][c];
+            d[u][nt][c + 2] = s[u][nt][c + 2] - m[nt][c];
+            f[u][nt][c] = ev_now[u] + (m[nt][c] - m2[nt][c]);
+          }
+          passes |= fmaxf(fmaxf(d[0][nt][c], d[0][nt][c + 2]), fmaxf(d[1][nt][c], d[1][nt][c + 2])) > kKv8Slack ||
+                    fmaxf(f[0][nt][c], f[1][nt][c]) > kKv8Weight;
+        }
+      return passes;
+    };
+    if (__any_sync(0xffffffffu, relate())) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float down[2];
@@ -422,6 +434,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
           o[nt][i][3] *= down[1];
         }
       }
+      relate();
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -429,11 +442,11 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
-        // from a probability to what it weighs in the output. (Value scales that are further apart than this has room for, over 2^126, lose the smaller ones.)
-        const float f0 = ex2_approx(fminf(ev_now[u] + m[nt][0] - m2[nt][0], 126.f)), f1 = ex2_approx(fminf(ev_now[u] + m[nt][1] - m2[nt][1], 126.f));
+        // (value scales that are further apart than this has room for, over 2^126, lose the smaller ones)
+        const float f0 = ex2_approx(fminf(f[u][nt][0], 126.f)), f1 = ex2_approx(fminf(f[u][nt][1], 126.f));
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float e = ex2_approx(s[u][nt][c] - m[nt][c & 1]);
+          const float e = ex2_approx(d[u][nt][c]);
           l[nt][c & 1] += e;
           w[c] = e * (c & 1 ? f1 : f0);
         }
@@ -445,28 +458,21 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
         pf[nt][1] = transposed(pack_f16x2(w[2], w[3]));
       }
       // ---- output
-      uint32_t vr[4][VW];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* row = from + u * PAGE_BYTES + PAGE_BYTES / 2 + (i >> 1) * 8 * D + (i & 1 ? (v_at ^ 64) + (D == 128 ? 128 : 0) : v_at);
-        if (VW == 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(row);
-          vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(row);
-          vr[i][0] = x.x; vr[i][1] = x.y;
+      for (int j = 0; j < D / 32; ++j) {
+        // channels 2g and 2g + 1 of a piece, tokens 2t, 2t + 1 and 8 more: bytes {2t: a, b; 2t + 1: a, b}
+        uint32_t v[4];
+        ldsm_x4_t(from + u * PAGE_BYTES + PAGE_BYTES / 2 + (out_at ^ (32 * j)), v[0], v[1], v[2], v[3]);
+        uint32_t a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          a[i] = kv8_parted<false>(v[i]);
+          b[i] = kv8_parted<true>(v[i]);
         }
-      }
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t a = vr[0][w] ^ 0x80808080u, bb = vr[1][w] ^ 0x80808080u, c = vr[2][w] ^ 0x80808080u, d = vr[3][w] ^ 0x80808080u;
-        const uint32_t x0 = __byte_perm(a, bb, 0x5140), x1 = __byte_perm(a, bb, 0x7362), y0 = __byte_perm(c, d, 0x5140), y1 = __byte_perm(c, d, 0x7362);
-        const uint32_t e0 = kv8_halves<0x4140>(x0), e1 = kv8_halves<0x4342>(x0), e2 = kv8_halves<0x4140>(y0), e3 = kv8_halves<0x4342>(y0);
-        const uint32_t f0 = kv8_halves<0x4140>(x1), f1 = kv8_halves<0x4342>(x1), f2 = kv8_halves<0x4140>(y1), f3 = kv8_halves<0x4342>(y1);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_f16(o[nt][2 * w], e0, e1, e2, e3, pf[nt][0], pf[nt][1]);
-          mma_f16(o[nt][2 * w + 1], f0, f1, f2, f3, pf[nt][0], pf[nt][1]);
+          mma_f16(o[nt][2 * j], a[0], b[0], a[1], b[1], pf[nt][0], pf[nt][1]);
+          mma_f16(o[nt][2 * j + 1], a[2], b[2], a[3], b[3], pf[nt][0], pf[nt][1]);
         }
       }
     }
@@ -487,9 +493,9 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       const int row = nt * 8 + 2 * t + c;
       if (g == 0) row_warp[warp * ROWS + row] = Kv8Row{m[nt][c], sum, m2[nt][c]};
-      float2* dst = reinterpret_cast<float2*>(o_warp + (warp * ROWS + row) * D + g * (D / 8));
+      float2* dst = reinterpret_cast<float2*>(o_warp + (warp * ROWS + row) * D + 2 * g);
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) dst[i] = make_float2(o[nt][i][c], o[nt][i][c + 2]);
+      for (int i = 0; i < STEPS; ++i) dst[8 * i] = make_float2(o[nt][i][c], o[nt][i][c + 2]);
     }
   __syncthreads();
   if (threadIdx.x < ROWS) {
