@@ -1,0 +1,119 @@
+// Rows of keys and values into blocks of 8 bits (kv8.cuh), rotated and normalised on the way.
+#pragma once
+#include "kv8.cuh"
+#include "ptx.cuh"
+
+namespace eredu {
+
+struct Kv8StoreParams {
+  const __nv_bfloat16 *q, *k, *v;   // [M, heads, D], rows of ld_q, ld_k, ld_v elements
+  __nv_bfloat16* q_out;             // [M, n_q, D]
+  int8_t *k_codes, *v_codes;        // [pages, n_kv, 16, D]
+  float *k_scales, *v_scales;       // [pages, n_kv]
+  const int* positions;             // [M]
+  const long long* slots;           // [M] page * 16 + offset, < 0: not stored
+  const float* inv_freq;            // [rot / 2]
+  const float *q_norm_w, *k_norm_w; // optional [D]
+  int M, ld_q, ld_k, ld_v, n_q, n_kv, rot, interleaved, tile, num_pages;
+  float attn_factor, norm_eps, norm_w_off;
+  int* status;
+};
+
+// Angle of a position: the product in two parts, so that far positions keep their digits.
+__device__ __forceinline__ float2 turn_of(int pos, float freq, float factor) {
+  const float p = static_cast<float>(pos);
+  const float a = p * freq, rest = fmaf(p, freq, -a);
+  float s, c;
+  sincosf(a, &s, &c);
+  return make_float2((c - s * rest) * factor, (s + c * rest) * factor);
+}
+
+template <int D>
+__device__ __forceinline__ float4 load_row4(const __nv_bfloat16* row, int lane) {
+  const uint2 u = *reinterpret_cast<const uint2*>(row + 4 * (lane & (D / 4 - 1)));
+  return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+}
+// The D / 4 lanes of a row together: norm, then rotation. `turns`: cosine and sine of the row's rot / 2 angles.
+template <int D>
+__device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, const float* w, const float2* turns, int lane) {
+  const int d = 4 * (lane & (D / 4 - 1));
+  if (w != nullptr) {
+    float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
+#pragma unroll
+    for (int o = D / 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss / static_cast<float>(D) + p.norm_eps);
+    x.x *= inv * (w[d] + p.norm_w_off);
+    x.y *= inv * (w[d + 1] + p.norm_w_off);
+    x.z *= inv * (w[d + 2] + p.norm_w_off);
+    x.w *= inv * (w[d + 3] + p.norm_w_off);
+  }
+  if (p.rot == 0) return x;
+  if (p.interleaved) {
+    if (d < p.rot) {
+      const float2 a = turns[d / 2], b = turns[d / 2 + 1];
+      x = make_float4(x.x * a.x - x.y * a.y, x.y * a.x + x.x * a.y, x.z * b.x - x.w * b.y, x.w * b.x + x.z * b.y);
+    }
+    return x;
+  }
+  const int half = p.rot / 2;
+  const int from = d < half ? lane + half / 4 : d < p.rot ? lane - half / 4 : lane;
+  const float4 o = make_float4(__shfl_sync(0xffffffffu, x.x, from), __shfl_sync(0xffffffffu, x.y, from), __shfl_sync(0xffffffffu, x.z, from),
+                               __shfl_sync(0xffffffffu, x.w, from));
+  if (d < p.rot) {
+    const float sign = d < half ? -1.f : 1.f;
+    const float2* t = turns + (d < half ? d : d - half);
+    x = make_float4(x.x * t[0].x + sign * o.x * t[0].y, x.y * t[1].x + sign * o.y * t[1].y, x.z * t[2].x + sign * o.z * t[2].y, x.w * t[3].x + sign * o.w * t[3].y);
+  }
+  return x;
+}
+
+// Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on; the whole warp.
+template <int D, bool KEYS>
+__device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float2* turns, int lane) {
+  constexpr int RPI = 128 / D;              // rows a warp holds at once
+  constexpr int STEPS = kKv8Page / RPI;
+  const __nv_bfloat16* src = KEYS ? p.k : p.v;
+  const int ld = KEYS ? p.ld_k : p.ld_v;
+  int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
+  float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
+  const int sub = RPI == 1 ? 0 : lane >> 4;
+  float4 x[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int r = i * RPI + sub;
+    x[i] = r < n ? load_row4<D>(src + static_cast<size_t>(row + r) * ld + h * D, lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const float before = first > 0 ? *at : 0.f;
+  uint32_t top = 0;   // as bits, so that what is no number wins
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    if (i * RPI >= n) break;
+    if (KEYS) {
+      const float4 y = prepared<D>(p, x[i], p.k_norm_w, turns + min(i * RPI + sub, n - 1) * (p.rot / 2), lane);
+      if (i * RPI + sub < n) x[i] = y;
+    }
+    top = max(max(top, __float_as_uint(fabsf(x[i].x))), __float_as_uint(fabsf(x[i].y)));
+    top = max(max(top, __float_as_uint(fabsf(x[i].z))), __float_as_uint(fabsf(x[i].w)));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  float scale = kv8_needed(__uint_as_float(top));
+  if (first > 0 && !(before <= scale)) scale = scale != scale ? scale : before;   // the larger, and what is no number stays none
+  const float inv = kv8_inverse(scale);
+  const int c = 4 * (lane & (D / 4 - 1));
+  if (first > 0 && scale != before) {
+    const float ratio = before * inv;
+    for (int r = sub; r < first; r += RPI) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + c);
+      const uint32_t u = *w;
+      *w = kv8_pack(kv8_code(u, 0) * ratio, kv8_code(u, 1) * ratio, kv8_code(u, 2) * ratio, kv8_code(u, 3) * ratio);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int r = i * RPI + sub;
+    if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x[i].x * inv, x[i].y * inv, x[i].z * inv, x[i].w * inv);
+  }
+  if (lane == 0) *at = scale;
+}
+
+}  // namespace eredu

@@ -14,18 +14,20 @@
 // own (m2, of s_j + log2 vs): the largest contribution to the output is near 1 whatever the scales are. The maxima are raised only where a score passes one by far.
 #include <cuda_bf16.h>
 
-#include "../common/kv8.cuh"
+#include "../common/kv8_store.cuh"
 #include "../common/launch.h"
 #include "../common/launch_count.h"
 #include "../common/mma.cuh"
 #include "../common/ptx.cuh"
 #include "../common/trace.cuh"
 
+extern "C" int eredu_kv8_store(const void*, const void*, const void*, void*, void*, void*, float*, float*, const int*, const long long*, const float*, const float*,
+                               const float*, int, int, int, int, int, int, int, int, int, int, float, float, float, int*, cudaStream_t);
+
 namespace eredu {
 
 struct AttnKv8Params {
-  const __nv_bfloat16* q;          // [B * q_per_seq, n_q, D], or
-  const float* q32;                // the same in 32 bits
+  const __nv_bfloat16* q;          // [B * q_per_seq] rows of ld_q elements, n_q heads of D
   const int8_t *k_codes, *v_codes; // [pages, n_kv, 16, D]
   const float *k_scales, *v_scales;
   __nv_bfloat16* out;              // [B * q_per_seq, n_q, D]
@@ -36,9 +38,16 @@ struct AttnKv8Params {
   float* part_ml;                  //              [CTAs, 2, rows of a tile, 4]
   int4* joins;                     //              [CTAs]: what of the CTA's first part is to be added up, see attn_kv8_combine_kernel
   int batch, max_pages, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
+  int ld_q;
   float scale_log2;
   int* status;
+  // A step from the projection's output (st.q = q, st.k, st.v in the same rows): queries are normalised and rotated as they are read and, `append`, the CTA
+  // that has the page of a new token writes its rows there.
+  Kv8StoreParams st;
+  int append;
 };
+constexpr int kKv8StepTokens = 8;   // new tokens that the rows of a tile span in a step
+
 constexpr int kKv8Warps = 4;         // three CTAs of four warps to an SM: four pages a warp fill shared memory
 constexpr int kKv8Threads = 32 * kKv8Warps;
 constexpr int kKv8Cluster = 8;      // splits that meet in a cluster
@@ -165,19 +174,17 @@ template <int D>
 __device__ __forceinline__ int kv8_piece(int r, int c) {
   return D == 128 ? r * 128 + (c ^ (r & 7)) * 16 : (r >> 1) * 128 + (((r & 1) << 2 | c) ^ (r >> 1 & 3)) * 16;
 }
-// Eight values of a query row times two powers of two, rounded to 16 bits: their upper bytes and their lower bytes.
-__device__ __forceinline__ uint4 query_bytes(const float (&x)[8], float up, float more) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = static_cast<uint32_t>(min(__float2int_rn(x[i] * up * more), 32767));
-  auto pick = [&](int i, uint32_t sel) { return __byte_perm(__byte_perm(w[i], w[i + 1], sel), __byte_perm(w[i + 2], w[i + 3], sel), 0x5410); };
-  return make_uint4(pick(0, 0x0051), pick(4, 0x0051), pick(0, 0x0040), pick(4, 0x0040));
+// Four values of a query row times two powers of two, rounded to 16 bits: their upper bytes and their lower bytes.
+__device__ __forceinline__ uint2 query_bytes(float4 x, float up, float more) {
+  auto whole = [&](float v) { return static_cast<uint32_t>(min(__float2int_rn(v * up * more), 32767)); };
+  const uint32_t a = whole(x.x), b = whole(x.y), c = whole(x.z), d = whole(x.w);
+  return make_uint2(__byte_perm(__byte_perm(a, b, 0x0051), __byte_perm(c, d, 0x0051), 0x5410), __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410));
 }
 
 // grid (splits, n_kv * tiles, B): the splits of a sequence and head form a cluster and meet in its shared memory.
 // EVEN: grid (CTAs): even shares of all pairs, so that long and short sequences, and few and many, fill the SMs alike. What a CTA has of a sequence and head
 // that others have a part of as well goes to memory, and attn_kv8_combine_kernel adds it up.
-template <int D, int NT, bool EVEN>
+template <int D, int NT, bool EVEN, bool STEP>
 __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params p) {
   constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16;
   constexpr int PAGE_BYTES = 2 * kKv8Page * D;
@@ -190,6 +197,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   Kv8Row* row_warp = reinterpret_cast<Kv8Row*>(o_s + ROWS * D);   // [warps][ROWS]
   Kv8Row* row_s = row_warp + kKv8Warps * ROWS;           // [ROWS]
   __shared__ float back_s[ROWS];
+  __shared__ float2 turns_s[STEP ? kKv8StepTokens * D / 2 : 1];   // angles of the tile's tokens
   pdl_launch_early();
   trace_mark(kTraceAttnDecode, kTraceStart);
   pdl_wait();
@@ -273,49 +281,75 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       }
     }
   };
-  if (turns > 0) fetch(0);
+  // a pair that new rows are written to is fetched behind the write
+  const int new_page = STEP && p.append ? pos_new / kKv8Page : 0x7fffffff;
+  auto waits = [&](int turn) { return STEP && page0 + 2 * (warp + kKv8Warps * turn) + 1 >= new_page; };
+  if (turns > 0 && !waits(0)) fetch(0);
   cp_async_commit();
-  if (turns > 1) fetch(1);
+  if (turns > 1 && !waits(1)) fetch(1);
   cp_async_commit();
 
-  // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
-  for (int nt = warp; nt < NT; nt += kKv8Warps) {
-    const int r = r0 + nt * 8 + g;
-    const bool in = nt * 8 + g < rows;
-    const size_t at = (static_cast<size_t>(b * p.q_per_seq + (in ? r / group : 0)) * p.n_q + kvh * group + (in ? r % group : 0)) * D + 4 * t;
-    float x[2 * KC][8];                           // channels 32 j + 4 t and three more, and 16 further on
-    float top = 0.f;
-    bool fine = true;
-#pragma unroll
-    for (int j = 0; j < 2 * KC; ++j) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const size_t from = at + 32 * j + 16 * h;
-        if (p.q32 != nullptr) {
-          const float4 u = *reinterpret_cast<const float4*>(p.q32 + from);
-          x[j][4 * h] = u.x; x[j][4 * h + 1] = u.y; x[j][4 * h + 2] = u.z; x[j][4 * h + 3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(p.q + from);
-          x[j][4 * h] = bf16_lo(u.x); x[j][4 * h + 1] = bf16_hi(u.x); x[j][4 * h + 2] = bf16_lo(u.y); x[j][4 * h + 3] = bf16_hi(u.y);
+  constexpr int RPI = 128 / D;                          // query rows a warp holds at once, four channels a lane
+  const int token0 = r0 / group, half = STEP ? p.st.rot / 2 : 0;
+  if (STEP) {
+    const int tokens = (r0 + rows - 1) / group - token0 + 1;
+    const int* positions = p.st.positions + static_cast<size_t>(b) * p.q_per_seq + token0;
+    for (int i = threadIdx.x; i < tokens * half; i += kKv8Threads) turns_s[i] = turn_of(positions[i / half], p.st.inv_freq[i % half], p.st.attn_factor);
+    __syncthreads();
+    // ---- the new rows of pages in this part: a warp for the keys or the values of a page (there are two such pages at most)
+    if (p.append) {
+      const int page = max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) + (warp >> 1);
+      if (page < page1) {
+        const int first = max(0, page * kKv8Page - pos_new), end_row = min(p.q_per_seq, (page + 1) * kKv8Page - pos_new), row0 = b * p.q_per_seq;
+        for (int r = first; r < end_row;) {
+          const long long to = p.st.slots[row0 + r];
+          int n = 1;
+          if (to >= 0 && (to >> 4) < p.num_pages) {
+            while (r + n < end_row && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
+            const long long cell = (to >> 4) * p.n_kv + kvh;
+            if ((warp & 1) == 0) store_block<D, true>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * half, lane);
+            else store_block<D, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane);
+          } else if (to >= 0) {
+            report_status(p.status, kStatusBadArgument);
+          }
+          r += n;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (!in) x[j][i] = 0.f;
-        top = fmaxf(top, fabsf(x[j][i]));
-        fine = fine && fabsf(x[j][i]) < INFINITY;
-      }
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t four = __ballot_sync(0xffffffffu, fine) >> (4 * g) & 15u;
-    const int e = static_cast<int>(__float_as_uint(top) >> 23);                  // 2^(e - 127) <= top
-    const int up = four != 15u || e == 0 ? 0 : 141 - e, half = up / 2;           // 2^up brings the largest to 2^14
+  }
+  // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
+  for (int i = warp * RPI; i < ROWS; i += kKv8Warps * RPI) {
+    const int row = i + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
+    const bool in = row < rows;
+    const int r = r0 + (in ? row : 0);
+    float4 x = load_row4<D>(p.q + static_cast<size_t>(b * p.q_per_seq + r / group) * p.ld_q + (kvh * group + r % group) * D, lane);
+    if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (r / group - token0) * half, lane);
+    if (!in) x = make_float4(0.f, 0.f, 0.f, 0.f);
+    uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))), max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
 #pragma unroll
-    for (int j = 0; j < 2 * KC; ++j) q_s[(nt * 2 * KC + j) * 32 + lane] = query_bytes(x[j], exp2_of(half), exp2_of(up - half));
-    if (t == 0) back_s[nt * 8 + g] = four == 15u ? p.scale_log2 * exp2_of(-half) * exp2_of(half - up) : __uint_as_float(0x7fc00000u);
+    for (int o = D / 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool fine = top < 0x7f800000u;
+    const int e = static_cast<int>(top >> 23), up = !fine || e == 0 ? 0 : 141 - e, up0 = up / 2;   // 2^(e - 127) <= top; 2^up brings it to 2^14
+    const uint2 bytes = query_bytes(x, exp2_of(up0), exp2_of(up - up0));
+    // the B fragments of lane 4 g + t: channels 32 j + 4 t and 32 j + 16 + 4 t of row g, upper bytes of either, then lower bytes
+    uint32_t* to = reinterpret_cast<uint32_t*>(q_s + ((row >> 3) * 2 * KC + (c >> 3)) * 32 + (row & 7) * 4 + (c & 3)) + (c >> 2 & 1);
+    to[0] = bytes.x;
+    to[2] = bytes.y;
+    if (c == 0) back_s[row] = fine ? p.scale_log2 * exp2_of(-up0) * exp2_of(up0 - up) : __uint_as_float(0x7fc00000u);
   }
   __syncthreads();
+  if (STEP && p.append) {
+    const bool first = turns > 0 && waits(0), second = turns > 1 && waits(1);
+    const int pg = page0 + 2 * (warp + kKv8Warps * (lane >> 1)) + (lane & 1);
+    if (turns > 0 && !first && pg >= new_page && pg < page1) {   // looked up in front of the write
+      ks = p.k_scales[static_cast<size_t>(ids) * p.n_kv + kvh];
+      ev = p.v_scales[static_cast<size_t>(ids) * p.n_kv + kvh];
+    }
+    if (first) fetch(0);
+    if (second) fetch(1);
+    cp_async_commit();
+    if (first || second) cp_async_wait<0>();   // (its places in the order of copies are taken)
+  }
   float back[NT][2];                                    // of the lane's columns 2t, 2t + 1
   int pos[NT][2];
   float o[NT][STEPS][4], m[NT][2], m2[NT][2], l[NT][2];
@@ -639,7 +673,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(At
       __float2bfloat16(kv8_finish(all, r, p.sinks == nullptr ? nullptr : p.sinks + head));
 }
 
-template <int D, int NT, bool EVEN>
+template <int D, int NT, bool EVEN, bool STEP>
 static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int ctas, cudaStream_t stream) {
   constexpr int ROWS = 8 * NT;
   constexpr size_t rings = static_cast<size_t>(kKv8Warps) * 4 * 2 * kKv8Page * D;
@@ -650,7 +684,7 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int ctas, cudaStream_
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<D, NT, EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<D, NT, EVEN, STEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
@@ -674,7 +708,7 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int ctas, cudaStream_
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv8_kernel<D, NT, EVEN>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv8_kernel<D, NT, EVEN, STEP>, p);
   eredu_count_launches(1);
   if (EVEN && e == cudaSuccess) {
     e = launch_pdl(attn_kv8_combine_kernel<D, NT>, dim3(ctas, p.tiles == 1 ? p.q_per_seq * (p.n_q / p.n_kv) : ROWS), dim3(32 * kCombineWarps), 0, stream, p);
@@ -692,18 +726,35 @@ EREDU_TRACE_INSTALLER(attention_kv8)
 // Query rows of one key / value head that a CTA takes at once; beyond 16, a tile more of them reads the pages again.
 static int kv8_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
 
-// splits 1 to 8: CTAs of a sequence and head. 0: even shares for `ctas` CTAs, with scratch for 2 * ctas tiles of 8 rows (16 where a head has more than 8).
-extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
-                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
-                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int D, int splits, int ctas, int window, int chunk,
-                                     float scale, int* status, cudaStream_t stream) {
-  if (batch <= 0) return 0;
-  if ((D != 64 && D != 128) || n_kv <= 0 || n_q % n_kv != 0 || n_q <= 0 || q_per_seq <= 0 || splits < 0 || splits > kKv8Cluster || max_pages <= 0 ||
-      num_pages <= 0 || window < 0 || chunk < 0)
+static int attn_kv8(AttnKv8Params& p, int D, int ctas, bool step, cudaStream_t stream) {
+  if (p.batch <= 0) return 0;
+  if ((D != 64 && D != 128) || p.n_kv <= 0 || p.n_q % p.n_kv != 0 || p.n_q <= 0 || p.q_per_seq <= 0 || p.splits < 0 || p.splits > kKv8Cluster ||
+      p.max_pages <= 0 || p.num_pages <= 0 || p.window < 0 || p.chunk < 0 || p.ld_q % 4 != 0)
     return -2;
+  const int rows = p.q_per_seq * (p.n_q / p.n_kv), tile = kv8_tile_rows(rows);
+  p.tiles = (rows + tile - 1) / tile;
+  const long long line = static_cast<long long>(p.batch) * p.n_kv * p.tiles * (p.max_pages / 2 + 1);
+  if (p.splits == 0 ? ctas <= 0 || p.part_o == nullptr || p.part_ml == nullptr || p.joins == nullptr || line > (1LL << 30)
+                    : p.batch > 65535 || static_cast<long long>(p.n_kv) * p.tiles > 65535)
+    return -2;
+  cudaError_t e;
+#define ER_KV8(D_, NT_)                                                                                                                            \
+  e = step ? (p.splits == 0 ? launch_attn_kv8<D_, NT_, true, true>(p, ctas, stream) : launch_attn_kv8<D_, NT_, false, true>(p, ctas, stream))      \
+           : (p.splits == 0 ? launch_attn_kv8<D_, NT_, true, false>(p, ctas, stream) : launch_attn_kv8<D_, NT_, false, false>(p, ctas, stream))
+  if (D == 128 && tile == 8) ER_KV8(128, 1);
+  else if (D == 128) ER_KV8(128, 2);
+  else if (tile == 8) ER_KV8(64, 1);
+  else ER_KV8(64, 2);
+#undef ER_KV8
+  return static_cast<int>(e);
+}
+
+static AttnKv8Params attn_kv8_params(const void* q, int ld_q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
+                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
+                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int splits, int window, int chunk, float scale, int* status) {
   AttnKv8Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q32 = nullptr;
+  p.ld_q = ld_q;
   p.k_codes = static_cast<const int8_t*>(k_codes);
   p.v_codes = static_cast<const int8_t*>(v_codes);
   p.k_scales = k_scales;
@@ -721,21 +772,60 @@ extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const v
   p.n_q = n_q;
   p.n_kv = n_kv;
   p.q_per_seq = q_per_seq;
-  const int rows = q_per_seq * (n_q / n_kv), tile = kv8_tile_rows(rows);
-  p.tiles = (rows + tile - 1) / tile;
   p.splits = splits;
   p.window = window;
   p.chunk = chunk;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status;
-  const long long line = static_cast<long long>(batch) * n_kv * p.tiles * (max_pages / 2 + 1);
-  if (splits == 0 ? ctas <= 0 || part_o == nullptr || part_ml == nullptr || joins == nullptr || line > (1LL << 30) : batch > 65535 || static_cast<long long>(n_kv) * p.tiles > 65535) return -2;
-  cudaError_t e;
-#define ER_KV8(D_, NT_) e = splits == 0 ? launch_attn_kv8<D_, NT_, true>(p, ctas, stream) : launch_attn_kv8<D_, NT_, false>(p, ctas, stream)
-  if (D == 128 && tile == 8) ER_KV8(128, 1);
-  else if (D == 128) ER_KV8(128, 2);
-  else if (tile == 8) ER_KV8(64, 1);
-  else ER_KV8(64, 2);
-#undef ER_KV8
-  return static_cast<int>(e);
+  return p;
+}
+
+// splits 1 to 8: CTAs of a sequence and head. 0: even shares for `ctas` CTAs, with scratch for 2 * ctas tiles of 8 rows (16 where a head has more than 8).
+extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
+                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
+                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int D, int splits, int ctas, int window, int chunk,
+                                     float scale, int* status, cudaStream_t stream) {
+  AttnKv8Params p = attn_kv8_params(q, n_q * D, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
+                                    max_pages, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
+  return attn_kv8(p, D, ctas, false, stream);
+}
+
+// The same from the projection's output qkv, rows [q heads | k heads | v heads] x D of ld elements. The attention kernel writes the new rows itself where
+// one tile holds all query rows of a head, so that one CTA has a page; else eredu_kv8_store goes in front.
+extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, void* k_codes, void* v_codes, float* k_scales, float* v_scales, void* out, const int* block_table,
+                                   const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, const int* positions,
+                                   const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int batch, int q_per_seq,
+                                   int max_pages, int num_pages, int n_q, int n_kv, int D, int rot, int interleaved, int splits, int ctas, int window, int chunk,
+                                   float scale, float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
+  if (batch <= 0) return 0;
+  if (n_kv <= 0 || n_q <= 0 || n_q % n_kv != 0 || q_per_seq <= 0 || rot < 0 || rot > D || rot % 8 != 0) return -2;
+  const int group = n_q / n_kv, rows = q_per_seq * group;
+  if (group == 1 && rows > kKv8StepTokens) return -2;
+  AttnKv8Params p = attn_kv8_params(qkv, ld, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
+                                    max_pages, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
+  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(qkv);
+  p.append = rows <= 16;
+  p.st.k = row + n_q * D;
+  p.st.v = row + (n_q + n_kv) * D;
+  p.st.ld_k = p.st.ld_v = ld;
+  p.st.k_codes = static_cast<int8_t*>(k_codes);
+  p.st.v_codes = static_cast<int8_t*>(v_codes);
+  p.st.k_scales = k_scales;
+  p.st.v_scales = v_scales;
+  p.st.positions = positions;
+  p.st.slots = slots;
+  p.st.inv_freq = inv_freq;
+  p.st.q_norm_w = q_norm_w;
+  p.st.k_norm_w = k_norm_w;
+  p.st.rot = rot;
+  p.st.interleaved = interleaved;
+  p.st.attn_factor = attn_factor;
+  p.st.norm_eps = norm_eps;
+  p.st.norm_w_off = norm_w_off;
+  if (!p.append) {
+    const int e = eredu_kv8_store(nullptr, p.st.k, p.st.v, nullptr, k_codes, v_codes, k_scales, v_scales, positions, slots, inv_freq, nullptr, k_norm_w,
+                                  batch * q_per_seq, 0, ld, ld, n_q, n_kv, D, rot, interleaved, num_pages, attn_factor, norm_eps, norm_w_off, status, stream);
+    if (e != 0) return e;
+  }
+  return attn_kv8(p, D, ctas, true, stream);
 }

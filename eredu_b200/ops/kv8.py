@@ -40,6 +40,7 @@ P, I, F = native.P, native.I, native.F
 native.register("eredu_kv8_store", I, [P] * 13 + [I] * 10 + [F] * 3 + [P] * 2)
 native.register("eredu_kv8_values", I, [P] * 10 + [I] * 8 + [P] * 2)
 native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 11 + [F] + [P] * 2)
+native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 16 + [I] * 13 + [F] * 4 + [P] * 2)
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 
@@ -152,14 +153,12 @@ def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
            (0, k.stride(0), v.stride(0)))
 
 
-def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
-             norm_eps, norm_w_off, q_out):
-    """The form of :func:`.core.rope_kv` for 8-bit pages on a GPU. Norm and rotation run in 32 bits throughout; a key is rounded once, to its code."""
+def _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, q_norm_w, k_norm_w):
     check_pages8(k_cache, v_cache, n_kv, head_dim)
-    dev, M = k_cache.device, qkv.shape[0]
-    if qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.stride(0) % 4 or qkv.data_ptr() % 8 \
-            or qkv.shape[1] < (n_q + 2 * n_kv) * head_dim or n_q % n_kv:
-        raise ValueError(f"qkv: bf16 rows of {n_q} + 2 * {n_kv} heads of {head_dim}, 8-byte aligned, on {dev} are expected")
+    dev = k_cache.codes.device
+    if qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 or qkv.shape[0] != M or qkv.stride(1) != 1 or qkv.stride(0) % 4 \
+            or qkv.data_ptr() % 8 or qkv.shape[1] < (n_q + 2 * n_kv) * head_dim or n_q % n_kv:
+        raise ValueError(f"qkv: {M} bf16 rows of {n_q} + 2 * {n_kv} heads of {head_dim}, 8-byte aligned, on {dev} are expected")
     if rot % 8 or rot > head_dim or inv_freq.numel() != rot // 2:
         raise ValueError(f"{rot} rotated dims with {inv_freq.numel()} frequencies: a multiple of 8 up to the head size, and half as many frequencies")
     if positions.shape != (M,) or slots.shape != (M,):
@@ -169,6 +168,13 @@ def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, 
     for w in (q_norm_w, k_norm_w):
         if w is not None and w.numel() != head_dim:
             raise ValueError(f"a norm has {w.numel()} weights for heads of {head_dim}")
+
+
+def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
+             norm_eps, norm_w_off, q_out):
+    """The form of :func:`.core.rope_kv` for 8-bit pages on a GPU. Norm and rotation run in 32 bits throughout; a key is rounded once, to its code."""
+    dev, M = k_cache.codes.device, qkv.shape[0]
+    _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, q_norm_w, k_norm_w)
     if q_out is None:
         q_out = torch.empty((M, n_q, head_dim), dtype=qkv.dtype, device=dev)
     else:
@@ -201,25 +207,38 @@ def page_values(k_cache: Pages8, v_cache: Pages8, pages):
     return out[0], out[1]
 
 
-def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q=None):
-    n_q, dim = q.shape[1:]
-    check_pages8(k_cache, v_cache, k_cache.shape[1], dim)
-    if n_q % k_cache.shape[1]:
-        raise ValueError(f"{n_q} query heads do not share {k_cache.shape[1]} key / value heads evenly")
-    dev = k_cache.device
-    if q.dtype != torch.bfloat16:
-        raise ValueError(f"queries over 8-bit pages are bf16 on a GPU, not {q.dtype}")
-    _on(dev, q=(q, torch.bfloat16), seq_lens=(seq_lens, torch.int32), sinks=(sinks, torch.float32), out=(out, q.dtype))
+def _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev):
+    if n_q % n_kv:
+        raise ValueError(f"{n_q} query heads do not share {n_kv} key / value heads evenly")
+    _on(dev, seq_lens=(seq_lens, torch.int32), sinks=(sinks, torch.float32))
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0] \
             or block_table.device != dev:
         raise ValueError("block_table: int32 rows, one per sequence")
-    _on(dev, cu_q=(cu_q, torch.int32))
-    if cu_q is not None and cu_q.shape[0] != seq_lens.shape[0] + 1:
-        raise ValueError(f"{cu_q.shape[0]} query offsets for {seq_lens.shape[0]} sequences")
     if sinks is not None and sinks.numel() != n_q:
         raise ValueError(f"{sinks.numel()} sinks for {n_q} query heads")
+
+
+def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q=None):
+    n_q, dim = q.shape[1:]
+    n_kv, dev = k_cache.codes.shape[1], k_cache.codes.device
+    check_pages8(k_cache, v_cache, n_kv, dim)
+    _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev)
+    _on(dev, q=(q, torch.bfloat16), out=(out, torch.bfloat16), cu_q=(cu_q, torch.int32))
+    if cu_q is not None and cu_q.shape[0] != seq_lens.shape[0] + 1:
+        raise ValueError(f"{cu_q.shape[0]} query offsets for {seq_lens.shape[0]} sequences")
     if out is not None and out.shape != q.shape:
         raise ValueError(f"out {tuple(out.shape)} for queries {tuple(q.shape)}")
+
+
+def _shares(splits, rows, dim, dev):
+    """(splits, CTAs, scratch, addresses in it) of a decode call."""
+    if 1 <= splits <= CLUSTER:
+        return splits, 0, None, None, None, None
+    ctas = EVEN_CTAS * _sm_count(dev)
+    n = 2 * ctas * (8 if rows <= 8 else 16)
+    part = torch.empty(n * (dim + 4) + 4 * ctas, dtype=torch.float32, device=dev)
+    at = part.data_ptr()
+    return 0, ctas, part, at, at + n * dim * 4, at + n * (dim + 4) * 4
 
 
 def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk):
@@ -234,19 +253,29 @@ def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
         raise ValueError(f"{q.shape[0]} query rows for {B} sequences of {q_per_seq}")
     if out is None:
         out = torch.empty_like(q)
-    part_o = part_ml = joins = None
-    ctas = 0
-    if splits > CLUSTER or splits < 1:
-        splits, ctas = 0, EVEN_CTAS * _sm_count(dev)
-        rows = 2 * ctas * (8 if q_per_seq * (n_q // n_kv) <= 8 else 16)
-        part = torch.empty(rows * (dim + 4) + 4 * ctas, dtype=torch.float32, device=dev)
-        part_o = part.data_ptr()
-        part_ml = part_o + rows * dim * 4
-        joins = part_ml + rows * 16
+    splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
     code = lib().eredu_attn_kv8_decode(q.data_ptr(), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
                                        block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins, B, q_per_seq, block_table.stride(0),
                                        k_cache.codes.shape[0], n_q, n_kv, dim, splits, ctas, int(window), int(chunk), scale, ptr(status_word(dev)), stream_ptr(dev))
     check(code, "eredu_attn_kv8_decode")
+    return out
+
+
+def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, q_per_seq, scale, positions, slots, inv_freq, n_q, n_kv, dim, rot, interleaved,
+                    attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, splits, window, sinks, chunk):
+    """The form of :func:`.core.attention_decode_rope` for 8-bit pages on a GPU: queries keep 16 bits from the rotation to the scores."""
+    dev, B = k_cache.codes.device, seq_lens.shape[0]
+    M = B * q_per_seq
+    _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, dim, rot, q_norm_w, k_norm_w)
+    _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev)
+    out = torch.empty((M, n_q, dim), dtype=torch.bfloat16, device=dev)
+    splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
+    code = lib().eredu_attn_kv8_step(qkv.data_ptr(), qkv.stride(0), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(),
+                                     v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins,
+                                     positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), B, q_per_seq,
+                                     block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window),
+                                     int(chunk), scale, attn_factor, norm_eps, norm_w_off, status_word(dev).data_ptr(), stream_ptr(dev))
+    check(code, "eredu_attn_kv8_step")
     return out
 
 
