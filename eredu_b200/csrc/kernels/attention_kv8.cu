@@ -39,6 +39,7 @@ struct AttnKv8Params {
   int4* joins;                     //              [CTAs]: what of the CTA's first part is to be added up, see attn_kv8_combine_kernel
   int batch, max_pages, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
   int ld_q;
+  uint32_t per_group;              // 2^32 / (n_q / n_kv), rounded up; 0 for a group of one
   float scale_log2;
   int* status;
   // A step from the projection's output (st.q = q, st.k, st.v in the same rows): queries are normalised and rotated as they are read and, `append`, the CTA
@@ -46,6 +47,8 @@ struct AttnKv8Params {
   Kv8StoreParams st;
   int append;
 };
+// Token of query row r among those that share a key / value head (r < 2^16: exact), in place of a division of some thirty instructions.
+__device__ __forceinline__ int kv8_token(const AttnKv8Params& p, int r) { return p.per_group == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.per_group)); }
 constexpr int kKv8StepTokens = 8;   // new tokens that the rows of a tile span in a step
 
 constexpr int kKv8Warps = 4;         // three CTAs of four warps to an SM: four pages a warp fill shared memory
@@ -96,6 +99,11 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ int kv8_lowest_key(const AttnKv8Params& p, int pos) {
   if (p.window > 0) return max(0, pos - p.window + 1);
   return p.chunk > 0 && pos > 0 ? pos - pos % p.chunk : 0;
@@ -106,8 +114,8 @@ struct Kv8Pages {
   int first, end;
 };
 __device__ __forceinline__ Kv8Pages kv8_pages(const AttnKv8Params& p, int kv_len) {
-  const int last = min((kv_len + kKv8Page - 1) / kKv8Page, p.max_pages);
-  return Kv8Pages{min(kv8_lowest_key(p, kv_len - p.q_per_seq) / kKv8Page, last), last};
+  const int last = min((kv_len + kKv8Page - 1) >> 4, p.max_pages);
+  return Kv8Pages{min(kv8_lowest_key(p, kv_len - p.q_per_seq) >> 4, last), last};
 }
 // Even shares: the pairs of pages of all sequences, heads and tiles of rows in one line, of which every CTA takes as many. A sequence has one pair at
 // least, so that somebody writes its rows.
@@ -155,8 +163,11 @@ __device__ __forceinline__ Kv8Place kv8_place(const AttnKv8Params& p, int i, int
 struct Kv8Row {
   float m, l, m2;
 };
-// Output of a row: `o` relative to 2^m2, the sum to 2^m; a sink is a key of zero value. A row that sees nothing is zero.
-__device__ __forceinline__ float kv8_finish(float o, const Kv8Row& r, const float* sink) {
+// What takes a row's output, relative to 2^m2, to the sum of its probabilities: o * over * up. A sink is a key of zero value. A row that sees nothing is zero.
+struct Kv8Finish {
+  float over, up;
+};
+__device__ __forceinline__ Kv8Finish kv8_finish(const Kv8Row& r, const float* sink) {
   float m = r.m, l = r.l;
   if (sink != nullptr) {
     const float s = *sink * 1.4426950408889634f;
@@ -164,7 +175,12 @@ __device__ __forceinline__ float kv8_finish(float o, const Kv8Row& r, const floa
     l = l * ex2_approx(m - top) + ex2_approx(s - top);
     m = top;
   }
-  return l == 0.f || r.l == 0.f ? 0.f : o / l * ex2_approx(r.m2 - m);
+  if (l == 0.f || r.l == 0.f) return Kv8Finish{0.f, 0.f};
+  return Kv8Finish{1.f / l, ex2_approx(r.m2 - m)};
+}
+__device__ __forceinline__ float4 fma4(float4 a, float w, float4 c) { return make_float4(fmaf(a.x, w, c.x), fmaf(a.y, w, c.y), fmaf(a.z, w, c.z), fmaf(a.w, w, c.w)); }
+__device__ __forceinline__ void store_out(__nv_bfloat16* to, float4 v, float up) {
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(v.x * up, v.y * up), pack_bf16x2(v.z * up, v.w * up));
 }
 
 __device__ __forceinline__ float exp2_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }   // -126 <= e <= 127
@@ -186,17 +202,19 @@ __device__ __forceinline__ uint2 query_bytes(float4 x, float up, float more) {
 // that others have a part of as well goes to memory, and attn_kv8_combine_kernel adds it up.
 template <int D, int NT, bool EVEN, bool STEP>
 __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params p) {
-  constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16;
+  constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16, WIDE = D + 4;   // WIDE: lanes of four rows meet all banks
   constexpr int PAGE_BYTES = 2 * kKv8Page * D;
   extern __shared__ __align__(16) uint8_t smem[];
   // queries as bytes [NT][2 KC][32 lanes], then the rings [warps][2 pairs][2 pages]; behind the last page, what the warps have gathered takes their place
   uint4* q_s = reinterpret_cast<uint4*>(smem);
   uint8_t* rings = smem + NT * 2 * KC * 512;
-  float* o_warp = reinterpret_cast<float*>(rings);       // [warps][ROWS][D]
-  float* o_s = o_warp + kKv8Warps * ROWS * D;            // [ROWS][D]
+  float* o_warp = reinterpret_cast<float*>(rings);       // [warps][ROWS][WIDE]
+  float* o_s = o_warp + kKv8Warps * ROWS * WIDE;         // [ROWS][D]
   Kv8Row* row_warp = reinterpret_cast<Kv8Row*>(o_s + ROWS * D);   // [warps][ROWS]
   Kv8Row* row_s = row_warp + kKv8Warps * ROWS;           // [ROWS]
-  __shared__ float back_s[ROWS];
+  float* weight = reinterpret_cast<float*>(row_s + ROWS);         // [warps, or splits][ROWS]
+  __shared__ float back_s[ROWS], up_s[ROWS];
+  __shared__ size_t out_s[ROWS];          // where a row's output goes
   __shared__ float2 turns_s[STEP ? kKv8StepTokens * D / 2 : 1];   // angles of the tile's tokens
   pdl_launch_early();
   trace_mark(kTraceAttnDecode, kTraceStart);
@@ -222,9 +240,9 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   }
   do {
   const int b = EVEN ? place.b : blockIdx.z, head_tile = EVEN ? (at - place.begin) / place.pairs : blockIdx.y, split = EVEN ? 0 : blockIdx.x;
-  const int kvh = head_tile / p.tiles, r0 = head_tile % p.tiles * ROWS, rows = min(ROWS, rows_all - r0);
+  const int kvh = p.tiles == 1 ? head_tile : head_tile / p.tiles, r0 = (head_tile - kvh * p.tiles) * ROWS, rows = min(ROWS, rows_all - r0);
   const int kv_len = p.seq_lens[b], pos_new = kv_len - p.q_per_seq;
-  const int pos_first = pos_new + r0 / group, pos_last = pos_new + (r0 + rows - 1) / group;   // positions of the tile's first and last row
+  const int token0 = kv8_token(p, r0), pos_first = pos_new + token0, pos_last = pos_new + kv8_token(p, r0 + rows - 1);   // positions of the tile's first and last row
   const Kv8Pages pages = kv8_pages(p, kv_len);
   int page0, page1;
   bool whole = p.splits == 1;                                                                 // nobody else has a part of these rows
@@ -235,7 +253,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     page0 = pages.first + 2 * first;
     page1 = min(pages.end, page0 + 2 * n);
   } else {
-    const int per = (pages.end - pages.first + p.splits - 1) / p.splits;
+    const int per = whole ? pages.end - pages.first : (pages.end - pages.first + p.splits - 1) / p.splits;
     page0 = pages.first + split * per;
     page1 = min(pages.end, page0 + per);
   }
@@ -290,11 +308,12 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   cp_async_commit();
 
   constexpr int RPI = 128 / D;                          // query rows a warp holds at once, four channels a lane
-  const int token0 = r0 / group, half = STEP ? p.st.rot / 2 : 0;
+  const int half = STEP ? p.st.rot / 2 : 0;
   if (STEP) {
-    const int tokens = (r0 + rows - 1) / group - token0 + 1;
+    const int tokens = pos_last - pos_first + 1;
     const int* positions = p.st.positions + static_cast<size_t>(b) * p.q_per_seq + token0;
-    for (int i = threadIdx.x; i < tokens * half; i += kKv8Threads) turns_s[i] = turn_of(positions[i / half], p.st.inv_freq[i % half], p.st.attn_factor);
+    for (int n = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); n < tokens; n += kKv8Threads / (D / 2))
+      if (i < half) turns_s[n * half + i] = turn_of(positions[n], p.st.inv_freq[i], p.st.attn_factor);
     __syncthreads();
     // ---- the new rows of pages in this part: a warp for the keys or the values of a page (there are two such pages at most)
     if (p.append) {
@@ -318,12 +337,19 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     }
   }
   // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
-  for (int i = warp * RPI; i < ROWS; i += kKv8Warps * RPI) {
-    const int row = i + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
+  constexpr int QUERIES = ROWS / (kKv8Warps * RPI);     // of a warp, all on their way before the first is looked at
+  float4 query[QUERIES];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int r = r0 + min((i * kKv8Warps + warp) * RPI + lane / (D / 4), rows - 1), token = kv8_token(p, r);
+    query[i] = load_row4<D>(p.q + static_cast<size_t>(b * p.q_per_seq + token) * p.ld_q + (kvh * group + r - token * group) * D, lane);
+  }
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int row = (i * kKv8Warps + warp) * RPI + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
     const bool in = row < rows;
-    const int r = r0 + (in ? row : 0);
-    float4 x = load_row4<D>(p.q + static_cast<size_t>(b * p.q_per_seq + r / group) * p.ld_q + (kvh * group + r % group) * D, lane);
-    if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (r / group - token0) * half, lane);
+    float4 x = query[i];
+    if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (kv8_token(p, r0 + min(row, rows - 1)) - token0) * half, lane);
     if (!in) x = make_float4(0.f, 0.f, 0.f, 0.f);
     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))), max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
 #pragma unroll
@@ -360,7 +386,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       back[nt][c] = back_s[nt * 8 + 2 * t + c];
-      pos[nt][c] = pos_new + (r0 + min(nt * 8 + 2 * t + c, rows - 1)) / group;
+      pos[nt][c] = pos_new + kv8_token(p, r0 + min(nt * 8 + 2 * t + c, rows - 1));
       m[nt][c] = m2[nt][c] = kLowest;
       l[nt][c] = 0.f;
     }
@@ -414,14 +440,16 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const bool edge = tok + 2 * kKv8Page - 1 > mask_hi || tok < mask_lo;
     if (edge) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int c = 0; c < 2; ++c) {
+          const int high = min(pos[nt][c], last_key) - tok - g, low = kv8_lowest_key(p, pos[nt][c]) - tok - g;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int key = tok + u * kKv8Page + g + (c >> 1) * 8, at = pos[nt][c & 1];
-            if (key > min(at, last_key) || key < kv8_lowest_key(p, at)) s[u][nt][c] = -INFINITY;
-          }
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (u * kKv8Page + h * 8 > high || u * kKv8Page + h * 8 < low) s[u][nt][c + 2 * h] = -INFINITY;
+        }
     }
     // ---- d: score against the maximum in use. f: what a probability weighs in the output, against m2
     float d[2][NT][4], f[2][NT][2];
@@ -527,37 +555,40 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       const int row = nt * 8 + 2 * t + c;
       if (g == 0) row_warp[warp * ROWS + row] = Kv8Row{m[nt][c], sum, m2[nt][c]};
-      float2* dst = reinterpret_cast<float2*>(o_warp + (warp * ROWS + row) * D + 2 * g);
+      float2* dst = reinterpret_cast<float2*>(o_warp + (warp * ROWS + row) * WIDE + 2 * g);
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) dst[8 * i] = make_float2(o[nt][i][c], o[nt][i][c + 2]);
     }
   __syncthreads();
   if (threadIdx.x < ROWS) {
+    const int row = threadIdx.x;
     Kv8Row r = {kLowest, 0.f, kLowest};
     for (int w = 0; w < kKv8Warps; ++w) {
-      r.m = fmaxf(r.m, row_warp[w * ROWS + threadIdx.x].m);
-      r.m2 = fmaxf(r.m2, row_warp[w * ROWS + threadIdx.x].m2);
+      r.m = fmaxf(r.m, row_warp[w * ROWS + row].m);
+      r.m2 = fmaxf(r.m2, row_warp[w * ROWS + row].m2);
     }
-    for (int w = 0; w < kKv8Warps; ++w) r.l += row_warp[w * ROWS + threadIdx.x].l * ex2_approx(row_warp[w * ROWS + threadIdx.x].m - r.m);
-    row_s[threadIdx.x] = r;
+    for (int w = 0; w < kKv8Warps; ++w) r.l += row_warp[w * ROWS + row].l * ex2_approx(row_warp[w * ROWS + row].m - r.m);
+    const int n = r0 + min(row, rows - 1), token = kv8_token(p, n), head = kvh * group + n - token * group;
+    out_s[row] = (static_cast<size_t>(b * p.q_per_seq + token) * p.n_q + head) * D;
+    const Kv8Finish f = whole ? kv8_finish(r, p.sinks == nullptr ? nullptr : p.sinks + head) : Kv8Finish{1.f, 1.f};
+    for (int w = 0; w < kKv8Warps; ++w) weight[w * ROWS + row] = ex2_approx(row_warp[w * ROWS + row].m2 - r.m2) * f.over;
+    up_s[row] = f.up;
+    row_s[row] = r;
   }
   __syncthreads();
   const size_t part = (static_cast<size_t>(blockIdx.x) * 2 + slot) * ROWS;
-  for (int i = threadIdx.x; i < rows * D; i += kKv8Threads) {
-    const int row = i / D, d = i % D;
-    const Kv8Row r = row_s[row];
-    float sum = 0.f;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kKv8Threads) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kKv8Warps; ++w) sum += o_warp[(w * ROWS + row) * D + d] * ex2_approx(row_warp[w * ROWS + row].m2 - r.m2);
+    for (int w = 0; w < kKv8Warps; ++w) sum = fma4(*reinterpret_cast<const float4*>(o_warp + (w * ROWS + row) * WIDE + d), weight[w * ROWS + row], sum);
     if (whole) {
-      const int n = r0 + row, head = kvh * group + n % group;
-      p.out[(static_cast<size_t>(b * p.q_per_seq + n / group) * p.n_q + head) * D + d] =
-          __float2bfloat16(kv8_finish(sum, r, p.sinks == nullptr ? nullptr : p.sinks + head));
+      store_out(p.out + out_s[row] + d, sum, up_s[row]);
     } else if (!EVEN) {
-      o_s[i] = sum;
+      *reinterpret_cast<float4*>(o_s + row * D + d) = sum;
     } else {
-      p.part_o[part * D + i] = sum;
-      if (d == 0) *reinterpret_cast<float4*>(p.part_ml + (part + row) * 4) = make_float4(r.m, r.l, r.m2, 0.f);
+      *reinterpret_cast<float4*>(p.part_o + (part + row) * D + d) = sum;
+      if (d == 0) *reinterpret_cast<float4*>(p.part_ml + (part + row) * 4) = make_float4(row_s[row].m, row_s[row].l, row_s[row].m2, 0.f);
     }
   }
   if (EVEN) {
@@ -573,27 +604,50 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   // ---- the splits: every CTA of the cluster finishes some of the values
   cluster_arrive_release();
   cluster_wait_acquire();
-  for (int i = split * kKv8Threads + threadIdx.x; i < rows * D; i += p.splits * kKv8Threads) {
-    const int row = i / D;
+  if (threadIdx.x < ROWS) {
+    const int row = threadIdx.x;
     Kv8Row part_row[kKv8Cluster], r = {kLowest, 0.f, kLowest};
 #pragma unroll
     for (int s = 0; s < kKv8Cluster; ++s) {
       if (s >= p.splits) break;
       const uint32_t at = mapa_shared(smem_u32(row_s + row), s);
       part_row[s] = Kv8Row{ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)};
+    }
+#pragma unroll
+    for (int s = 0; s < kKv8Cluster; ++s) {
+      if (s >= p.splits) break;
       r.m = fmaxf(r.m, part_row[s].m);
       r.m2 = fmaxf(r.m2, part_row[s].m2);
     }
-    float sum = 0.f;
 #pragma unroll
     for (int s = 0; s < kKv8Cluster; ++s) {
       if (s >= p.splits) break;
       r.l += part_row[s].l * ex2_approx(part_row[s].m - r.m);
-      sum += ld_cluster_f32(mapa_shared(smem_u32(o_s + i), s)) * ex2_approx(part_row[s].m2 - r.m2);
     }
-    const int n = r0 + row, head = kvh * group + n % group;
-    p.out[(static_cast<size_t>(b * p.q_per_seq + n / group) * p.n_q + head) * D + i % D] =
-        __float2bfloat16(kv8_finish(sum, r, p.sinks == nullptr ? nullptr : p.sinks + head));
+    const int n = r0 + min(row, rows - 1);
+    const Kv8Finish f = kv8_finish(r, p.sinks == nullptr ? nullptr : p.sinks + kvh * group + n - kv8_token(p, n) * group);
+#pragma unroll
+    for (int s = 0; s < kKv8Cluster; ++s) {
+      if (s >= p.splits) break;
+      weight[s * ROWS + row] = ex2_approx(part_row[s].m2 - r.m2) * f.over;
+    }
+    up_s[row] = f.up;
+  }
+  __syncthreads();
+  for (int i = split * kKv8Threads + threadIdx.x; i < rows * (D / 4); i += p.splits * kKv8Threads) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float4 o4[kKv8Cluster], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < kKv8Cluster; ++s) {
+      if (s >= p.splits) break;
+      o4[s] = ld_cluster_f32x4(mapa_shared(smem_u32(o_s + row * D + d), s));
+    }
+#pragma unroll
+    for (int s = 0; s < kKv8Cluster; ++s) {
+      if (s >= p.splits) break;
+      sum = fma4(o4[s], weight[s * ROWS + row], sum);
+    }
+    store_out(p.out + out_s[row] + d, sum, up_s[row]);
   }
   cluster_arrive_release();   // nobody leaves while its shared memory is read
   cluster_wait_acquire();
@@ -613,7 +667,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(At
   pdl_launch_dependents();
   const int4 join = p.joins[blockIdx.x];
   const int parts = join.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.n_q / p.n_kv;
-  const int kvh = join.z / p.tiles, n = join.z % p.tiles * ROWS + row, c0 = blockIdx.x - 1;
+  const int kvh = p.tiles == 1 ? join.z : join.z / p.tiles, n = (join.z - kvh * p.tiles) * ROWS + row, c0 = blockIdx.x - 1;
   if (parts == 0 || n >= p.q_per_seq * group) return;
   // the first of the CTAs has it as its last part, the others as their first
   auto place_of = [&](int s) { return (static_cast<size_t>(c0 + s) * 2 + (s == 0 && join.w == 0 ? 1 : 0)) * ROWS + row; };
@@ -668,16 +722,16 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(At
     r.l += row_s[w].l * ex2_approx(row_s[w].m - r.m);
     all += sum_s[w][threadIdx.x] * ex2_approx(row_s[w].m2 - r.m2);
   }
-  const int head = kvh * group + n % group;
-  p.out[(static_cast<size_t>(join.y * p.q_per_seq + n / group) * p.n_q + head) * D + threadIdx.x] =
-      __float2bfloat16(kv8_finish(all, r, p.sinks == nullptr ? nullptr : p.sinks + head));
+  const int token = kv8_token(p, n), head = kvh * group + n - token * group;
+  const Kv8Finish f = kv8_finish(r, p.sinks == nullptr ? nullptr : p.sinks + head);
+  p.out[(static_cast<size_t>(join.y * p.q_per_seq + token) * p.n_q + head) * D + threadIdx.x] = __float2bfloat16(all * f.over * f.up);
 }
 
 template <int D, int NT, bool EVEN, bool STEP>
 static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int ctas, cudaStream_t stream) {
   constexpr int ROWS = 8 * NT;
   constexpr size_t rings = static_cast<size_t>(kKv8Warps) * 4 * 2 * kKv8Page * D;
-  constexpr size_t gathered = static_cast<size_t>(kKv8Warps + 1) * ROWS * (D * sizeof(float) + sizeof(Kv8Row));
+  constexpr size_t gathered = static_cast<size_t>(ROWS) * ((kKv8Warps * (D + 4) + D) * sizeof(float) + (kKv8Warps + 1) * sizeof(Kv8Row) + kKv8Cluster * sizeof(float));
   constexpr size_t smem = NT * (D / 32) * 512 + (rings > gathered ? rings : gathered);
   static bool configured[64] = {};
   int dev = 0;
@@ -732,7 +786,10 @@ static int attn_kv8(AttnKv8Params& p, int D, int ctas, bool step, cudaStream_t s
       p.max_pages <= 0 || p.num_pages <= 0 || p.window < 0 || p.chunk < 0 || p.ld_q % 4 != 0)
     return -2;
   const int rows = p.q_per_seq * (p.n_q / p.n_kv), tile = kv8_tile_rows(rows);
+  if (rows >= 1 << 16) return -2;
   p.tiles = (rows + tile - 1) / tile;
+  const uint32_t group = p.n_q / p.n_kv;
+  p.per_group = group == 1 ? 0 : static_cast<uint32_t>(((1ULL << 32) + group - 1) / group);
   const long long line = static_cast<long long>(p.batch) * p.n_kv * p.tiles * (p.max_pages / 2 + 1);
   if (p.splits == 0 ? ctas <= 0 || p.part_o == nullptr || p.part_ml == nullptr || p.joins == nullptr || line > (1LL << 30)
                     : p.batch > 65535 || static_cast<long long>(p.n_kv) * p.tiles > 65535)
