@@ -36,6 +36,7 @@ class ModelLoadOptions:
     max_batch: int = 8
     max_seq_len: int = 4096
     kv_pages: Optional[int] = None
+    kv_bits: Optional[int] = None        # 8: keys and values are cached in 8 bits with a scale per page and head
     state_slots: Optional[int] = None    # recurrent-state slots of hybrid models (None: twice the decode batch)
     prefix_cache: bool = False           # later requests lease the published KV pages of an equal prompt prefix
     kv_host_tier_bytes: int = 0          # with prefix_cache: evicted published pages are kept in pinned host memory ...
@@ -226,7 +227,7 @@ class LoadedModel:
         engine = Engine(model, max_batch=opt.max_batch, max_seq_len=opt.max_seq_len, num_pages=opt.kv_pages,
                         use_cuda_graph=opt.use_cuda_graph, prefix_cache=opt.prefix_cache,
                         kv_host_tier_bytes=opt.kv_host_tier_bytes, kv_disk_tier_dir=opt.kv_disk_tier_dir,
-                        kv_disk_tier_bytes=opt.kv_disk_tier_bytes, state_slots=opt.state_slots)
+                        kv_disk_tier_bytes=opt.kv_disk_tier_bytes, state_slots=opt.state_slots, kv_bits=opt.kv_bits)
         tokenizer = None
         try:
             from ..text.tokenizer import load_tokenizer
@@ -659,6 +660,8 @@ class LoadedModel:
         par = opt.parallel
         if par is not None and par.tp_size * par.pp_size * par.ep_size > 1:
             raise NotImplementedError(f"{src.cfg.model_type}: tensor / pipeline / expert parallelism is not built for this family")
+        if opt.kv_bits == 8:
+            raise NotImplementedError(f"{src.cfg.model_type}: this family's attention does not take 8-bit pages")
         if opt.weight_residency != "device" or opt.expert_cache or opt.prefix_cache:
             raise NotImplementedError(f"{src.cfg.model_type}: weight residency tiers, expert caches and prefix reuse are not built for this family")
         if src.cfg.model_type == "inkling_mm_model":

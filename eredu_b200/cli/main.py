@@ -67,6 +67,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--expert-cache-prefill-bank-bytes", type=int, default=1 << 30)
     p.add_argument("--expert-cache-eviction", choices=["lru", "lfu"], default="lru")
     p.add_argument("--expert-cache-benchmark", action="store_true")
+    p.add_argument("--kv-bits", type=int, choices=[8, 16], default=16, help="8: keys and values cached in 8 bits with a scale per page and head")
     p.add_argument("--mapped-shards", type=int, default=4)
     p.add_argument("--raw", action="store_true", help="no chat template: the prompt is fed verbatim")
     p.add_argument("--image", action="append", default=[], metavar="PATH", help="image part of the prompt (vision-language models)")
@@ -375,7 +376,7 @@ def main(argv=None) -> int:
             ec_budget = ec_budget or plan.expert_cache.get("device_budget_bytes")
             ec_eviction = plan.expert_cache.get("eviction", ec_eviction)
     t0 = time.perf_counter()
-    lm = LoadedModel.load(model_path, ModelLoadOptions(device=device, quantization=quant, mapped_shards=a.mapped_shards,
+    lm = LoadedModel.load(model_path, ModelLoadOptions(device=device, quantization=quant, mapped_shards=a.mapped_shards, kv_bits=a.kv_bits,
                                                        max_batch=1, max_seq_len=max(4096, a.max_tokens + 2048),
                                                        weight_residency=("dense_disk_stream" if dense_disk else
                                                                          "layerwise_host" if layerwise else "device"),

@@ -157,6 +157,57 @@ class BlockManager {
 
   int refcount(int64_t page) const { return refs_.at(page); }
 
+  // Pages somebody holds, in order.
+  std::vector<int64_t> held() const {
+    std::vector<int64_t> out;
+    for (int64_t p = 1; p < num_pages_; ++p)
+      if (refs_[p] > 0) out.push_back(p);
+    return out;
+  }
+
+  // Renames pages so that those with contents (held or published) are the lowest ones: (old, new) pairs, all old ones behind all new ones. The
+  // caller copies the contents and renames the pages wherever it keeps them, before anything else is written.
+  std::vector<std::pair<int64_t, int64_t>> compact() {
+    std::vector<std::pair<int64_t, int64_t>> moves;
+    auto live = [&](int64_t p) { return refs_[p] > 0 || cached_.count(p) > 0; };
+    int64_t lo = 1, hi = num_pages_ - 1;
+    for (;;) {
+      while (lo < hi && live(lo)) ++lo;
+      while (hi > lo && !live(hi)) --hi;
+      if (lo >= hi) break;
+      refs_[lo] = refs_[hi];
+      hash_of_[lo] = hash_of_[hi];
+      has_hash_[lo] = has_hash_[hi];
+      uses_[lo] = uses_[hi];
+      stamp_[lo] = stamp_[hi];
+      refs_[hi] = 0;
+      uses_[hi] = stamp_[hi] = 0;
+      if (has_hash_[hi]) {
+        auto it = by_hash_.find(hash_of_[hi]);
+        if (it != by_hash_.end() && it->second == hi) it->second = lo;
+        has_hash_[hi] = false;
+      }
+      if (cached_.erase(hi) > 0) cached_.insert(lo);
+      moves.emplace_back(hi, lo);
+    }
+    rebuild_free();
+    return moves;
+  }
+
+  // Another number of pages; those that go must have no contents (compact() first).
+  void resize(int64_t num_pages) {
+    if (num_pages < 2) throw std::invalid_argument("need at least 2 pages");
+    for (int64_t p = num_pages; p < num_pages_; ++p)
+      if (refs_[p] > 0 || cached_.count(p) > 0) throw std::invalid_argument("page " + std::to_string(p) + " has contents");
+    num_pages_ = num_pages;
+    refs_.resize(num_pages, 0);
+    hash_of_.resize(num_pages, 0);
+    has_hash_.resize(num_pages, false);
+    uses_.resize(num_pages, 0);
+    stamp_.resize(num_pages, 0);
+    rebuild_free();
+  }
+
   // The page published under `hash` on the device, or -1.
   int64_t lookup(uint64_t hash) const {
     auto it = by_hash_.find(hash);
@@ -175,6 +226,11 @@ class BlockManager {
  private:
   void check(int64_t p) const {
     if (p <= 0 || p >= num_pages_) throw std::out_of_range("page id out of range");
+  }
+  void rebuild_free() {
+    free_.clear();
+    for (int64_t p = num_pages_ - 1; p >= 1; --p)
+      if (refs_[p] == 0 && cached_.count(p) == 0) free_.push_back(p);
   }
   int64_t evict_one() {
     if (cached_.empty()) throw std::runtime_error("no evictable page");
@@ -473,6 +529,9 @@ void bind_runtime(py::module_& m) {
       .def("match_prefix", &BlockManager::match_prefix)
       .def("seal_prefix", &BlockManager::seal_prefix)
       .def("refcount", &BlockManager::refcount)
+      .def("held", &BlockManager::held)
+      .def("compact", &BlockManager::compact)
+      .def("resize", &BlockManager::resize)
       .def("lookup", &BlockManager::lookup)
       .def("take_evicted", &BlockManager::take_evicted)
       .def_static("chain_hash", &BlockManager::chain_hash);

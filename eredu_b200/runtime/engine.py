@@ -51,7 +51,8 @@ class Engine:
     def __init__(self, model: CausalLM, max_batch: int = 32, max_seq_len: int = 4096, num_pages: Optional[int] = None,
                  use_cuda_graph: Optional[bool] = None, prefill_chunk: int = 8192, hist_cap: int = 1024,
                  prefix_cache: bool = False, kv_host_tier_bytes: int = 0, kv_disk_tier_dir=None, kv_disk_tier_bytes: int = 0,
-                 state_slots: Optional[int] = None):
+                 state_slots: Optional[int] = None, kv_bits: Optional[int] = None):
+        """``kv_bits`` = 8: keys and values are cached in 8 bits (:mod:`eredu_b200.ops.kv8`)."""
         self.model = model
         self.cfg = model.cfg
         self.device = model.device
@@ -69,13 +70,15 @@ class Engine:
             layer_dims = {li: self.cfg.layer_kv_dims(li) for li in kv_layers}
             donors = {li: self.cfg.layer_kv_donor(li) for li in local if self.cfg.layer_kv_donor(li) is not None}
             layer_pools = {li: self.cfg.layer_kv_pool(li) for li in kv_layers if self.cfg.layer_kv_pool(li)}
+        if kv_bits == 8:
+            self._check_8bit_pages()
         self.kv = PagedKVCache(model.num_local_layers(), model.n_kv_local, key_dim, num_pages, model.dtype,
                                self.device, first_layer=model.first_layer, value_dim=value_dim,
                                attention_layers=kv_layers,
                                conv_layers=conv_layers,
                                conv_channels=self.cfg.hidden_size // model.par.tp_size if conv_layers else 0,
                                conv_hist=self.cfg.conv_l_cache - 1, layer_dims=layer_dims, donors=donors,
-                               layer_pools=layer_pools)
+                               layer_pools=layer_pools, kv_bits=kv_bits)
         # recurrent-state slots: by default twice the decode batch, so that prompts can be prefilled while a batch decodes
         slots = max(2 * max_batch, 8) if state_slots is None else state_slots
         shapes = {li: self.cfg.layer_state_shape(li) for li in local if self.cfg.layer_state_shape(li) is not None}
@@ -134,6 +137,16 @@ class Engine:
         # Pipeline parallelism: ``forward`` returns None on stages without the output head and ``token_sync``
         # distributes the tokens sampled on the last stage (set by parallel.pipeline.PipelineRunner).
         self.token_sync = None
+
+    def _check_8bit_pages(self) -> None:
+        """The families whose attention layers reach their cache through the operators that take 8-bit pages."""
+        cfg = self.cfg
+        own = (cfg.mixers is not None or cfg.is_mla or getattr(self.model, "family", None) is not None
+               or any(getattr(self.model, name, None) is not None for name in ("g4", "mg")))
+        if own:
+            raise NotImplementedError(f"{cfg.model_type}: this family's attention does not take 8-bit pages")
+        if self.device.type == "cuda" and cfg.head_dim not in ops.KV8_HEAD_DIMS:
+            raise NotImplementedError(f"8-bit pages are built for head sizes {ops.KV8_HEAD_DIMS}, not {cfg.head_dim}")
 
     # ------------------------------------------------------------------------------------------ requests
     def new_sequence(self, prompt, sampling=None, max_new_tokens=256, eos_ids=()) -> Sequence:
@@ -243,6 +256,54 @@ class Engine:
             self.kv.allocator.release(seq.pages)
             seq.pages = []
 
+    def fork(self, seq: Sequence) -> Sequence:
+        """A second sequence at the same point: same prompt, output and cached tokens. Full pages are shared, which nobody writes to any more; the page that is
+        being filled is copied (in all layers, one launch). It draws random numbers of its own."""
+        other = Sequence(self._next_id, list(seq.prompt), seq.sampling, seq.max_new_tokens, seq.eos_ids, list(seq.output), kv_len=seq.kv_len,
+                         cached_tokens=seq.cached_tokens)
+        if getattr(seq, "rope_delta", 0):
+            other.rope_delta = seq.rope_delta
+        self._next_id += 1
+        if seq.pages:
+            other.pages = self.kv.fork(seq.pages, seq.kv_len)
+            try:
+                if self.kv.page_to_slot is not None:
+                    self.kv.bind_state(other.pages[0])
+                self.kv.restore_state(other.pages[0], self.kv.snapshot_state(seq.pages[0]))
+            except RuntimeError:
+                self.kv.allocator.release(other.pages)
+                raise
+        return other
+
+    def compact(self, seqs) -> int:
+        """Moves the cached pages to the front of the pool and renames them in ``seqs`` (all sequences that have pages) and in the decode state, whose
+        captured graph stays valid. Returns the number of pages moved."""
+        named = {int(p) for s in seqs for p in s.pages}
+        missing = [p for p in self.kv.allocator.held() if p not in named]
+        if missing:
+            raise ValueError(f"{len(missing)} pages are held by none of the sequences given")
+        moves = self.kv.compact()
+        if moves:
+            for s in seqs:
+                s.pages = [moves.get(int(p), int(p)) for p in s.pages]
+            st = self._decode_state
+            if st is not None:
+                names = np.arange(self.kv.num_pages, dtype=np.int64)
+                names[list(moves)] = list(moves.values())
+                names = self._t(names, torch.int64)
+                st["block_table"].copy_(names[st["block_table"].long()])
+                slots = st["slots"]
+                slots.copy_(torch.where(slots >= 0, names[slots.clamp_min(0) // PAGE] * PAGE + slots.clamp_min(0) % PAGE, slots))
+        return len(moves)
+
+    def resize_cache(self, num_pages: int, seqs=()) -> None:
+        """Another number of pages while ``seqs`` (all sequences that have pages) keep theirs: gives memory back, or takes more. Not during a decode
+        state, whose graph reads the pool where it is."""
+        if self._decode_state is not None:
+            raise RuntimeError("the pool does not change its size under a decode state")
+        self.compact(seqs)
+        self.kv.resize(num_pages)
+
     def snapshot_state(self, seq: Sequence):
         """Recurrent state of a hybrid model's sequence at its current length (None when there is none to keep)."""
         return self.kv.snapshot_state(seq.pages[0]) if seq.pages else None
@@ -258,8 +319,10 @@ class Engine:
             t = t.pin_memory().to(self.device, non_blocking=True)
         return t
 
-    def decode_splits(self, batch: int, longest: int) -> int:
-        """Split-KV factor of a step of ``batch`` sequences that bring one token each, the longest context of them ``longest`` tokens."""
+    def decode_splits(self, batch: int, longest: int, tokens: int = 1) -> int:
+        """Split-KV factor of a step of ``batch`` sequences that bring one token each (8-bit pages: ``tokens``), the longest context of them ``longest`` tokens."""
+        if self.cuda and self.kv.kv_bits:
+            return ops.decode_splits(batch, self.model.n_kv_local, longest, self.sm_count, tokens * self.model.n_q_local // self.model.n_kv_local, bits=8)
         rows = self.model.decode_rows
         return ops.decode_splits(batch, self.model.n_kv_local, longest, self.sm_count, rows, self.cfg.head_dim) if self.cuda else 1
 
@@ -752,14 +815,26 @@ class Engine:
     # ------------------------------------------------------------------------------------------ generate
     @torch.no_grad()
     def generate(self, prompts: list[list[int]], sampling: Optional[SamplingParams] = None, max_new_tokens: int = 64,
-                 eos_ids=(), on_token=None) -> list[list[int]]:
+                 eos_ids=(), on_token=None, samples: int = 1) -> list[list[int]]:
         """Greedy / stochastic generation for a batch of token-id prompts. ``on_token(seq_index, token)`` is called
         as tokens are committed; a truthy return value ends that sequence with the value as its finish reason.
-        ``self.last_finish_reasons`` holds the per-sequence reasons afterwards."""
-        seqs = [self.new_sequence(p, sampling, max_new_tokens, eos_ids) for p in prompts]
+        ``self.last_finish_reasons`` holds the per-sequence reasons afterwards.
+        ``samples`` > 1: that many continuations of every prompt, one behind the other in the result. The prompt is run and cached once; its sequence is
+        forked in front of its last token, which is every continuation's first step."""
+        seqs = []
         try:
-            first = self.prefill(seqs)
-            first_host = first.tolist()
+            for p in prompts:
+                seqs.append(self.new_sequence(p, sampling, max_new_tokens, eos_ids))
+                if samples > 1:
+                    s, known = seqs[-1], len(p) - 1
+                    if known > s.kv_len:
+                        self.prefill([s], limits=[known - s.kv_len])
+                    seqs.extend(self.fork(s) for _ in range(samples - 1))
+            if samples > 1:
+                first = torch.tensor([s.prompt[-1] for s in seqs], dtype=torch.int32)
+            else:
+                first = self.prefill(seqs)
+            first_host = first.tolist() if samples == 1 else []
             for i, (s, t) in enumerate(zip(seqs, first_host)):
                 s.output.append(int(t))
                 if on_token:

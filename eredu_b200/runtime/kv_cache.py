@@ -12,6 +12,8 @@ from typing import Optional
 
 import torch
 
+from ..ops.kv8 import FLOOR, Pages8, copy_pages
+
 PAGE = 16
 
 
@@ -36,13 +38,31 @@ class PageAllocator:
     def release(self, pages) -> None:
         self._free.extend(reversed(list(pages)))
 
+    def held(self) -> list[int]:
+        return sorted(set(range(1, self.num_pages)) - set(self._free))
+
+    def compact(self) -> list[tuple[int, int]]:
+        held = self.held()
+        kept = set(held)
+        moves = list(zip([p for p in held if p > len(held)][::-1], [p for p in range(1, len(held) + 1) if p not in kept]))
+        self._free = list(range(self.num_pages - 1, len(held), -1))
+        return moves
+
+    def resize(self, num_pages: int) -> None:
+        if num_pages < 2 or any(p >= num_pages for p in self.held()):
+            raise ValueError(f"pages behind {num_pages} have contents")
+        held = set(self.held())
+        self.num_pages = num_pages
+        self._free = [p for p in range(num_pages - 1, 0, -1) if p not in held]
+
 
 class PagedKVCache:
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, num_pages: int, dtype, device,
                  first_layer: int = 0, attention_layers=None, conv_layers=None, conv_channels: int = 0, conv_hist: int = 0,
                  value_dim: Optional[int] = None, layer_dims: Optional[dict] = None, donors: Optional[dict] = None,
-                 layer_pools: Optional[dict] = None):
-        """``layer_dims``: layer -> (kv heads, key width, value width) for families whose layers differ; layers of one
+                 layer_pools: Optional[dict] = None, kv_bits: Optional[int] = None):
+        """``kv_bits`` = 8: keys and values are held as int8 codes with a scale per page and head (:mod:`eredu_b200.ops.kv8`), about half the memory of bf16;
+        :meth:`layer` then gives a pair of ``Pages8``. ``layer_dims``: layer -> (kv heads, key width, value width) for families whose layers differ; layers of one
         geometry share a pool tensor, so a page id is valid in every layer. ``donors``: layer -> the earlier layer whose
         keys and values it reads (it keeps none of its own). ``layer_pools``: layer -> tokens of a block whose mean key and
         value are kept as well; a page holds the means of the blocks that end in it, so they come and go with the page.
@@ -61,8 +81,18 @@ class PagedKVCache:
             groups.setdefault(tuple((layer_dims or {}).get(li, default)), []).append(li)
         if not groups:
             groups[default] = []
+        if kv_bits not in (None, 8, 16):
+            raise ValueError(f"kv_bits is 8 or 16, not {kv_bits}")
+        self.kv_bits = 8 if kv_bits == 8 else None
+        if self.kv_bits and (layer_pools or any(dk != dv for _, dk, dv in groups)):
+            raise NotImplementedError("8-bit pages hold keys and values of one width, without means of blocks")
+        if self.kv_bits:
+            dtype = torch.int8
         self.pools, self._kv_index = [], {}
+        self.scales: list = []               # 8-bit pages: fp32 [layers, pages, heads] of keys and of values, per pool
         for g, ((heads, dk, dv), members) in enumerate(groups.items()):
+            if self.kv_bits:
+                self.scales.append(tuple(torch.full((len(members), num_pages, heads), FLOOR, dtype=torch.float32, device=device) for _ in "kv"))
             k = torch.zeros((len(members), num_pages, heads, PAGE, dk), dtype=dtype, device=device)
             # latent-attention models cache one row per token in ``k`` and nothing in ``v`` (value_dim 1 keeps the plumbing)
             v = torch.zeros_like(k) if dv == dk else torch.zeros((len(members), num_pages, heads, PAGE, dv), dtype=dtype,
@@ -206,10 +236,74 @@ class PagedKVCache:
     def layer(self, li: int):
         g, i = self._kv_index[li]
         k, v = self.pools[g]
+        if self.kv_bits:
+            ks, vs = self.scales[g]
+            return Pages8(k[i], ks[i]), Pages8(v[i], vs[i])
         return k[i], v[i]
 
+    # ---- whole pages
+    def page_tensors(self) -> list:
+        """Everything that belongs to a page, as tensors [layers, pages, ...]."""
+        pooled = [t[None] for pair in self.pooled.values() for t in pair]
+        return [t for pair in (*self.pools, *self.scales) for t in pair if t.shape[0]] + pooled
+
+    def copy_pages(self, src, dst) -> None:
+        """Page ``src[i]`` to page ``dst[i]`` in every layer (:func:`eredu_b200.ops.copy_pages`, with its checks); page 0 is nobody's."""
+        if any(int(p) == 0 for p in (*src, *dst)):
+            raise IndexError("page 0 belongs to nobody")
+        copy_pages(self.page_tensors(), src, dst)
+
+    def fork(self, pages, kv_len: int) -> list:
+        """Pages of a second sequence with the same ``kv_len`` cached tokens and as many pages: full ones are shared (leased once more), the others are new,
+        with a copy of what they hold. Sequences with a recurrent state, which is found by their first page, share none."""
+        al = self.allocator
+        held = self.pages_for(kv_len)
+        shared = kv_len // PAGE if hasattr(al, "retain") and not self.has_recurrent_state() else 0
+        fresh = self.alloc(len(pages) - shared)
+        if shared:
+            al.retain(list(pages[:shared]))
+        self.copy_pages(list(pages[shared:held]), fresh[:held - shared])
+        return list(pages[:shared]) + fresh
+
+    def compact(self) -> dict:
+        """Moves pages so that those with contents are the lowest ones; {old page: new page} of those that moved. Whoever keeps page numbers renames them."""
+        moves = self.allocator.compact()
+        if moves:
+            tensors = self.page_tensors() + ([self.conv_state] if self.conv_state is not None else [])
+            copy_pages(tensors, [a for a, _ in moves], [b for _, b in moves])
+        if self.page_to_slot is not None:
+            names = {a: b for a, b in moves}
+            self._slot_of_page = {names.get(p, p): slot for p, slot in self._slot_of_page.items()}
+            for p, slot in self._slot_of_page.items():
+                self.page_to_slot[p] = slot
+        return dict(moves)
+
+    def resize(self, num_pages: int) -> None:
+        """Another number of pages, with the contents of those that stay; the pages that go must have none (:meth:`compact`)."""
+        self.allocator.resize(num_pages)
+        keep = min(num_pages, self.num_pages)
+
+        def other(t, dim=1):
+            shape = list(t.shape)
+            shape[dim] = num_pages
+            new = t.new_zeros(shape)
+            new.narrow(dim, 0, keep).copy_(t.narrow(dim, 0, keep))
+            return new
+
+        self.pools = [tuple(other(t) for t in pair) for pair in self.pools]
+        self.scales = [tuple(other(t) for t in pair) for pair in self.scales]
+        self.pooled = {li: tuple(other(t, 0) for t in pair) for li, pair in self.pooled.items()}
+        self.k, self.v = self.pools[0]
+        if self.conv_state is not None:
+            self.conv_state = other(self.conv_state)
+        if self.page_to_slot is not None:
+            self.page_to_slot = other(self.page_to_slot, 0)
+        self.num_pages = num_pages
+
     def require_uniform(self, what: str) -> None:
-        """Raised by the features that move pages of one geometry (lower tiers, parking)."""
+        """Raised by the features that move pages of one geometry (lower tiers, parking, prompt caches)."""
+        if self.kv_bits:
+            raise NotImplementedError(f"{what} does not take 8-bit pages")
         if len(self.pools) > 1:
             raise NotImplementedError(f"{what} needs one key / value geometry for all layers; this model has {len(self.pools)}")
         if self.pooled:
@@ -224,6 +318,7 @@ class PagedKVCache:
             extra += self.la_rec_state.numel() * 4 + self.la_conv_state.numel() * self.la_conv_state.element_size()
         extra += sum(t.numel() * 4 for t in self.layer_state.values())
         pools = (*self.pools, *self.pooled.values())
+        extra += sum(4 * (k.numel() + v.numel()) for k, v in self.scales)
         return sum((k.numel() + v.numel()) * k.element_size() for k, v in pools) + extra
 
     @staticmethod

@@ -269,6 +269,8 @@ def save_prompt_cache(engine, seq, directory, checkpoint_fingerprint: str, prefi
     from ..formats.checkpoint import _np
     from ..lib import _eredu_host as H
 
+    if engine.kv.kv_bits:
+        engine.kv.require_uniform("a prompt cache")
     ident = model_identity(engine, checkpoint_fingerprint)
     topo: PromptCacheTopology = ident["topology"]
     n = seq.kv_len if prefix_tokens is None else int(prefix_tokens)
@@ -377,6 +379,8 @@ def load_prompt_cache(engine, directory, tokens, checkpoint_fingerprint: str, sa
     of ``tokens`` (checked by hash); at least the last token is left to prefill so that logits exist."""
     from ..lib import _eredu_host as H
 
+    if engine.kv.kv_bits:
+        engine.kv.require_uniform("a prompt cache")
     ident = model_identity(engine, checkpoint_fingerprint)
     man = open_prompt_cache(directory, ident["topology"])
     for key in ("model_family", "effective_model_type", "checkpoint_fingerprint", "architecture_fingerprint", "layer_count",
