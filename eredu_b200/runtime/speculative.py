@@ -70,7 +70,9 @@ class SpeculativeDecoder:
     @staticmethod
     def _splits(eng: Engine, batch: int, tokens: int, longest: int) -> int:
         """Split-KV factor of a step of ``tokens`` per sequence: a drafter's single tokens are split like those of any decode step."""
-        if tokens == 1 or getattr(eng.kv, "kv_bits", None):
+        if tokens == 1:
+            return eng.decode_splits(batch, longest)
+        if getattr(eng.kv, "kv_bits", None):
             return eng.decode_splits(batch, longest, tokens)
         return ops.decode_splits(batch, eng.model.n_kv_local, longest, eng.sm_count) if eng.cuda else 1
 
