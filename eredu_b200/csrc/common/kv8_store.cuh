@@ -19,13 +19,16 @@ struct Kv8StoreParams {
   int* status;
 };
 
-// Angle of a position: the product in two parts, so that far positions keep their digits.
-__device__ __forceinline__ float2 turn_of(int pos, float freq, float factor) {
+// Cosine and sine of pos * freq, times `factor`. The product in two parts, so that far positions keep their digits; then whole turns are taken off with
+// 2 pi in two parts (the reduction of Cody and Waite; fma makes the first difference exact), which leaves an angle the fast functions are good for: off by 2^-20
+// in all for angles below 2^24, where sincosf costs four times as much.
+__device__ __forceinline__ void turn_of(int pos, float freq, float factor, float& c, float& s) {
   const float p = static_cast<float>(pos);
   const float a = p * freq, rest = fmaf(p, freq, -a);
-  float s, c;
-  sincosf(a, &s, &c);
-  return make_float2((c - s * rest) * factor, (s + c * rest) * factor);
+  const float k = rintf(a * 0.15915494f);
+  const float r = fmaf(-k, -1.7484556e-7f, fmaf(-k, 6.2831855f, a)) + rest;
+  s = __sinf(r) * factor;
+  c = __cosf(r) * factor;
 }
 
 template <int D>
@@ -33,9 +36,9 @@ __device__ __forceinline__ float4 load_row4(const __nv_bfloat16* row, int lane) 
   const uint2 u = *reinterpret_cast<const uint2*>(row + 4 * (lane & (D / 4 - 1)));
   return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
 }
-// The D / 4 lanes of a row together: norm, then rotation. `turns`: cosine and sine of the row's rot / 2 angles.
+// The D / 4 lanes of a row together: norm, then rotation. `turns`: rot / 2 cosines of the row's angles, then as many sines.
 template <int D>
-__device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, const float* w, const float2* turns, int lane) {
+__device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, const float* w, const float* turns, int lane) {
   const int d = 4 * (lane & (D / 4 - 1));
   if (w != nullptr) {
     float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
@@ -48,61 +51,71 @@ __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, co
     x.w *= inv * (w[d + 3] + p.norm_w_off);
   }
   if (p.rot == 0) return x;
+  const int half = p.rot / 2;
   if (p.interleaved) {
     if (d < p.rot) {
-      const float2 a = turns[d / 2], b = turns[d / 2 + 1];
-      x = make_float4(x.x * a.x - x.y * a.y, x.y * a.x + x.x * a.y, x.z * b.x - x.w * b.y, x.w * b.x + x.z * b.y);
+      const float2 c = *reinterpret_cast<const float2*>(turns + d / 2), n = *reinterpret_cast<const float2*>(turns + half + d / 2);
+      x = make_float4(x.x * c.x - x.y * n.x, x.y * c.x + x.x * n.x, x.z * c.y - x.w * n.y, x.w * c.y + x.z * n.y);
     }
     return x;
   }
-  const int half = p.rot / 2;
   const int from = d < half ? lane + half / 4 : d < p.rot ? lane - half / 4 : lane;
   const float4 o = make_float4(__shfl_sync(0xffffffffu, x.x, from), __shfl_sync(0xffffffffu, x.y, from), __shfl_sync(0xffffffffu, x.z, from),
                                __shfl_sync(0xffffffffu, x.w, from));
   if (d < p.rot) {
     const float sign = d < half ? -1.f : 1.f;
-    const float2* t = turns + (d < half ? d : d - half);
-    x = make_float4(x.x * t[0].x + sign * o.x * t[0].y, x.y * t[1].x + sign * o.y * t[1].y, x.z * t[2].x + sign * o.z * t[2].y, x.w * t[3].x + sign * o.w * t[3].y);
+    const int i = d < half ? d : d - half;
+    const float4 c = *reinterpret_cast<const float4*>(turns + i), n = *reinterpret_cast<const float4*>(turns + half + i);
+    x = make_float4(x.x * c.x + sign * o.x * n.x, x.y * c.y + sign * o.y * n.y, x.z * c.z + sign * o.z * n.z, x.w * c.w + sign * o.w * n.w);
   }
   return x;
 }
 
-// Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on; the whole warp.
-template <int D, bool KEYS>
-__device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float2* turns, int lane) {
+// Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on. SHARE warps together (`part` of them; 1: a warp by itself);
+// `tops` has a word for each, and all threads of the CTA are here then.
+template <int D, bool KEYS, int SHARE>
+__device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, int part,
+                                            uint32_t* tops) {
   constexpr int RPI = 128 / D;              // rows a warp holds at once
-  constexpr int STEPS = kKv8Page / RPI;
+  constexpr int STEPS = kKv8Page / (RPI * SHARE);
   const __nv_bfloat16* src = KEYS ? p.k : p.v;
   const int ld = KEYS ? p.ld_k : p.ld_v;
   int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
   float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
-  const int sub = RPI == 1 ? 0 : lane >> 4;
+  const int sub = (RPI == 1 ? 0 : lane >> 4) + part * RPI;
   float4 x[STEPS];
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int r = i * RPI + sub;
+    const int r = i * RPI * SHARE + sub;
     x[i] = r < n ? load_row4<D>(src + static_cast<size_t>(row + r) * ld + h * D, lane) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float before = first > 0 ? *at : 0.f;
   uint32_t top = 0;   // as bits, so that what is no number wins
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    if (i * RPI >= n) break;
+    if (i * RPI * SHARE + part * RPI >= n) break;
+    const int r = i * RPI * SHARE + sub;
     if (KEYS) {
-      const float4 y = prepared<D>(p, x[i], p.k_norm_w, turns + min(i * RPI + sub, n - 1) * (p.rot / 2), lane);
-      if (i * RPI + sub < n) x[i] = y;
+      const float4 y = prepared<D>(p, x[i], p.k_norm_w, turns + min(r, n - 1) * p.rot, lane);
+      if (r < n) x[i] = y;
     }
     top = max(max(top, __float_as_uint(fabsf(x[i].x))), __float_as_uint(fabsf(x[i].y)));
     top = max(max(top, __float_as_uint(fabsf(x[i].z))), __float_as_uint(fabsf(x[i].w)));
   }
   top = __reduce_max_sync(0xffffffffu, top);
+  if (SHARE > 1) {
+    if (lane == 0) tops[part] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SHARE; ++i) top = max(top, tops[i]);
+  }
   float scale = kv8_needed(__uint_as_float(top));
   if (first > 0 && !(before <= scale)) scale = scale != scale ? scale : before;   // the larger, and what is no number stays none
   const float inv = kv8_inverse(scale);
   const int c = 4 * (lane & (D / 4 - 1));
   if (first > 0 && scale != before) {
     const float ratio = before * inv;
-    for (int r = sub; r < first; r += RPI) {
+    for (int r = sub; r < first; r += RPI * SHARE) {
       uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + c);
       const uint32_t u = *w;
       *w = kv8_pack(kv8_code(u, 0) * ratio, kv8_code(u, 1) * ratio, kv8_code(u, 2) * ratio, kv8_code(u, 3) * ratio);
@@ -110,10 +123,11 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
   }
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int r = i * RPI + sub;
+    const int r = i * RPI * SHARE + sub;
     if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x[i].x * inv, x[i].y * inv, x[i].z * inv, x[i].w * inv);
   }
-  if (lane == 0) *at = scale;
+  if (SHARE > 1) __syncthreads();   // the words, and the scale that others may still be reading
+  if (lane == 0 && part == 0) *at = scale;
 }
 
 }  // namespace eredu

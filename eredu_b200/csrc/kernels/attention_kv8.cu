@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   float* weight = reinterpret_cast<float*>(row_s + ROWS);         // [warps, or splits][ROWS]
   __shared__ float back_s[ROWS], up_s[ROWS];
   __shared__ size_t out_s[ROWS];          // where a row's output goes
-  __shared__ float2 turns_s[STEP ? kKv8StepTokens * D / 2 : 1];   // angles of the tile's tokens
+  __shared__ __align__(16) float turns_s[STEP ? kKv8StepTokens * D : 1];   // cosines and sines of the tile's tokens
   pdl_launch_early();
   trace_mark(kTraceAttnDecode, kTraceStart);
   pdl_wait();
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const int tokens = pos_last - pos_first + 1;
     const int* positions = p.st.positions + static_cast<size_t>(b) * p.q_per_seq + token0;
     for (int n = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); n < tokens; n += kKv8Threads / (D / 2))
-      if (i < half) turns_s[n * half + i] = turn_of(positions[n], p.st.inv_freq[i], p.st.attn_factor);
+      if (i < half) turn_of(positions[n], p.st.inv_freq[i], p.st.attn_factor, turns_s[n * p.st.rot + i], turns_s[n * p.st.rot + half + i]);
     __syncthreads();
     // ---- the new rows of pages in this part: a warp for the keys or the values of a page (there are two such pages at most)
     if (p.append) {
@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
           if (to >= 0 && (to >> 4) < p.num_pages) {
             while (r + n < end_row && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
             const long long cell = (to >> 4) * p.n_kv + kvh;
-            if ((warp & 1) == 0) store_block<D, true>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * half, lane);
-            else store_block<D, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane);
+            if ((warp & 1) == 0) store_block<D, true, 1>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * p.st.rot, lane, 0, nullptr);
+            else store_block<D, false, 1>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane, 0, nullptr);
           } else if (to >= 0) {
             report_status(p.status, kStatusBadArgument);
           }
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const int row = (i * kKv8Warps + warp) * RPI + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
     const bool in = row < rows;
     float4 x = query[i];
-    if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (kv8_token(p, r0 + min(row, rows - 1)) - token0) * half, lane);
+    if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (kv8_token(p, r0 + min(row, rows - 1)) - token0) * p.st.rot, lane);
     if (!in) x = make_float4(0.f, 0.f, 0.f, 0.f);
     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))), max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
 #pragma unroll

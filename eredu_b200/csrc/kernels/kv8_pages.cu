@@ -12,43 +12,46 @@ namespace eredu {
 // ============================================================================ rows into their blocks
 // q, k rotated by their positions (optional RMSNorm per head in front), k and v rounded into their blocks, q stored as it is.
 //
-// A run is a stretch of rows that follow one another in one page; its rows share a scale per head, so one warp holds all of a run's rows of a
-// head in registers (16 x 128 / 32 values a lane), finds the largest and stores the codes: one read, no shared memory. A lane has four
-// neighbouring values of a row; the partner of a rotation sits `rot / 8` lanes further. The angles of a tile of rows are computed once for all heads.
-constexpr int kStoreThreads = 256;
+// A run is a stretch of rows that follow one another in one page; its rows share a scale per head. Four warps have the run's keys in registers and four its
+// values (16 x 128 / 128 values a thread), find the largest together and store the codes: one read. A lane has four neighbouring values of a row; the
+// partner of a rotation sits `rot / 8` lanes further. The angles of a tile of rows are computed once for the head's keys and its query heads.
+// 4096 rows, 32 heads of 128 over 8: a warp to a run's keys, in 128 registers, 92 us.
+constexpr int kStoreThreads = 256, kStoreShare = kStoreThreads / 64;   // half of the warps for keys, half for values
 constexpr int kStoreRows = 32;      // a tile of 16 rows and what the last run of it has behind them
 
-// grid (tiles of rows, groups of key / value heads)
+// grid (tiles of rows, n_kv)
 template <int D>
-__global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams p, int heads) {
+__global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams p) {
   constexpr int RPI = 128 / D;
-  extern __shared__ float2 turns[];          // [rows of the tile and the last run][rot / 2]
+  extern __shared__ __align__(16) float turns[];          // [rows of the tile and the last run][rot / 2 cosines, rot / 2 sines]
   __shared__ int run_row[kKv8Page], run_len[kKv8Page];
+  __shared__ long long run_slot[kKv8Page];
+  __shared__ uint32_t tops[kStoreThreads / 32];
   __shared__ int runs, behind;
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
-  const int row0 = blockIdx.x * p.tile, rows = min(p.tile, p.M - row0);
-  const int h0 = blockIdx.y * heads, hn = min(heads, p.n_kv - h0);
+  const int row0 = blockIdx.x * p.tile, rows = min(p.tile, p.M - row0), h0 = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.rot / 2;
   if (warp == 0) {
-    // lane r < 16: row r of the tile; its run, where it begins one
+    // lane r has the slots of rows r - 1 and r of the tile and the 16 behind it: a row continues the one in front where its slot is the next of the same page
     const int r = row0 + lane;
-    const bool in = lane < rows;
-    const long long slot = in ? p.slots[r] : -1;
-    bool begins = in && slot >= 0 && (r == 0 || (slot & 15) == 0 || p.slots[r - 1] != slot - 1);
+    const bool known = r < p.M && lane < rows + kKv8Page;
+    const long long slot = known ? p.slots[r] : -1, front = known && r > 0 ? p.slots[r - 1] : -1;
+    const bool follows = slot >= 0 && (slot & 15) != 0 && front == slot - 1;
+    bool begins = lane < rows && slot >= 0 && !follows;
     if (begins && (slot >> 4) >= p.num_pages) {
       report_status(p.status, kStatusBadArgument);
       begins = false;
     }
-    int n = begins ? 1 : 0;
-    if (begins)
-      while (n < kKv8Page - static_cast<int>(slot & 15) && r + n < p.M && p.slots[r + n] == slot + n) ++n;
-    const uint32_t mask = __ballot_sync(0xffffffffu, begins);
+    const uint32_t mask = __ballot_sync(0xffffffffu, begins), more = __ballot_sync(0xffffffffu, follows);
+    // (a tile of 16 rows and 15 more at most: what follows the last row of the warp's 32 cannot belong to a run of this tile)
+    const int n = begins ? 1 + __ffs(~(more >> lane >> 1)) - 1 : 0;
     if (begins) {
       const int i = __popc(mask & ((1u << lane) - 1));
       run_row[i] = lane;
       run_len[i] = n;
+      run_slot[i] = slot;
     }
     const int end = __reduce_max_sync(0xffffffffu, begins ? lane + n : 0);
     if (lane == 0) {
@@ -57,25 +60,39 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < behind * half; i += kStoreThreads)
-    turns[i] = turn_of(p.positions[row0 + i / half], p.inv_freq[i % half], p.attn_factor);
+  for (int r = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); r < behind; r += kStoreThreads / (D / 2))
+    if (i < half) turn_of(p.positions[row0 + r], p.inv_freq[i], p.attn_factor, turns[r * p.rot + i], turns[r * p.rot + half + i]);
   __syncthreads();
-  for (int i = warp; i < runs * hn * 2; i += kStoreThreads / 32) {
-    const int run = i / (2 * hn), h = h0 + (i >> 1) % hn;
-    const int at = run_row[run], row = row0 + at, n = run_len[run];
-    const long long slot = p.slots[row], cell = (slot >> 4) * p.n_kv + h;
-    if ((i & 1) == 0) store_block<D, true>(p, row, n, static_cast<int>(slot & 15), cell, h, turns + at * half, lane);
-    else store_block<D, false>(p, row, n, static_cast<int>(slot & 15), cell, h, turns, lane);
+  for (int i = 0; i < runs; ++i) {
+    const int at = run_row[i];
+    const long long cell = (run_slot[i] >> 4) * p.n_kv + h0;
+    const int first = static_cast<int>(run_slot[i] & 15);
+    if (warp < kStoreShare) store_block<D, true, kStoreShare>(p, row0 + at, run_len[i], first, cell, h0, turns + at * p.rot, lane, warp, tops);
+    else store_block<D, false, kStoreShare>(p, row0 + at, run_len[i], first, cell, h0, turns, lane, warp - kStoreShare, tops + kStoreShare);
   }
-  if (p.q_out == nullptr) return;
-  const int group = p.n_q / p.n_kv, mine = hn * group;     // query heads of this CTA
-  const int sub = RPI == 1 ? 0 : lane >> 4;
-  for (int i = warp * RPI; i < rows * mine; i += kStoreThreads / 32 * RPI) {
-    const int item = min(i + sub, rows * mine - 1), r = item / mine, head = h0 * group + item % mine;
-    const size_t row = row0 + r;
-    const float4 x = prepared<D>(p, load_row4<D>(p.q + row * p.ld_q + head * D, lane), p.q_norm_w, turns + r * half, lane);
-    if (i + sub < rows * mine)
-      *reinterpret_cast<uint2*>(p.q_out + (row * p.n_q + head) * D + 4 * (lane & (D / 4 - 1))) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+  // ---- query rows of this head, four at a time on their way
+  constexpr int WARPS = kStoreThreads / 32, DEEP = 4;
+  const int mine = p.q_out == nullptr ? 1 : p.n_q / p.n_kv, items = p.q_out == nullptr ? 0 : rows * mine, sub = RPI == 1 ? 0 : lane >> 4;
+  const uint32_t per_mine = ((1u << 20) + mine - 1) / mine;     // item / mine by a product: exact below 2^20 / mine, and there are 16 mine of them at most
+  float4 query[DEEP];
+  auto load_queries = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < DEEP; ++j) {
+      const int item = min(i0 + j * WARPS * RPI + sub, items - 1), r = static_cast<int>(item * per_mine >> 20);
+      query[j] = load_row4<D>(p.q + static_cast<size_t>(row0 + r) * p.ld_q + (h0 * mine + item - r * mine) * D, lane);
+    }
+  };
+  for (int i0 = warp * RPI; i0 < items; i0 += WARPS * RPI * DEEP) {
+    load_queries(i0);
+#pragma unroll
+    for (int j = 0; j < DEEP; ++j) {
+      const int item = i0 + j * WARPS * RPI + sub, r = static_cast<int>(min(item, items - 1) * per_mine >> 20), head = h0 * mine + min(item, items - 1) - r * mine;
+      if (i0 + j * WARPS * RPI >= items) break;
+      const float4 x = prepared<D>(p, query[j], p.q_norm_w, turns + r * p.rot, lane);
+      if (item < items)
+        *reinterpret_cast<uint2*>(p.q_out + (static_cast<size_t>(row0 + r) * p.n_q + head) * D + 4 * (lane & (D / 4 - 1))) =
+            make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+    }
   }
 }
 
@@ -91,10 +108,13 @@ struct Kv8ValuesParams {
   const int* seq_lens;     // optional [rows]
   const int* cu_q;         // with seq_lens: query offsets
   int* table_out;          // with seq_lens: [rows, wide]
-  int pitch, wide, n_kv, block, num_pages, window, chunk;   // block = 16 D
+  int pitch, wide, n_kv, num_pages, window, chunk;
   int* status;
 };
-__global__ void __launch_bounds__(256) kv8_values_kernel(Kv8ValuesParams p) {
+constexpr int kValuesThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kValuesThreads) kv8_values_kernel(Kv8ValuesParams p) {
+  constexpr int BLOCK = kKv8Page * D, DEEP = 4;   // codes of a block; pieces of eight codes a thread has on their way
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
@@ -112,21 +132,27 @@ __global__ void __launch_bounds__(256) kv8_values_kernel(Kv8ValuesParams p) {
     if (threadIdx.x == 0) report_status(p.status, kStatusBadArgument);
     page = 0;
   }
-  const int8_t* codes = (blockIdx.z == 0 ? p.k_codes : p.v_codes) + static_cast<size_t>(page) * p.n_kv * p.block;
+  const size_t all = static_cast<size_t>(p.n_kv) * BLOCK;
+  const int8_t* codes = (blockIdx.z == 0 ? p.k_codes : p.v_codes) + page * all;
   const float* scales = (blockIdx.z == 0 ? p.k_scales : p.v_scales) + static_cast<size_t>(page) * p.n_kv;
-  __nv_bfloat16* out = (blockIdx.z == 0 ? p.k_out : p.v_out) + entry * p.n_kv * p.block;
-  for (int c = threadIdx.x * 16; c < p.n_kv * p.block; c += 256 * 16) {
-    const uint4 u = *reinterpret_cast<const uint4*>(codes + c);
-    const float s = scales[c / p.block];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    uint32_t o[8];
+  __nv_bfloat16* out = (blockIdx.z == 0 ? p.k_out : p.v_out) + entry * all;
+  for (int c0 = threadIdx.x * 8; c0 < p.n_kv * BLOCK; c0 += kValuesThreads * 8 * DEEP) {
+    uint2 u[DEEP];
+    float s[DEEP];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      o[2 * j] = pack_bf16x2(kv8_code(w[j], 0) * s, kv8_code(w[j], 1) * s);
-      o[2 * j + 1] = pack_bf16x2(kv8_code(w[j], 2) * s, kv8_code(w[j], 3) * s);
+    for (int j = 0; j < DEEP; ++j) {
+      const int c = min(c0 + j * kValuesThreads * 8, p.n_kv * BLOCK - 8);
+      u[j] = *reinterpret_cast<const uint2*>(codes + c);
+      s[j] = scales[c / BLOCK];
     }
-    *reinterpret_cast<uint4*>(out + c) = make_uint4(o[0], o[1], o[2], o[3]);
-    *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+    for (int j = 0; j < DEEP; ++j) {
+      const int c = c0 + j * kValuesThreads * 8;
+      if (c < p.n_kv * BLOCK)
+        *reinterpret_cast<uint4*>(out + c) =
+            make_uint4(pack_bf16x2(kv8_code(u[j].x, 0) * s[j], kv8_code(u[j].x, 1) * s[j]), pack_bf16x2(kv8_code(u[j].x, 2) * s[j], kv8_code(u[j].x, 3) * s[j]),
+                       pack_bf16x2(kv8_code(u[j].y, 0) * s[j], kv8_code(u[j].y, 1) * s[j]), pack_bf16x2(kv8_code(u[j].y, 2) * s[j], kv8_code(u[j].y, 3) * s[j]));
+    }
   }
 }
 
@@ -202,14 +228,12 @@ extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void
   p.norm_eps = norm_eps;
   p.norm_w_off = norm_w_off;
   p.status = status;
-  // few rows: a row and a head per CTA; many: a tile of 16 rows, in which most runs are whole, and all heads
-  const bool few = M <= 256;
-  p.tile = few ? 1 : 16;
-  const int heads = few ? 1 : n_kv;
-  const dim3 grid((M + p.tile - 1) / p.tile, (n_kv + heads - 1) / heads);
-  const size_t smem = static_cast<size_t>(kStoreRows) * (rot / 2) * sizeof(float2);
-  const cudaError_t e = D == 128 ? launch_pdl(kv8_store_kernel<128>, grid, dim3(kStoreThreads), smem, stream, p, heads)
-                                 : launch_pdl(kv8_store_kernel<64>, grid, dim3(kStoreThreads), smem, stream, p, heads);
+  // a key / value head with its query heads per CTA, and a row or, where there are many, 16, in which most runs are whole
+  p.tile = M <= 256 ? 1 : 16;
+  const dim3 grid((M + p.tile - 1) / p.tile, n_kv);
+  const size_t smem = static_cast<size_t>(kStoreRows) * rot * sizeof(float);
+  const cudaError_t e = D == 128 ? launch_pdl(kv8_store_kernel<128>, grid, dim3(kStoreThreads), smem, stream, p)
+                                 : launch_pdl(kv8_store_kernel<64>, grid, dim3(kStoreThreads), smem, stream, p);
   eredu_count_launches(1);
   return static_cast<int>(e);
 }
@@ -218,7 +242,7 @@ extern "C" int eredu_kv8_values(const void* k_codes, const void* v_codes, const 
                                 const int* pages, const int* seq_lens, const int* cu_q, int* table_out, int rows, int pitch, int wide, int n_kv, int D,
                                 int num_pages, int window, int chunk, int* status, cudaStream_t stream) {
   if (rows <= 0 || wide <= 0) return 0;
-  if (D % 16 != 0 || n_kv <= 0 || rows > 65535 || num_pages <= 0) return -2;
+  if ((D != 64 && D != 128) || n_kv <= 0 || rows > 65535 || num_pages <= 0) return -2;
   Kv8ValuesParams p = {};
   p.k_codes = static_cast<const int8_t*>(k_codes);
   p.v_codes = static_cast<const int8_t*>(v_codes);
@@ -233,12 +257,12 @@ extern "C" int eredu_kv8_values(const void* k_codes, const void* v_codes, const 
   p.pitch = pitch;
   p.wide = wide;
   p.n_kv = n_kv;
-  p.block = kKv8Page * D;
   p.num_pages = num_pages;
   p.window = window;
   p.chunk = chunk;
   p.status = status;
-  const cudaError_t e = launch_pdl(kv8_values_kernel, dim3(wide, rows, 2), dim3(256), 0, stream, p);
+  const cudaError_t e = D == 128 ? launch_pdl(kv8_values_kernel<128>, dim3(wide, rows, 2), dim3(kValuesThreads), 0, stream, p)
+                                 : launch_pdl(kv8_values_kernel<64>, dim3(wide, rows, 2), dim3(kValuesThreads), 0, stream, p);
   eredu_count_launches(1);
   return static_cast<int>(e);
 }

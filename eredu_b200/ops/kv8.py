@@ -13,6 +13,7 @@ makes the scale, and with it the whole block, no number until the block is opene
 """
 from __future__ import annotations
 
+import struct
 from typing import NamedTuple
 
 import torch
@@ -74,25 +75,31 @@ class Pages8(NamedTuple):
 
 
 def check_pages8(k: Pages8, v: Pages8, n_kv: int, head_dim: int) -> None:
+    if type(k) is not Pages8 or type(v) is not Pages8:
+        raise TypeError("keys and values: a pair of Pages8 is expected, both or neither")
+    (kc, ks), (vc, vs) = k, v
+    shape = kc.shape
+    # (one condition for the common case: these checks are a good part of what a short call costs)
+    if (kc.dtype is torch.int8 and vc.dtype is torch.int8 and ks.dtype is torch.float32 and vs.dtype is torch.float32 and vc.shape == shape and len(shape) == 4
+            and shape[1] == n_kv and shape[2] == PAGE and shape[3] == head_dim and ks.shape == shape[:2] and vs.shape == shape[:2]
+            and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+            and kc.get_device() == vc.get_device() == ks.get_device() == vs.get_device() and (head_dim in KV8_HEAD_DIMS or not kc.is_cuda)):
+        return
     for name, t in (("keys", k), ("values", v)):
-        if not isinstance(t, Pages8):
-            raise TypeError(f"{name}: a pair of Pages8 is expected, both or neither")
         if t.codes.dtype != torch.int8 or t.scales.dtype != torch.float32 or tuple(t.codes.shape[1:]) != (n_kv, PAGE, head_dim) \
                 or t.scales.shape != t.codes.shape[:2]:
             raise ValueError(f"{name}: codes {tuple(t.codes.shape)} {t.codes.dtype} with scales {tuple(t.scales.shape)} {t.scales.dtype} are no pages of "
                              f"{n_kv} heads of {head_dim}")
         if not t.codes.is_contiguous() or not t.scales.is_contiguous() or t.scales.device != t.codes.device:
             raise ValueError(f"{name}: codes and scales have to be contiguous and on one device")
-    if k.codes.shape[0] != v.codes.shape[0] or k.device != v.device:
+    if kc.shape[0] != vc.shape[0] or kc.device != vc.device:
         raise ValueError("keys and values have to have the same pages")
-    if k.is_cuda and head_dim not in KV8_HEAD_DIMS:
-        raise NotImplementedError(f"the kernels of 8-bit pages are built for head sizes {KV8_HEAD_DIMS}, not {head_dim}")
+    raise NotImplementedError(f"the kernels of 8-bit pages are built for head sizes {KV8_HEAD_DIMS}, not {head_dim}")
 
 
-def _on(device, **tensors) -> None:
-    for name, (t, dtype) in tensors.items():
-        if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.device != device):
-            raise ValueError(f"{name}: a contiguous {dtype} tensor on {device} is expected, not {t.dtype} on {t.device}")
+def _need(name, t, dtype, device) -> None:
+    if t is not None and (t.dtype is not dtype or not t.is_contiguous() or t.device != device):
+        raise ValueError(f"{name}: a contiguous {dtype} tensor on {device} is expected, not {t.dtype} on {t.device}")
 
 
 # ------------------------------------------------------------------------------------------ writing
@@ -146,7 +153,7 @@ def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
         store_rows_ref(k, slots, k_cache)
         store_rows_ref(v, slots, v_cache)
         return
-    _on(k_cache.device, slots=(slots, torch.int64))
+    _need("slots", slots, torch.int64, k_cache.device)
     k, v = (t if t.dtype == torch.bfloat16 and t.stride()[1:] == (head_dim, 1) and t.stride(0) % 4 == 0 and t.data_ptr() % 8 == 0
             else t.to(torch.bfloat16).contiguous() for t in (k, v))
     _store(None, k.data_ptr(), v.data_ptr(), slots, k_cache, v_cache, None, None, None, 0, n_kv, head_dim, 0, False, 1.0, None, None, 0.0, 0.0,
@@ -163,11 +170,14 @@ def _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, 
         raise ValueError(f"{rot} rotated dims with {inv_freq.numel()} frequencies: a multiple of 8 up to the head size, and half as many frequencies")
     if positions.shape != (M,) or slots.shape != (M,):
         raise ValueError("one position and one slot per row are expected")
-    _on(dev, positions=(positions, torch.int32), slots=(slots, torch.int64), inv_freq=(inv_freq, torch.float32), q_norm_w=(q_norm_w, torch.float32),
-        k_norm_w=(k_norm_w, torch.float32))
+    _need("positions", positions, torch.int32, dev)
+    _need("slots", slots, torch.int64, dev)
+    _need("inv_freq", inv_freq, torch.float32, dev)
     for w in (q_norm_w, k_norm_w):
-        if w is not None and w.numel() != head_dim:
-            raise ValueError(f"a norm has {w.numel()} weights for heads of {head_dim}")
+        if w is not None:
+            _need("norm weights", w, torch.float32, dev)
+            if w.numel() != head_dim:
+                raise ValueError(f"a norm has {w.numel()} weights for heads of {head_dim}")
 
 
 def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
@@ -176,9 +186,9 @@ def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, 
     dev, M = k_cache.codes.device, qkv.shape[0]
     _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, q_norm_w, k_norm_w)
     if q_out is None:
-        q_out = torch.empty((M, n_q, head_dim), dtype=qkv.dtype, device=dev)
+        q_out = qkv.new_empty((M, n_q, head_dim))
     else:
-        _on(dev, q_out=(q_out, qkv.dtype))
+        _need("q_out", q_out, qkv.dtype, dev)
         if q_out.numel() != M * n_q * head_dim:
             raise ValueError(f"q_out has {q_out.numel()} elements for {M} rows of {n_q} heads of {head_dim}")
     ld, at = qkv.stride(0), qkv.data_ptr()
@@ -190,27 +200,29 @@ def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, 
 # ------------------------------------------------------------------------------------------ reading
 def page_values(k_cache: Pages8, v_cache: Pages8, pages):
     """Keys and values of ``pages`` [n] int32 as bf16 [n, heads, 16, head size] each (exact: a code has seven bits)."""
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("keys and values have to have the same pages")
-    check_pages8(k_cache, v_cache, *k_cache.shape[1::2])
-    if not k_cache.is_cuda:
+    if type(k_cache) is not Pages8:
+        raise TypeError("keys and values: a pair of Pages8 is expected")
+    (kc, ks), (vc, vs) = k_cache, v_cache
+    num, n_kv, _, dim = kc.shape
+    check_pages8(k_cache, v_cache, n_kv, dim)
+    if not kc.is_cuda:
         return tuple(t.values(pages.long()).to(torch.bfloat16) for t in (k_cache, v_cache))
-    dev, (num, n_kv, _, dim) = k_cache.device, k_cache.shape
-    _on(dev, pages=(pages, torch.int32))
-    n = pages.shape[0]
-    out = torch.empty((2, n, n_kv, PAGE, dim), dtype=torch.bfloat16, device=dev)
+    dev, n = kc.device, pages.shape[0]
+    _need("pages", pages, torch.int32, dev)
+    out = kc.new_empty((2, n, n_kv, PAGE, dim), dtype=torch.bfloat16)
     if n:
-        half = out.data_ptr()
-        code = lib().eredu_kv8_values(ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), half, half + out.nbytes // 2,
-                                      ptr(pages), None, None, None, 1, n, n, n_kv, dim, num, 0, 0, ptr(status_word(dev)), stream_ptr(dev))
+        at = out.data_ptr()
+        code = lib().eredu_kv8_values(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + 2 * n * n_kv * PAGE * dim, pages.data_ptr(), None, None,
+                                      None, 1, n, n, n_kv, dim, num, 0, 0, status_word(dev).data_ptr(), stream_ptr(dev))
         check(code, "eredu_kv8_values")
-    return out[0], out[1]
+    return out.unbind(0)
 
 
 def _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev):
     if n_q % n_kv:
         raise ValueError(f"{n_q} query heads do not share {n_kv} key / value heads evenly")
-    _on(dev, seq_lens=(seq_lens, torch.int32), sinks=(sinks, torch.float32))
+    _need("seq_lens", seq_lens, torch.int32, dev)
+    _need("sinks", sinks, torch.float32, dev)
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0] \
             or block_table.device != dev:
         raise ValueError("block_table: int32 rows, one per sequence")
@@ -223,7 +235,9 @@ def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_
     n_kv, dev = k_cache.codes.shape[1], k_cache.codes.device
     check_pages8(k_cache, v_cache, n_kv, dim)
     _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev)
-    _on(dev, q=(q, torch.bfloat16), out=(out, torch.bfloat16), cu_q=(cu_q, torch.int32))
+    _need("q", q, torch.bfloat16, dev)
+    _need("out", out, torch.bfloat16, dev)
+    _need("cu_q", cu_q, torch.int32, dev)
     if cu_q is not None and cu_q.shape[0] != seq_lens.shape[0] + 1:
         raise ValueError(f"{cu_q.shape[0]} query offsets for {seq_lens.shape[0]} sequences")
     if out is not None and out.shape != q.shape:
@@ -268,7 +282,7 @@ def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
     M = B * q_per_seq
     _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, dim, rot, q_norm_w, k_norm_w)
     _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev)
-    out = torch.empty((M, n_q, dim), dtype=torch.bfloat16, device=dev)
+    out = qkv.new_empty((M, n_q, dim))
     splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
     code = lib().eredu_attn_kv8_step(qkv.data_ptr(), qkv.stride(0), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(),
                                      v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins,
@@ -329,17 +343,23 @@ def copy_pages(pools, src, dst) -> None:
     """Page ``src[i]`` to page ``dst[i]`` in every layer of every tensor of ``pools``, in one launch (for eight tensors). ``pools``: tensors
     [layers, pages, ...] with pages that are contiguous. ``src``, ``dst``: page numbers on the host, which are checked (in range, no destination twice, none
     that is a source as well), or int32 tensors on the pools' device, for which that is the caller's part (pages out of range are not copied, and reported)."""
-    pools = [t for t in pools]
     if not pools:
         return
     dev, num = pools[0].device, pools[0].shape[1]
+    words = []                  # address, bytes between layers, bytes of a page, layers
     for t in pools:
-        if t.device != dev or t.dim() < 2 or t.shape[1] != num:
+        shape, size = t.shape, t.element_size()
+        if t.device != dev or len(shape) < 2 or shape[1] != num:
             raise ValueError("the pools have to have the same pages, on one device")
-        if not t[0].is_contiguous() if t.shape[0] else False:
+        if not shape[0]:
+            continue
+        if not t.is_contiguous() and not t[0].is_contiguous():
             raise ValueError("the pages of a layer have to be contiguous")
-        if (t[0, 0].numel() if t.shape[0] and num else 0) * t.element_size() % 4 or t.data_ptr() % 4:
+        page = t.stride(1) * size if num > 1 else t[0].numel() * size
+        at = t.data_ptr()
+        if page % 4 or at % 4:
             raise ValueError("pages have to be whole words")
+        words.append((at, t.stride(0) * size, page, shape[0]))
     on_host = [x for x in (src, dst) if not (torch.is_tensor(x) and x.is_cuda)]
     if len(on_host) == 2:
         a, b = ([int(i) for i in (x.tolist() if torch.is_tensor(x) else x)] for x in (src, dst))
@@ -363,13 +383,11 @@ def copy_pages(pools, src, dst) -> None:
     if on_host:
         both = _page_list(src + dst, dev)
         src, dst = both[:len(src)], both[len(src):]
-    if src.shape[0] == 0:
+    n = src.shape[0]
+    if n == 0:
         return
-    import ctypes
-
-    for i in range(0, len(pools), 8):
-        part = [t for t in pools[i:i + 8] if t.shape[0]]
-        words = [w for t in part for w in (t.data_ptr(), t.stride(0) * t.element_size(), t[0, 0].numel() * t.element_size(), t.shape[0])]
-        code = lib().eredu_copy_pages((ctypes.c_longlong * len(words))(*words), len(part), src.data_ptr(), dst.data_ptr(), src.shape[0], num,
-                                      ptr(status_word(dev)), stream_ptr(dev))
+    for i in range(0, len(words), 8):
+        part = words[i:i + 8]
+        code = lib().eredu_copy_pages(struct.pack(f"{4 * len(part)}q", *(w for t in part for w in t)), len(part), src.data_ptr(), dst.data_ptr(), n, num,
+                                      status_word(dev).data_ptr(), stream_ptr(dev))
         check(code, "eredu_copy_pages")
