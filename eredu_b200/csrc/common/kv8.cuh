@@ -26,9 +26,12 @@ __device__ __forceinline__ float kv8_inverse(float scale) {
   const uint32_t u = __float_as_uint(scale);
   return u >= 0x7f800000u ? scale : __uint_as_float(0x7f000000u - u);
 }
-__device__ __forceinline__ uint32_t kv8_pack(float a, float b, float c, float d) {
-  const int i = __float2int_rn(a), j = __float2int_rn(b), k = __float2int_rn(c), l = __float2int_rn(d);
-  return (i & 0xff) | (j & 0xff) << 8 | (k & 0xff) << 16 | static_cast<uint32_t>(l) << 24;
+// Codes of four values times `inv`, a power of two: the sum with 1.5 * 2^23 rounds to a whole number, ties to even, and ends in its byte.
+__device__ __forceinline__ uint32_t kv8_pack(float a, float b, float c, float d, float inv) {
+  constexpr float kWhole = 12582912.f;
+  const uint32_t i = __float_as_uint(fmaf(a, inv, kWhole)), j = __float_as_uint(fmaf(b, inv, kWhole)), k = __float_as_uint(fmaf(c, inv, kWhole)),
+                 l = __float_as_uint(fmaf(d, inv, kWhole));
+  return __byte_perm(__byte_perm(i, j, 0x0040), __byte_perm(k, l, 0x0040), 0x5410);
 }
 __device__ __forceinline__ float kv8_code(uint32_t word, int i) { return static_cast<float>(static_cast<int8_t>(word >> (8 * i))); }
 

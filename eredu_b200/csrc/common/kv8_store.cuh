@@ -36,8 +36,8 @@ __device__ __forceinline__ float4 load_row4(const __nv_bfloat16* row, int lane) 
   const uint2 u = *reinterpret_cast<const uint2*>(row + 4 * (lane & (D / 4 - 1)));
   return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
 }
-// The D / 4 lanes of a row together: norm, then rotation. `turns`: rot / 2 cosines of the row's angles, then as many sines.
-template <int D>
+// The D / 4 lanes of a row together: norm, then rotation. WHOLE: all of a row is rotated, in halves, and nothing of that is asked at run time. `turns`: rot / 2 cosines of the row's angles, then as many sines.
+template <int D, bool WHOLE>
 __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, const float* w, const float* turns, int lane) {
   const int d = 4 * (lane & (D / 4 - 1));
   if (w != nullptr) {
@@ -50,14 +50,23 @@ __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, co
     x.z *= inv * (w[d + 2] + p.norm_w_off);
     x.w *= inv * (w[d + 3] + p.norm_w_off);
   }
-  if (p.rot == 0) return x;
-  const int half = p.rot / 2;
-  if (p.interleaved) {
+  if (!WHOLE && p.rot == 0) return x;
+  const int rot = WHOLE ? D : p.rot, half = rot / 2;
+  if (!WHOLE && p.interleaved) {
     if (d < p.rot) {
       const float2 c = *reinterpret_cast<const float2*>(turns + d / 2), n = *reinterpret_cast<const float2*>(turns + half + d / 2);
       x = make_float4(x.x * c.x - x.y * n.x, x.y * c.x + x.x * n.x, x.z * c.y - x.w * n.y, x.w * c.y + x.z * n.y);
     }
     return x;
+  }
+  if (WHOLE) {
+    const float4 o = make_float4(__shfl_xor_sync(0xffffffffu, x.x, D / 8), __shfl_xor_sync(0xffffffffu, x.y, D / 8), __shfl_xor_sync(0xffffffffu, x.z, D / 8),
+                                 __shfl_xor_sync(0xffffffffu, x.w, D / 8));
+    const int i = d & (D / 2 - 1);
+    const float4 c = *reinterpret_cast<const float4*>(turns + i);
+    float4 n = *reinterpret_cast<const float4*>(turns + D / 2 + i);
+    if (d < D / 2) n = make_float4(-n.x, -n.y, -n.z, -n.w);
+    return make_float4(x.x * c.x + o.x * n.x, x.y * c.y + o.y * n.y, x.z * c.z + o.z * n.z, x.w * c.w + o.w * n.w);
   }
   const int from = d < half ? lane + half / 4 : d < p.rot ? lane - half / 4 : lane;
   const float4 o = make_float4(__shfl_sync(0xffffffffu, x.x, from), __shfl_sync(0xffffffffu, x.y, from), __shfl_sync(0xffffffffu, x.z, from),
@@ -73,7 +82,7 @@ __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, co
 
 // Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on. SHARE warps together (`part` of them; 1: a warp by itself);
 // `tops` has a word for each, and all threads of the CTA are here then.
-template <int D, bool KEYS, int SHARE>
+template <int D, bool KEYS, int SHARE, bool WHOLE>
 __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, int part,
                                             uint32_t* tops) {
   constexpr int RPI = 128 / D;              // rows a warp holds at once
@@ -96,7 +105,7 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
     if (i * RPI * SHARE + part * RPI >= n) break;
     const int r = i * RPI * SHARE + sub;
     if (KEYS) {
-      const float4 y = prepared<D>(p, x[i], p.k_norm_w, turns + min(r, n - 1) * p.rot, lane);
+      const float4 y = prepared<D, WHOLE>(p, x[i], p.k_norm_w, turns + min(r, n - 1) * (WHOLE ? D : p.rot), lane);
       if (r < n) x[i] = y;
     }
     top = max(max(top, __float_as_uint(fabsf(x[i].x))), __float_as_uint(fabsf(x[i].y)));
@@ -118,13 +127,13 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
     for (int r = sub; r < first; r += RPI * SHARE) {
       uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + c);
       const uint32_t u = *w;
-      *w = kv8_pack(kv8_code(u, 0) * ratio, kv8_code(u, 1) * ratio, kv8_code(u, 2) * ratio, kv8_code(u, 3) * ratio);
+      *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), ratio);
     }
   }
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int r = i * RPI * SHARE + sub;
-    if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x[i].x * inv, x[i].y * inv, x[i].z * inv, x[i].w * inv);
+    if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x[i].x, x[i].y, x[i].z, x[i].w, inv);
   }
   if (SHARE > 1) __syncthreads();   // the words, and the scale that others may still be reading
   if (lane == 0 && part == 0) *at = scale;

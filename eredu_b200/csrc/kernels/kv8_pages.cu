@@ -20,7 +20,7 @@ constexpr int kStoreThreads = 256, kStoreShare = kStoreThreads / 64;   // half o
 constexpr int kStoreRows = 32;      // a tile of 16 rows and what the last run of it has behind them
 
 // grid (tiles of rows, n_kv)
-template <int D>
+template <int D, bool WHOLE>
 __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams p) {
   constexpr int RPI = 128 / D;
   extern __shared__ __align__(16) float turns[];          // [rows of the tile and the last run][rot / 2 cosines, rot / 2 sines]
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams
   pdl_wait();
   pdl_launch_dependents();
   const int row0 = blockIdx.x * p.tile, rows = min(p.tile, p.M - row0), h0 = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.rot / 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rot = WHOLE ? D : p.rot, half = rot / 2;
   if (warp == 0) {
     // lane r has the slots of rows r - 1 and r of the tile and the 16 behind it: a row continues the one in front where its slot is the next of the same page
     const int r = row0 + lane;
@@ -61,14 +61,14 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams
   }
   __syncthreads();
   for (int r = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); r < behind; r += kStoreThreads / (D / 2))
-    if (i < half) turn_of(p.positions[row0 + r], p.inv_freq[i], p.attn_factor, turns[r * p.rot + i], turns[r * p.rot + half + i]);
+    if (i < half) turn_of(p.positions[row0 + r], p.inv_freq[i], p.attn_factor, turns[r * rot + i], turns[r * rot + half + i]);
   __syncthreads();
   for (int i = 0; i < runs; ++i) {
     const int at = run_row[i];
     const long long cell = (run_slot[i] >> 4) * p.n_kv + h0;
     const int first = static_cast<int>(run_slot[i] & 15);
-    if (warp < kStoreShare) store_block<D, true, kStoreShare>(p, row0 + at, run_len[i], first, cell, h0, turns + at * p.rot, lane, warp, tops);
-    else store_block<D, false, kStoreShare>(p, row0 + at, run_len[i], first, cell, h0, turns, lane, warp - kStoreShare, tops + kStoreShare);
+    if (warp < kStoreShare) store_block<D, true, kStoreShare, WHOLE>(p, row0 + at, run_len[i], first, cell, h0, turns + at * rot, lane, warp, tops);
+    else store_block<D, false, kStoreShare, WHOLE>(p, row0 + at, run_len[i], first, cell, h0, turns, lane, warp - kStoreShare, tops + kStoreShare);
   }
   // ---- query rows of this head, four at a time on their way
   constexpr int WARPS = kStoreThreads / 32, DEEP = 4;
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams
     for (int j = 0; j < DEEP; ++j) {
       const int item = i0 + j * WARPS * RPI + sub, r = static_cast<int>(min(item, items - 1) * per_mine >> 20), head = h0 * mine + min(item, items - 1) - r * mine;
       if (i0 + j * WARPS * RPI >= items) break;
-      const float4 x = prepared<D>(p, query[j], p.q_norm_w, turns + r * p.rot, lane);
+      const float4 x = prepared<D, WHOLE>(p, query[j], p.q_norm_w, turns + r * rot, lane);
       if (item < items)
         *reinterpret_cast<uint2*>(p.q_out + (static_cast<size_t>(row0 + r) * p.n_q + head) * D + 4 * (lane & (D / 4 - 1))) =
             make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
@@ -232,8 +232,11 @@ extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void
   p.tile = M <= 256 ? 1 : 16;
   const dim3 grid((M + p.tile - 1) / p.tile, n_kv);
   const size_t smem = static_cast<size_t>(kStoreRows) * rot * sizeof(float);
-  const cudaError_t e = D == 128 ? launch_pdl(kv8_store_kernel<128>, grid, dim3(kStoreThreads), smem, stream, p)
-                                 : launch_pdl(kv8_store_kernel<64>, grid, dim3(kStoreThreads), smem, stream, p);
+  const bool whole = rot == D && interleaved == 0;
+  const cudaError_t e = D == 128 ? (whole ? launch_pdl(kv8_store_kernel<128, true>, grid, dim3(kStoreThreads), smem, stream, p)
+                                          : launch_pdl(kv8_store_kernel<128, false>, grid, dim3(kStoreThreads), smem, stream, p))
+                                 : (whole ? launch_pdl(kv8_store_kernel<64, true>, grid, dim3(kStoreThreads), smem, stream, p)
+                                          : launch_pdl(kv8_store_kernel<64, false>, grid, dim3(kStoreThreads), smem, stream, p));
   eredu_count_launches(1);
   return static_cast<int>(e);
 }
