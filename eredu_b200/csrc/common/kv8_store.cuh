@@ -7,7 +7,8 @@ namespace eredu {
 
 struct Kv8StoreParams {
   const __nv_bfloat16 *q, *k, *v;   // [M, heads, D], rows of ld_q, ld_k, ld_v elements
-  __nv_bfloat16* q_out;             // [M, n_q, D]
+  void* q_out;                      // [M, n_q, D] bf16, or fp32
+  int q_out_fp32;
   int8_t *k_codes, *v_codes;        // [pages, n_kv, 16, D]
   float *k_scales, *v_scales;       // [pages, n_kv]
   const int* positions;             // [M]
@@ -80,8 +81,19 @@ __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, co
   return x;
 }
 
-// Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on. SHARE warps together (`part` of them; 1: a warp by itself);
-// `tops` has a word for each, and all threads of the CTA are here then.
+// The scale of a block whose new rows have the largest magnitude `top` (as bits); `before`: that of the rows in front, if any. The larger of the two, and what is
+// no number stays none.
+__device__ __forceinline__ float kv8_raised(uint32_t top, int first, float before) {
+  const float scale = kv8_needed(__uint_as_float(top));
+  return first > 0 && !(before <= scale) ? (scale != scale ? scale : before) : scale;
+}
+__device__ __forceinline__ uint32_t kv8_top(uint32_t top, float4 x) {
+  top = max(max(top, __float_as_uint(fabsf(x.x))), __float_as_uint(fabsf(x.y)));
+  return max(max(top, __float_as_uint(fabsf(x.z))), __float_as_uint(fabsf(x.w)));
+}
+
+// Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on. SHARE warps together, all threads of the CTA; `part`: which of them
+// this is, `tops`: a word for each.
 template <int D, bool KEYS, int SHARE, bool WHOLE>
 __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, int part,
                                             uint32_t* tops) {
@@ -108,18 +120,14 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
       const float4 y = prepared<D, WHOLE>(p, x[i], p.k_norm_w, turns + min(r, n - 1) * (WHOLE ? D : p.rot), lane);
       if (r < n) x[i] = y;
     }
-    top = max(max(top, __float_as_uint(fabsf(x[i].x))), __float_as_uint(fabsf(x[i].y)));
-    top = max(max(top, __float_as_uint(fabsf(x[i].z))), __float_as_uint(fabsf(x[i].w)));
+    top = kv8_top(top, x[i]);
   }
   top = __reduce_max_sync(0xffffffffu, top);
-  if (SHARE > 1) {
-    if (lane == 0) tops[part] = top;
-    __syncthreads();
+  if (lane == 0) tops[part] = top;
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < SHARE; ++i) top = max(top, tops[i]);
-  }
-  float scale = kv8_needed(__uint_as_float(top));
-  if (first > 0 && !(before <= scale)) scale = scale != scale ? scale : before;   // the larger, and what is no number stays none
+  for (int i = 0; i < SHARE; ++i) top = max(top, tops[i]);
+  const float scale = kv8_raised(top, first, before);
   const float inv = kv8_inverse(scale);
   const int c = 4 * (lane & (D / 4 - 1));
   if (first > 0 && scale != before) {
@@ -135,8 +143,42 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
     const int r = i * RPI * SHARE + sub;
     if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x[i].x, x[i].y, x[i].z, x[i].w, inv);
   }
-  if (SHARE > 1) __syncthreads();   // the words, and the scale that others may still be reading
+  __syncthreads();   // the words, and the scale that others may still be reading
   if (lane == 0 && part == 0) *at = scale;
+}
+
+// The same for a few rows by one warp that has other things in its registers: the rows are looked at twice.
+template <int D, bool KEYS>
+__device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane) {
+  constexpr int RPI = 128 / D;
+  int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
+  float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
+  const int sub = RPI == 1 ? 0 : lane >> 4, c = 4 * (lane & (D / 4 - 1));
+  auto row_of = [&](int r) {
+    const int in = min(r, n - 1);
+    float4 x = load_row4<D>((KEYS ? p.k : p.v) + static_cast<size_t>(row + in) * (KEYS ? p.ld_k : p.ld_v) + h * D, lane);
+    return KEYS ? prepared<D, false>(p, x, p.k_norm_w, turns + in * p.rot, lane) : x;
+  };
+  const float before = first > 0 ? *at : 0.f;
+  uint32_t top = 0;
+#pragma unroll 1
+  for (int r = sub; r - sub < n; r += RPI) top = kv8_top(top, row_of(r));
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float scale = kv8_raised(top, first, before), inv = kv8_inverse(scale);
+  if (first > 0 && scale != before) {
+#pragma unroll 1
+    for (int r = sub; r < first; r += RPI) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + c);
+      const uint32_t u = *w;
+      *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), before * inv);
+    }
+  }
+#pragma unroll 1
+  for (int r = sub; r - sub < n; r += RPI) {
+    const float4 x = row_of(r);
+    if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x.x, x.y, x.z, x.w, inv);
+  }
+  if (lane == 0) *at = scale;
 }
 
 }  // namespace eredu

@@ -22,12 +22,13 @@
 #include "../common/trace.cuh"
 
 extern "C" int eredu_kv8_store(const void*, const void*, const void*, void*, void*, void*, float*, float*, const int*, const long long*, const float*, const float*,
-                               const float*, int, int, int, int, int, int, int, int, int, int, float, float, float, int*, cudaStream_t);
+                               const float*, int, int, int, int, int, int, int, int, int, int, int, float, float, float, int*, cudaStream_t);
 
 namespace eredu {
 
 struct AttnKv8Params {
-  const __nv_bfloat16* q;          // [B * q_per_seq] rows of ld_q elements, n_q heads of D
+  const __nv_bfloat16* q;          // [B * q_per_seq] rows of ld_q elements, n_q heads of D; or
+  const float* q32;                // the same in 32 bits
   const int8_t *k_codes, *v_codes; // [pages, n_kv, 16, D]
   const float *k_scales, *v_scales;
   __nv_bfloat16* out;              // [B * q_per_seq, n_q, D]
@@ -42,10 +43,9 @@ struct AttnKv8Params {
   uint32_t per_group;              // 2^32 / (n_q / n_kv), rounded up; 0 for a group of one
   float scale_log2;
   int* status;
-  // A step from the projection's output (st.q = q, st.k, st.v in the same rows): queries are normalised and rotated as they are read and, `append`, the CTA
-  // that has the page of a new token writes its rows there.
+  // A step from the projection's output (q, st.k and st.v in the same rows): queries are normalised and rotated as they are read, and the CTA that has the
+  // page of a new token writes its rows there.
   Kv8StoreParams st;
-  int append;
 };
 // Token of query row r among those that share a key / value head (r < 2^16: exact), in place of a division of some thirty instructions.
 __device__ __forceinline__ int kv8_token(const AttnKv8Params& p, int r) { return p.per_group == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.per_group)); }
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     }
   };
   // a pair that new rows are written to is fetched behind the write
-  const int new_page = STEP && p.append ? pos_new / kKv8Page : 0x7fffffff;
+  const int new_page = STEP ? pos_new / kKv8Page : 0x7fffffff;
   auto waits = [&](int turn) { return STEP && page0 + 2 * (warp + kKv8Warps * turn) + 1 >= new_page; };
   if (turns > 0 && !waits(0)) fetch(0);
   cp_async_commit();
@@ -316,23 +316,21 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       if (i < half) turn_of(positions[n], p.st.inv_freq[i], p.st.attn_factor, turns_s[n * p.st.rot + i], turns_s[n * p.st.rot + half + i]);
     __syncthreads();
     // ---- the new rows of pages in this part: a warp for the keys or the values of a page (there are two such pages at most)
-    if (p.append) {
-      const int page = max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) + (warp >> 1);
-      if (page < page1) {
-        const int first = max(0, page * kKv8Page - pos_new), end_row = min(p.q_per_seq, (page + 1) * kKv8Page - pos_new), row0 = b * p.q_per_seq;
-        for (int r = first; r < end_row;) {
-          const long long to = p.st.slots[row0 + r];
-          int n = 1;
-          if (to >= 0 && (to >> 4) < p.num_pages) {
-            while (r + n < end_row && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
-            const long long cell = (to >> 4) * p.n_kv + kvh;
-            if ((warp & 1) == 0) store_block<D, true, 1, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * p.st.rot, lane, 0, nullptr);
-            else store_block<D, false, 1, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane, 0, nullptr);
-          } else if (to >= 0) {
-            report_status(p.status, kStatusBadArgument);
-          }
-          r += n;
+    const int page = max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) + (warp >> 1);
+    if (page < page1) {
+      const int first = max(0, page * kKv8Page - pos_new), end_row = min(p.q_per_seq, (page + 1) * kKv8Page - pos_new), row0 = b * p.q_per_seq;
+      for (int r = first; r < end_row;) {
+        const long long to = p.st.slots[row0 + r];
+        int n = 1;
+        if (to >= 0 && (to >> 4) < p.num_pages) {
+          while (r + n < end_row && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
+          const long long cell = (to >> 4) * p.n_kv + kvh;
+          if ((warp & 1) == 0) store_few<D, true>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * p.st.rot, lane);
+          else store_few<D, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane);
+        } else if (to >= 0) {
+          report_status(p.status, kStatusBadArgument);
         }
+        r += n;
       }
     }
   }
@@ -342,7 +340,8 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int r = r0 + min((i * kKv8Warps + warp) * RPI + lane / (D / 4), rows - 1), token = kv8_token(p, r);
-    query[i] = load_row4<D>(p.q + static_cast<size_t>(b * p.q_per_seq + token) * p.ld_q + (kvh * group + r - token * group) * D, lane);
+    const size_t at = static_cast<size_t>(b * p.q_per_seq + token) * p.ld_q + (kvh * group + r - token * group) * D;
+    query[i] = !STEP && p.q32 != nullptr ? *reinterpret_cast<const float4*>(p.q32 + at + lane % (D / 4) * 4) : load_row4<D>(p.q + at, lane);
   }
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     if (c == 0) back_s[row] = fine ? p.scale_log2 * exp2_of(-up0) * exp2_of(up0 - up) : __uint_as_float(0x7fc00000u);
   }
   __syncthreads();
-  if (STEP && p.append) {
+  if (STEP) {
     const bool first = turns > 0 && waits(0), second = turns > 1 && waits(1);
     const int pg = page0 + 2 * (warp + kKv8Warps * (lane >> 1)) + (lane & 1);
     if (turns > 0 && !first && pg >= new_page && pg < page1) {   // looked up in front of the write
@@ -847,21 +846,31 @@ extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const v
   return attn_kv8(p, D, ctas, false, stream);
 }
 
-// The same from the projection's output qkv, rows [q heads | k heads | v heads] x D of ld elements. The attention kernel writes the new rows itself where
-// one tile holds all query rows of a head, so that one CTA has a page; else eredu_kv8_store goes in front.
-extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, void* k_codes, void* v_codes, float* k_scales, float* v_scales, void* out, const int* block_table,
+// The same from the projection's output qkv, rows [q heads | k heads | v heads] x D of ld elements. The attention kernel rotates queries and writes the new
+// rows itself where one tile holds all query rows of a head, so that one CTA has a page; else eredu_kv8_store goes in front and leaves the queries in
+// q32 [batch * q_per_seq, n_q, D] (four sequences of 3000 tokens, five new ones, 32 heads over 4: 18 us; rotated in each of three tiles 20).
+extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, float* q32, void* k_codes, void* v_codes, float* k_scales, float* v_scales, void* out, const int* block_table,
                                    const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, const int* positions,
                                    const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int batch, int q_per_seq,
                                    int max_pages, int num_pages, int n_q, int n_kv, int D, int rot, int interleaved, int splits, int ctas, int window, int chunk,
                                    float scale, float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
   if (batch <= 0) return 0;
   if (n_kv <= 0 || n_q <= 0 || n_q % n_kv != 0 || q_per_seq <= 0 || rot < 0 || rot > D || rot % 8 != 0) return -2;
-  const int group = n_q / n_kv, rows = q_per_seq * group;
-  if (group == 1 && rows > kKv8StepTokens) return -2;
+  const int group = n_q / n_kv;
+  const bool own = q_per_seq * group <= 16 && q_per_seq <= kKv8StepTokens;
+  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(qkv);
   AttnKv8Params p = attn_kv8_params(qkv, ld, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
                                     max_pages, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
-  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(qkv);
-  p.append = rows <= 16;
+  if (!own) {
+    if (q32 == nullptr) return -2;
+    const int e = eredu_kv8_store(qkv, row + n_q * D, row + (n_q + n_kv) * D, q32, k_codes, v_codes, k_scales, v_scales, positions, slots, inv_freq, q_norm_w,
+                                  k_norm_w, batch * q_per_seq, ld, ld, ld, n_q, n_kv, D, rot, interleaved, num_pages, 1, attn_factor, norm_eps, norm_w_off, status,
+                                  stream);
+    if (e != 0) return e;
+    p.q32 = q32;
+    p.ld_q = n_q * D;
+    return attn_kv8(p, D, ctas, false, stream);
+  }
   p.st.k = row + n_q * D;
   p.st.v = row + (n_q + n_kv) * D;
   p.st.ld_k = p.st.ld_v = ld;
@@ -879,10 +888,5 @@ extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, void* k_codes, void*
   p.st.attn_factor = attn_factor;
   p.st.norm_eps = norm_eps;
   p.st.norm_w_off = norm_w_off;
-  if (!p.append) {
-    const int e = eredu_kv8_store(nullptr, p.st.k, p.st.v, nullptr, k_codes, v_codes, k_scales, v_scales, positions, slots, inv_freq, nullptr, k_norm_w,
-                                  batch * q_per_seq, 0, ld, ld, n_q, n_kv, D, rot, interleaved, num_pages, attn_factor, norm_eps, norm_w_off, status, stream);
-    if (e != 0) return e;
-  }
   return attn_kv8(p, D, ctas, true, stream);
 }

@@ -89,9 +89,10 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams
       const int item = i0 + j * WARPS * RPI + sub, r = static_cast<int>(min(item, items - 1) * per_mine >> 20), head = h0 * mine + min(item, items - 1) - r * mine;
       if (i0 + j * WARPS * RPI >= items) break;
       const float4 x = prepared<D, WHOLE>(p, query[j], p.q_norm_w, turns + r * rot, lane);
-      if (item < items)
-        *reinterpret_cast<uint2*>(p.q_out + (static_cast<size_t>(row0 + r) * p.n_q + head) * D + 4 * (lane & (D / 4 - 1))) =
-            make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+      const size_t at = (static_cast<size_t>(row0 + r) * p.n_q + head) * D + 4 * (lane & (D / 4 - 1));
+      if (item >= items) continue;
+      if (p.q_out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.q_out) + at) = x;
+      else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.q_out) + at) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
     }
   }
 }
@@ -195,8 +196,8 @@ using namespace eredu;
 
 extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void* q_out, void* k_codes, void* v_codes, float* k_scales, float* v_scales,
                                const int* positions, const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int M,
-                               int ld_q, int ld_k, int ld_v, int n_q, int n_kv, int D, int rot, int interleaved, int num_pages, float attn_factor,
-                               float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
+                               int ld_q, int ld_k, int ld_v, int n_q, int n_kv, int D, int rot, int interleaved, int num_pages, int q_out_fp32,
+                               float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
   if (M <= 0) return 0;
   if ((D != 64 && D != 128) || n_kv <= 0 || num_pages <= 0 || rot < 0 || rot > D || rot % 8 != 0 || ld_q % 4 != 0 || ld_k % 4 != 0 || ld_v % 4 != 0 ||
       (q_out != nullptr && (n_q <= 0 || n_q % n_kv != 0)))
@@ -205,7 +206,8 @@ extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
-  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.q_out = q_out;
+  p.q_out_fp32 = q_out_fp32;
   p.k_codes = static_cast<int8_t*>(k_codes);
   p.v_codes = static_cast<int8_t*>(v_codes);
   p.k_scales = k_scales;

@@ -752,7 +752,7 @@ def attention_decode_rope(qkv, k_cache, v_cache, block_table, seq_lens, q_per_se
     if isinstance(k_cache, Pages8):
         if norm_whole or value_norm or not append or value_dim != head_dim:
             raise NotImplementedError("8-bit pages: norms per head, values as wide as keys, and rows that are appended")
-        if qkv.is_cuda and positions.dim() == 1 and (n_q > n_kv or q_per_seq <= FUSED_ROPE_MAX_NEW):
+        if qkv.is_cuda and positions.dim() == 1:
             return attention_step8(qkv, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, positions, slots, inv_freq, n_q, n_kv, head_dim,
                                    rot or head_dim, interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, splits, window, sinks, chunk)
         q = rope_kv(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off)

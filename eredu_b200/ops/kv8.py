@@ -38,10 +38,10 @@ def _sm_count(device) -> int:
 
 
 P, I, F = native.P, native.I, native.F
-native.register("eredu_kv8_store", I, [P] * 13 + [I] * 10 + [F] * 3 + [P] * 2)
+native.register("eredu_kv8_store", I, [P] * 13 + [I] * 11 + [F] * 3 + [P] * 2)
 native.register("eredu_kv8_values", I, [P] * 10 + [I] * 8 + [P] * 2)
 native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 11 + [F] + [P] * 2)
-native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 16 + [I] * 13 + [F] * 4 + [P] * 2)
+native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 17 + [I] * 13 + [F] * 4 + [P] * 2)
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 
@@ -138,7 +138,7 @@ def _store(q, k, v, slots, k_cache, v_cache, q_out, positions, inv_freq, n_q, n_
     dev = k_cache.device
     code = lib().eredu_kv8_store(q, k, v, ptr(q_out), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), ptr(positions),
                                  ptr(slots), ptr(inv_freq), ptr(q_norm_w), ptr(k_norm_w), slots.shape[0], ld[0], ld[1], ld[2], n_q, n_kv, head_dim, rot,
-                                 1 if interleaved else 0, k_cache.codes.shape[0], attn_factor, norm_eps, norm_w_off, ptr(status_word(dev)), stream_ptr(dev))
+                                 1 if interleaved else 0, k_cache.codes.shape[0], 0, attn_factor, norm_eps, norm_w_off, ptr(status_word(dev)), stream_ptr(dev))
     check(code, "eredu_kv8_store")
 
 
@@ -283,8 +283,10 @@ def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
     _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, dim, rot, q_norm_w, k_norm_w)
     _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev)
     out = qkv.new_empty((M, n_q, dim))
-    splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
-    code = lib().eredu_attn_kv8_step(qkv.data_ptr(), qkv.stride(0), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(),
+    rows = q_per_seq * (n_q // n_kv)
+    splits, ctas, part, part_o, part_ml, joins = _shares(splits, rows, dim, dev)
+    q32 = torch.empty(M * n_q * dim, dtype=torch.float32, device=dev) if rows > 16 or q_per_seq > 8 else None
+    code = lib().eredu_attn_kv8_step(qkv.data_ptr(), qkv.stride(0), ptr(q32), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(),
                                      v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins,
                                      positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), B, q_per_seq,
                                      block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window),
