@@ -298,18 +298,24 @@ def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
 def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     """Split factor of the decode kernel for 8-bit pages: 1 to 8 CTAs for a sequence and head, or 0 for even shares.
 
-    Three CTAs fit an SM, clusters not quite: as many splits as find room on nine tenths of that, with a pair of pages for each of a CTA's four warps. Even
-    shares cost a second kernel and the way to a CTA's place, 3 to 5 us, and pay where clusters leave SMs empty and a CTA has many pairs (us, 32 heads of 128 over 8, even /
-    best cluster: one sequence of 8192 tokens 16 / 14, of 32768 22 / 33; four of 32768 47 / 52; eight of 8192 28 / 26, of 32768 85 / 88; 16 of 8192 both 44).
-    More sequences and heads than the SMs have room for go one CTA each, or three where sequences are long enough for their tail to count (us with 1 / 3 / even:
-    32 of 512 10.0 / 15.2 / 15.4; 64 of 2048 44 / 48 / 45; 64 of 8192 154 / 138 / 144)."""
+    Three CTAs fit an SM, clusters not quite: as many splits as find room on nine tenths of that (two where that is all), with a pair of pages for each of a CTA's
+    four warps. Even shares cost a second kernel and the way to a CTA's place, 3 to 5 us, and pay where clusters leave SMs empty and a CTA has many pairs (us, 32
+    heads of 128 over 8, even / best cluster: one sequence of 8192 tokens 16 / 14, of 32768 22 / 33; four of 32768 47 / 52; eight of 8192 28 / 26, of 32768
+    85 / 88; 20 of 8192 50 / 53).
+    More sequences and heads than that go one CTA each, or, where they are long enough for the tail of the longest to count, two or three or even shares
+    (us with 1 / 2 / 3 / even: 32 of 1024 15 / 18 / 18 / 18, of 4096 48 / 47 / 43 / 44, of 8192 84 / 86 / 74 / 73; 64 of 2048 43 / 44 / 48 / 44, of 4096 77 / 73 / 76 / 74,
+    of 8192 152 / 141 / 136 / 142, with four new tokens 176 / 156 / 159 / 154)."""
     tiles = -(-max(rows, 1) // (8 if rows <= 8 else 16))
     heads = max(1, batch * n_kv * tiles)
     pairs = max(1, -(-max_kv_len // (2 * PAGE)))
     room = EVEN_CTAS * sm_count
-    if heads * 20 > room * 9:
-        return 1 if pairs < 64 or heads > 3 * room else 3 if pairs < 384 else 0
-    splits = max(1, min(room * 9 // 10 // heads, pairs // 4, CLUSTER))
+    if heads > room // 2 + 2:
+        if pairs < 96:
+            return 1
+        if pairs < 192:
+            return 3 if 3 * heads <= 2 * room else 2
+        return 3 if heads > room and rows <= 8 else 0
+    splits = max(1, min(max(2, room * 9 // 10 // heads), pairs // 4, CLUSTER))
     if splits == 7:             # six or eight fill a GPC better
         splits = 6
     return 0 if pairs > 96 * splits else splits
