@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import native
-from .kv8 import Pages8, attention_decode8, attention_step8, check_attention8, decode_splits8, gather_values, rope_kv8, store_kv
+from .kv8 import Pages8, attention_decode8, attention_prefill8, attention_step8, decode_splits8, rope_kv8, store_kv
 from .native import check, lib, ptr, status_word, stream_ptr
 
 PAGE = 16
@@ -612,7 +612,7 @@ def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_le
     Caches of :class:`Pages8`: the pages that some query sees are brought to bf16 first - once for all query tiles and heads that read them -, in memory
     that the call allocates (``max_kv_len`` bounds it, and then has to be that of the longest sequence at least)."""
     if isinstance(k_cache, Pages8) and q.is_cuda:
-        return _attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len)
+        return attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
         if not _tensor_core_dims(q, k_cache, v_cache):
             return _attention_simt(q, k_cache, v_cache, block_table, seq_lens, cu_q, 0, max_q_len, scale, window, chunk, sinks)
@@ -641,16 +641,6 @@ def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_le
                                     k_cache.shape[1], q.shape[2], window, scale, stream_ptr(q.device))
     check(code, "eredu_attn_prefill")
     return out
-
-
-def _attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len):
-    check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q)
-    if out is None:
-        out = torch.empty_like(q)
-    if q.shape[0] == 0 or seq_lens.shape[0] == 0:
-        return out
-    k, v, table = gather_values(k_cache, v_cache, block_table, seq_lens, cu_q, max_kv_len, window, chunk)
-    return attention_prefill(q, k, v, table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len)
 
 
 import os as _os

@@ -321,22 +321,35 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     return 0 if pairs > 96 * splits else splits
 
 
-def gather_values(k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_kv_len, window, chunk):
-    """The pages that some query sees, as bf16 pages of their own, and the block table that finds them: (keys, values, table). Entries of the
-    table that nobody sees point behind the last page, where the tensor maps of prefill attention read zeros; rows of eight pages, a key tile."""
-    dev, B = k_cache.device, seq_lens.shape[0]
-    num, n_kv, _, dim = k_cache.shape
+def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len):
+    """The form of :func:`.core.attention_prefill` for 8-bit pages on a GPU. The pages that some query sees are brought to bf16, in pages and a block table of
+    their own, and the prefill kernel reads these: once for all query tiles and heads that share them, where a kernel that reads codes would convert
+    each tile again for every one of them. Entries of that table that nobody sees point behind the last page, where the kernel's tensor maps read
+    zeros; its rows are whole key tiles of eight pages."""
+    check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q)
+    (kc, ks), (vc, vs) = k_cache, v_cache
+    dev, B, (total, n_q, dim) = q.device, seq_lens.shape[0], q.shape
+    num, n_kv = kc.shape[:2]
+    if out is None:
+        out = torch.empty_like(q)
+    if total == 0 or B == 0:
+        return out
     wide = block_table.shape[1]
     if max_kv_len > 0:
         wide = min(wide, -(-max_kv_len // PAGE))
     wide = -(-wide // 8) * 8
-    out = torch.empty((2, B * wide, n_kv, PAGE, dim), dtype=torch.bfloat16, device=dev)
-    table = torch.empty((B, wide), dtype=torch.int32, device=dev)
-    code = lib().eredu_kv8_values(ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
-                                  out.data_ptr() + out.nbytes // 2, ptr(block_table), ptr(seq_lens), ptr(cu_q), ptr(table), B, block_table.stride(0), wide,
-                                  n_kv, dim, num, int(window), int(chunk), ptr(status_word(dev)), stream_ptr(dev))
+    half = B * wide * n_kv * PAGE * dim * 2                                  # bytes of the keys
+    held = torch.empty(2 * half + 4 * B * wide, dtype=torch.uint8, device=dev)
+    at = held.data_ptr()
+    table, status, stream = at + 2 * half, status_word(dev).data_ptr(), stream_ptr(dev)
+    lens, cu = seq_lens.data_ptr(), cu_q.data_ptr()
+    code = lib().eredu_kv8_values(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + half, block_table.data_ptr(), lens, cu, table, B,
+                                  block_table.stride(0), wide, n_kv, dim, num, int(window), int(chunk), status, stream)
     check(code, "eredu_kv8_values")
-    return out[0], out[1], table
+    code = lib().eredu_attn_prefill_tc(q.data_ptr(), at, at + half, out.data_ptr(), table, lens, cu, ptr(sinks), B, total, max_q_len, wide, B * wide, n_q, n_kv, dim, dim,
+                                       int(window), int(chunk), int(max_kv_len), _sm_count(dev), scale, status, stream)
+    check(code, "eredu_attn_prefill_tc")
+    return out
 
 
 # ------------------------------------------------------------------------------------------ moving
