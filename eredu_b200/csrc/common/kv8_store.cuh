@@ -20,16 +20,20 @@ struct Kv8StoreParams {
   int* status;
 };
 
-// Cosine and sine of pos * freq, times `factor`. The product in two parts, so that far positions keep their digits; then whole turns are taken off with
-// 2 pi in two parts (the reduction of Cody and Waite; fma makes the first difference exact), which leaves an angle the fast functions are good for: off by 2^-20
-// in all for angles below 2^24, where sincosf costs four times as much.
+// Cosine and sine of pos * freq, times `factor`, off by 2^-23 or so. The product in two parts, so that far positions keep their digits; quarter turns are taken
+// off with pi / 2 in two parts (the reduction of Cody and Waite; fma makes the first difference exact), and what is left, pi / 4 at most, goes into the Taylor
+// series up to x^9 and x^10 (the next terms are below 2^-28). For angles below 2^22; sincosf costs more than twice as much, and its fast forms are off by 2^-21.
 __device__ __forceinline__ void turn_of(int pos, float freq, float factor, float& c, float& s) {
+  constexpr float kWhole = 12582912.f;                       // 1.5 * 2^23
   const float p = static_cast<float>(pos);
   const float a = p * freq, rest = fmaf(p, freq, -a);
-  const float k = rintf(a * 0.15915494f);
-  const float r = fmaf(-k, -1.7484556e-7f, fmaf(-k, 6.2831855f, a)) + rest;
-  s = __sinf(r) * factor;
-  c = __cosf(r) * factor;
+  const float t = fmaf(a, 0.636619772f, kWhole), k = t - kWhole;
+  const float r = fmaf(-k, -4.37113883e-8f, fmaf(-k, 1.57079637f, a)) + rest, z = r * r;
+  const float sine = fmaf(r * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), r);
+  const float cosine = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+  const int quarter = __float_as_int(t);
+  s = ((quarter & 1) ? cosine : sine) * ((quarter & 2) ? -factor : factor);
+  c = ((quarter & 1) ? sine : cosine) * (((quarter + 1) & 2) ? -factor : factor);
 }
 
 template <int D>

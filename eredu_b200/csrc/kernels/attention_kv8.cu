@@ -11,7 +11,8 @@
 //           and a lower accumulator row. P^T comes from S^T by movmatrix.
 // The 8 query rows of a tile are the query heads that share the key / value head, times the new tokens; two tiles side by side above 8.
 // Probabilities are rounded to f16 (11 bits; codes are exact in it). The page's value scale goes into what a probability weighs, relative to a running maximum of its
-// own (m2, of s_j + log2 vs): the largest contribution to the output is near 1 whatever the scales are. The maxima are raised only where a score passes one by far.
+// own (m2, of s_j + log2 vs): the largest weight of a row is near 1 whatever the scales are, and one
+// below 2^-14 of it is off by 2^-25 of it at most. The maxima are raised only where a score passes one by far.
 #include <cuda_bf16.h>
 
 #include "../common/kv8_store.cuh"

@@ -304,7 +304,7 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     85 / 88; 20 of 8192 50 / 53).
     More sequences and heads than that go one CTA each, or, where they are long enough for the tail of the longest to count, two or three or even shares
     (us with 1 / 2 / 3 / even: 32 of 1024 15 / 18 / 18 / 18, of 4096 48 / 47 / 43 / 44, of 8192 84 / 86 / 74 / 73; 64 of 2048 43 / 44 / 48 / 44, of 4096 77 / 73 / 76 / 74,
-    of 8192 152 / 141 / 136 / 142, with four new tokens 176 / 156 / 159 / 154)."""
+    of 8192 156 / 142 / 146 / 142, with four new tokens 176 / 156 / 159 / 154)."""
     tiles = -(-max(rows, 1) // (8 if rows <= 8 else 16))
     heads = max(1, batch * n_kv * tiles)
     pairs = max(1, -(-max_kv_len // (2 * PAGE)))
@@ -314,7 +314,7 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
             return 1
         if pairs < 192:
             return 3 if 3 * heads <= 2 * room else 2
-        return 3 if heads > room and rows <= 8 else 0
+        return 0
     splits = max(1, min(max(2, room * 9 // 10 // heads), pairs // 4, CLUSTER))
     if splits == 7:             # six or eight fill a GPC better
         splits = 6
