@@ -151,9 +151,9 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
   if (lane == 0 && part == 0) *at = scale;
 }
 
-// The same for a few rows by one warp that has other things in its registers: the rows are looked at twice.
+// The same for a few rows by one warp that has other things in its registers: the rows are looked at twice. `before`: the block's scale.
 template <int D, bool KEYS>
-__device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane) {
+__device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, float before) {
   constexpr int RPI = 128 / D;
   int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
   float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
@@ -163,7 +163,6 @@ __device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int 
     float4 x = load_row4<D>((KEYS ? p.k : p.v) + static_cast<size_t>(row + in) * (KEYS ? p.ld_k : p.ld_v) + h * D, lane);
     return KEYS ? prepared<D, false>(p, x, p.k_norm_w, turns + in * p.rot, lane) : x;
   };
-  const float before = first > 0 ? *at : 0.f;
   uint32_t top = 0;
 #pragma unroll 1
   for (int r = sub; r - sub < n; r += RPI) top = kv8_top(top, row_of(r));

@@ -47,6 +47,7 @@ struct AttnKv8Params {
   // A step from the projection's output (q, st.k and st.v in the same rows): queries are normalised and rotated as they are read, and the CTA that has the
   // page of a new token writes its rows there.
   Kv8StoreParams st;
+  int settled;      // the kernel just before this one writes the projection's output only: no pages, tables, lengths, positions, slots or frequencies
 };
 // Token of query row r among those that share a key / value head (r < 2^16: exact), in place of a division of some thirty instructions.
 __device__ __forceinline__ int kv8_token(const AttnKv8Params& p, int r) { return p.per_group == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.per_group)); }
@@ -219,25 +220,34 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   __shared__ __align__(16) float turns_s[STEP ? kKv8StepTokens * D : 1];   // cosines and sines of the tile's tokens
   pdl_launch_early();
   trace_mark(kTraceAttnDecode, kTraceStart);
-  pdl_wait();
-  trace_mark(kTraceAttnDecode, kTraceAfterWait);
-  pdl_launch_dependents();
+  // settled: what lies in front of the projection's output in time - places, pages, angles - is read ahead of the wait; nothing is written
+  bool waited = !(STEP && p.settled);
+  auto wait_for_input = [&]() {
+    pdl_wait();
+    trace_mark(kTraceAttnDecode, kTraceAfterWait);
+    pdl_launch_dependents();
+    waited = true;
+  };
+  if (waited) wait_for_input();
   const int warp = static_cast<int>(warp_uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = p.n_q / p.n_kv, rows_all = p.q_per_seq * group;
   // the CTA's share: pairs [at, end) of the line; or one split
   Kv8Place place = {};
   int at = 0, end = 0, slot = 0;
+  int4 join = make_int4(0, 0, 0, 0);
   if (EVEN) {
     place = kv8_place(p, blockIdx.x, gridDim.x, lane);
     at = place.share * blockIdx.x;
-    if (threadIdx.x == 0) {
-      const int head_tile = place.b < 0 ? 0 : (at - place.begin) / place.pairs, begin = place.begin + head_tile * place.pairs;
-      // of the CTAs that have a part of these rows, the second one stands for all: it begins behind their first pair, and the CTA in front does not
-      const bool second = place.b >= 0 && at > begin && at - place.share <= begin;
-      p.joins[blockIdx.x] = second ? make_int4((begin + place.pairs - 1) / place.share - blockIdx.x + 2, place.b, head_tile, at - place.share == begin) : make_int4(0, 0, 0, 0);
+    if (place.b < 0) {
+      if (!waited) wait_for_input();
+      if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
     }
-    if (place.b < 0) return;
     end = min(place.total, at + place.share);
+    // of the CTAs that have a part of the first rows, the second one stands for all: it begins behind their first pair, and the CTA in front does not
+    const int head_tile = (at - place.begin) / place.pairs, begin = place.begin + head_tile * place.pairs;
+    if (at > begin && at - place.share <= begin)
+      join = make_int4((begin + place.pairs - 1) / place.share - blockIdx.x + 2, place.b, head_tile, at - place.share == begin);
   }
   do {
   const int b = EVEN ? place.b : blockIdx.z, head_tile = EVEN ? (at - place.begin) / place.pairs : blockIdx.y, split = EVEN ? 0 : blockIdx.x;
@@ -316,26 +326,18 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     for (int n = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); n < tokens; n += kKv8Threads / (D / 2))
       if (i < half) turn_of(positions[n], p.st.inv_freq[i], p.st.attn_factor, turns_s[n * p.st.rot + i], turns_s[n * p.st.rot + half + i]);
     __syncthreads();
-    // ---- the new rows of pages in this part: a warp for the keys or the values of a page (there are two such pages at most)
-    const int page = max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) + (warp >> 1);
-    if (page < page1) {
-      const int first = max(0, page * kKv8Page - pos_new), end_row = min(p.q_per_seq, (page + 1) * kKv8Page - pos_new), row0 = b * p.q_per_seq;
-      for (int r = first; r < end_row;) {
-        const long long to = p.st.slots[row0 + r];
-        int n = 1;
-        if (to >= 0 && (to >> 4) < p.num_pages) {
-          while (r + n < end_row && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
-          const long long cell = (to >> 4) * p.n_kv + kvh;
-          if ((warp & 1) == 0) store_few<D, true>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * p.st.rot, lane);
-          else store_few<D, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane);
-        } else if (to >= 0) {
-          report_status(p.status, kStatusBadArgument);
-        }
-        r += n;
-      }
-    }
   }
-  // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
+  // this warp's share of the write: keys or values of a page in this part (there are two such pages at most)
+  const int my_page = STEP ? max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) + (warp >> 1) : 0;
+  const int my_row = STEP ? max(0, my_page * kKv8Page - pos_new) : 0, my_end = STEP && my_page < page1 ? min(p.q_per_seq, (my_page + 1) * kKv8Page - pos_new) : 0;
+  long long my_slot = -1;
+  float my_scale = 0.f;
+  if (STEP && my_row < my_end) {
+    my_slot = p.st.slots[b * p.q_per_seq + my_row];
+    if (my_slot >= 0 && (my_slot >> 4) < p.num_pages) my_scale = ((warp & 1) == 0 ? p.k_scales : p.v_scales)[(my_slot >> 4) * p.n_kv + kvh];
+  }
+  if (STEP && !waited) wait_for_input();
+  if (EVEN && slot == 0 && threadIdx.x == 0) p.joins[blockIdx.x] = join;
   constexpr int QUERIES = ROWS / (kKv8Warps * RPI);     // of a warp, all on their way before the first is looked at
   float4 query[QUERIES];
 #pragma unroll
@@ -344,6 +346,26 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const size_t at = static_cast<size_t>(b * p.q_per_seq + token) * p.ld_q + (kvh * group + r - token * group) * D;
     query[i] = !STEP && p.q32 != nullptr ? *reinterpret_cast<const float4*>(p.q32 + at + lane % (D / 4) * 4) : load_row4<D>(p.q + at, lane);
   }
+  // ---- the new rows
+  if (STEP) {
+    const int row0 = b * p.q_per_seq;
+#pragma unroll 1
+    for (int r = my_row; r < my_end;) {
+      const long long to = r == my_row ? my_slot : p.st.slots[row0 + r];
+      int n = 1;
+      if (to >= 0 && (to >> 4) < p.num_pages) {
+        while (r + n < my_end && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
+        const long long cell = (to >> 4) * p.n_kv + kvh;
+        const float before = r == my_row ? my_scale : ((warp & 1) == 0 ? p.k_scales : p.v_scales)[cell];
+        if ((warp & 1) == 0) store_few<D, true>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * p.st.rot, lane, before);
+        else store_few<D, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane, before);
+      } else if (to >= 0) {
+        report_status(p.status, kStatusBadArgument);
+      }
+      r += n;
+    }
+  }
+  // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int row = (i * kKv8Warps + warp) * RPI + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
@@ -854,7 +876,7 @@ extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, float* q32, void* k_
                                    const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, const int* positions,
                                    const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int batch, int q_per_seq,
                                    int max_pages, int num_pages, int n_q, int n_kv, int D, int rot, int interleaved, int splits, int ctas, int window, int chunk,
-                                   float scale, float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
+                                   int settled, float scale, float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
   if (batch <= 0) return 0;
   if (n_kv <= 0 || n_q <= 0 || n_q % n_kv != 0 || q_per_seq <= 0 || rot < 0 || rot > D || rot % 8 != 0) return -2;
   const int group = n_q / n_kv;
@@ -872,6 +894,7 @@ extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, float* q32, void* k_
     p.ld_q = n_q * D;
     return attn_kv8(p, D, ctas, false, stream);
   }
+  p.settled = !EREDU_PDL_EARLY && pdl_enabled() && settled != 0;
   p.st.k = row + n_q * D;
   p.st.v = row + (n_q + n_kv) * D;
   p.st.ld_k = p.st.ld_v = ld;

@@ -744,7 +744,7 @@ def attention_decode_rope(qkv, k_cache, v_cache, block_table, seq_lens, q_per_se
             raise NotImplementedError("8-bit pages: norms per head, values as wide as keys, and rows that are appended")
         if qkv.is_cuda and positions.dim() == 1:
             return attention_step8(qkv, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, positions, slots, inv_freq, n_q, n_kv, head_dim,
-                                   rot or head_dim, interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, splits, window, sinks, chunk)
+                                   rot or head_dim, interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, splits, window, sinks, chunk, settled)
         q = rope_kv(qkv, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off)
         return attention_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, chunk=chunk)
     if norm_whole or value_norm or not append or value_dim != head_dim or chunk:

@@ -41,7 +41,7 @@ P, I, F = native.P, native.I, native.F
 native.register("eredu_kv8_store", I, [P] * 13 + [I] * 11 + [F] * 3 + [P] * 2)
 native.register("eredu_kv8_values", I, [P] * 10 + [I] * 8 + [P] * 2)
 native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 11 + [F] + [P] * 2)
-native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 17 + [I] * 13 + [F] * 4 + [P] * 2)
+native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 17 + [I] * 14 + [F] * 4 + [P] * 2)
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 
@@ -276,7 +276,7 @@ def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
 
 
 def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, q_per_seq, scale, positions, slots, inv_freq, n_q, n_kv, dim, rot, interleaved,
-                    attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, splits, window, sinks, chunk):
+                    attn_factor, q_norm_w, k_norm_w, norm_eps, norm_w_off, splits, window, sinks, chunk, settled):
     """The form of :func:`.core.attention_decode_rope` for 8-bit pages on a GPU: queries keep 16 bits from the rotation to the scores."""
     dev, B = k_cache.codes.device, seq_lens.shape[0]
     M = B * q_per_seq
@@ -290,7 +290,7 @@ def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
                                      v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins,
                                      positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), B, q_per_seq,
                                      block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window),
-                                     int(chunk), scale, attn_factor, norm_eps, norm_w_off, status_word(dev).data_ptr(), stream_ptr(dev))
+                                     int(chunk), 1 if settled else 0, scale, attn_factor, norm_eps, norm_w_off, status_word(dev).data_ptr(), stream_ptr(dev))
     check(code, "eredu_attn_kv8_step")
     return out
 
