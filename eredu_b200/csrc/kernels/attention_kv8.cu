@@ -33,13 +33,13 @@ struct AttnKv8Params {
   const int8_t *k_codes, *v_codes; // [pages, n_kv, 16, D]
   const float *k_scales, *v_scales;
   __nv_bfloat16* out;              // [B * q_per_seq, n_q, D]
-  const int* block_table;          // [B, max_pages]
+  const int* block_table;          // [B rows of `pitch`], max_pages of them
   const int* seq_lens;             // [B], new tokens included
   const float* sinks;              // optional [n_q]
   float* part_o;                   // even shares: [CTAs, 2, rows of a tile, D]
   float* part_ml;                  //              [CTAs, 2, rows of a tile, 4]
   int4* joins;                     //              [CTAs]: what of the CTA's first part is to be added up, see attn_kv8_combine_kernel
-  int batch, max_pages, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
+  int batch, max_pages, pitch, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
   int ld_q;
   uint32_t per_group;              // 2^32 / (n_q / n_kv), rounded up; 0 for a group of one
   float scale_log2;
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   const int mask_hi = min(pos_first, last_key), mask_lo = kv8_lowest_key(p, pos_last);        // pages inside need no mask
 
   // ---- pairs warp, warp + 4, ... of the part. Lanes 2 i and 2 i + 1 hold page ids and scales of the i-th of 16 turns; those of the 16 before stay at hand.
-  const int* table = p.block_table + static_cast<size_t>(b) * p.max_pages;
+  const int* table = p.block_table + static_cast<size_t>(b) * p.pitch;
   const int turns = page1 > page0 + 2 * warp ? (page1 - page0 - 2 * warp + 2 * kKv8Warps - 1) / (2 * kKv8Warps) : 0;
   int ids = 0;
   float ks = 0.f, ev = 0.f, ks_before = 0.f, ev_before = 0.f;
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     }
     store_out(p.out + out_s[row] + d, sum, up_s[row]);
   }
-  cluster_arrive_release();   // nobody leaves while its shared memory is read
+  cluster_arrive_relaxed();   // nobody leaves while its shared memory is read; nothing is handed over (with release: 0.1 to 0.3 us for stores on their way)
   cluster_wait_acquire();
   } while (EVEN && at < end);
 }
@@ -830,7 +830,8 @@ static int attn_kv8(AttnKv8Params& p, int D, int ctas, bool step, cudaStream_t s
 
 static AttnKv8Params attn_kv8_params(const void* q, int ld_q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
                                      const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
-                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int splits, int window, int chunk, float scale, int* status) {
+                                     int q_per_seq, int max_pages, int pitch, int num_pages, int n_q, int n_kv, int splits, int window, int chunk, float scale,
+                                     int* status) {
   AttnKv8Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.ld_q = ld_q;
@@ -847,6 +848,7 @@ static AttnKv8Params attn_kv8_params(const void* q, int ld_q, const void* k_code
   p.joins = static_cast<int4*>(joins);
   p.batch = batch;
   p.max_pages = max_pages;
+  p.pitch = pitch;
   p.num_pages = num_pages;
   p.n_q = n_q;
   p.n_kv = n_kv;
@@ -862,10 +864,10 @@ static AttnKv8Params attn_kv8_params(const void* q, int ld_q, const void* k_code
 // splits 1 to 8: CTAs of a sequence and head. 0: even shares for `ctas` CTAs, with scratch for 2 * ctas tiles of 8 rows (16 where a head has more than 8).
 extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
                                      const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
-                                     int q_per_seq, int max_pages, int num_pages, int n_q, int n_kv, int D, int splits, int ctas, int window, int chunk,
+                                     int q_per_seq, int max_pages, int pitch, int num_pages, int n_q, int n_kv, int D, int splits, int ctas, int window, int chunk,
                                      float scale, int* status, cudaStream_t stream) {
   AttnKv8Params p = attn_kv8_params(q, n_q * D, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
-                                    max_pages, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
+                                    max_pages, pitch, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
   return attn_kv8(p, D, ctas, false, stream);
 }
 
@@ -875,7 +877,7 @@ extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const v
 extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, float* q32, void* k_codes, void* v_codes, float* k_scales, float* v_scales, void* out, const int* block_table,
                                    const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, const int* positions,
                                    const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int batch, int q_per_seq,
-                                   int max_pages, int num_pages, int n_q, int n_kv, int D, int rot, int interleaved, int splits, int ctas, int window, int chunk,
+                                   int max_pages, int pitch, int num_pages, int n_q, int n_kv, int D, int rot, int interleaved, int splits, int ctas, int window, int chunk,
                                    int settled, float scale, float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
   if (batch <= 0) return 0;
   if (n_kv <= 0 || n_q <= 0 || n_q % n_kv != 0 || q_per_seq <= 0 || rot < 0 || rot > D || rot % 8 != 0) return -2;
@@ -883,7 +885,7 @@ extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, float* q32, void* k_
   const bool own = q_per_seq * group <= 16 && q_per_seq <= kKv8StepTokens;
   const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(qkv);
   AttnKv8Params p = attn_kv8_params(qkv, ld, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
-                                    max_pages, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
+                                    max_pages, pitch, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
   if (!own) {
     if (q32 == nullptr) return -2;
     const int e = eredu_kv8_store(qkv, row + n_q * D, row + (n_q + n_kv) * D, q32, k_codes, v_codes, k_scales, v_scales, positions, slots, inv_freq, q_norm_w,

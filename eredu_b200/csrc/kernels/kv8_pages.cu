@@ -109,7 +109,7 @@ struct Kv8ValuesParams {
   const int* seq_lens;     // optional [rows]
   const int* cu_q;         // with seq_lens: query offsets
   int* table_out;          // with seq_lens: [rows, wide]
-  int pitch, wide, n_kv, num_pages, window, chunk;
+  int pitch, table_wide, wide, n_kv, num_pages, window, chunk;   // table_wide: entries of a row of `pages`; wide: of a row of the output
   int* status;
 };
 constexpr int kValuesThreads = 256;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kValuesThreads) kv8_values_kernel(Kv8ValuesPar
   if (p.seq_lens != nullptr) {
     const int len = p.seq_lens[row], first = len - (p.cu_q[row + 1] - p.cu_q[row]);
     const int low = p.window > 0 ? first - p.window + 1 : p.chunk > 0 && first > 0 ? first - first % p.chunk : 0;
-    const bool seen = i * kKv8Page < len && i * kKv8Page + kKv8Page > low && first < len && i < p.pitch;
+    const bool seen = i * kKv8Page < len && i * kKv8Page + kKv8Page > low && first < len && i < p.table_wide;
     if (threadIdx.x == 0 && blockIdx.z == 0) p.table_out[entry] = static_cast<int>(seen ? entry : static_cast<size_t>(gridDim.y) * p.wide);
     if (!seen) return;
   }
@@ -244,7 +244,7 @@ extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void
 }
 
 extern "C" int eredu_kv8_values(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* k_out, void* v_out,
-                                const int* pages, const int* seq_lens, const int* cu_q, int* table_out, int rows, int pitch, int wide, int n_kv, int D,
+                                const int* pages, const int* seq_lens, const int* cu_q, int* table_out, int rows, int pitch, int table_wide, int wide, int n_kv, int D,
                                 int num_pages, int window, int chunk, int* status, cudaStream_t stream) {
   if (rows <= 0 || wide <= 0) return 0;
   if ((D != 64 && D != 128) || n_kv <= 0 || rows > 65535 || num_pages <= 0) return -2;
@@ -261,6 +261,7 @@ extern "C" int eredu_kv8_values(const void* k_codes, const void* v_codes, const 
   p.table_out = table_out;
   p.pitch = pitch;
   p.wide = wide;
+  p.table_wide = table_wide;
   p.n_kv = n_kv;
   p.num_pages = num_pages;
   p.window = window;

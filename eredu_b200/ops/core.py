@@ -611,7 +611,7 @@ def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_le
     computed; 0: unknown). Key and value widths are those of the caches. Returns [total_q, n_q, value width].
     Caches of :class:`Pages8`: the pages that some query sees are brought to bf16 first - once for all query tiles and heads that read them -, in memory
     that the call allocates (``max_kv_len`` bounds it, and then has to be that of the longest sequence at least)."""
-    if isinstance(k_cache, Pages8) and q.is_cuda:
+    if q.is_cuda and (isinstance(k_cache, Pages8) or isinstance(v_cache, Pages8)):
         return attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
         if not _tensor_core_dims(q, k_cache, v_cache):
@@ -698,7 +698,7 @@ def attention_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scal
                      scratch=None, out=None, chunk=0):
     """q: [B * q_per_seq, n_q, D]; ``window`` / ``chunk`` as in :func:`attention_prefill`. ``scratch`` = (part_o, part_ml, counters) from :func:`decode_scratch` when
     splits > 1 (fp32 partials and zeroed int32 arrival tickets). Caches of :class:`Pages8` need no ``scratch``; a query that sees no key gives zeros."""
-    if isinstance(k_cache, Pages8) and q.is_cuda:
+    if q.is_cuda and (isinstance(k_cache, Pages8) or isinstance(v_cache, Pages8)):
         return attention_decode8(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
         if not _tensor_core_dims(q, k_cache, v_cache) or q.shape[1] // k_cache.shape[1] > 32:

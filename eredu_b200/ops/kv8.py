@@ -39,9 +39,9 @@ def _sm_count(device) -> int:
 
 P, I, F = native.P, native.I, native.F
 native.register("eredu_kv8_store", I, [P] * 13 + [I] * 11 + [F] * 3 + [P] * 2)
-native.register("eredu_kv8_values", I, [P] * 10 + [I] * 8 + [P] * 2)
-native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 11 + [F] + [P] * 2)
-native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 17 + [I] * 14 + [F] * 4 + [P] * 2)
+native.register("eredu_kv8_values", I, [P] * 10 + [I] * 9 + [P] * 2)
+native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 12 + [F] + [P] * 2)
+native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 17 + [I] * 15 + [F] * 4 + [P] * 2)
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 
@@ -68,15 +68,19 @@ class Pages8(NamedTuple):
         return codes.float() * scales[..., None, None]
 
     @classmethod
-    def empty(cls, pages: int, heads: int, head_dim: int, device, layers: int = 0) -> "Pages8":
-        """Zeroed blocks; with ``layers``, [layers, pages, ...]."""
-        lead = (layers, pages, heads) if layers else (pages, heads)
-        return cls(torch.zeros((*lead, PAGE, head_dim), dtype=torch.int8, device=device), torch.full(lead, FLOOR, dtype=torch.float32, device=device))
+    def empty(cls, pages: int, heads: int, head_dim: int, device) -> "Pages8":
+        """Zeroed blocks."""
+        return cls(torch.zeros((pages, heads, PAGE, head_dim), dtype=torch.int8, device=device),
+                   torch.full((pages, heads), FLOOR, dtype=torch.float32, device=device))
+
+
+def _check_pair(k, v) -> None:
+    if type(k) is not Pages8 or type(v) is not Pages8:
+        raise TypeError("keys and values: a pair of Pages8 is expected, both or neither")
 
 
 def check_pages8(k: Pages8, v: Pages8, n_kv: int, head_dim: int) -> None:
-    if type(k) is not Pages8 or type(v) is not Pages8:
-        raise TypeError("keys and values: a pair of Pages8 is expected, both or neither")
+    _check_pair(k, v)
     (kc, ks), (vc, vs) = k, v
     shape = kc.shape
     # (one condition for the common case: these checks are a good part of what a short call costs)
@@ -182,7 +186,8 @@ def _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, 
 
 def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
              norm_eps, norm_w_off, q_out):
-    """The form of :func:`.core.rope_kv` for 8-bit pages on a GPU. Norm and rotation run in 32 bits throughout; a key is rounded once, to its code."""
+    """The form of :func:`.core.rope_kv` for 8-bit pages on a GPU. Norm and rotation run in 32 bits throughout; a key is rounded once, to its code.
+    Angles (position times frequency) are good below 2^22."""
     dev, M = k_cache.codes.device, qkv.shape[0]
     _check_qkv(qkv, M, positions, slots, inv_freq, k_cache, v_cache, n_q, n_kv, head_dim, rot, q_norm_w, k_norm_w)
     if q_out is None:
@@ -200,8 +205,7 @@ def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, 
 # ------------------------------------------------------------------------------------------ reading
 def page_values(k_cache: Pages8, v_cache: Pages8, pages):
     """Keys and values of ``pages`` [n] int32 as bf16 [n, heads, 16, head size] each (exact: a code has seven bits)."""
-    if type(k_cache) is not Pages8:
-        raise TypeError("keys and values: a pair of Pages8 is expected")
+    _check_pair(k_cache, v_cache)
     (kc, ks), (vc, vs) = k_cache, v_cache
     num, n_kv, _, dim = kc.shape
     check_pages8(k_cache, v_cache, n_kv, dim)
@@ -213,7 +217,7 @@ def page_values(k_cache: Pages8, v_cache: Pages8, pages):
     if n:
         at = out.data_ptr()
         code = lib().eredu_kv8_values(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + 2 * n * n_kv * PAGE * dim, pages.data_ptr(), None, None,
-                                      None, 1, n, n, n_kv, dim, num, 0, 0, status_word(dev).data_ptr(), stream_ptr(dev))
+                                      None, 1, n, n, n, n_kv, dim, num, 0, 0, status_word(dev).data_ptr(), stream_ptr(dev))
         check(code, "eredu_kv8_values")
     return out.unbind(0)
 
@@ -231,6 +235,7 @@ def _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev):
 
 
 def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q=None):
+    _check_pair(k_cache, v_cache)
     n_q, dim = q.shape[1:]
     n_kv, dev = k_cache.codes.shape[1], k_cache.codes.device
     check_pages8(k_cache, v_cache, n_kv, dim)
@@ -269,7 +274,7 @@ def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
         out = torch.empty_like(q)
     splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
     code = lib().eredu_attn_kv8_decode(q.data_ptr(), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
-                                       block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins, B, q_per_seq, block_table.stride(0),
+                                       block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins, B, q_per_seq, block_table.shape[1], block_table.stride(0),
                                        k_cache.codes.shape[0], n_q, n_kv, dim, splits, ctas, int(window), int(chunk), scale, ptr(status_word(dev)), stream_ptr(dev))
     check(code, "eredu_attn_kv8_decode")
     return out
@@ -289,7 +294,7 @@ def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
     code = lib().eredu_attn_kv8_step(qkv.data_ptr(), qkv.stride(0), ptr(q32), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(),
                                      v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins,
                                      positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), B, q_per_seq,
-                                     block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window),
+                                     block_table.shape[1], block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window),
                                      int(chunk), 1 if settled else 0, scale, attn_factor, norm_eps, norm_w_off, status_word(dev).data_ptr(), stream_ptr(dev))
     check(code, "eredu_attn_kv8_step")
     return out
@@ -344,7 +349,7 @@ def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_len
     table, status, stream = at + 2 * half, status_word(dev).data_ptr(), stream_ptr(dev)
     lens, cu = seq_lens.data_ptr(), cu_q.data_ptr()
     code = lib().eredu_kv8_values(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + half, block_table.data_ptr(), lens, cu, table, B,
-                                  block_table.stride(0), wide, n_kv, dim, num, int(window), int(chunk), status, stream)
+                                  block_table.stride(0), block_table.shape[1], wide, n_kv, dim, num, int(window), int(chunk), status, stream)
     check(code, "eredu_kv8_values")
     code = lib().eredu_attn_prefill_tc(q.data_ptr(), at, at + half, out.data_ptr(), table, lens, cu, ptr(sinks), B, total, max_q_len, wide, B * wide, n_q, n_kv, dim, dim,
                                        int(window), int(chunk), int(max_kv_len), _sm_count(dev), scale, status, stream)

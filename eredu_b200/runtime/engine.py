@@ -261,6 +261,8 @@ class Engine:
         being filled is copied (in all layers, one launch). It draws random numbers of its own."""
         other = Sequence(self._next_id, list(seq.prompt), seq.sampling, seq.max_new_tokens, seq.eos_ids, list(seq.output), kv_len=seq.kv_len,
                          cached_tokens=seq.cached_tokens)
+        if seq.kv_len and not seq.pages:
+            raise RuntimeError("a sequence whose pages are parked is not forked")
         if getattr(seq, "rope_delta", 0):
             other.rope_delta = seq.rope_delta
         self._next_id += 1
@@ -277,7 +279,7 @@ class Engine:
 
     def compact(self, seqs) -> int:
         """Moves the cached pages to the front of the pool and renames them in ``seqs`` (all sequences that have pages) and in the decode state, whose
-        captured graph stays valid. Returns the number of pages moved."""
+        captured graph stays valid (not in the tables of a speculative round: not under one). Returns the number of pages moved."""
         named = {int(p) for s in seqs for p in s.pages}
         missing = [p for p in self.kv.allocator.held() if p not in named]
         if missing:
@@ -821,6 +823,8 @@ class Engine:
         ``self.last_finish_reasons`` holds the per-sequence reasons afterwards.
         ``samples`` > 1: that many continuations of every prompt, one behind the other in the result. The prompt is run and cached once; its sequence is
         forked in front of its last token, which is every continuation's first step."""
+        if samples < 1:
+            raise ValueError(f"{samples} continuations of a prompt")
         seqs = []
         try:
             for p in prompts:

@@ -21,7 +21,7 @@ from ..ops import native
 KERNELS = {1: "gemm", 2: "gemm_persistent", 3: "qgemm", 4: "attn_decode", 5: "attn_prefill", 6: "rope_kv", 7: "rmsnorm",
            8: "embedding", 9: "sampler", 10: "decode_advance", 11: "moe", 12: "silu_mul", 13: "comm"}
 PHASES = {0: "start", 1: "after_wait", 2: "end"}
-_UNITS = ("gemm", "gemm_persistent", "attention", "norm_rope", "sampler")
+_UNITS = ("gemm", "gemm_persistent", "attention", "attention_kv8", "norm_rope", "sampler")
 
 
 class DeviceTrace:

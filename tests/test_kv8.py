@@ -337,6 +337,27 @@ def test_what_is_no_number_reaches_only_those_who_see_it():
 
 
 @pytest.mark.gpu
+def test_block_tables_that_are_part_of_a_wider_one():
+    """Rows of another pitch than their width; lengths that say more than the table has are cut there, and nothing behind the table is read."""
+    seq_lens = (70, 33)
+    num, table = layout(seq_lens, "cuda")
+    k, v = (filled(num, 2, 64, "cuda", seed=i) for i in range(2))
+    q = torch.randn((2, 8, 64), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    lens, cu = ints(seq_lens, "cuda"), ints([0, 1, 2], "cuda")
+    wide = torch.full((2, 40), 1 << 20, dtype=torch.int32, device="cuda")
+    part = wide[:, 30:30 + table.shape[1]]
+    part.copy_(table)
+    for splits in (1, 3, 0):
+        assert torch.equal(ops.attention_decode(q, k, v, part, lens, 1, 0.1, splits=splits), ops.attention_decode(q, k, v, table, lens, 1, 0.1, splits=splits))
+    assert torch.equal(ops.attention_prefill(q, k, v, part, lens, cu, 1, 0.1), ops.attention_prefill(q, k, v, table, lens, cu, 1, 0.1))
+    short = wide[:, 30:32]
+    for splits in (1, 3, 0):
+        got = ops.attention_decode(q, k, v, short, lens, 1, 0.1, splits=splits)
+        within(got, *attended(q, k.values(), v.values(), table, (32, 32), (1, 1), 0.1), 2.0 ** -11)
+    ops.native.check_status(torch.device("cuda"))
+
+
+@pytest.mark.gpu
 def test_pages_behind_four_gigabytes():
     """Codes at offsets that no 32-bit number holds."""
     heads, dim, num = 8, 128, 270_000
@@ -536,8 +557,11 @@ def test_calls_that_are_refused_on_a_gpu():
         a = dict(q=q, table=table, lens=lens, sinks=None, out=None) | change
         with pytest.raises(ValueError):
             ops.attention_decode(a["q"], k, v, a["table"], a["lens"], 1, 1.0, sinks=a["sinks"], out=a["out"])
-    with pytest.raises(TypeError):
-        ops.attention_decode(q, k, v.codes, table, lens, 1, 1.0)
+    for pair in ((k, v.codes), (k.codes, v)):
+        with pytest.raises(TypeError):
+            ops.attention_decode(q, *pair, table, lens, 1, 1.0)
+        with pytest.raises(TypeError):
+            ops.attention_prefill(q, *pair, table, lens, ints([0, 1, 2], dev), 1, 1.0)
     with pytest.raises(NotImplementedError):
         wide = [Pages8.empty(4, 2, 256, dev) for _ in "kv"]
         ops.attention_decode(torch.zeros((2, 4, 256), dtype=torch.bfloat16, device=dev), *wide, table, lens, 1, 1.0)

@@ -176,6 +176,27 @@ def test_several_continuations_of_a_prompt(device):
     assert all(1 <= len(o) <= 6 for o in hist)
 
 
+def test_forks_and_continuations_that_are_refused():
+    eng = Engine(build(), max_batch=2, max_seq_len=64)
+    with pytest.raises(ValueError, match="continuations"):
+        eng.generate([prompt(4)], GREEDY, samples=0)
+    seq = eng.new_sequence(prompt(20), GREEDY, max_new_tokens=4)
+    eng.prefill([seq])
+    pages, seq.pages = seq.pages, []                 # as a parked sequence has none
+    with pytest.raises(RuntimeError, match="parked"):
+        eng.fork(seq)
+    seq.pages = pages
+    small = Engine(build(), max_batch=1, max_seq_len=64, num_pages=4)
+    s = small.new_sequence(prompt(20), GREEDY, max_new_tokens=4)
+    small.prefill([s])
+    free = small.kv.allocator.free_pages()
+    big = small.fork(s)                              # one page more
+    with pytest.raises(RuntimeError, match="exhausted"):
+        small.fork(s)
+    assert small.kv.allocator.free_pages() == free - 1 and small.kv.allocator.refcount(s.pages[0]) == 2
+    small.release(big)
+
+
 def test_hybrid_models_fork_their_states():
     from test_lfm2 import lfm2_cfg           # a model with convolution states, found by a sequence's first page
 
