@@ -15,6 +15,8 @@
 // below 2^-14 of it is off by 2^-25 of it at most. The maxima are raised only where a score passes one by far.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "../common/kv8_store.cuh"
 #include "../common/launch.h"
 #include "../common/launch_count.h"
@@ -40,6 +42,7 @@ struct AttnKv8Params {
   float* part_ml;                  //              [CTAs, 2, rows of a tile, 4]
   int4* joins;                     //              [CTAs]: what of the CTA's first part is to be added up, see attn_kv8_combine_kernel
   int batch, max_pages, pitch, num_pages, n_q, n_kv, q_per_seq, tiles, splits, window, chunk;
+  int ctas, stretch;               // of even shares; joins that a CTA of the second kernel looks through, 32 at most
   int ld_q;
   uint32_t per_group;              // 2^32 / (n_q / n_kv), rounded up; 0 for a group of one
   float scale_log2;
@@ -676,8 +679,11 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   } while (EVEN && at < end);
 }
 
-// Rows of a sequence and head of which several CTAs have a part. grid (CTAs, rows of a tile): joins[i] = {parts, sequence, head and tile, whether the first
-// part, that of CTA i - 1, is also the first of that CTA}, no parts where there is nothing to add up. Four warps take some parts each.
+// Rows of a sequence and head of which several CTAs have a part: joins[i] = {parts, sequence, head and tile, whether the first part, that of CTA i - 1, is also
+// the first of that CTA}, no parts where there is nothing to add up. grid (stretches of joins, rows of a tile): two stretches for each sequence and head, a CTA
+// for each of all joins, mostly without work, only where there are no fewer of those. Four warps take some parts each.
+// One sequence of 65536 tokens, attention in all: a CTA for every join 33.1 (64 query heads 35.0) us, stretches 31.6 (31.9), with eight warps 30.8 (31.5); 64 of
+// 8192, where parts are two or three: 141.7, 142.8, with eight warps 148.7.
 constexpr int kCombineWarps = 4;
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(AttnKv8Params p) {
@@ -687,66 +693,74 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attn_kv8_combine_kernel(At
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
-  const int4 join = p.joins[blockIdx.x];
-  const int parts = join.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.n_q / p.n_kv;
-  const int kvh = p.tiles == 1 ? join.z : join.z / p.tiles, n = (join.z - kvh * p.tiles) * ROWS + row, c0 = blockIdx.x - 1;
-  if (parts == 0 || n >= p.q_per_seq * group) return;
-  // the first of the CTAs has it as its last part, the others as their first
-  auto place_of = [&](int s) { return (static_cast<size_t>(c0 + s) * 2 + (s == 0 && join.w == 0 ? 1 : 0)) * ROWS + row; };
-  Kv8Row r = {kLowest, 0.f, kLowest};
-  float sum[PER] = {};
-  // up to eight splits a warp at once, so that their loads are on the way together
-  for (int s0 = warp; s0 < parts; s0 += 8 * kCombineWarps) {
-    float4 ml[8];
-    float part[8][PER];
+  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.n_q / p.n_kv;
+  const int i0 = blockIdx.x * p.stretch;
+  const int4 held = lane < p.stretch && i0 + lane < p.ctas ? p.joins[i0 + lane] : make_int4(0, 0, 0, 0);
+  for (uint32_t there = __ballot_sync(0xffffffffu, held.x != 0); there != 0; there &= there - 1) {
+    const int from = __ffs(there) - 1, c0 = i0 + from - 1;
+    const int parts = __shfl_sync(0xffffffffu, held.x, from), b = __shfl_sync(0xffffffffu, held.y, from), head_tile = __shfl_sync(0xffffffffu, held.z, from);
+    const int first = __shfl_sync(0xffffffffu, held.w, from);
+    const int kvh = p.tiles == 1 ? head_tile : head_tile / p.tiles, n = (head_tile - kvh * p.tiles) * ROWS + row;
+    if (n >= p.q_per_seq * group) continue;
+    // the first of the CTAs has it as its last part, the others as their first
+    auto place_of = [&](int s) { return (static_cast<size_t>(c0 + s) * 2 + (s == 0 && first == 0 ? 1 : 0)) * ROWS + row; };
+    Kv8Row r = {kLowest, 0.f, kLowest};
+    float sum[PER] = {};
+    // up to eight parts a warp at once, so that their loads are on the way together
+    for (int s0 = warp; s0 < parts; s0 += 8 * kCombineWarps) {
+      float4 ml[8];
+      float part[8][PER];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = s0 + i * kCombineWarps;
-      const size_t from = place_of(min(s, parts - 1));
-      ml[i] = s < parts ? *reinterpret_cast<const float4*>(p.part_ml + from * 4) : make_float4(kLowest, 0.f, kLowest, 0.f);
+      for (int i = 0; i < 8; ++i) {
+        const int s = s0 + i * kCombineWarps;
+        const size_t at = place_of(min(s, parts - 1));
+        ml[i] = s < parts ? *reinterpret_cast<const float4*>(p.part_ml + at * 4) : make_float4(kLowest, 0.f, kLowest, 0.f);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) part[i][j] = s < parts ? p.part_o[from * D + lane + 32 * j] : 0.f;
+        for (int j = 0; j < PER; ++j) part[i][j] = s < parts ? p.part_o[at * D + lane + 32 * j] : 0.f;
+      }
+      float m = r.m, m2 = r.m2;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        m = fmaxf(m, ml[i].x);
+        m2 = fmaxf(m2, ml[i].z);
+      }
+      r.l *= ex2_approx(r.m - m);
+      const float down = ex2_approx(r.m2 - m2);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) sum[j] *= down;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        r.l += ml[i].y * ex2_approx(ml[i].x - m);
+        const float w = ex2_approx(ml[i].z - m2);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum[j] += part[i][j] * w;
+      }
+      r.m = m;
+      r.m2 = m2;
     }
-    float m = r.m, m2 = r.m2;
+    if (lane == 0) row_s[warp] = r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m = fmaxf(m, ml[i].x);
-      m2 = fmaxf(m2, ml[i].z);
+    for (int j = 0; j < PER; ++j) sum_s[warp][lane + 32 * j] = sum[j];
+    __syncthreads();
+    if (threadIdx.x < D) {   // (D is at most the number of threads)
+      r = Kv8Row{kLowest, 0.f, kLowest};
+#pragma unroll
+      for (int w = 0; w < kCombineWarps; ++w) {
+        r.m = fmaxf(r.m, row_s[w].m);
+        r.m2 = fmaxf(r.m2, row_s[w].m2);
+      }
+      float all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kCombineWarps; ++w) {
+        r.l += row_s[w].l * ex2_approx(row_s[w].m - r.m);
+        all += sum_s[w][threadIdx.x] * ex2_approx(row_s[w].m2 - r.m2);
+      }
+      const int token = kv8_token(p, n), head = kvh * group + n - token * group;
+      const Kv8Finish f = kv8_finish(r, p.sinks == nullptr ? nullptr : p.sinks + head);
+      p.out[(static_cast<size_t>(b * p.q_per_seq + token) * p.n_q + head) * D + threadIdx.x] = __float2bfloat16(all * f.over * f.up);
     }
-    r.l *= ex2_approx(r.m - m);
-    const float down = ex2_approx(r.m2 - m2);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) sum[j] *= down;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      r.l += ml[i].y * ex2_approx(ml[i].x - m);
-      const float w = ex2_approx(ml[i].z - m2);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) sum[j] += part[i][j] * w;
-    }
-    r.m = m;
-    r.m2 = m2;
+    if ((there & (there - 1)) != 0) __syncthreads();   // the next rows go to the same places
   }
-  if (lane == 0) row_s[warp] = r;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) sum_s[warp][lane + 32 * j] = sum[j];
-  __syncthreads();
-  if (threadIdx.x >= D) return;   // (D is at most the number of threads)
-  r = Kv8Row{kLowest, 0.f, kLowest};
-#pragma unroll
-  for (int w = 0; w < kCombineWarps; ++w) {
-    r.m = fmaxf(r.m, row_s[w].m);
-    r.m2 = fmaxf(r.m2, row_s[w].m2);
-  }
-  float all = 0.f;
-#pragma unroll
-  for (int w = 0; w < kCombineWarps; ++w) {
-    r.l += row_s[w].l * ex2_approx(row_s[w].m - r.m);
-    all += sum_s[w][threadIdx.x] * ex2_approx(row_s[w].m2 - r.m2);
-  }
-  const int token = kv8_token(p, n), head = kvh * group + n - token * group;
-  const Kv8Finish f = kv8_finish(r, p.sinks == nullptr ? nullptr : p.sinks + head);
-  p.out[(static_cast<size_t>(join.y * p.q_per_seq + token) * p.n_q + head) * D + threadIdx.x] = __float2bfloat16(all * f.over * f.up);
 }
 
 template <int D, int NT, bool EVEN, bool STEP>
@@ -787,7 +801,7 @@ static cudaError_t launch_attn_kv8(const AttnKv8Params& p, int ctas, cudaStream_
   cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kv8_kernel<D, NT, EVEN, STEP>, p);
   eredu_count_launches(1);
   if (EVEN && e == cudaSuccess) {
-    e = launch_pdl(attn_kv8_combine_kernel<D, NT>, dim3(ctas, p.tiles == 1 ? p.q_per_seq * (p.n_q / p.n_kv) : ROWS), dim3(32 * kCombineWarps), 0, stream, p);
+    e = launch_pdl(attn_kv8_combine_kernel<D, NT>, dim3((ctas + p.stretch - 1) / p.stretch, p.tiles == 1 ? p.q_per_seq * (p.n_q / p.n_kv) : ROWS), dim3(32 * kCombineWarps), 0, stream, p);
     eredu_count_launches(1);
   }
   return e;
@@ -810,6 +824,8 @@ static int attn_kv8(AttnKv8Params& p, int D, int ctas, bool step, cudaStream_t s
   const int rows = p.q_per_seq * (p.n_q / p.n_kv), tile = kv8_tile_rows(rows);
   if (rows >= 1 << 16) return -2;
   p.tiles = (rows + tile - 1) / tile;
+  p.ctas = ctas;
+  p.stretch = static_cast<int>(std::clamp(ctas / (2LL * p.batch * p.n_kv * p.tiles), 1LL, 32LL));
   const uint32_t group = p.n_q / p.n_kv;
   p.per_group = group == 1 ? 0 : static_cast<uint32_t>(((1ULL << 32) + group - 1) / group);
   const long long line = static_cast<long long>(p.batch) * p.n_kv * p.tiles * (p.max_pages / 2 + 1);
