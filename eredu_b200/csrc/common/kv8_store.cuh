@@ -41,8 +41,8 @@ __device__ __forceinline__ float4 load_row4(const __nv_bfloat16* row, int lane) 
   const uint2 u = *reinterpret_cast<const uint2*>(row + 4 * (lane & (D / 4 - 1)));
   return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
 }
-// The D / 4 lanes of a row together: norm, then rotation. WHOLE: all of a row is rotated, in halves, and nothing of that is asked at run time. `turns`: rot / 2 cosines of the row's angles, then as many sines.
-template <int D, bool WHOLE>
+// The D / 4 lanes of a row together: norm, then rotation. `turns`: rot / 2 cosines of the row's angles, then as many sines.
+template <int D>
 __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, const float* w, const float* turns, int lane) {
   const int d = 4 * (lane & (D / 4 - 1));
   if (w != nullptr) {
@@ -55,23 +55,14 @@ __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, co
     x.z *= inv * (w[d + 2] + p.norm_w_off);
     x.w *= inv * (w[d + 3] + p.norm_w_off);
   }
-  if (!WHOLE && p.rot == 0) return x;
-  const int rot = WHOLE ? D : p.rot, half = rot / 2;
-  if (!WHOLE && p.interleaved) {
+  if (p.rot == 0) return x;
+  const int half = p.rot / 2;
+  if (p.interleaved) {
     if (d < p.rot) {
       const float2 c = *reinterpret_cast<const float2*>(turns + d / 2), n = *reinterpret_cast<const float2*>(turns + half + d / 2);
       x = make_float4(x.x * c.x - x.y * n.x, x.y * c.x + x.x * n.x, x.z * c.y - x.w * n.y, x.w * c.y + x.z * n.y);
     }
     return x;
-  }
-  if (WHOLE) {
-    const float4 o = make_float4(__shfl_xor_sync(0xffffffffu, x.x, D / 8), __shfl_xor_sync(0xffffffffu, x.y, D / 8), __shfl_xor_sync(0xffffffffu, x.z, D / 8),
-                                 __shfl_xor_sync(0xffffffffu, x.w, D / 8));
-    const int i = d & (D / 2 - 1);
-    const float4 c = *reinterpret_cast<const float4*>(turns + i);
-    float4 n = *reinterpret_cast<const float4*>(turns + D / 2 + i);
-    if (d < D / 2) n = make_float4(-n.x, -n.y, -n.z, -n.w);
-    return make_float4(x.x * c.x + o.x * n.x, x.y * c.y + o.y * n.y, x.z * c.z + o.z * n.z, x.w * c.w + o.w * n.w);
   }
   const int from = d < half ? lane + half / 4 : d < p.rot ? lane - half / 4 : lane;
   const float4 o = make_float4(__shfl_sync(0xffffffffu, x.x, from), __shfl_sync(0xffffffffu, x.y, from), __shfl_sync(0xffffffffu, x.z, from),
@@ -84,6 +75,50 @@ __device__ __forceinline__ float4 prepared(const Kv8StoreParams& p, float4 x, co
   }
   return x;
 }
+// How a warp holds rows. WHOLE, all of a row is rotated, in halves: a lane has four channels of the lower half and their partners of the upper, so that a rotation
+// stays in the lane and a warp holds two rows of 128 (or four of 64). Else a lane has four neighbouring channels, and `prepared` above finds the partners.
+template <int D, bool WHOLE>
+struct Kv8Rows {
+  static constexpr int PER = WHOLE ? 2 : 1, LANES = D / (4 * PER), ROWS = 32 / LANES;
+  float4 x[PER];
+  static __device__ __forceinline__ int row(int lane) { return LANES == 32 ? 0 : lane / LANES; }
+  static __device__ __forceinline__ int channel(int lane, int j) { return 4 * (lane & (LANES - 1)) + j * (D / 2); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint2 u = *reinterpret_cast<const uint2*>(row + channel(lane, j));
+      x[j] = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // Norm, then rotation, by the LANES lanes of a row together.
+  __device__ __forceinline__ void prepare(const Kv8StoreParams& p, const float* w, const float* turns, int lane) {
+    if constexpr (!WHOLE) {
+      x[0] = prepared<D>(p, x[0], w, turns, lane);
+    } else {
+      float4 &a = x[0], &b = x[1];
+      const int d = channel(lane, 0);
+      if (w != nullptr) {
+        float ss = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z + b.w * b.w;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(ss / static_cast<float>(D) + p.norm_eps);
+        const float* u = w + D / 2;
+        a = make_float4(a.x * (inv * (w[d] + p.norm_w_off)), a.y * (inv * (w[d + 1] + p.norm_w_off)), a.z * (inv * (w[d + 2] + p.norm_w_off)),
+                        a.w * (inv * (w[d + 3] + p.norm_w_off)));
+        b = make_float4(b.x * (inv * (u[d] + p.norm_w_off)), b.y * (inv * (u[d + 1] + p.norm_w_off)), b.z * (inv * (u[d + 2] + p.norm_w_off)),
+                        b.w * (inv * (u[d + 3] + p.norm_w_off)));
+      }
+      const float4 c = *reinterpret_cast<const float4*>(turns + d), n = *reinterpret_cast<const float4*>(turns + D / 2 + d);
+      const float4 lo = make_float4(a.x * c.x - b.x * n.x, a.y * c.y - b.y * n.y, a.z * c.z - b.z * n.z, a.w * c.w - b.w * n.w);
+      b = make_float4(b.x * c.x + a.x * n.x, b.y * c.y + a.y * n.y, b.z * c.z + a.z * n.z, b.w * c.w + a.w * n.w);
+      a = lo;
+    }
+  }
+};
 
 // The scale of a block whose new rows have the largest magnitude `top` (as bits); `before`: that of the rows in front, if any. The larger of the two, and what is
 // no number stays none.
@@ -101,30 +136,28 @@ __device__ __forceinline__ uint32_t kv8_top(uint32_t top, float4 x) {
 template <int D, bool KEYS, int SHARE, bool WHOLE>
 __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, int part,
                                             uint32_t* tops) {
-  constexpr int RPI = 128 / D;              // rows a warp holds at once
-  constexpr int STEPS = kKv8Page / (RPI * SHARE);
+  using Rows = Kv8Rows<D, WHOLE>;
+  constexpr int STRIDE = Rows::ROWS * SHARE, STEPS = kKv8Page / STRIDE;
   const __nv_bfloat16* src = KEYS ? p.k : p.v;
   const int ld = KEYS ? p.ld_k : p.ld_v;
   int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
   float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
-  const int sub = (RPI == 1 ? 0 : lane >> 4) + part * RPI;
-  float4 x[STEPS];
+  const int sub = Rows::row(lane) + part * Rows::ROWS;
+  Rows rows[STEPS];
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int r = i * RPI * SHARE + sub;
-    x[i] = r < n ? load_row4<D>(src + static_cast<size_t>(row + r) * ld + h * D, lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const int r = i * STRIDE + sub;
+    if (r < n) rows[i].load(src + static_cast<size_t>(row + r) * ld + h * D, lane);
+    else rows[i].clear();
   }
   const float before = first > 0 ? *at : 0.f;
   uint32_t top = 0;   // as bits, so that what is no number wins
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    if (i * RPI * SHARE + part * RPI >= n) break;
-    const int r = i * RPI * SHARE + sub;
-    if (KEYS) {
-      const float4 y = prepared<D, WHOLE>(p, x[i], p.k_norm_w, turns + min(r, n - 1) * (WHOLE ? D : p.rot), lane);
-      if (r < n) x[i] = y;
-    }
-    top = kv8_top(top, x[i]);
+    if (i * STRIDE + part * Rows::ROWS >= n) break;
+    if (KEYS) rows[i].prepare(p, p.k_norm_w, turns + min(i * STRIDE + sub, n - 1) * (WHOLE ? D : p.rot), lane);   // (rows behind the last are zero: they stay so)
+#pragma unroll
+    for (int j = 0; j < Rows::PER; ++j) top = kv8_top(top, rows[i].x[j]);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) tops[part] = top;
@@ -133,24 +166,30 @@ __device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, in
   for (int i = 0; i < SHARE; ++i) top = max(top, tops[i]);
   const float scale = kv8_raised(top, first, before);
   const float inv = kv8_inverse(scale);
-  const int c = 4 * (lane & (D / 4 - 1));
   if (first > 0 && scale != before) {
     const float ratio = before * inv;
-    for (int r = sub; r < first; r += RPI * SHARE) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + c);
-      const uint32_t u = *w;
-      *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), ratio);
+    for (int r = sub; r < first; r += STRIDE) {
+#pragma unroll
+      for (int j = 0; j < Rows::PER; ++j) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + Rows::channel(lane, j));
+        const uint32_t u = *w;
+        *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), ratio);
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int r = i * RPI * SHARE + sub;
-    if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x[i].x, x[i].y, x[i].z, x[i].w, inv);
+    const int r = i * STRIDE + sub;
+    if (r >= n) continue;
+#pragma unroll
+    for (int j = 0; j < Rows::PER; ++j) {
+      const float4 x = rows[i].x[j];
+      *reinterpret_cast<uint32_t*>(codes + (first + r) * D + Rows::channel(lane, j)) = kv8_pack(x.x, x.y, x.z, x.w, inv);
+    }
   }
   __syncthreads();   // the words, and the scale that others may still be reading
   if (lane == 0 && part == 0) *at = scale;
 }
-
 // The same for a few rows by one warp that has other things in its registers: the rows are looked at twice. `before`: the block's scale.
 template <int D, bool KEYS>
 __device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, float before) {
@@ -161,7 +200,7 @@ __device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int 
   auto row_of = [&](int r) {
     const int in = min(r, n - 1);
     float4 x = load_row4<D>((KEYS ? p.k : p.v) + static_cast<size_t>(row + in) * (KEYS ? p.ld_k : p.ld_v) + h * D, lane);
-    return KEYS ? prepared<D, false>(p, x, p.k_norm_w, turns + in * p.rot, lane) : x;
+    return KEYS ? prepared<D>(p, x, p.k_norm_w, turns + in * p.rot, lane) : x;
   };
   uint32_t top = 0;
 #pragma unroll 1

@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const int row = (i * kKv8Warps + warp) * RPI + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
     const bool in = row < rows;
     float4 x = query[i];
-    if (STEP) x = prepared<D, false>(p.st, x, p.st.q_norm_w, turns_s + (kv8_token(p, r0 + min(row, rows - 1)) - token0) * p.st.rot, lane);
+    if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (kv8_token(p, r0 + min(row, rows - 1)) - token0) * p.st.rot, lane);
     if (!in) x = make_float4(0.f, 0.f, 0.f, 0.f);
     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))), max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
 #pragma unroll

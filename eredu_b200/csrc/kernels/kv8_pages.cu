@@ -22,7 +22,7 @@ constexpr int kStoreRows = 32;      // a tile of 16 rows and what the last run o
 // grid (tiles of rows, n_kv)
 template <int D, bool WHOLE>
 __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams p) {
-  constexpr int RPI = 128 / D;
+  using Rows = Kv8Rows<D, WHOLE>;
   extern __shared__ __align__(16) float turns[];          // [rows of the tile and the last run][rot / 2 cosines, rot / 2 sines]
   __shared__ int run_row[kKv8Page], run_len[kKv8Page];
   __shared__ long long run_slot[kKv8Page];
@@ -71,28 +71,29 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams
     else store_block<D, false, kStoreShare, WHOLE>(p, row0 + at, run_len[i], first, cell, h0, turns, lane, warp - kStoreShare, tops + kStoreShare);
   }
   // ---- query rows of this head, four at a time on their way
-  constexpr int WARPS = kStoreThreads / 32, DEEP = 4;
-  const int mine = p.q_out == nullptr ? 1 : p.n_q / p.n_kv, items = p.q_out == nullptr ? 0 : rows * mine, sub = RPI == 1 ? 0 : lane >> 4;
+  constexpr int DEEP = 4, STRIDE = kStoreThreads / 32 * Rows::ROWS;
+  const int mine = p.q_out == nullptr ? 1 : p.n_q / p.n_kv, items = p.q_out == nullptr ? 0 : rows * mine, sub = Rows::row(lane);
   const uint32_t per_mine = ((1u << 20) + mine - 1) / mine;     // item / mine by a product: exact below 2^20 / mine, and there are 16 mine of them at most
-  float4 query[DEEP];
-  auto load_queries = [&](int i0) {
+  for (int i0 = warp * Rows::ROWS; i0 < items; i0 += STRIDE * DEEP) {
+    Rows query[DEEP];
 #pragma unroll
     for (int j = 0; j < DEEP; ++j) {
-      const int item = min(i0 + j * WARPS * RPI + sub, items - 1), r = static_cast<int>(item * per_mine >> 20);
-      query[j] = load_row4<D>(p.q + static_cast<size_t>(row0 + r) * p.ld_q + (h0 * mine + item - r * mine) * D, lane);
+      const int item = min(i0 + j * STRIDE + sub, items - 1), r = static_cast<int>(item * per_mine >> 20);
+      query[j].load(p.q + static_cast<size_t>(row0 + r) * p.ld_q + (h0 * mine + item - r * mine) * D, lane);
     }
-  };
-  for (int i0 = warp * RPI; i0 < items; i0 += WARPS * RPI * DEEP) {
-    load_queries(i0);
 #pragma unroll
     for (int j = 0; j < DEEP; ++j) {
-      const int item = i0 + j * WARPS * RPI + sub, r = static_cast<int>(min(item, items - 1) * per_mine >> 20), head = h0 * mine + min(item, items - 1) - r * mine;
-      if (i0 + j * WARPS * RPI >= items) break;
-      const float4 x = prepared<D, WHOLE>(p, query[j], p.q_norm_w, turns + r * rot, lane);
-      const size_t at = (static_cast<size_t>(row0 + r) * p.n_q + head) * D + 4 * (lane & (D / 4 - 1));
+      const int item = i0 + j * STRIDE + sub, r = static_cast<int>(min(item, items - 1) * per_mine >> 20), head = h0 * mine + min(item, items - 1) - r * mine;
+      if (i0 + j * STRIDE >= items) break;
+      query[j].prepare(p, p.q_norm_w, turns + r * rot, lane);
       if (item >= items) continue;
-      if (p.q_out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.q_out) + at) = x;
-      else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.q_out) + at) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+      const size_t at = (static_cast<size_t>(row0 + r) * p.n_q + head) * D;
+#pragma unroll
+      for (int i = 0; i < Rows::PER; ++i) {
+        const float4 x = query[j].x[i];
+        if (p.q_out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.q_out) + at + Rows::channel(lane, i)) = x;
+        else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.q_out) + at + Rows::channel(lane, i)) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+      }
     }
   }
 }
@@ -200,7 +201,7 @@ extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void
                                float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
   if (M <= 0) return 0;
   if ((D != 64 && D != 128) || n_kv <= 0 || num_pages <= 0 || rot < 0 || rot > D || rot % 8 != 0 || ld_q % 4 != 0 || ld_k % 4 != 0 || ld_v % 4 != 0 ||
-      (q_out != nullptr && (n_q <= 0 || n_q % n_kv != 0)))
+      (q_out != nullptr && (n_q <= 0 || n_q % n_kv != 0 || n_q / n_kv > 256)))
     return -2;
   Kv8StoreParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
