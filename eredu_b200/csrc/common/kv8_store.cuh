@@ -83,12 +83,15 @@ struct Kv8Rows {
   float4 x[PER];
   static __device__ __forceinline__ int row(int lane) { return LANES == 32 ? 0 : lane / LANES; }
   static __device__ __forceinline__ int channel(int lane, int j) { return 4 * (lane & (LANES - 1)) + j * (D / 2); }
-  __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane) {
+  __device__ __forceinline__ void take(const uint2 (&u)[PER]) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint2 u = *reinterpret_cast<const uint2*>(row + channel(lane, j));
-      x[j] = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
-    }
+    for (int j = 0; j < PER; ++j) x[j] = make_float4(bf16_lo(u[j].x), bf16_hi(u[j].x), bf16_lo(u[j].y), bf16_hi(u[j].y));
+  }
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int lane) {
+    uint2 u[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) u[j] = *reinterpret_cast<const uint2*>(row + channel(lane, j));
+    take(u);
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -131,65 +134,6 @@ __device__ __forceinline__ uint32_t kv8_top(uint32_t top, float4 x) {
   return max(max(top, __float_as_uint(fabsf(x.z))), __float_as_uint(fabsf(x.w)));
 }
 
-// Rows [row, row + n) of head h into the block at `cell` = (page, head), from offset `first` on. SHARE warps together, all threads of the CTA; `part`: which of them
-// this is, `tops`: a word for each.
-template <int D, bool KEYS, int SHARE, bool WHOLE>
-__device__ __forceinline__ void store_block(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, int part,
-                                            uint32_t* tops) {
-  using Rows = Kv8Rows<D, WHOLE>;
-  constexpr int STRIDE = Rows::ROWS * SHARE, STEPS = kKv8Page / STRIDE;
-  const __nv_bfloat16* src = KEYS ? p.k : p.v;
-  const int ld = KEYS ? p.ld_k : p.ld_v;
-  int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
-  float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
-  const int sub = Rows::row(lane) + part * Rows::ROWS;
-  Rows rows[STEPS];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int r = i * STRIDE + sub;
-    if (r < n) rows[i].load(src + static_cast<size_t>(row + r) * ld + h * D, lane);
-    else rows[i].clear();
-  }
-  const float before = first > 0 ? *at : 0.f;
-  uint32_t top = 0;   // as bits, so that what is no number wins
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    if (i * STRIDE + part * Rows::ROWS >= n) break;
-    if (KEYS) rows[i].prepare(p, p.k_norm_w, turns + min(i * STRIDE + sub, n - 1) * (WHOLE ? D : p.rot), lane);   // (rows behind the last are zero: they stay so)
-#pragma unroll
-    for (int j = 0; j < Rows::PER; ++j) top = kv8_top(top, rows[i].x[j]);
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) tops[part] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < SHARE; ++i) top = max(top, tops[i]);
-  const float scale = kv8_raised(top, first, before);
-  const float inv = kv8_inverse(scale);
-  if (first > 0 && scale != before) {
-    const float ratio = before * inv;
-    for (int r = sub; r < first; r += STRIDE) {
-#pragma unroll
-      for (int j = 0; j < Rows::PER; ++j) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + Rows::channel(lane, j));
-        const uint32_t u = *w;
-        *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), ratio);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int r = i * STRIDE + sub;
-    if (r >= n) continue;
-#pragma unroll
-    for (int j = 0; j < Rows::PER; ++j) {
-      const float4 x = rows[i].x[j];
-      *reinterpret_cast<uint32_t*>(codes + (first + r) * D + Rows::channel(lane, j)) = kv8_pack(x.x, x.y, x.z, x.w, inv);
-    }
-  }
-  __syncthreads();   // the words, and the scale that others may still be reading
-  if (lane == 0 && part == 0) *at = scale;
-}
 // The same for a few rows by one warp that has other things in its registers: the rows are looked at twice. `before`: the block's scale.
 template <int D, bool KEYS>
 __device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, float before) {

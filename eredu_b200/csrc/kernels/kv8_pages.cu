@@ -17,82 +17,143 @@ namespace eredu {
 // partner of a rotation sits `rot / 8` lanes further. The angles of a tile of rows are computed once for the head's keys and its query heads.
 // 4096 rows, 32 heads of 128 over 8: a warp to a run's keys, in 128 registers, 92 us.
 constexpr int kStoreThreads = 256, kStoreShare = kStoreThreads / 64;   // half of the warps for keys, half for values
+constexpr int kStoreRoom = 3 * 148;
 constexpr int kStoreRows = 32;      // a tile of 16 rows and what the last run of it has behind them
 
 // grid (tiles of rows, n_kv)
 template <int D, bool WHOLE>
-__global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(Kv8StoreParams p) {
+__global__ void __launch_bounds__(kStoreThreads, 4) kv8_store_kernel(Kv8StoreParams p) {
   using Rows = Kv8Rows<D, WHOLE>;
+  constexpr int PER = Rows::PER, SHARED = Rows::ROWS * kStoreShare, STEPS = kKv8Page / SHARED;   // rows that the warps of a run hold at once, and how often
   extern __shared__ __align__(16) float turns[];          // [rows of the tile and the last run][rot / 2 cosines, rot / 2 sines]
-  __shared__ int run_row[kKv8Page], run_len[kKv8Page];
-  __shared__ long long run_slot[kKv8Page];
-  __shared__ uint32_t tops[kStoreThreads / 32];
-  __shared__ int runs, behind;
+  __shared__ uint32_t tops[2][kStoreShare];
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
   const int row0 = blockIdx.x * p.tile, rows = min(p.tile, p.M - row0), h0 = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rot = WHOLE ? D : p.rot, half = rot / 2;
-  if (warp == 0) {
-    // lane r has the slots of rows r - 1 and r of the tile and the 16 behind it: a row continues the one in front where its slot is the next of the same page
-    const int r = row0 + lane;
-    const bool known = r < p.M && lane < rows + kKv8Page;
-    const long long slot = known ? p.slots[r] : -1, front = known && r > 0 ? p.slots[r - 1] : -1;
-    const bool follows = slot >= 0 && (slot & 15) != 0 && front == slot - 1;
-    bool begins = lane < rows && slot >= 0 && !follows;
-    if (begins && (slot >> 4) >= p.num_pages) {
-      report_status(p.status, kStatusBadArgument);
-      begins = false;
-    }
-    const uint32_t mask = __ballot_sync(0xffffffffu, begins), more = __ballot_sync(0xffffffffu, follows);
-    // (a tile of 16 rows and 15 more at most: what follows the last row of the warp's 32 cannot belong to a run of this tile)
-    const int n = begins ? 1 + __ffs(~(more >> lane >> 1)) - 1 : 0;
-    if (begins) {
-      const int i = __popc(mask & ((1u << lane) - 1));
-      run_row[i] = lane;
-      run_len[i] = n;
-      run_slot[i] = slot;
-    }
-    const int end = __reduce_max_sync(0xffffffffu, begins ? lane + n : 0);
-    if (lane == 0) {
-      runs = __popc(mask);
-      behind = max(rows, end);
-    }
-  }
-  __syncthreads();
-  for (int r = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); r < behind; r += kStoreThreads / (D / 2))
-    if (i < half) turn_of(p.positions[row0 + r], p.inv_freq[i], p.attn_factor, turns[r * rot + i], turns[r * rot + half + i]);
-  __syncthreads();
-  for (int i = 0; i < runs; ++i) {
-    const int at = run_row[i];
-    const long long cell = (run_slot[i] >> 4) * p.n_kv + h0;
-    const int first = static_cast<int>(run_slot[i] & 15);
-    if (warp < kStoreShare) store_block<D, true, kStoreShare, WHOLE>(p, row0 + at, run_len[i], first, cell, h0, turns + at * rot, lane, warp, tops);
-    else store_block<D, false, kStoreShare, WHOLE>(p, row0 + at, run_len[i], first, cell, h0, turns, lane, warp - kStoreShare, tops + kStoreShare);
-  }
-  // ---- query rows of this head, four at a time on their way
+  // lane r has the slots of rows r - 1 and r of the tile and the 16 behind it: a row continues the one in front where its slot is the next of the same page
+  const bool known = row0 + lane < p.M && lane < rows + kKv8Page;
+  const long long slot = known ? p.slots[row0 + lane] : -1, front = known && row0 + lane > 0 ? p.slots[row0 + lane - 1] : -1;
+  // ---- query rows of this head, a warp has DEEP (times as many as it holds at once) on their way
   constexpr int DEEP = 4, STRIDE = kStoreThreads / 32 * Rows::ROWS;
   const int mine = p.q_out == nullptr ? 1 : p.n_q / p.n_kv, items = p.q_out == nullptr ? 0 : rows * mine, sub = Rows::row(lane);
   const uint32_t per_mine = ((1u << 20) + mine - 1) / mine;     // item / mine by a product: exact below 2^20 / mine, and there are 16 mine of them at most
-  for (int i0 = warp * Rows::ROWS; i0 < items; i0 += STRIDE * DEEP) {
-    Rows query[DEEP];
+  uint2 query[DEEP][PER];
+  auto load_queries = [&](int i0) {
 #pragma unroll
     for (int j = 0; j < DEEP; ++j) {
       const int item = min(i0 + j * STRIDE + sub, items - 1), r = static_cast<int>(item * per_mine >> 20);
-      query[j].load(p.q + static_cast<size_t>(row0 + r) * p.ld_q + (h0 * mine + item - r * mine) * D, lane);
+      const __nv_bfloat16* from = p.q + static_cast<size_t>(row0 + r) * p.ld_q + (h0 * mine + item - r * mine) * D;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) query[j][i] = *reinterpret_cast<const uint2*>(from + Rows::channel(lane, i));
     }
+  };
+  if (warp * Rows::ROWS < items) load_queries(warp * Rows::ROWS);
+  // ---- the tile's runs, by every warp for itself: bits of `begin`; their first lanes have length and slot
+  const bool follows = slot >= 0 && (slot & 15) != 0 && front == slot - 1;
+  bool begins = lane < rows && slot >= 0 && !follows;
+  if (begins && (slot >> 4) >= p.num_pages) {
+    report_status(p.status, kStatusBadArgument);
+    begins = false;
+  }
+  uint32_t begin = __ballot_sync(0xffffffffu, begins);
+  const uint32_t more = __ballot_sync(0xffffffffu, follows);
+  // (a tile of 16 rows and 15 more at most: what follows the last row of the warp's 32 cannot belong to a run of this tile)
+  const int length = begins ? __ffs(~(more >> lane >> 1)) : 0;
+  const int behind = max(rows, __reduce_max_sync(0xffffffffu, begins ? lane + length : 0));
+  // ---- a run: half of the warps have its keys, half its values
+  const bool keys = warp < kStoreShare;
+  const int part = keys ? warp : warp - kStoreShare, mine0 = sub + part * Rows::ROWS, ld = keys ? p.ld_k : p.ld_v;
+  const __nv_bfloat16* src = (keys ? p.k : p.v) + static_cast<size_t>(row0) * ld + h0 * D;
+  uint2 raw[STEPS][PER];
+  int at = 0, n = 0, first = 0;
+  size_t cell = 0;
+  float before = 0.f;
+  auto next_run = [&]() {
+    at = __ffs(begin) - 1;
+    begin &= begin - 1;
+    n = __shfl_sync(0xffffffffu, length, at);
+    const long long to = __shfl_sync(0xffffffffu, slot, at);
+    first = static_cast<int>(to & 15);
+    cell = static_cast<size_t>(to >> 4) * p.n_kv + h0;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int r = i * SHARED + mine0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) raw[i][j] = r < n ? *reinterpret_cast<const uint2*>(src + static_cast<size_t>(at + r) * ld + Rows::channel(lane, j)) : make_uint2(0, 0);
+    }
+    before = first > 0 ? (keys ? p.k_scales : p.v_scales)[cell] : 0.f;
+  };
+  bool left = begin != 0;
+  if (left) next_run();
+  for (int r = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2); r < behind; r += kStoreThreads / (D / 2))
+    if (i < half) turn_of(p.positions[row0 + r], p.inv_freq[i], p.attn_factor, turns[r * rot + i], turns[r * rot + half + i]);
+  __syncthreads();
+  while (left) {
+    const int at_now = at, n_now = n, first_now = first;
+    const float before_now = before;
+    int8_t* codes = (keys ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
+    float* scale_at = (keys ? p.k_scales : p.v_scales) + cell;
+    Rows held[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) held[i].take(raw[i]);
+    left = begin != 0;
+    if (left) next_run();
+    uint32_t top = 0;   // as bits, so that what is no number wins
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (i * SHARED + part * Rows::ROWS >= n_now) break;
+      if (keys) held[i].prepare(p, p.k_norm_w, turns + (at_now + min(i * SHARED + mine0, n_now - 1)) * rot, lane);   // (rows behind the last are zero: they stay so)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) top = kv8_top(top, held[i].x[j]);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[keys ? 0 : 1][part] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kStoreShare; ++i) top = max(top, tops[keys ? 0 : 1][i]);
+    const float scale = kv8_raised(top, first_now, before_now), inv = kv8_inverse(scale);
+    if (first_now > 0 && scale != before_now) {
+      const float ratio = before_now * inv;
+      for (int r = mine0; r < first_now; r += SHARED) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + Rows::channel(lane, j));
+          const uint32_t u = *w;
+          *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), ratio);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int r = i * SHARED + mine0;
+      if (r >= n_now) continue;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float4 x = held[i].x[j];
+        *reinterpret_cast<uint32_t*>(codes + (first_now + r) * D + Rows::channel(lane, j)) = kv8_pack(x.x, x.y, x.z, x.w, inv);
+      }
+    }
+    if (lane == 0 && part == 0) *scale_at = scale;
+    if (left) __syncthreads();   // the next run's words
+  }
+  for (int i0 = warp * Rows::ROWS; i0 < items; i0 += STRIDE * DEEP) {
+    if (i0 >= STRIDE * DEEP) load_queries(i0);
 #pragma unroll
     for (int j = 0; j < DEEP; ++j) {
       const int item = i0 + j * STRIDE + sub, r = static_cast<int>(min(item, items - 1) * per_mine >> 20), head = h0 * mine + min(item, items - 1) - r * mine;
       if (i0 + j * STRIDE >= items) break;
-      query[j].prepare(p, p.q_norm_w, turns + r * rot, lane);
+      Rows x;
+      x.take(query[j]);
+      x.prepare(p, p.q_norm_w, turns + r * rot, lane);
       if (item >= items) continue;
       const size_t at = (static_cast<size_t>(row0 + r) * p.n_q + head) * D;
 #pragma unroll
       for (int i = 0; i < Rows::PER; ++i) {
-        const float4 x = query[j].x[i];
-        if (p.q_out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.q_out) + at + Rows::channel(lane, i)) = x;
-        else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.q_out) + at + Rows::channel(lane, i)) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+        const float4 y = x.x[i];
+        if (p.q_out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.q_out) + at + Rows::channel(lane, i)) = y;
+        else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.q_out) + at + Rows::channel(lane, i)) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
       }
     }
   }
@@ -231,8 +292,9 @@ extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void
   p.norm_eps = norm_eps;
   p.norm_w_off = norm_w_off;
   p.status = status;
-  // a key / value head with its query heads per CTA, and a row or, where there are many, 16, in which most runs are whole
-  p.tile = M <= 256 ? 1 : 16;
+  // a key / value head with its query heads per CTA, and as few rows as find room at once
+  p.tile = 1;
+  while (p.tile < kKv8Page && static_cast<long long>((M + p.tile - 1) / p.tile) * n_kv > kStoreRoom) p.tile *= 2;
   const dim3 grid((M + p.tile - 1) / p.tile, n_kv);
   const size_t smem = static_cast<size_t>(kStoreRows) * rot * sizeof(float);
   const bool whole = rot == D && interleaved == 0;
