@@ -304,12 +304,13 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     """Split factor of the decode kernel for 8-bit pages: 1 to 8 CTAs for a sequence and head, or 0 for even shares.
 
     Three CTAs fit an SM, clusters not quite: as many splits as find room on nine tenths of that (two where that is all), with a pair of pages for each of a CTA's
-    four warps. Even shares cost a second kernel and the way to a CTA's place, 3 to 5 us, and pay where clusters leave SMs empty and a CTA has many pairs (us, 32
-    heads of 128 over 8, even / best cluster: one sequence of 8192 tokens 16 / 14, of 32768 22 / 33; four of 32768 47 / 52; eight of 8192 28 / 26, of 32768
-    85 / 88; 20 of 8192 50 / 53).
+    four warps. Even shares cost a second kernel and the way to a CTA's place, 2 to 4 us, and pay where clusters leave SMs empty and a CTA has many pairs: more
+    than 48 of eight splits, which most often are all that a cluster may have and not all there is room for, and more than 84 of fewer (us, 32 heads of 128 over 8,
+    even / best cluster: one sequence of 8192 tokens 13.3 / 11.9, of 12000 14.5 / 13.9, of 16384 15.2 / 17.6, of 65536 32 / 54; four of 8192 16.4 / 15.3, of 16384
+    22.5 / 26.0; eight of 8192 24.2 / 23.1, of 12000 35.6 / 34.2, of 16384 43.2 / 43.6, of 32768 79 / 81; 20 of 8192 51 / 52).
     More sequences and heads than that go one CTA each, or, where they are long enough for the tail of the longest to count, two or three or even shares
-    (us with 1 / 2 / 3 / even: 32 of 1024 15 / 18 / 18 / 18, of 4096 48 / 47 / 43 / 44, of 8192 84 / 86 / 74 / 73; 64 of 2048 43 / 44 / 48 / 44, of 4096 77 / 73 / 76 / 74,
-    of 8192 156 / 142 / 146 / 142, with four new tokens 176 / 156 / 159 / 154)."""
+    (us with 1 / 2 / 3 / even: 32 of 1024 16 / 17 / 17 / 19, of 4096 48 / 46 / 42 / 44, of 8192 85 / 84 / 73 / 73; 64 of 2048 43 / 43 / 46 / 46, of 4096 77 / 72 / 75 / 74,
+    of 8192 152 / 140 / 135 / 144 captured and 149 / 142 / 146 / 142 call by call; with four new tokens 175 / 156 / 158 / 155)."""
     tiles = -(-max(rows, 1) // (8 if rows <= 8 else 16))
     heads = max(1, batch * n_kv * tiles)
     pairs = max(1, -(-max_kv_len // (2 * PAGE)))
@@ -323,7 +324,7 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     splits = max(1, min(max(2, room * 9 // 10 // heads), pairs // 4, CLUSTER))
     if splits == 7:             # six or eight fill a GPC better
         splits = 6
-    return 0 if pairs > 96 * splits else splits
+    return 0 if pairs > (48 if splits == CLUSTER else 84) * splits else splits
 
 
 def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len):
