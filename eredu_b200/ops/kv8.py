@@ -308,9 +308,10 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     than 48 of eight splits, which most often are all that a cluster may have and not all there is room for, and more than 84 of fewer (us, 32 heads of 128 over 8,
     even / best cluster: one sequence of 8192 tokens 13.3 / 11.9, of 12000 14.5 / 13.9, of 16384 15.2 / 17.6, of 65536 32 / 54; four of 8192 16.4 / 15.3, of 16384
     22.5 / 26.0; eight of 8192 24.2 / 23.1, of 12000 35.6 / 34.2, of 16384 43.2 / 43.6, of 32768 79 / 81; 20 of 8192 51 / 52).
-    More sequences and heads than that go one CTA each, or, where they are long enough for the tail of the longest to count, two or three or even shares
-    (us with 1 / 2 / 3 / even: 32 of 1024 16 / 17 / 17 / 19, of 4096 48 / 46 / 42 / 44, of 8192 85 / 84 / 73 / 73; 64 of 2048 43 / 43 / 46 / 46, of 4096 77 / 72 / 75 / 74,
-    of 8192 152 / 140 / 135 / 144 captured and 149 / 142 / 146 / 142 call by call; with four new tokens 175 / 156 / 158 / 155)."""
+    More sequences and heads than that go one CTA each, or, where they are long enough for the tail of the longest to count, two or three
+    (us with 1 / 2 / 3 / even: 32 of 1024 16 / 17 / 17 / 19, of 4096 48 / 46 / 42 / 44; 64 of 2048 43 / 43 / 46 / 46, of 4096 77 / 72 / 75 / 74), or even shares where
+    they are longer still. Three splits are up to a twentieth faster there when all are about as long, and far slower when one is longer than the others
+    (3 / even: 64 of 8192 136 / 142, 32 of 16384 132 / 135, one of 16384 with 31 of 1024 48 / 23; 64 of 8192 with four new tokens 158 / 155)."""
     tiles = -(-max(rows, 1) // (8 if rows <= 8 else 16))
     heads = max(1, batch * n_kv * tiles)
     pairs = max(1, -(-max_kv_len // (2 * PAGE)))
