@@ -43,4 +43,12 @@ __device__ __forceinline__ uint32_t kv8_parted(uint32_t word) {
   return h;
 }
 
+
+// Where 16-byte piece c of token row r lies in a page's half of a ring slot: pieces change places within 128 bytes, so that the eight rows of an 8 x 8 matrix
+// that ldmatrix reads meet all banks.
+template <int D>
+__device__ __forceinline__ int kv8_piece(int r, int c) {
+  return D == 128 ? r * 128 + (c ^ (r & 7)) * 16 : (r >> 1) * 128 + (((r & 1) << 2 | c) ^ (r >> 1 & 3)) * 16;
+}
+
 }  // namespace eredu

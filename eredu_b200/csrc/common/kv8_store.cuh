@@ -134,37 +134,72 @@ __device__ __forceinline__ uint32_t kv8_top(uint32_t top, float4 x) {
   return max(max(top, __float_as_uint(fabsf(x.z))), __float_as_uint(fabsf(x.w)));
 }
 
-// The same for a few rows by one warp that has other things in its registers: the rows are looked at twice. `before`: the block's scale.
+constexpr int kKv8StepTokens = 8;   // new tokens of a sequence in a step that writes its own rows
+// The keys or values of a step's new rows, as they are, on their way to one warp: two registers for every 128 values.
+template <int D>
+struct Kv8Few {
+  static constexpr int RPI = 128 / D, N = kKv8StepTokens / RPI;
+  uint2 raw[N];
+  // rows [0, n) of head h from `from` on
+  __device__ __forceinline__ void load(const __nv_bfloat16* from, int ld, int n, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * RPI < n) raw[i] = *reinterpret_cast<const uint2*>(from + static_cast<size_t>(min(i * RPI + lane / (D / 4), n - 1)) * ld + 4 * (lane & (D / 4 - 1)));
+  }
+  // row `at`, one of this lane's
+  __device__ __forceinline__ float4 row(int at) const {
+    uint2 u = raw[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      if (at / RPI == i) u = raw[i];
+    return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+  }
+};
+
+// Rows [row, row + n) of a step, of `few`, into the block at `cell` = (page, head), from offset `first` on, by one warp that has other things in its registers: they are
+// looked at twice, one after the other. A lane has rows lane / (D / 4) + RPI i of them (those in front of `row`, and behind, do not count). `before`: the block's
+// scale. `held`: where the page's codes of the head lie in shared memory as well, if they do (kv8_piece). Gives the scale.
 template <int D, bool KEYS>
-__device__ __forceinline__ void store_few(const Kv8StoreParams& p, int row, int n, int first, long long cell, int h, const float* turns, int lane, float before) {
+__device__ __forceinline__ float store_few(const Kv8StoreParams& p, const Kv8Few<D>& few, int row, int n, int first, long long cell, const float* turns, int lane, float before,
+                                           uint8_t* held) {
   constexpr int RPI = 128 / D;
   int8_t* codes = (KEYS ? p.k_codes : p.v_codes) + cell * (kKv8Page * D);
-  float* at = (KEYS ? p.k_scales : p.v_scales) + cell;
-  const int sub = RPI == 1 ? 0 : lane >> 4, c = 4 * (lane & (D / 4 - 1));
-  auto row_of = [&](int r) {
-    const int in = min(r, n - 1);
-    float4 x = load_row4<D>((KEYS ? p.k : p.v) + static_cast<size_t>(row + in) * (KEYS ? p.ld_k : p.ld_v) + h * D, lane);
-    return KEYS ? prepared<D>(p, x, p.k_norm_w, turns + in * p.rot, lane) : x;
+  const int sub = RPI == 1 ? 0 : lane >> 4, c = 4 * (lane & (D / 4 - 1)), row0 = row / RPI * RPI;
+  auto row_of = [&](int r) {      // (all lanes of the warp)
+    const float4 y = few.row(r);
+    return KEYS ? prepared<D>(p, y, p.k_norm_w, turns + min(r, row + n - 1) * p.rot, lane) : y;
   };
+  auto beside = [&](int r) { return reinterpret_cast<uint32_t*>(held + kv8_piece<D>(r, c >> 4) + (c & 15)); };
   uint32_t top = 0;
+  float4 x;
 #pragma unroll 1
-  for (int r = sub; r - sub < n; r += RPI) top = kv8_top(top, row_of(r));
+  for (int r = row0 + sub; r - sub < row + n; r += RPI) {
+    x = row_of(r);
+    if (r >= row && r < row + n) top = kv8_top(top, x);
+  }
   top = __reduce_max_sync(0xffffffffu, top);
   const float scale = kv8_raised(top, first, before), inv = kv8_inverse(scale);
   if (first > 0 && scale != before) {
 #pragma unroll 1
     for (int r = sub; r < first; r += RPI) {
       uint32_t* w = reinterpret_cast<uint32_t*>(codes + r * D + c);
-      const uint32_t u = *w;
-      *w = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), before * inv);
+      const uint32_t u = held != nullptr ? *beside(r) : *w;
+      const uint32_t now = kv8_pack(kv8_code(u, 0), kv8_code(u, 1), kv8_code(u, 2), kv8_code(u, 3), before * inv);
+      *w = now;
+      if (held != nullptr) *beside(r) = now;
     }
   }
 #pragma unroll 1
-  for (int r = sub; r - sub < n; r += RPI) {
-    const float4 x = row_of(r);
-    if (r < n) *reinterpret_cast<uint32_t*>(codes + (first + r) * D + c) = kv8_pack(x.x, x.y, x.z, x.w, inv);
+  for (int r = row0 + sub; r - sub < row + n; r += RPI) {
+    if (row + n - row0 > RPI) x = row_of(r);
+    const uint32_t now = kv8_pack(x.x, x.y, x.z, x.w, inv);
+    if (r >= row && r < row + n) {
+      *reinterpret_cast<uint32_t*>(codes + (first + r - row) * D + c) = now;
+      if (held != nullptr) *beside(first + r - row) = now;
+    }
   }
-  if (lane == 0) *at = scale;
+  if (lane == 0) (KEYS ? p.k_scales : p.v_scales)[cell] = scale;
+  return scale;
 }
 
 }  // namespace eredu

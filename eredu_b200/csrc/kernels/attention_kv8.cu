@@ -59,7 +59,6 @@ struct AttnKv8Params {
 };
 // Token of query row r among those that share a key / value head (r < 2^16: exact), in place of a division of some thirty instructions.
 __device__ __forceinline__ int kv8_token(const AttnKv8Params& p, int r) { return p.per_group == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.per_group)); }
-constexpr int kKv8StepTokens = 8;   // new tokens that the rows of a tile span in a step
 
 constexpr int kKv8Warps = 4;         // three CTAs of four warps to an SM: four pages a warp fill shared memory
 constexpr int kKv8Threads = 32 * kKv8Warps;
@@ -67,6 +66,7 @@ constexpr int kKv8Cluster = 8;      // splits that meet in a cluster
 // log2 units by which a score may pass the maximum in use, and a probability's weight the probability: what they give together, 2^14, f16 holds.
 constexpr float kKv8Slack = 6.f, kKv8Weight = 8.f;
 constexpr float kLowest = -3.402823466e38f;
+constexpr uint32_t kNone = 0xffffffffu;   // bits of no scale
 // Integer sums start at the bits of 1.5 * 2^23: as floats they are that plus the sum, which stays below 2^22 (128 * 127 * 255).
 constexpr int kMagicBits = 0x4b400000;
 constexpr float kMagic = 12582912.f;
@@ -194,12 +194,6 @@ __device__ __forceinline__ void store_out(__nv_bfloat16* to, float4 v, float up)
 }
 
 __device__ __forceinline__ float exp2_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }   // -126 <= e <= 127
-// Where 16-byte piece c of token row r lies in a page's half of a ring slot: pieces change places within 128 bytes, so that the eight rows of an 8 x 8 matrix
-// that ldmatrix reads meet all banks.
-template <int D>
-__device__ __forceinline__ int kv8_piece(int r, int c) {
-  return D == 128 ? r * 128 + (c ^ (r & 7)) * 16 : (r >> 1) * 128 + (((r & 1) << 2 | c) ^ (r >> 1 & 3)) * 16;
-}
 // Four values of a query row times two powers of two, rounded to 16 bits: their upper bytes and their lower bytes.
 __device__ __forceinline__ uint2 query_bytes(float4 x, float up, float more) {
   auto whole = [&](float v) { return static_cast<uint32_t>(min(__float2int_rn(v * up * more), 32767)); };
@@ -214,7 +208,8 @@ template <int D, int NT, bool EVEN, bool STEP>
 __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params p) {
   constexpr int ROWS = 8 * NT, KC = D / 64, STEPS = D / 16, WIDE = D + 4;   // WIDE: lanes of four rows meet all banks
   constexpr int PAGE_BYTES = 2 * kKv8Page * D;
-  extern __shared__ __align__(16) uint8_t smem[];
+  // on lines of 128 bytes: rings 16 bytes off them cost 17 % (32 sequences of 2048 29.8 -> 34.9 us)
+  extern __shared__ __align__(128) uint8_t smem[];
   // queries as bytes [NT][2 KC][32 lanes], then the rings [warps][2 pairs][2 pages]; behind the last page, what the warps have gathered takes their place
   uint4* q_s = reinterpret_cast<uint4*>(smem);
   uint8_t* rings = smem + NT * 2 * KC * 512;
@@ -225,6 +220,7 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
   float* weight = reinterpret_cast<float*>(row_s + ROWS);         // [warps, or splits][ROWS]
   __shared__ float back_s[ROWS], up_s[ROWS];
   __shared__ size_t out_s[ROWS];          // where a row's output goes
+  __shared__ float scale_s[kKv8Warps];    // scales of blocks with new rows
   __shared__ __align__(16) float turns_s[STEP ? kKv8StepTokens * D : 1];   // cosines and sines of the tile's tokens
   pdl_launch_early();
   trace_mark(kTraceAttnDecode, kTraceStart);
@@ -318,12 +314,9 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       }
     }
   };
-  // a pair that new rows are written to is fetched behind the write
-  const int new_page = STEP ? pos_new / kKv8Page : 0x7fffffff;
-  auto waits = [&](int turn) { return STEP && page0 + 2 * (warp + kKv8Warps * turn) + 1 >= new_page; };
-  if (turns > 0 && !waits(0)) fetch(0);
+  if (turns > 0) fetch(0);
   cp_async_commit();
-  if (turns > 1 && !waits(1)) fetch(1);
+  if (turns > 1) fetch(1);
   cp_async_commit();
 
   constexpr int RPI = 128 / D;                          // query rows a warp holds at once, four channels a lane
@@ -335,14 +328,23 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
       if (i < half) turn_of(positions[n], p.st.inv_freq[i], p.st.attn_factor, turns_s[n * p.st.rot + i], turns_s[n * p.st.rot + half + i]);
     __syncthreads();
   }
-  // this warp's share of the write: keys or values of a page in this part (there are two such pages at most)
-  const int my_page = STEP ? max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) + (warp >> 1) : 0;
+  // The new rows lie in two pages of this part at most, from new_page on. Warps 0 and 2 write their keys, 1 and 3 their values - to memory, and to the ring where
+  // the page is on its way to it already.
+  const int new_page = STEP ? max(page0, pos_new < 0 ? 0 : pos_new / kKv8Page) : page1;
+  const bool news = new_page < page1;
+  const int my_page = new_page + (warp >> 1);
   const int my_row = STEP ? max(0, my_page * kKv8Page - pos_new) : 0, my_end = STEP && my_page < page1 ? min(p.q_per_seq, (my_page + 1) * kKv8Page - pos_new) : 0;
   long long my_slot = -1;
   float my_scale = 0.f;
+  int my_id = -1;                  // the page's number in the table
+  uint8_t* my_held = nullptr;
   if (STEP && my_row < my_end) {
     my_slot = p.st.slots[b * p.q_per_seq + my_row];
     if (my_slot >= 0 && (my_slot >> 4) < p.num_pages) my_scale = ((warp & 1) == 0 ? p.k_scales : p.v_scales)[(my_slot >> 4) * p.n_kv + kvh];
+    my_id = table[my_page];
+    const int i = my_page - page0;
+    if (i < 4 * kKv8Warps)
+      my_held = rings + (i >> 1) % kKv8Warps * (4 * PAGE_BYTES) + (i / (2 * kKv8Warps) * 2 + (i & 1)) * PAGE_BYTES + (warp & 1) * (PAGE_BYTES / 2);
   }
   if (STEP && !waited) wait_for_input();
   if (EVEN && slot == 0 && threadIdx.x == 0) p.joins[blockIdx.x] = join;
@@ -354,25 +356,10 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     const size_t at = static_cast<size_t>(b * p.q_per_seq + token) * p.ld_q + (kvh * group + r - token * group) * D;
     query[i] = !STEP && p.q32 != nullptr ? *reinterpret_cast<const float4*>(p.q32 + at + lane % (D / 4) * 4) : load_row4<D>(p.q + at, lane);
   }
-  // ---- the new rows
-  if (STEP) {
-    const int row0 = b * p.q_per_seq;
-#pragma unroll 1
-    for (int r = my_row; r < my_end;) {
-      const long long to = r == my_row ? my_slot : p.st.slots[row0 + r];
-      int n = 1;
-      if (to >= 0 && (to >> 4) < p.num_pages) {
-        while (r + n < my_end && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
-        const long long cell = (to >> 4) * p.n_kv + kvh;
-        const float before = r == my_row ? my_scale : ((warp & 1) == 0 ? p.k_scales : p.v_scales)[cell];
-        if ((warp & 1) == 0) store_few<D, true>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s + r * p.st.rot, lane, before);
-        else store_few<D, false>(p.st, row0 + r, n, static_cast<int>(to & 15), cell, kvh, turns_s, lane, before);
-      } else if (to >= 0) {
-        report_status(p.status, kStatusBadArgument);
-      }
-      r += n;
-    }
-  }
+  Kv8Few<D> few;
+  if (STEP && my_row < my_end)
+    few.load(((warp & 1) == 0 ? p.st.k : p.st.v) + static_cast<size_t>(b * p.q_per_seq + my_row) * ((warp & 1) == 0 ? p.st.ld_k : p.st.ld_v) + kvh * D,
+             (warp & 1) == 0 ? p.st.ld_k : p.st.ld_v, my_end - my_row, lane);
   // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
@@ -393,18 +380,42 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     to[2] = bytes.y;
     if (c == 0) back_s[row] = fine ? p.scale_log2 * exp2_of(-up0) * exp2_of(up0 - up) : __uint_as_float(0x7fc00000u);
   }
-  __syncthreads();
-  if (STEP) {
-    const bool first = turns > 0 && waits(0), second = turns > 1 && waits(1);
-    const int pg = page0 + 2 * (warp + kKv8Warps * (lane >> 1)) + (lane & 1);
-    if (turns > 0 && !first && pg >= new_page && pg < page1) {   // looked up in front of the write
-      ks = p.k_scales[static_cast<size_t>(ids) * p.n_kv + kvh];
-      ev = p.v_scales[static_cast<size_t>(ids) * p.n_kv + kvh];
+  // ---- the new rows
+  if (STEP && news) {
+    float scale = __uint_as_float(kNone);
+    const int row0 = b * p.q_per_seq;
+    cp_async_wait<0>();
+    __syncthreads();      // what the rings hold of all warps has landed
+#pragma unroll 1
+    for (int r = my_row; r < my_end;) {
+      const long long to = r == my_row ? my_slot : p.st.slots[row0 + r];
+      int n = 1;
+      if (to >= 0 && (to >> 4) < p.num_pages) {
+        while (r + n < my_end && (to + n) % kKv8Page != 0 && p.st.slots[row0 + r + n] == to + n) ++n;
+        const long long cell = (to >> 4) * p.n_kv + kvh;
+        const float before = r == my_row ? my_scale : ((warp & 1) == 0 ? p.k_scales : p.v_scales)[cell];
+        const bool seen = to >> 4 == my_id;
+        uint8_t* held = seen ? my_held : nullptr;
+        float now;
+        if ((warp & 1) == 0) now = store_few<D, true>(p.st, few, r - my_row, n, static_cast<int>(to & 15), cell, turns_s + my_row * p.st.rot, lane, before, held);
+        else now = store_few<D, false>(p.st, few, r - my_row, n, static_cast<int>(to & 15), cell, turns_s, lane, before, held);
+        __syncwarp();
+        if (seen) scale = now;
+      } else if (to >= 0) {
+        report_status(p.status, kStatusBadArgument);
+      }
+      r += n;
     }
-    if (first) fetch(0);
-    if (second) fetch(1);
-    cp_async_commit();
-    if (first || second) cp_async_wait<0>();   // (its places in the order of copies are taken)
+    if (lane == 0) scale_s[warp] = scale;
+  }
+  __syncthreads();
+  if (STEP && news) {      // looked up in front of the write
+    const int i = page0 + 2 * (warp + kKv8Warps * (lane >> 1)) + (lane & 1) - new_page;
+    if (i >= 0 && i < page1 - new_page) {
+      const float k = scale_s[2 * min(i, 1)], v = scale_s[2 * min(i, 1) + 1];
+      if (__float_as_uint(k) != kNone) ks = k;
+      if (__float_as_uint(v) != kNone) ev = v;
+    }
   }
   float back[NT][2];                                    // of the lane's columns 2t, 2t + 1
   int pos[NT][2];

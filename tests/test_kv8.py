@@ -456,6 +456,45 @@ def test_decode_step_from_the_projection(device, n_q, n_kv, dim, old, new, norm,
     assert ((got - want).abs() <= bound).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q, n_kv, dim", [(8, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("old, new", [((4203,), 3), ((2046, 250), 4), ((127, 4095), 1)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_steps_far_behind_what_a_warp_reads_first(n_q, n_kv, dim, old, new, splits):
+    """New rows in pages that a CTA comes to late, and in the first ones of its second look at the table."""
+    test_decode_step_from_the_projection("cuda", n_q, n_kv, dim, old, new, False, splits)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n_q, n_kv, dim", [(4, 4, 64), (16, 4, 128)])
+@pytest.mark.parametrize("settled", [False, True])
+def test_rows_of_a_step_that_are_not_stored(device, n_q, n_kv, dim, settled):
+    """Sequences of which the first, the last or no new rows go to their pages: attention reads what is there."""
+    new, old = 4, (30, 13, 44, 100)
+    seq_lens = [a + new for a in old]
+    num, table = layout(seq_lens, device)
+    g = torch.Generator().manual_seed(dim)
+    qkv = torch.randn((len(old) * new, (n_q + 2 * n_kv) * dim), generator=g).bfloat16().to(device)
+    freq = torch.tensor([1e4 ** (-2 * j / dim) for j in range(dim // 2)], device=device)
+    at = torch.cat([torch.arange(a, a + new) for a in old])
+    seq = torch.repeat_interleave(torch.arange(len(old)), new)
+    slots = table.cpu()[seq, at // PAGE].long() * PAGE + at % PAGE
+    slots[[0, 1, 7, 8, 9, 10, 11]] = -1
+    slots, at = slots.to(device), at.to(torch.int32).to(device)
+    pages = [filled(num, n_kv, dim, device, seed=i) for i in range(2)]
+    again = [Pages8(p.codes.clone(), p.scales.clone()) for p in pages]
+    got = ops.attention_decode_rope(qkv, *pages, table, ints(seq_lens, device), new, dim ** -0.5, at, slots, freq, n_q, n_kv, dim, splits=2, settled=settled)
+    q = ops.rope_kv(qkv, at, slots, freq, *again, n_q, n_kv, dim)
+    for a, b in zip(pages, again):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    want, size = attended(q, pages[0].values(), pages[1].values(), table, seq_lens, [new] * len(old), dim ** -0.5)
+    keys = pages[0].values().double().abs().amax((0, 2)).cpu()                 # [n_kv, dim]: no key is larger
+    most = (q.double().cpu().abs().view(-1, n_kv, n_q // n_kv, dim) * keys[None, :, None]).sum(-1).max()
+    moved = float(most) * dim ** -0.5 * 2.0 ** -8                              # half a bf16 step in every component of a query
+    bound = (2 * 2.0 ** -11 + 2.0 ** -13 + 2 * math.expm1(moved)) * size + 2.0 ** -8 * want.abs() + 2.0 ** -120
+    assert ((got.double().cpu() - want).abs() <= bound).all()
+
+
 # ------------------------------------------------------------------------------------------ moving
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("kind, heads, dim", [(torch.bfloat16, 8, 128), (torch.float32, 1, 4), (torch.int8, 3, 64), (torch.bfloat16, 1, 1)])
