@@ -22,15 +22,13 @@
 
 #include <algorithm>
 
+#include "../common/kv8_args.h"
 #include "../common/kv8_store.cuh"
 #include "../common/launch.h"
 #include "../common/launch_count.h"
 #include "../common/mma.cuh"
 #include "../common/ptx.cuh"
 #include "../common/trace.cuh"
-
-extern "C" int eredu_kv8_store(const void*, const void*, const void*, void*, void*, void*, float*, float*, const int*, const long long*, const float*, const float*,
-                               const float*, int, int, int, int, int, int, int, int, int, int, int, float, float, float, int*, cudaStream_t);
 
 namespace eredu {
 
@@ -860,91 +858,82 @@ static int attn_kv8(AttnKv8Params& p, int D, int ctas, bool step, cudaStream_t s
   return static_cast<int>(e);
 }
 
-static AttnKv8Params attn_kv8_params(const void* q, int ld_q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
-                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
-                                     int q_per_seq, int max_pages, int pitch, int num_pages, int n_q, int n_kv, int splits, int window, int chunk, float scale,
-                                     int* status) {
+static AttnKv8Params attn_kv8_params(const Kv8AttentionArgs& a, int ld_q) {
   AttnKv8Params p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.ld_q = ld_q;
-  p.k_codes = static_cast<const int8_t*>(k_codes);
-  p.v_codes = static_cast<const int8_t*>(v_codes);
-  p.k_scales = k_scales;
-  p.v_scales = v_scales;
-  p.out = static_cast<__nv_bfloat16*>(out);
-  p.block_table = block_table;
-  p.seq_lens = seq_lens;
-  p.sinks = sinks;
-  p.part_o = part_o;
-  p.part_ml = part_ml;
-  p.joins = static_cast<int4*>(joins);
-  p.batch = batch;
-  p.max_pages = max_pages;
-  p.pitch = pitch;
-  p.num_pages = num_pages;
-  p.n_q = n_q;
-  p.n_kv = n_kv;
-  p.q_per_seq = q_per_seq;
-  p.splits = splits;
-  p.window = window;
-  p.chunk = chunk;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.status = status;
+  p.k_codes = static_cast<const int8_t*>(a.k_codes);
+  p.v_codes = static_cast<const int8_t*>(a.v_codes);
+  p.k_scales = a.k_scales;
+  p.v_scales = a.v_scales;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.block_table = a.block_table;
+  p.seq_lens = a.seq_lens;
+  p.sinks = a.sinks;
+  p.part_o = a.part_o;
+  p.part_ml = a.part_ml;
+  p.joins = static_cast<int4*>(a.joins);
+  p.batch = a.batch;
+  p.max_pages = a.max_pages;
+  p.pitch = a.pitch;
+  p.num_pages = a.num_pages;
+  p.n_q = a.n_q;
+  p.n_kv = a.n_kv;
+  p.q_per_seq = a.q_per_seq;
+  p.splits = a.splits;
+  p.window = a.window;
+  p.chunk = a.chunk;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.status = a.status;
   return p;
 }
 
 // splits 1 to 8: CTAs of a sequence and head. 0: even shares for `ctas` CTAs, with scratch for 2 * ctas tiles of 8 rows (16 where a head has more than 8).
-extern "C" int eredu_attn_kv8_decode(const void* q, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* out,
-                                     const int* block_table, const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, int batch,
-                                     int q_per_seq, int max_pages, int pitch, int num_pages, int n_q, int n_kv, int D, int splits, int ctas, int window, int chunk,
-                                     float scale, int* status, cudaStream_t stream) {
-  AttnKv8Params p = attn_kv8_params(q, n_q * D, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
-                                    max_pages, pitch, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
-  return attn_kv8(p, D, ctas, false, stream);
+extern "C" int eredu_attn_kv8_decode(const void* args, int bytes) {
+  Kv8AttentionArgs a;
+  if (!kv8_args(a, args, bytes)) return -2;
+  AttnKv8Params p = attn_kv8_params(a, a.n_q * a.D);
+  return attn_kv8(p, a.D, a.ctas, false, a.stream);
 }
 
-// The same from the projection's output qkv, rows [q heads | k heads | v heads] x D of ld elements. The attention kernel rotates queries and writes the new
-// rows itself where one tile holds all query rows of a head, so that one CTA has a page; else eredu_kv8_store goes in front and leaves the queries in
-// q32 [batch * q_per_seq, n_q, D] (four sequences of 3000 tokens, five new ones, 32 heads over 4: 18 us; rotated in each of three tiles 20).
-extern "C" int eredu_attn_kv8_step(const void* qkv, int ld, float* q32, void* k_codes, void* v_codes, float* k_scales, float* v_scales, void* out, const int* block_table,
-                                   const int* seq_lens, const float* sinks, float* part_o, float* part_ml, void* joins, const int* positions,
-                                   const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int batch, int q_per_seq,
-                                   int max_pages, int pitch, int num_pages, int n_q, int n_kv, int D, int rot, int interleaved, int splits, int ctas, int window, int chunk,
-                                   int settled, float scale, float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
-  if (batch <= 0) return 0;
-  if (n_kv <= 0 || n_q <= 0 || n_q % n_kv != 0 || q_per_seq <= 0 || rot < 0 || rot > D || rot % 8 != 0) return -2;
-  const int group = n_q / n_kv;
-  const bool own = q_per_seq * group <= 16 && q_per_seq <= kKv8StepTokens;
-  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(qkv);
-  AttnKv8Params p = attn_kv8_params(qkv, ld, k_codes, v_codes, k_scales, v_scales, out, block_table, seq_lens, sinks, part_o, part_ml, joins, batch, q_per_seq,
-                                    max_pages, pitch, num_pages, n_q, n_kv, splits, window, chunk, scale, status);
+// The same from the projection's output, rows [q heads | k heads | v heads] x D of ld elements. The attention kernel rotates queries and writes the new
+// rows itself where one tile holds all query rows of a head, so that one CTA has a page; else kv8_store goes in front and leaves the queries in
+// q32 [batch * q_per_seq, n_q, D] (four sequences of 3000 tokens, five new ones, 32 heads over 4: 17 us; rotated in each of three tiles 20).
+extern "C" int eredu_attn_kv8_step(const void* args, int bytes) {
+  Kv8AttentionArgs a;
+  if (!kv8_args(a, args, bytes)) return -2;
+  if (a.batch <= 0) return 0;
+  if (a.n_kv <= 0 || a.n_q <= 0 || a.n_q % a.n_kv != 0 || a.q_per_seq <= 0 || a.rot < 0 || a.rot > a.D || a.rot % 8 != 0) return -2;
+  const bool own = a.q_per_seq * (a.n_q / a.n_kv) <= 16 && a.q_per_seq <= kKv8StepTokens;
+  const __nv_bfloat16 *row = static_cast<const __nv_bfloat16*>(a.q), *k = row + a.n_q * a.D, *v = k + a.n_kv * a.D;
+  AttnKv8Params p = attn_kv8_params(a, a.ld);
   if (!own) {
-    if (q32 == nullptr) return -2;
-    const int e = eredu_kv8_store(qkv, row + n_q * D, row + (n_q + n_kv) * D, q32, k_codes, v_codes, k_scales, v_scales, positions, slots, inv_freq, q_norm_w,
-                                  k_norm_w, batch * q_per_seq, ld, ld, ld, n_q, n_kv, D, rot, interleaved, num_pages, 1, attn_factor, norm_eps, norm_w_off, status,
-                                  stream);
+    if (a.q32 == nullptr) return -2;
+    const int e = kv8_store(Kv8StoreArgs{a.q, k, v, a.q32, a.k_codes, a.v_codes, a.k_scales, a.v_scales, a.positions, a.slots, a.inv_freq, a.q_norm_w, a.k_norm_w, a.status,
+                                         a.stream, a.batch * a.q_per_seq, a.ld, a.ld, a.ld, a.n_q, a.n_kv, a.D, a.rot, a.interleaved, a.num_pages, 1, a.attn_factor,
+                                         a.norm_eps, a.norm_w_off});
     if (e != 0) return e;
-    p.q32 = q32;
-    p.ld_q = n_q * D;
-    return attn_kv8(p, D, ctas, false, stream);
+    p.q32 = a.q32;
+    p.ld_q = a.n_q * a.D;
+    return attn_kv8(p, a.D, a.ctas, false, a.stream);
   }
-  p.settled = !EREDU_PDL_EARLY && pdl_enabled() && settled != 0;
-  p.st.k = row + n_q * D;
-  p.st.v = row + (n_q + n_kv) * D;
-  p.st.ld_k = p.st.ld_v = ld;
-  p.st.k_codes = static_cast<int8_t*>(k_codes);
-  p.st.v_codes = static_cast<int8_t*>(v_codes);
-  p.st.k_scales = k_scales;
-  p.st.v_scales = v_scales;
-  p.st.positions = positions;
-  p.st.slots = slots;
-  p.st.inv_freq = inv_freq;
-  p.st.q_norm_w = q_norm_w;
-  p.st.k_norm_w = k_norm_w;
-  p.st.rot = rot;
-  p.st.interleaved = interleaved;
-  p.st.attn_factor = attn_factor;
-  p.st.norm_eps = norm_eps;
-  p.st.norm_w_off = norm_w_off;
-  return attn_kv8(p, D, ctas, true, stream);
+  p.settled = !EREDU_PDL_EARLY && pdl_enabled() && a.settled != 0;
+  p.st.k = k;
+  p.st.v = v;
+  p.st.ld_k = p.st.ld_v = a.ld;
+  p.st.k_codes = static_cast<int8_t*>(a.k_codes);
+  p.st.v_codes = static_cast<int8_t*>(a.v_codes);
+  p.st.k_scales = a.k_scales;
+  p.st.v_scales = a.v_scales;
+  p.st.positions = a.positions;
+  p.st.slots = a.slots;
+  p.st.inv_freq = a.inv_freq;
+  p.st.q_norm_w = a.q_norm_w;
+  p.st.k_norm_w = a.k_norm_w;
+  p.st.rot = a.rot;
+  p.st.interleaved = a.interleaved;
+  p.st.attn_factor = a.attn_factor;
+  p.st.norm_eps = a.norm_eps;
+  p.st.norm_w_off = a.norm_w_off;
+  return attn_kv8(p, a.D, a.ctas, true, a.stream);
 }

@@ -1,6 +1,7 @@
 // Pages of a cache held in 8 bits (common/kv8.cuh): rows are written, values read back, and pages of any cache copied.
 #include <algorithm>
 
+#include "../common/kv8_args.h"
 #include "../common/kv8_store.cuh"
 #include "../common/launch.h"
 #include "../common/launch_count.h"
@@ -259,82 +260,85 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(PageCopyParams p) {
 
 using namespace eredu;
 
-extern "C" int eredu_kv8_store(const void* q, const void* k, const void* v, void* q_out, void* k_codes, void* v_codes, float* k_scales, float* v_scales,
-                               const int* positions, const long long* slots, const float* inv_freq, const float* q_norm_w, const float* k_norm_w, int M,
-                               int ld_q, int ld_k, int ld_v, int n_q, int n_kv, int D, int rot, int interleaved, int num_pages, int q_out_fp32,
-                               float attn_factor, float norm_eps, float norm_w_off, int* status, cudaStream_t stream) {
+int eredu::kv8_store(const Kv8StoreArgs& a) {
+  const int M = a.M, n_kv = a.n_kv, rot = a.rot;
   if (M <= 0) return 0;
-  if ((D != 64 && D != 128) || n_kv <= 0 || num_pages <= 0 || rot < 0 || rot > D || rot % 8 != 0 || ld_q % 4 != 0 || ld_k % 4 != 0 || ld_v % 4 != 0 ||
-      (q_out != nullptr && (n_q <= 0 || n_q % n_kv != 0 || n_q / n_kv > 256)))
+  if ((a.D != 64 && a.D != 128) || n_kv <= 0 || a.num_pages <= 0 || rot < 0 || rot > a.D || rot % 8 != 0 || a.ld_q % 4 != 0 || a.ld_k % 4 != 0 || a.ld_v % 4 != 0 ||
+      (a.q_out != nullptr && (a.n_q <= 0 || a.n_q % n_kv != 0 || a.n_q / n_kv > 256)))
     return -2;
   Kv8StoreParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.v = static_cast<const __nv_bfloat16*>(v);
-  p.q_out = q_out;
-  p.q_out_fp32 = q_out_fp32;
-  p.k_codes = static_cast<int8_t*>(k_codes);
-  p.v_codes = static_cast<int8_t*>(v_codes);
-  p.k_scales = k_scales;
-  p.v_scales = v_scales;
-  p.positions = positions;
-  p.slots = slots;
-  p.inv_freq = inv_freq;
-  p.q_norm_w = q_norm_w;
-  p.k_norm_w = k_norm_w;
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.k = static_cast<const __nv_bfloat16*>(a.k);
+  p.v = static_cast<const __nv_bfloat16*>(a.v);
+  p.q_out = a.q_out;
+  p.q_out_fp32 = a.q_out_fp32;
+  p.k_codes = static_cast<int8_t*>(a.k_codes);
+  p.v_codes = static_cast<int8_t*>(a.v_codes);
+  p.k_scales = a.k_scales;
+  p.v_scales = a.v_scales;
+  p.positions = a.positions;
+  p.slots = a.slots;
+  p.inv_freq = a.inv_freq;
+  p.q_norm_w = a.q_norm_w;
+  p.k_norm_w = a.k_norm_w;
   p.M = M;
-  p.ld_q = ld_q;
-  p.ld_k = ld_k;
-  p.ld_v = ld_v;
-  p.n_q = n_q;
+  p.ld_q = a.ld_q;
+  p.ld_k = a.ld_k;
+  p.ld_v = a.ld_v;
+  p.n_q = a.n_q;
   p.n_kv = n_kv;
   p.rot = rot;
-  p.interleaved = interleaved;
-  p.num_pages = num_pages;
-  p.attn_factor = attn_factor;
-  p.norm_eps = norm_eps;
-  p.norm_w_off = norm_w_off;
-  p.status = status;
+  p.interleaved = a.interleaved;
+  p.num_pages = a.num_pages;
+  p.attn_factor = a.attn_factor;
+  p.norm_eps = a.norm_eps;
+  p.norm_w_off = a.norm_w_off;
+  p.status = a.status;
   // a key / value head with its query heads per CTA, and as few rows as find room at once
   p.tile = 1;
   while (p.tile < kKv8Page && static_cast<long long>((M + p.tile - 1) / p.tile) * n_kv > kStoreRoom) p.tile *= 2;
   const dim3 grid((M + p.tile - 1) / p.tile, n_kv);
   const size_t smem = static_cast<size_t>(kStoreRows) * rot * sizeof(float);
-  const bool whole = rot == D && interleaved == 0;
-  const cudaError_t e = D == 128 ? (whole ? launch_pdl(kv8_store_kernel<128, true>, grid, dim3(kStoreThreads), smem, stream, p)
-                                          : launch_pdl(kv8_store_kernel<128, false>, grid, dim3(kStoreThreads), smem, stream, p))
-                                 : (whole ? launch_pdl(kv8_store_kernel<64, true>, grid, dim3(kStoreThreads), smem, stream, p)
-                                          : launch_pdl(kv8_store_kernel<64, false>, grid, dim3(kStoreThreads), smem, stream, p));
+  const bool whole = rot == a.D && a.interleaved == 0;
+  const cudaError_t e = a.D == 128 ? (whole ? launch_pdl(kv8_store_kernel<128, true>, grid, dim3(kStoreThreads), smem, a.stream, p)
+                                            : launch_pdl(kv8_store_kernel<128, false>, grid, dim3(kStoreThreads), smem, a.stream, p))
+                                   : (whole ? launch_pdl(kv8_store_kernel<64, true>, grid, dim3(kStoreThreads), smem, a.stream, p)
+                                            : launch_pdl(kv8_store_kernel<64, false>, grid, dim3(kStoreThreads), smem, a.stream, p));
   eredu_count_launches(1);
   return static_cast<int>(e);
 }
 
-extern "C" int eredu_kv8_values(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, void* k_out, void* v_out,
-                                const int* pages, const int* seq_lens, const int* cu_q, int* table_out, int rows, int pitch, int table_wide, int wide, int n_kv, int D,
-                                int num_pages, int window, int chunk, int* status, cudaStream_t stream) {
-  if (rows <= 0 || wide <= 0) return 0;
-  if ((D != 64 && D != 128) || n_kv <= 0 || rows > 65535 || num_pages <= 0) return -2;
+extern "C" int eredu_kv8_store(const void* args, int bytes) {
+  Kv8StoreArgs a;
+  return kv8_args(a, args, bytes) ? kv8_store(a) : -2;
+}
+
+extern "C" int eredu_kv8_values(const void* args, int bytes) {
+  Kv8ValuesArgs a;
+  if (!kv8_args(a, args, bytes)) return -2;
+  if (a.rows <= 0 || a.wide <= 0) return 0;
+  if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.rows > 65535 || a.num_pages <= 0) return -2;
   Kv8ValuesParams p = {};
-  p.k_codes = static_cast<const int8_t*>(k_codes);
-  p.v_codes = static_cast<const int8_t*>(v_codes);
-  p.k_scales = k_scales;
-  p.v_scales = v_scales;
-  p.k_out = static_cast<__nv_bfloat16*>(k_out);
-  p.v_out = static_cast<__nv_bfloat16*>(v_out);
-  p.pages = pages;
-  p.seq_lens = seq_lens;
-  p.cu_q = cu_q;
-  p.table_out = table_out;
-  p.pitch = pitch;
-  p.wide = wide;
-  p.table_wide = table_wide;
-  p.n_kv = n_kv;
-  p.num_pages = num_pages;
-  p.window = window;
-  p.chunk = chunk;
-  p.status = status;
-  const cudaError_t e = D == 128 ? launch_pdl(kv8_values_kernel<128>, dim3(wide, rows, 2), dim3(kValuesThreads), 0, stream, p)
-                                 : launch_pdl(kv8_values_kernel<64>, dim3(wide, rows, 2), dim3(kValuesThreads), 0, stream, p);
+  p.k_codes = static_cast<const int8_t*>(a.k_codes);
+  p.v_codes = static_cast<const int8_t*>(a.v_codes);
+  p.k_scales = a.k_scales;
+  p.v_scales = a.v_scales;
+  p.k_out = static_cast<__nv_bfloat16*>(a.k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(a.v_out);
+  p.pages = a.pages;
+  p.seq_lens = a.seq_lens;
+  p.cu_q = a.cu_q;
+  p.table_out = a.table_out;
+  p.pitch = a.pitch;
+  p.wide = a.wide;
+  p.table_wide = a.table_wide;
+  p.n_kv = a.n_kv;
+  p.num_pages = a.num_pages;
+  p.window = a.window;
+  p.chunk = a.chunk;
+  p.status = a.status;
+  const cudaError_t e = a.D == 128 ? launch_pdl(kv8_values_kernel<128>, dim3(a.wide, a.rows, 2), dim3(kValuesThreads), 0, a.stream, p)
+                                   : launch_pdl(kv8_values_kernel<64>, dim3(a.wide, a.rows, 2), dim3(kValuesThreads), 0, a.stream, p);
   eredu_count_launches(1);
   return static_cast<int>(e);
 }

@@ -13,6 +13,7 @@ makes the scale, and with it the whole block, no number until the block is opene
 """
 from __future__ import annotations
 
+import ctypes
 import struct
 from typing import NamedTuple
 
@@ -38,10 +39,10 @@ def _sm_count(device) -> int:
 
 
 P, I, F = native.P, native.I, native.F
-native.register("eredu_kv8_store", I, [P] * 13 + [I] * 11 + [F] * 3 + [P] * 2)
-native.register("eredu_kv8_values", I, [P] * 10 + [I] * 9 + [P] * 2)
-native.register("eredu_attn_kv8_decode", I, [P] * 12 + [I] * 12 + [F] + [P] * 2)
-native.register("eredu_attn_kv8_step", I, [P, I] + [P] * 17 + [I] * 15 + [F] * 4 + [P] * 2)
+# the arguments of a call in one block, laid out as csrc/common/kv8_args.h has them
+_STORE, _VALUES, _ATTENTION = struct.Struct("15Q11i3f"), struct.Struct("12Q10i"), struct.Struct("20Q16i4f")
+for _name in ("eredu_kv8_store", "eredu_kv8_values", "eredu_attn_kv8_decode", "eredu_attn_kv8_step"):
+    native.register(_name, I, [ctypes.c_char_p, I])
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 
@@ -101,6 +102,11 @@ def check_pages8(k: Pages8, v: Pages8, n_kv: int, head_dim: int) -> None:
     raise NotImplementedError(f"the kernels of 8-bit pages are built for head sizes {KV8_HEAD_DIMS}, not {head_dim}")
 
 
+def address(t) -> int:
+    """Where a tensor lies, 0 for none."""
+    return 0 if t is None else t.data_ptr()
+
+
 def _need(name, t, dtype, device) -> None:
     if t is not None and (t.dtype is not dtype or not t.is_contiguous() or t.device != device):
         raise ValueError(f"{name}: a contiguous {dtype} tensor on {device} is expected, not {t.dtype} on {t.device}")
@@ -140,9 +146,10 @@ def store_rows_ref(x, slots, pages: Pages8) -> None:
 def _store(q, k, v, slots, k_cache, v_cache, q_out, positions, inv_freq, n_q, n_kv, head_dim, rot, interleaved, attn_factor, q_norm_w, k_norm_w,
            norm_eps, norm_w_off, ld):
     dev = k_cache.device
-    code = lib().eredu_kv8_store(q, k, v, ptr(q_out), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), ptr(positions),
-                                 ptr(slots), ptr(inv_freq), ptr(q_norm_w), ptr(k_norm_w), slots.shape[0], ld[0], ld[1], ld[2], n_q, n_kv, head_dim, rot,
-                                 1 if interleaved else 0, k_cache.codes.shape[0], 0, attn_factor, norm_eps, norm_w_off, ptr(status_word(dev)), stream_ptr(dev))
+    code = lib().eredu_kv8_store(_STORE.pack(
+        q, k, v, address(q_out), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(), v_cache.scales.data_ptr(), address(positions), slots.data_ptr(),
+        address(inv_freq), address(q_norm_w), address(k_norm_w), status_word(dev).data_ptr(), stream_ptr(dev), slots.shape[0], *ld, n_q, n_kv, head_dim, rot,
+        1 if interleaved else 0, k_cache.codes.shape[0], 0, attn_factor, norm_eps, norm_w_off), _STORE.size)
     check(code, "eredu_kv8_store")
 
 
@@ -160,7 +167,7 @@ def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
     _need("slots", slots, torch.int64, k_cache.device)
     k, v = (t if t.dtype == torch.bfloat16 and t.stride()[1:] == (head_dim, 1) and t.stride(0) % 4 == 0 and t.data_ptr() % 8 == 0
             else t.to(torch.bfloat16).contiguous() for t in (k, v))
-    _store(None, k.data_ptr(), v.data_ptr(), slots, k_cache, v_cache, None, None, None, 0, n_kv, head_dim, 0, False, 1.0, None, None, 0.0, 0.0,
+    _store(0, k.data_ptr(), v.data_ptr(), slots, k_cache, v_cache, None, None, None, 0, n_kv, head_dim, 0, False, 1.0, None, None, 0.0, 0.0,
            (0, k.stride(0), v.stride(0)))
 
 
@@ -216,8 +223,9 @@ def page_values(k_cache: Pages8, v_cache: Pages8, pages):
     out = kc.new_empty((2, n, n_kv, PAGE, dim), dtype=torch.bfloat16)
     if n:
         at = out.data_ptr()
-        code = lib().eredu_kv8_values(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + 2 * n * n_kv * PAGE * dim, pages.data_ptr(), None, None,
-                                      None, 1, n, n, n, n_kv, dim, num, 0, 0, status_word(dev).data_ptr(), stream_ptr(dev))
+        code = lib().eredu_kv8_values(_VALUES.pack(
+            kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + 2 * n * n_kv * PAGE * dim, pages.data_ptr(), 0, 0, 0, status_word(dev).data_ptr(),
+            stream_ptr(dev), 1, n, n, n, n_kv, dim, num, 0, 0, 0), _VALUES.size)
         check(code, "eredu_kv8_values")
     return out.unbind(0)
 
@@ -252,7 +260,7 @@ def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_
 def _shares(splits, rows, dim, dev):
     """(splits, CTAs, scratch, addresses in it) of a decode call."""
     if 1 <= splits <= CLUSTER:
-        return splits, 0, None, None, None, None
+        return splits, 0, None, 0, 0, 0
     ctas = EVEN_CTAS * _sm_count(dev)
     n = 2 * ctas * (8 if rows <= 8 else 16)
     part = torch.empty(n * (dim + 4) + 4 * ctas, dtype=torch.float32, device=dev)
@@ -273,9 +281,10 @@ def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
     if out is None:
         out = torch.empty_like(q)
     splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
-    code = lib().eredu_attn_kv8_decode(q.data_ptr(), ptr(k_cache.codes), ptr(v_cache.codes), ptr(k_cache.scales), ptr(v_cache.scales), out.data_ptr(),
-                                       block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins, B, q_per_seq, block_table.shape[1], block_table.stride(0),
-                                       k_cache.codes.shape[0], n_q, n_kv, dim, splits, ctas, int(window), int(chunk), scale, ptr(status_word(dev)), stream_ptr(dev))
+    code = lib().eredu_attn_kv8_decode(_ATTENTION.pack(
+        q.data_ptr(), 0, k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(), v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), address(sinks), part_o, part_ml, joins, 0, 0, 0, 0, 0, status_word(dev).data_ptr(), stream_ptr(dev), 0, B, q_per_seq, block_table.shape[1],
+        block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, 0, 0, splits, ctas, int(window), int(chunk), 0, scale, 0.0, 0.0, 0.0), _ATTENTION.size)
     check(code, "eredu_attn_kv8_decode")
     return out
 
@@ -291,11 +300,12 @@ def attention_step8(qkv, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
     rows = q_per_seq * (n_q // n_kv)
     splits, ctas, part, part_o, part_ml, joins = _shares(splits, rows, dim, dev)
     q32 = torch.empty(M * n_q * dim, dtype=torch.float32, device=dev) if rows > 16 or q_per_seq > 8 else None
-    code = lib().eredu_attn_kv8_step(qkv.data_ptr(), qkv.stride(0), ptr(q32), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(),
-                                     v_cache.scales.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptr(sinks), part_o, part_ml, joins,
-                                     positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), B, q_per_seq,
-                                     block_table.shape[1], block_table.stride(0), k_cache.codes.shape[0], n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window),
-                                     int(chunk), 1 if settled else 0, scale, attn_factor, norm_eps, norm_w_off, status_word(dev).data_ptr(), stream_ptr(dev))
+    code = lib().eredu_attn_kv8_step(_ATTENTION.pack(
+        qkv.data_ptr(), address(q32), k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), k_cache.scales.data_ptr(), v_cache.scales.data_ptr(), out.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(), address(sinks), part_o, part_ml, joins, positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), address(q_norm_w),
+        address(k_norm_w), status_word(dev).data_ptr(), stream_ptr(dev), qkv.stride(0), B, q_per_seq, block_table.shape[1], block_table.stride(0), k_cache.codes.shape[0],
+        n_q, n_kv, dim, rot, 1 if interleaved else 0, splits, ctas, int(window), int(chunk), 1 if settled else 0, scale, attn_factor, norm_eps, norm_w_off),
+        _ATTENTION.size)
     check(code, "eredu_attn_kv8_step")
     return out
 
@@ -350,8 +360,9 @@ def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_len
     at = held.data_ptr()
     table, status, stream = at + 2 * half, status_word(dev).data_ptr(), stream_ptr(dev)
     lens, cu = seq_lens.data_ptr(), cu_q.data_ptr()
-    code = lib().eredu_kv8_values(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + half, block_table.data_ptr(), lens, cu, table, B,
-                                  block_table.stride(0), block_table.shape[1], wide, n_kv, dim, num, int(window), int(chunk), status, stream)
+    code = lib().eredu_kv8_values(_VALUES.pack(
+        kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + half, block_table.data_ptr(), lens, cu, table, status, stream, B, block_table.stride(0),
+        block_table.shape[1], wide, n_kv, dim, num, int(window), int(chunk), 0), _VALUES.size)
     check(code, "eredu_kv8_values")
     code = lib().eredu_attn_prefill_tc(q.data_ptr(), at, at + half, out.data_ptr(), table, lens, cu, ptr(sinks), B, total, max_q_len, wide, B * wide, n_q, n_kv, dim, dim,
                                        int(window), int(chunk), int(max_kv_len), _sm_count(dev), scale, status, stream)

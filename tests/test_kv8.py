@@ -495,6 +495,15 @@ def test_rows_of_a_step_that_are_not_stored(device, n_q, n_kv, dim, settled):
     assert ((got.double().cpu() - want).abs() <= bound).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name, block", [("eredu_kv8_store", kv8._STORE), ("eredu_kv8_values", kv8._VALUES), ("eredu_attn_kv8_decode", kv8._ATTENTION),
+                                         ("eredu_attn_kv8_step", kv8._ATTENTION)])
+def test_argument_blocks_are_as_long_as_the_library_has_them(name, block):
+    call, nothing = getattr(ops.native.lib(), name), bytes(block.size)        # no rows, no sequences: nothing is launched
+    assert call(nothing, block.size) == 0
+    assert call(nothing + b"    ", block.size + 4) != 0 and call(nothing, 8) != 0
+
+
 # ------------------------------------------------------------------------------------------ moving
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("kind, heads, dim", [(torch.bfloat16, 8, 128), (torch.float32, 1, 4), (torch.int8, 3, 64), (torch.bfloat16, 1, 1)])
