@@ -359,11 +359,14 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
     few.load(((warp & 1) == 0 ? p.st.k : p.st.v) + static_cast<size_t>(b * p.q_per_seq + my_row) * ((warp & 1) == 0 ? p.st.ld_k : p.st.ld_v) + kvh * D,
              (warp & 1) == 0 ? p.st.ld_k : p.st.ld_v, my_end - my_row, lane);
   // ---- the query rows: bytes into shared memory, and what takes a score back to log2 units
-#pragma unroll
-  for (int i = 0; i < QUERIES; ++i) {
+#pragma unroll(STEP ? 1 : QUERIES)
+  for (int i = 0; i < QUERIES; ++i) {      // (a step's rows one after the other: what rotates them is long, and read once)
     const int row = (i * kKv8Warps + warp) * RPI + lane / (D / 4), c = lane % (D / 4);       // this lane has channels 4 c and three more
     const bool in = row < rows;
-    float4 x = query[i];
+    float4 x = query[0];
+#pragma unroll
+    for (int j = 1; j < QUERIES; ++j)
+      if (i == j) x = query[j];
     if (STEP) x = prepared<D>(p.st, x, p.st.q_norm_w, turns_s + (kv8_token(p, r0 + min(row, rows - 1)) - token0) * p.st.rot, lane);
     if (!in) x = make_float4(0.f, 0.f, 0.f, 0.f);
     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))), max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
