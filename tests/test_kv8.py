@@ -496,6 +496,33 @@ def test_rows_of_a_step_that_are_not_stored(device, n_q, n_kv, dim, settled):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [33, 300, 700, 2000])
+@pytest.mark.parametrize("n_q, n_kv, dim, rot", [(8, 8, 128, 128), (14, 2, 64, 64), (3, 3, 128, 32), (32, 2, 64, 8)])
+def test_runs_of_all_kinds_whatever_tile_they_begin_in(rows, n_q, n_kv, dim, rot):
+    """Runs of any length and offset with rows between them that are not stored. The angles are zero, so that codes and scales are those of the rows themselves."""
+    g = torch.Generator().manual_seed(rows + n_q)
+    draw = lambda low, high: int(torch.randint(low, high + 1, (), generator=g))     # noqa: E731
+    slots, page = [], 0
+    while len(slots) < rows:
+        if draw(0, 9) == 0:
+            slots += [-1] * draw(1, 5)
+        first = draw(0, 15) if draw(0, 2) == 0 else 0
+        slots += [page * PAGE + first + i for i in range(16 - first if draw(0, 1) else draw(1, 16 - first))]
+        page += 1
+    slots = torch.tensor(slots[:rows])
+    x = (torch.randn((rows, (n_q + 2 * n_kv) * dim), generator=g) * torch.exp(torch.randn((rows, 1), generator=g))).bfloat16()
+    pages = [filled(page, n_kv, dim, "cpu", seed=i) for i in range(2)]
+    have = [Pages8(p.codes.cuda(), p.scales.cuda()) for p in pages]
+    k, v = x.view(rows, -1, dim)[:, n_q:].split(n_kv, 1)
+    for part, p in zip((k, v), pages):
+        kv8.store_rows_ref(part, slots, p)
+    q = ops.rope_kv(x.cuda(), torch.arange(rows, dtype=torch.int32, device="cuda"), slots.cuda(), torch.zeros(rot // 2, device="cuda"), *have, n_q, n_kv, dim, rot=rot)
+    assert torch.equal(q.cpu().view(rows, -1), x[:, :n_q * dim])
+    for a, b in zip(have, pages):
+        assert torch.equal(a.scales.cpu(), b.scales) and torch.equal(a.codes.cpu(), b.codes)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name, block", [("eredu_kv8_store", kv8._STORE), ("eredu_kv8_values", kv8._VALUES), ("eredu_attn_kv8_decode", kv8._ATTENTION),
                                          ("eredu_attn_kv8_step", kv8._ATTENTION)])
 def test_argument_blocks_are_as_long_as_the_library_has_them(name, block):
