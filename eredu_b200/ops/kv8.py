@@ -13,7 +13,6 @@ makes the scale, and with it the whole block, no number until the block is opene
 """
 from __future__ import annotations
 
-import ctypes
 import struct
 from typing import NamedTuple
 
@@ -41,8 +40,10 @@ def _sm_count(device) -> int:
 P, I, F = native.P, native.I, native.F
 # the arguments of a call in one block, laid out as csrc/common/kv8_args.h has them
 _STORE, _VALUES, _ATTENTION = struct.Struct("15Q11i3f"), struct.Struct("12Q10i"), struct.Struct("20Q16i4f")
-for _name in ("eredu_kv8_store", "eredu_kv8_values", "eredu_attn_kv8_decode", "eredu_attn_kv8_step"):
-    native.register(_name, I, [ctypes.c_char_p, I])
+native.register("eredu_kv8_store", I, [P, I])
+native.register("eredu_kv8_values", I, [P, I])
+native.register("eredu_attn_kv8_decode", I, [P, I])
+native.register("eredu_attn_kv8_step", I, [P, I])
 native.register("eredu_copy_pages", I, [P, I, P, P, I, I, P, P])
 
 

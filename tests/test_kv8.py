@@ -1,5 +1,7 @@
 """Keys and values held in 8 bits: pages written, read, attended to and moved, against the definition in 64 bits."""
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -520,6 +522,18 @@ def test_runs_of_all_kinds_whatever_tile_they_begin_in(rows, n_q, n_kv, dim, rot
     assert torch.equal(q.cpu().view(rows, -1), x[:, :n_q * dim])
     for a, b in zip(have, pages):
         assert torch.equal(a.scales.cpu(), b.scales) and torch.equal(a.codes.cpu(), b.codes)
+
+
+def test_argument_blocks_hold_what_the_header_declares():
+    """Pointers, then ints, then floats, as many of each as the formats have."""
+    header = (Path(ops.__file__).resolve().parent.parent / "csrc/common/kv8_args.h").read_text()
+    for name, block in (("Kv8StoreArgs", kv8._STORE), ("Kv8ValuesArgs", kv8._VALUES), ("Kv8AttentionArgs", kv8._ATTENTION)):
+        body = re.sub(r"//.*", "", re.search(rf"struct {name} {{(.*?)}};", header, re.S).group(1))
+        kinds = ""
+        for line in filter(None, (part.strip() for part in body.split(";"))):
+            pointer = "*" in line or line.startswith("cudaStream_t")
+            kinds += ("Q" if pointer else "f" if line.startswith("float ") else "i") * len(line.split(","))
+        assert "".join(letter * int(n) for n, letter in re.findall(r"(\d+)([Qif])", block.format)) == kinds, name
 
 
 @pytest.mark.gpu
