@@ -274,11 +274,15 @@ def attention_decode8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens
     any other number: even shares of all pages whatever the sequences' lengths are, partial sums in memory that the call allocates, and a second kernel
     that adds them up."""
     check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out)
+    if q.shape[0] != seq_lens.shape[0] * q_per_seq:
+        raise ValueError(f"{q.shape[0]} query rows for {seq_lens.shape[0]} sequences of {q_per_seq}")
+    return _decode8(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk)
+
+
+def _decode8(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk):
     dev, B = q.device, seq_lens.shape[0]
     n_q, dim = q.shape[1:]
     n_kv = k_cache.codes.shape[1]
-    if q.shape[0] != B * q_per_seq:
-        raise ValueError(f"{q.shape[0]} query rows for {B} sequences of {q_per_seq}")
     if out is None:
         out = torch.empty_like(q)
     splits, ctas, part, part_o, part_ml, joins = _shares(splits, q_per_seq * (n_q // n_kv), dim, dev)
@@ -339,11 +343,30 @@ def decode_splits8(batch, n_kv, max_kv_len, sm_count=148, rows=0):
     return 0 if pairs > (48 if splits == CLUSTER else 84) * splits else splits
 
 
+def decode_pays(batch, new, n_q, n_kv, dim, seen, sm_count=148):
+    """Whether the decode kernel takes ``new`` query rows of each of ``batch`` sequences behind ``seen`` tokens in less time than the prefill kernel (estimates of either in us).
+    The former reads the pages once for every 16 rows that share a head, 0.6 ns a page, and a tile of them costs 9 ns beside that (head size 128, about half of 64).
+    The latter has a CTA for every head and 256 rows, however few they are. Those of one round take 2.1 us for 1000 keys; of more rounds each takes 4 us, and they read
+    keys and values, in bf16 and once for each query head, at 6.5 TB/s. Before, the pages are brought to bf16, three bytes a value.
+    Measured, decode / prefill, 32 heads of 128 over 8: 45 rows behind 512 10.4 / 15.5, behind 4096 24.2 / 24.9, behind 32768 123 / 104; 16 rows behind 32768 52 / 92; 64
+    behind 4096 29 / 26; 32 sequences with 9 rows behind 200 17 / 61; 64 with 9 behind 500 46 / 187; 100 with 20 rows 53 / 129, 8 with 100 25 / 17; one with 128
+    7.4 / 8.8, with 256 14.7 / 12.0. Heads of 64: 45 rows behind 4096 17.3 / 19.6, 64 rows 20.7 / 19.8, 300 rows 13.8 / 9.6."""
+    part = dim / 128
+    tiles = batch * n_kv * -(-new * (n_q // n_kv) // 16)
+    decode = 7 + tiles * (0.002 + 0.007 * part + 0.6e-3 * part * seen / PAGE)
+    ctas, keys = batch * n_q * -(-new // 256), -(-seen // 128) * 128
+    attention = 2.1e-3 * part * keys
+    if ctas > sm_count:
+        attention = max(attention, ctas * keys * 4 * dim / 6.5e6) + 4 * (ctas / sm_count - 1)
+    prefill = 12 + attention + batch * n_kv * seen * 6 * dim / 6.5e6
+    return decode < prefill
+
+
 def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len):
     """The form of :func:`.core.attention_prefill` for 8-bit pages on a GPU. The pages that some query sees are brought to bf16, in pages and a block table of
     their own, and the prefill kernel reads these: once for all query tiles and heads that share them, where a kernel that reads codes would convert
     each tile again for every one of them. Entries of that table that nobody sees point behind the last page, where the kernel's tensor maps read
-    zeros; its rows are whole key tiles of eight pages."""
+    zeros; its rows are whole key tiles of eight pages. Sequences that bring equally many rows, and few of them, go to the decode kernel."""
     check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q)
     (kc, ks), (vc, vs) = k_cache, v_cache
     dev, B, (total, n_q, dim) = q.device, seq_lens.shape[0], q.shape
@@ -352,6 +375,11 @@ def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_len
         out = torch.empty_like(q)
     if total == 0 or B == 0:
         return out
+    if total == B * max_q_len and max_kv_len > 0:
+        seen = min(max_kv_len, window + max_q_len if window > 0 else chunk + max_q_len if chunk > 0 else max_kv_len)
+        if decode_pays(B, max_q_len, n_q, n_kv, dim, seen, _sm_count(dev)):
+            splits = decode_splits8(B, n_kv, seen, _sm_count(dev), max_q_len * (n_q // n_kv))
+            return _decode8(q, k_cache, v_cache, block_table, seq_lens, max_q_len, scale, splits, window, sinks, out, chunk)
     wide = block_table.shape[1]
     if max_kv_len > 0:
         wide = min(wide, -(-max_kv_len // PAGE))

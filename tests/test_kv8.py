@@ -282,6 +282,16 @@ def test_prefill_attention(device, n_q, n_kv, dim, old, new, window, chunk, sink
         within(got, *attended(q, k.values(), v.values(), table, seq_lens, new, dim ** -0.5, window, chunk, s), 2.0 ** -8)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q, n_kv, dim", [(8, 2, 64), (32, 8, 128), (7, 1, 128)])
+@pytest.mark.parametrize("old, rows, window, chunk, sinks", [((4000,), 17, 0, 0, False), ((0, 500, 37), 9, 0, 0, True), ((300, 290), 33, 70, 0, False), ((90, 300), 12, 0, 64, True),
+                                                             ((9000,), 21, 0, 0, False), ((100,), 130, 0, 0, False)])
+def test_portions_of_equally_many_rows(n_q, n_kv, dim, old, rows, window, chunk, sinks):
+    """Few rows behind what is cached, as many for every sequence, with and without the longest length known."""
+    assert kv8.decode_pays(1, 45, 32, 8, 128, 512) and not kv8.decode_pays(1, 64, 32, 8, 128, 4160) and not kv8.decode_pays(1, 4096, 32, 8, 64, 4096)
+    test_prefill_attention("cuda", n_q, n_kv, dim, old, (rows,) * len(old), window, chunk, sinks)
+
+
 def expanded(pages, dim):
     """Pages whose scales differ by far more than f16 holds."""
     g = torch.Generator().manual_seed(5)
