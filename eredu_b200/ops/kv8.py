@@ -362,11 +362,12 @@ def decode_pays(batch, new, n_q, n_kv, dim, seen, sm_count=148):
     return decode < prefill
 
 
-def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len):
+def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len, equal=False):
     """The form of :func:`.core.attention_prefill` for 8-bit pages on a GPU. The pages that some query sees are brought to bf16, in pages and a block table of
     their own, and the prefill kernel reads these: once for all query tiles and heads that share them, where a kernel that reads codes would convert
     each tile again for every one of them. Entries of that table that nobody sees point behind the last page, where the kernel's tensor maps read
-    zeros; its rows are whole key tiles of eight pages. Sequences that bring equally many rows, and few of them, go to the decode kernel."""
+    zeros; its rows are whole key tiles of eight pages. Where the caller says that sequences bring equally many rows (what ``cu_q`` holds is not known
+    here, and rows behind its last entry are left as they are), few of them go to the decode kernel."""
     check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q)
     (kc, ks), (vc, vs) = k_cache, v_cache
     dev, B, (total, n_q, dim) = q.device, seq_lens.shape[0], q.shape
@@ -375,7 +376,7 @@ def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_len
         out = torch.empty_like(q)
     if total == 0 or B == 0:
         return out
-    if total == B * max_q_len and max_kv_len > 0:
+    if equal and max_kv_len > 0:
         seen = min(max_kv_len, window + max_q_len if window > 0 else chunk + max_q_len if chunk > 0 else max_kv_len)
         if decode_pays(B, max_q_len, n_q, n_kv, dim, seen, _sm_count(dev)):
             splits = decode_splits8(B, n_kv, seen, _sm_count(dev), max_q_len * (n_q // n_kv))

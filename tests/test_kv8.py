@@ -292,6 +292,36 @@ def test_portions_of_equally_many_rows(n_q, n_kv, dim, old, rows, window, chunk,
     test_prefill_attention("cuda", n_q, n_kv, dim, old, (rows,) * len(old), window, chunk, sinks)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q, n_kv, dim", [(8, 2, 64), (32, 8, 128), (7, 1, 128)])
+@pytest.mark.parametrize("old, rows, window, chunk, sinks", [((4000,), 17, 0, 0, False), ((0, 500, 37), 9, 0, 0, True), ((300, 290), 33, 70, 0, False), ((90, 300), 12, 0, 64, True),
+                                                             ((9000,), 21, 0, 0, False), ((100,), 130, 0, 0, False)])
+def test_portions_that_the_caller_knows_to_be_equal(n_q, n_kv, dim, old, rows, window, chunk, sinks):
+    seq_lens = [a + rows for a in old]
+    num, table = layout(seq_lens, "cuda", wider=1)
+    k, v = (filled(num, n_kv, dim, "cuda", seed=i) for i in range(2))
+    q = torch.randn((rows * len(old), n_q, dim), generator=torch.Generator().manual_seed(rows)).bfloat16().cuda()
+    s = torch.randn(n_q, device="cuda") if sinks else None
+    cu = ints([rows * i for i in range(len(old) + 1)], "cuda")
+    got = ops.attention_prefill(q, k, v, table, ints(seq_lens, "cuda"), cu, rows, dim ** -0.5, window=window, sinks=s, chunk=chunk, max_kv_len=max(seq_lens), equal=True)
+    within(got, *attended(q, k.values(), v.values(), table, seq_lens, [rows] * len(old), dim ** -0.5, window, chunk, s), 2.0 ** -8)
+    with pytest.raises(ValueError):
+        ops.attention_prefill(q[1:], k, v, table, ints(seq_lens, "cuda"), cu, rows, dim ** -0.5, max_kv_len=max(seq_lens), equal=True)
+
+
+@pytest.mark.gpu
+def test_padded_rows_of_a_prefill_are_left_as_they_were():
+    """As many rows as sequences times the longest portion, some of them behind the last sequence."""
+    n_q, n_kv, dim, lens, new = 8, 2, 128, (300, 40), (32, 20)
+    num, table = layout(lens, "cuda")
+    k, v = (filled(num, n_kv, dim, "cuda", seed=i) for i in range(2))
+    q = torch.randn((64, n_q, dim), generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    out = torch.full_like(q, 7.0)
+    ops.attention_prefill(q, k, v, table, ints(lens, "cuda"), ints([0, 32, 52], "cuda"), 32, dim ** -0.5, out=out, max_kv_len=300)
+    within(out[:52], *attended(q[:52], k.values(), v.values(), table, lens, new, dim ** -0.5), 2.0 ** -8)
+    assert (out[52:] == 7).all()
+
+
 def expanded(pages, dim):
     """Pages whose scales differ by far more than f16 holds."""
     g = torch.Generator().manual_seed(5)
