@@ -86,16 +86,16 @@ class PagedKVCache:
         self.kv_bits = 8 if kv_bits == 8 else None
         if self.kv_bits and (layer_pools or any(dk != dv for _, dk, dv in groups)):
             raise NotImplementedError("8-bit pages hold keys and values of one width, without means of blocks")
-        if self.kv_bits:
-            dtype = torch.int8
+        # pages alone are held in 8 bits: recurrent states and means of blocks are values of the model's type
+        self.state_dtype, page_dtype = dtype, torch.int8 if self.kv_bits else dtype
         self.pools, self._kv_index = [], {}
         self.scales: list = []               # 8-bit pages: fp32 [layers, pages, heads] of keys and of values, per pool
         for g, ((heads, dk, dv), members) in enumerate(groups.items()):
             if self.kv_bits:
                 self.scales.append(tuple(torch.full((len(members), num_pages, heads), FLOOR, dtype=torch.float32, device=device) for _ in "kv"))
-            k = torch.zeros((len(members), num_pages, heads, PAGE, dk), dtype=dtype, device=device)
+            k = torch.zeros((len(members), num_pages, heads, PAGE, dk), dtype=page_dtype, device=device)
             # latent-attention models cache one row per token in ``k`` and nothing in ``v`` (value_dim 1 keeps the plumbing)
-            v = torch.zeros_like(k) if dv == dk else torch.zeros((len(members), num_pages, heads, PAGE, dv), dtype=dtype,
+            v = torch.zeros_like(k) if dv == dk else torch.zeros((len(members), num_pages, heads, PAGE, dv), dtype=page_dtype,
                                                                  device=device)
             self.pools.append((k, v))
             self._kv_index.update({li: (g, i) for i, li in enumerate(members)})
@@ -136,7 +136,7 @@ class PagedKVCache:
         return pages
 
     def enable_linear_attention_state(self, layers, slots: int, conv_hist: int, conv_channels: int, heads: int, dk: int, dv: int):
-        dev, dt = self.k.device, self.k.dtype
+        dev, dt = self.k.device, self.state_dtype
         self._la_index = {li: i for i, li in enumerate(layers)}
         n = len(self._la_index)
         self.la_conv_state = torch.zeros((n, slots, conv_hist, conv_channels), dtype=dt, device=dev)
