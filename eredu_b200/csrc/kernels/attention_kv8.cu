@@ -90,6 +90,12 @@ __device__ __forceinline__ float lg2_approx(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The smaller one, or no number where one of them is none (fminf gives the other).
+__device__ __forceinline__ float min_or_none(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
   return v;
@@ -546,8 +552,8 @@ __global__ void __launch_bounds__(kKv8Threads, 3) attn_kv8_kernel(AttnKv8Params 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
-        // (value scales that are further apart than this has room for, over 2^126, lose the smaller ones)
-        const float f0 = ex2_approx(fminf(f[u][nt][0], 126.f)), f1 = ex2_approx(fminf(f[u][nt][1], 126.f));
+        // (value scales that are further apart than this has room for, over 2^126, lose the smaller ones; the scale of a block that is no number stays none)
+        const float f0 = ex2_approx(min_or_none(f[u][nt][0], 126.f)), f1 = ex2_approx(min_or_none(f[u][nt][1], 126.f));
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float e = ex2_approx(d[u][nt][c]);

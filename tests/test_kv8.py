@@ -379,6 +379,34 @@ def test_what_is_no_number_reaches_only_those_who_see_it():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim, n_q, n_kv", [(64, 4, 1), (128, 32, 2)])
+@pytest.mark.parametrize("splits", [1, 3, 0])
+@pytest.mark.parametrize("apart", [0.0, 200.0])
+def test_values_that_are_no_numbers_give_none(dim, n_q, n_kv, splits, apart):
+    """A block of values that a write has marked: every code is the same, so that no sum of products of both signs stands in for what is no number. Also where the
+    block's tokens weigh nothing (scores that are ``apart`` below the others' in units of log2: a product of zero and no number is none)."""
+    seq_lens = (400, 90)
+    num, table = layout(seq_lens, "cuda")
+    k, v = (filled(num, n_kv, dim, "cuda", seed=i) for i in range(2))
+    q = torch.ones((2, n_q, dim), dtype=torch.bfloat16, device="cuda")
+    k.codes.fill_(1)
+    k.scales.fill_(1.0)
+    marked = table[0, 7].item()
+    rows = torch.full((PAGE, n_kv, dim), 1 - apart / dim, dtype=torch.bfloat16, device="cuda")
+    bad = torch.ones_like(rows)
+    bad[3, :, 5] = math.nan
+    ops.store_kv(rows, bad, torch.arange(marked * PAGE, (marked + 1) * PAGE, device="cuda"), k, v)
+    assert v.scales[marked].isnan().all()
+    got = ops.attention_decode(q, k, v, table, ints(seq_lens, "cuda"), 1, math.log(2.0), splits=splits)
+    assert got[0].isnan().all() and torch.isfinite(got[1]).all()
+    cu = ints([0, 1, 2], "cuda")
+    assert ops.attention_prefill(q, k, v, table, ints(seq_lens, "cuda"), cu, 1, math.log(2.0))[0].isnan().all()
+    # and where nobody sees it, nobody has it
+    got = ops.attention_decode(q, k, v, table, ints(seq_lens, "cuda"), 1, math.log(2.0), splits=splits, window=200)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.gpu
 def test_block_tables_that_are_part_of_a_wider_one():
     """Rows of another pitch than their width; lengths that say more than the table has are cut there, and nothing behind the table is read."""
     seq_lens = (70, 33)
