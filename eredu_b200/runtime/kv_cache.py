@@ -283,15 +283,15 @@ class PagedKVCache:
         self.allocator.resize(num_pages)
         keep = min(num_pages, self.num_pages)
 
-        def other(t, dim=1):
+        def other(t, dim=1, fill=0):
             shape = list(t.shape)
             shape[dim] = num_pages
-            new = t.new_zeros(shape)
+            new = t.new_full(shape, fill)
             new.narrow(dim, 0, keep).copy_(t.narrow(dim, 0, keep))
             return new
 
         self.pools = [tuple(other(t) for t in pair) for pair in self.pools]
-        self.scales = [tuple(other(t) for t in pair) for pair in self.scales]
+        self.scales = [tuple(other(t, fill=FLOOR) for t in pair) for pair in self.scales]
         self.pooled = {li: tuple(other(t, 0) for t in pair) for li, pair in self.pooled.items()}
         self.k, self.v = self.pools[0]
         if self.conv_state is not None:

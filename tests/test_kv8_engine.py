@@ -279,6 +279,14 @@ def test_the_pool_changes_its_size(bits):
         eng.resize_cache(50, [seqs[1], seqs[3]])
 
 
+def test_scales_of_new_pages_are_those_of_a_new_pool():
+    """A block that nobody has opened has the smallest scale there is."""
+    kv = PagedKVCache(2, 3, 64, 6, torch.float32, "cpu", kv_bits=8)
+    kv.scales[0][0][:, 2] = 0.5
+    kv.resize(11)
+    assert (kv.scales[0][0][:, 2] == 0.5).all() and (kv.scales[0][0][:, 3:] == 2.0 ** -100).all() and (kv.scales[0][1] == 2.0 ** -100).all()
+
+
 def allocators(n):
     from eredu_b200.lib import _eredu_host
 
