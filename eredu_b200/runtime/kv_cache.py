@@ -278,26 +278,46 @@ class PagedKVCache:
                 self.page_to_slot[p] = slot
         return dict(moves)
 
+    def _paged(self) -> list:
+        """Every tensor with an entry per page: (what holds it, its place there, the dimension of the pages, what a new page holds)."""
+        places = [(self.pools, g, j, 1, 0) for g in range(len(self.pools)) for j in range(2)]
+        places += [(self.scales, g, j, 1, FLOOR) for g in range(len(self.scales)) for j in range(2)]
+        places += [(self.pooled, li, j, 0, 0) for li in self.pooled for j in range(2)]
+        places += [(vars(self), name, None, dim, 0) for name, dim in (("conv_state", 1), ("page_to_slot", 0)) if getattr(self, name) is not None]
+        return places
+
     def resize(self, num_pages: int) -> None:
-        """Another number of pages, with the contents of those that stay; the pages that go must have none (:meth:`compact`)."""
-        self.allocator.resize(num_pages)
+        """Another number of pages, with the contents of those that stay; the pages that go must have none (:meth:`compact`). One tensor after the other is
+        replaced, so that one is there twice at most. Where memory does not suffice, the error leaves a cache that works: pages that go are given up
+        ahead of all tensors (as views of the old ones, until each has its own memory), pages that come are counted when every tensor has them."""
         keep = min(num_pages, self.num_pages)
 
-        def other(t, dim=1, fill=0):
+        def take(where, key, j):
+            return where[key] if j is None else where[key][j]
+
+        def put(where, key, j, t):
+            where[key] = t if j is None else tuple(t if i == j else other for i, other in enumerate(where[key]))
+            self.k, self.v = self.pools[0]
+
+        places = self._paged()
+        if num_pages < self.num_pages:
+            self.allocator.resize(num_pages)
+            self.num_pages = num_pages
+            for where, key, j, dim, _ in places:
+                put(where, key, j, take(where, key, j).narrow(dim, 0, keep))
+        whole = []
+        for where, key, j, dim, fill in places:
+            t = take(where, key, j)
             shape = list(t.shape)
             shape[dim] = num_pages
             new = t.new_full(shape, fill)
             new.narrow(dim, 0, keep).copy_(t.narrow(dim, 0, keep))
-            return new
-
-        self.pools = [tuple(other(t) for t in pair) for pair in self.pools]
-        self.scales = [tuple(other(t, fill=FLOOR) for t in pair) for pair in self.scales]
-        self.pooled = {li: tuple(other(t, 0) for t in pair) for li, pair in self.pooled.items()}
-        self.k, self.v = self.pools[0]
-        if self.conv_state is not None:
-            self.conv_state = other(self.conv_state)
-        if self.page_to_slot is not None:
-            self.page_to_slot = other(self.page_to_slot, 0)
+            put(where, key, j, new.narrow(dim, 0, keep))
+            whole.append(new)
+        if num_pages > self.num_pages:
+            self.allocator.resize(num_pages)
+        for (where, key, j, *_), new in zip(places, whole):
+            put(where, key, j, new)
         self.num_pages = num_pages
 
     def require_uniform(self, what: str) -> None:

@@ -3,6 +3,7 @@ import dataclasses
 
 import pytest
 import torch
+import torch.utils._python_dispatch
 
 from eredu_b200 import ops
 from eredu_b200.models import config as C
@@ -277,6 +278,100 @@ def test_the_pool_changes_its_size(bits):
     eng.start_decode([seqs[1]], torch.tensor([1], dtype=torch.int32))
     with pytest.raises(RuntimeError, match="decode state"):
         eng.resize_cache(50, [seqs[1], seqs[3]])
+
+
+class Failing(torch.utils._python_dispatch.TorchDispatchMode):
+    """The n-th new tensor of the pool's shapes cannot be had."""
+
+    def __init__(self, n, pages):
+        super().__init__()
+        self.left, self.pages, self.seen = n, pages, []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        name = func.overloadpacket.__name__
+        out = func(*args, **(kwargs or {}))
+        if (name.startswith("new_") or name in ("empty", "zeros", "full", "clone")) and torch.is_tensor(out) and self.pages in out.shape:
+            self.left -= 1
+            self.seen.append(name)
+            if self.left < 0:
+                raise torch.OutOfMemoryError("no memory left")
+        return out
+
+
+@pytest.mark.parametrize("bits", [None, 8])
+@pytest.mark.parametrize("pages", [9, 41])
+@pytest.mark.parametrize("hybrid", [False, True])
+def test_a_pool_that_cannot_change_its_size_goes_on(bits, pages, hybrid):
+    """Whichever of the new tensors cannot be had: every tensor has the pages that the allocator gives, contents are what they were, and the next attempt succeeds."""
+    if hybrid:
+        from test_lfm2 import lfm2_cfg
+
+        cfg = lfm2_cfg(vocab_size=512)
+        sd = random_state(cfg, seed=1, std=0.08)
+        model = build_from_tensors(cfg, sd.__getitem__, sd.__contains__, "cpu", torch.float32)
+    else:
+        model = build()
+    twin = Engine(model, max_batch=4, max_seq_len=64, kv_bits=bits)
+    t = twin.new_sequence(prompt(20), GREEDY, max_new_tokens=20)
+    twin.feed_logits(t, t.prompt)
+    want = [twin.feed_logits(t, [x]).clone() for x in (5, 6)]
+    want.append(twin.feed_logits(twin.new_sequence(prompt(20), GREEDY, max_new_tokens=20), prompt(20) + [5]).clone())
+    for n in range(20):
+        eng = Engine(model, max_batch=4, max_seq_len=64, kv_bits=bits)
+        gone = eng.new_sequence(prompt(30), GREEDY, max_new_tokens=20)
+        seq = eng.new_sequence(prompt(20), GREEDY, max_new_tokens=20)
+        eng.feed_logits(seq, seq.prompt)
+        eng.release(gone)
+        try:
+            with Failing(n, pages):
+                eng.resize_cache(pages, [seq])
+            failed = False
+        except torch.OutOfMemoryError:
+            failed = True
+        kv = eng.kv
+
+        def consistent():
+            assert all(x.shape[1] == kv.num_pages for x in kv.page_tensors() + ([] if kv.conv_state is None else [kv.conv_state]))
+            assert kv.k is kv.pools[0][0] and kv.v is kv.pools[0][1]
+            assert len(kv.allocator.held()) + kv.allocator.free_pages() == kv.num_pages - 1
+            taken = kv.allocator.alloc(kv.allocator.free_pages())
+            assert max(taken) < kv.num_pages
+            kv.allocator.release(taken)
+
+        consistent()
+        assert kv.num_pages in ((pages,) if not failed else (17, min(17, pages)))
+        assert torch.equal(eng.feed_logits(seq, [5]), want[0])
+        eng.resize_cache(pages, [seq])
+        consistent()
+        assert kv.num_pages == pages and torch.equal(eng.feed_logits(seq, [6]), want[1])
+        last = eng.new_sequence(prompt(20), GREEDY, max_new_tokens=20)
+        assert torch.equal(eng.feed_logits(last, last.prompt + [5]), want[2])
+        if not failed:
+            break
+    assert not failed and n == (2 if bits is None else 4) + hybrid
+
+
+def test_new_pages_of_a_pool_are_those_of_a_new_pool():
+    """And no more than one tensor of the pool is there twice at a time."""
+    import weakref
+
+    kv = PagedKVCache(2, 3, 64, 6, torch.float32, "cpu", kv_bits=8)
+    old = [weakref.ref(t) for t in kv.pools[0]]
+    alive = []
+
+    class Watched(Failing):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            before = len(self.seen)
+            out = super().__torch_dispatch__(func, types, args, kwargs)
+            if len(self.seen) > before:
+                alive.append(sum(ref() is not None for ref in old))
+            return out
+
+    with Watched(99, 11):
+        kv.resize(11)
+    assert alive[:2] == [2, 1] and alive[-1] == 0
+    assert kv.scales[0][0].shape == (2, 11, 3) and all((s == 2.0 ** -100).all() for s in kv.scales[0])
+    assert not kv.k.any() and not kv.v.any()
 
 
 def test_scales_of_new_pages_are_those_of_a_new_pool():
