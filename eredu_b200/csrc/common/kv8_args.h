@@ -29,7 +29,8 @@ struct Kv8ValuesArgs {
   int* table_out;
   int* status;
   cudaStream_t stream;
-  int rows, pitch, table_wide, wide, n_kv, D, num_pages, window, chunk, spare;
+  int rows, pitch, table_wide, wide, n_kv, D, num_pages, window, chunk;
+  int entries;                            // with seq_lens: room of k_out and v_out where the rows follow one another; 0: rows of `wide`
 };
 
 struct Kv8AttentionArgs {

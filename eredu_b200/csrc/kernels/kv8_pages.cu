@@ -165,7 +165,9 @@ __global__ void __launch_bounds__(kStoreThreads, 4) kv8_store_kernel(Kv8StorePar
 // ============================================================================ values of pages
 // Codes times scale as bf16 (exact: 8 significant bits): [entries, n_kv, 16, D] for keys and for values. The pages are a list, or (seq_lens given)
 // the rows of a block table: then entries that no query of the sequence sees are left out, and `table_out` [rows, wide] says where each one is - those left out
-// lie behind the last one, where a tensor map reads zeros. One byte in, two out, bound by memory: 8192 tokens of 8 heads of 128, 7.6 us (50 MB, 6.6 TB/s).
+// lie behind the last one, where a tensor map reads zeros. With `entries` the rows of the table follow one another without what is left out: the memory is the
+// sum of what sequences see, not as many times the longest as there are sequences, and every CTA adds up the rows in front of its own (two numbers each, 256 at once).
+// One byte in, two out, bound by memory: 8192 tokens of 8 heads of 128, 7.6 us (50 MB, 6.6 TB/s).
 struct Kv8ValuesParams {
   const int8_t *k_codes, *v_codes;
   const float *k_scales, *v_scales;
@@ -175,9 +177,18 @@ struct Kv8ValuesParams {
   const int* cu_q;         // with seq_lens: query offsets
   int* table_out;          // with seq_lens: [rows, wide]
   int pitch, table_wide, wide, n_kv, num_pages, window, chunk;   // table_wide: entries of a row of `pages`; wide: of a row of the output
+  int entries;             // with seq_lens: entries that the output has room for, where rows follow one another; 0: rows of `wide`
   int* status;
 };
 constexpr int kValuesThreads = 256;
+// Entries [first, end) of a row that one of its sequence's queries sees.
+__device__ __forceinline__ int2 seen_entries(const Kv8ValuesParams& p, int row) {
+  const int len = p.seq_lens[row], first = len - (p.cu_q[row + 1] - p.cu_q[row]);
+  if (first >= len || len <= 0) return make_int2(0, 0);
+  const int low = p.window > 0 ? max(0, first - p.window + 1) : p.chunk > 0 && first > 0 ? first - first % p.chunk : 0;
+  const int end = min(min((len - 1) / kKv8Page + 1, p.wide), p.table_wide);
+  return make_int2(min(low / kKv8Page, end), end);
+}
 template <int D>
 __global__ void __launch_bounds__(kValuesThreads) kv8_values_kernel(Kv8ValuesParams p) {
   constexpr int BLOCK = kKv8Page * D, DEEP = 4;   // codes of a block; pieces of eight codes a thread has on their way
@@ -185,12 +196,30 @@ __global__ void __launch_bounds__(kValuesThreads) kv8_values_kernel(Kv8ValuesPar
   pdl_wait();
   pdl_launch_dependents();
   const int row = blockIdx.y, i = blockIdx.x;
-  const size_t entry = static_cast<size_t>(row) * p.wide + i;
+  size_t entry = static_cast<size_t>(row) * p.wide + i;
   if (p.seq_lens != nullptr) {
-    const int len = p.seq_lens[row], first = len - (p.cu_q[row + 1] - p.cu_q[row]);
-    const int low = p.window > 0 ? first - p.window + 1 : p.chunk > 0 && first > 0 ? first - first % p.chunk : 0;
-    const bool seen = i * kKv8Page < len && i * kKv8Page + kKv8Page > low && first < len && i < p.table_wide;
-    if (threadIdx.x == 0 && blockIdx.z == 0) p.table_out[entry] = static_cast<int>(seen ? entry : static_cast<size_t>(gridDim.y) * p.wide);
+    const size_t place = entry;
+    const int2 mine = seen_entries(p, row);
+    bool seen = i >= mine.x && i < mine.y;      // (for all of the CTA)
+    if (seen && p.entries > 0) {
+      __shared__ int parts[kValuesThreads / 32];
+      int front = 0;
+      for (int r = threadIdx.x; r < row; r += kValuesThreads) {
+        const int2 other = seen_entries(p, r);
+        front += other.y - other.x;
+      }
+      front = __reduce_add_sync(0xffffffffu, front);
+      if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = front;
+      __syncthreads();
+      entry = i - mine.x;
+#pragma unroll
+      for (int w = 0; w < kValuesThreads / 32; ++w) entry += parts[w];
+      if (entry >= static_cast<size_t>(p.entries)) {      // sequences are longer than the caller has said
+        if (threadIdx.x == 0) report_status(p.status, kStatusBadArgument);
+        seen = false;
+      }
+    }
+    if (threadIdx.x == 0 && blockIdx.z == 0) p.table_out[place] = static_cast<int>(seen ? entry : p.entries > 0 ? static_cast<size_t>(p.entries) : static_cast<size_t>(gridDim.y) * p.wide);
     if (!seen) return;
   }
   int page = p.pages[static_cast<size_t>(row) * p.pitch + i];
@@ -317,7 +346,7 @@ extern "C" int eredu_kv8_values(const void* args, int bytes) {
   Kv8ValuesArgs a;
   if (!kv8_args(a, args, bytes)) return -2;
   if (a.rows <= 0 || a.wide <= 0) return 0;
-  if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.rows > 65535 || a.num_pages <= 0) return -2;
+  if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.rows > 65535 || a.num_pages <= 0 || a.entries < 0) return -2;
   Kv8ValuesParams p = {};
   p.k_codes = static_cast<const int8_t*>(a.k_codes);
   p.v_codes = static_cast<const int8_t*>(a.v_codes);
@@ -336,6 +365,7 @@ extern "C" int eredu_kv8_values(const void* args, int bytes) {
   p.num_pages = a.num_pages;
   p.window = a.window;
   p.chunk = a.chunk;
+  p.entries = a.entries;
   p.status = a.status;
   const cudaError_t e = a.D == 128 ? launch_pdl(kv8_values_kernel<128>, dim3(a.wide, a.rows, 2), dim3(kValuesThreads), 0, a.stream, p)
                                    : launch_pdl(kv8_values_kernel<64>, dim3(a.wide, a.rows, 2), dim3(kValuesThreads), 0, a.stream, p);

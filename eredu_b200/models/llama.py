@@ -313,7 +313,7 @@ class CausalLM:
             attn = ops.attention_prefill(q, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.cu_q,
                                          batch.max_q_len, self.scale, window=window, sinks=lw.sinks,
                                          max_kv_len=max((a + n for a, n in batch.portions), default=0) if batch.portions else 0,
-                                         equal=bool(batch.portions) and all(n == batch.max_q_len for _, n in batch.portions))
+                                         portions=batch.portions)
         else:
             attn = ops.attention_decode(q, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.q_per_seq,
                                         self.scale, splits=batch.splits, window=window, sinks=lw.sinks,

@@ -144,7 +144,7 @@ def block_forward(model, li, lw, h, batch, kv):
                         cfg.head_dim, rot=cfg.head_dim)         # inv_freq is zero for this family: rotation is the identity
         if batch.is_prefill:
             attn = ops.attention_prefill(q, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.cu_q, batch.max_q_len,
-                                         model.scale)
+                                         model.scale, portions=batch.portions)
         else:
             attn = ops.attention_decode(q, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.q_per_seq, model.scale,
                                         splits=batch.splits, scratch=batch.scratch)

@@ -605,17 +605,18 @@ def _tensor_core_dims(q, k_cache, v_cache) -> bool:
 
 
 def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window=0, sinks=None,
-                      out=None, chunk=0, max_kv_len=0, equal=False):
+                      out=None, chunk=0, max_kv_len=0, equal=False, portions=None):
     """``window`` > 0: a query at position p sees keys in (p - window, p]; ``chunk`` > 0: the keys of its own chunk of
     positions. ``max_kv_len``: the largest of ``seq_lens`` where the host knows it (it chooses how the work is split, never what is
     computed; 0: unknown). Key and value widths are those of the caches. Returns [total_q, n_q, value width].
     Caches of :class:`Pages8`: the pages that some query sees are brought to bf16 first - once for all query tiles and heads that read them -, in memory
-    that the call allocates (``max_kv_len`` bounds it, and then has to be that of the longest sequence at least).
+    that the call allocates: as many pages as sequences see in all where ``portions`` states (cached tokens, new tokens) of every sequence, as the device has
+    them, else as many times the longest as there are sequences (``max_kv_len`` bounds it, and then has to be that of the longest sequence at least).
     ``equal``: the caller knows that every sequence brings max_q_len rows and that ``q`` has no others; few rows behind 8-bit pages then go to the decode kernel."""
     if equal and q.shape[0] != seq_lens.shape[0] * max_q_len:
         raise ValueError(f"{q.shape[0]} query rows are not {max_q_len} for each of {seq_lens.shape[0]} sequences")
     if q.is_cuda and (isinstance(k_cache, Pages8) or isinstance(v_cache, Pages8)):
-        return attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len, equal)
+        return attention_prefill8(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len, equal, portions)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
         if not _tensor_core_dims(q, k_cache, v_cache):
             return _attention_simt(q, k_cache, v_cache, block_table, seq_lens, cu_q, 0, max_q_len, scale, window, chunk, sinks)

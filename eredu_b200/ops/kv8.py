@@ -362,11 +362,23 @@ def decode_pays(batch, new, n_q, n_kv, dim, seen, sm_count=148):
     return decode < prefill
 
 
-def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len, equal=False):
+def seen_pages(portions, window, chunk, wide):
+    """Pages that some query of a sequence sees, of the first ``wide`` of its table, added up over sequences of (cached tokens, new tokens)."""
+    count = 0
+    for old, new in portions:
+        if new > 0:
+            low = max(0, old - window + 1) if window > 0 else old - old % chunk if chunk > 0 else 0
+            count += max(0, min(wide, -(-(old + new) // PAGE)) - low // PAGE)
+    return count
+
+
+def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, out, chunk, max_kv_len, equal=False,
+                       portions=None):
     """The form of :func:`.core.attention_prefill` for 8-bit pages on a GPU. The pages that some query sees are brought to bf16, in pages and a block table of
     their own, and the prefill kernel reads these: once for all query tiles and heads that share them, where a kernel that reads codes would convert
     each tile again for every one of them. Entries of that table that nobody sees point behind the last page, where the kernel's tensor maps read
-    zeros; its rows are whole key tiles of eight pages. Where the caller says that sequences bring equally many rows (what ``cu_q`` holds is not known
+    zeros; its rows are whole key tiles of eight pages. Memory: as many pages as sequences see in all where the caller states ``portions``, else as many times the
+    longest row of the table as there are sequences. Where the caller says that sequences bring equally many rows (what ``cu_q`` holds is not known
     here, and rows behind its last entry are left as they are), few of them go to the decode kernel."""
     check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_q)
     (kc, ks), (vc, vs) = k_cache, v_cache
@@ -376,6 +388,11 @@ def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_len
         out = torch.empty_like(q)
     if total == 0 or B == 0:
         return out
+    if portions:
+        if len(portions) != B:
+            raise ValueError(f"{len(portions)} portions for {B} sequences")
+        max_kv_len = max_kv_len or max(old + new for old, new in portions)
+        equal = equal or (total == B * max_q_len and all(new == max_q_len for _, new in portions))
     if equal and max_kv_len > 0:
         seen = min(max_kv_len, window + max_q_len if window > 0 else chunk + max_q_len if chunk > 0 else max_kv_len)
         if decode_pays(B, max_q_len, n_q, n_kv, dim, seen, _sm_count(dev)):
@@ -385,16 +402,21 @@ def attention_prefill8(q, k_cache: Pages8, v_cache: Pages8, block_table, seq_len
     if max_kv_len > 0:
         wide = min(wide, -(-max_kv_len // PAGE))
     wide = -(-wide // 8) * 8
-    half = B * wide * n_kv * PAGE * dim * 2                                  # bytes of the keys
+    room, entries = B * wide, 0
+    if portions:
+        seen = max(1, seen_pages(portions, window, chunk, block_table.shape[1]))
+        if seen < room:
+            room = entries = seen
+    half = room * n_kv * PAGE * dim * 2                                      # bytes of the keys
     held = torch.empty(2 * half + 4 * B * wide, dtype=torch.uint8, device=dev)
     at = held.data_ptr()
     table, status, stream = at + 2 * half, status_word(dev).data_ptr(), stream_ptr(dev)
     lens, cu = seq_lens.data_ptr(), cu_q.data_ptr()
     code = lib().eredu_kv8_values(_VALUES.pack(
         kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), at, at + half, block_table.data_ptr(), lens, cu, table, status, stream, B, block_table.stride(0),
-        block_table.shape[1], wide, n_kv, dim, num, int(window), int(chunk), 0), _VALUES.size)
+        block_table.shape[1], wide, n_kv, dim, num, int(window), int(chunk), entries), _VALUES.size)
     check(code, "eredu_kv8_values")
-    code = lib().eredu_attn_prefill_tc(q.data_ptr(), at, at + half, out.data_ptr(), table, lens, cu, ptr(sinks), B, total, max_q_len, wide, B * wide, n_q, n_kv, dim, dim,
+    code = lib().eredu_attn_prefill_tc(q.data_ptr(), at, at + half, out.data_ptr(), table, lens, cu, ptr(sinks), B, total, max_q_len, wide, room, n_q, n_kv, dim, dim,
                                        int(window), int(chunk), int(max_kv_len), _sm_count(dev), scale, status, stream)
     check(code, "eredu_attn_prefill_tc")
     return out

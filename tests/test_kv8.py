@@ -309,6 +309,64 @@ def test_portions_that_the_caller_knows_to_be_equal(n_q, n_kv, dim, old, rows, w
         ops.attention_prefill(q[1:], k, v, table, ints(seq_lens, "cuda"), cu, rows, dim ** -0.5, max_kv_len=max(seq_lens), equal=True)
 
 
+def test_pages_that_are_seen():
+    """Counted as defined: a page is seen when a key of it lies in some query's reach."""
+    g = torch.Generator().manual_seed(0)
+    for _ in range(300):
+        old, new, wide = (int(torch.randint(0, n, (), generator=g)) for n in (200, 50, 20))
+        window, chunk = ((0, 0), (1 + old % 70, 0), (0, 1 + new))[int(torch.randint(0, 3, (), generator=g))]
+        seen = set()
+        for pos in range(old, old + new):
+            low = max(0, pos - window + 1) if window else pos - pos % chunk if chunk else 0
+            seen |= {j // PAGE for j in range(low, pos + 1)}
+        # (pages between those of the first and of the last query count, and so does the chunk of the first query)
+        span = range(min(seen), max(seen) + 1) if seen else ()
+        assert kv8.seen_pages([(old, new)], window, chunk, wide) == len([p for p in span if p < wide])
+    assert kv8.seen_pages([(10, 3), (0, 0), (100, 0), (31, 2)], 0, 0, 99) == 1 + 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q, n_kv, dim", [(8, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("window, chunk, sinks", [(0, 0, False), (100, 0, True), (0, 64, False)])
+@pytest.mark.parametrize("old, new", [((8000,) + (30,) * 40, (3,) + tuple(range(40))), ((500, 0, 900, 17), (40, 0, 200, 1)), ((0, 5), (1, 0)), ((3000,), (70,)), ((40,) * 300 + (600,), (2,) * 300 + (9,))])
+def test_memory_of_a_prefill_is_what_its_sequences_see(n_q, n_kv, dim, window, chunk, sinks, old, new):
+    """Beside the output and two tables; and the values are those of rows that are as wide as the longest."""
+    seq_lens = [a + n for a, n in zip(old, new)]
+    num, table = layout(seq_lens, "cuda", wider=2)
+    k, v = (filled(num, n_kv, dim, "cuda", seed=i) for i in range(2))
+    q = torch.randn((sum(new) + 5, n_q, dim), generator=torch.Generator().manual_seed(n_q)).bfloat16().cuda()   # rows behind the last: left as they were
+    s = torch.randn(n_q, device="cuda") if sinks else None
+    cu, lens = ints([sum(new[:i]) for i in range(len(new) + 1)], "cuda"), ints(seq_lens, "cuda")
+    how = dict(window=window, sinks=s, chunk=chunk)
+    want = ops.attention_prefill(q, k, v, table, lens, cu, max(new), dim ** -0.5, out=torch.full_like(q, 3.0), max_kv_len=max(seq_lens), **how)
+    out = torch.full_like(q, 3.0)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.attention_prefill(q, k, v, table, lens, cu, max(new), dim ** -0.5, out=out, max_kv_len=max(seq_lens), portions=list(zip(old, new)), **how)
+    peak = torch.cuda.max_memory_allocated() - before
+    seen = kv8.seen_pages(zip(old, new), window, chunk, table.shape[1])
+    # the allocator rounds up to 2 MB at most where a block is taken apart
+    assert peak <= 2 * 2 * max(1, seen) * n_kv * PAGE * dim + 4 * len(old) * (table.shape[1] + 8) + (2 << 20)
+    assert torch.equal(out, want) and (out[sum(new):] == 3).all()
+    ops.native.check_status(torch.device("cuda"))
+
+
+@pytest.mark.gpu
+def test_portions_that_are_not_those_of_the_device():
+    """Sequences that are longer than the caller says: nothing is written behind what was allocated, and the status word says so. Wrong numbers of portions are refused."""
+    lens, new = (400, 300), (20, 30)
+    num, table = layout(lens, "cuda")
+    k, v = (filled(num, 2, 64, "cuda", seed=i) for i in range(2))
+    q = torch.randn((50, 8, 64), device="cuda").bfloat16()
+    cu = ints([0, 20, 50], "cuda")
+    with pytest.raises(ValueError, match="portions"):
+        ops.attention_prefill(q, k, v, table, ints(lens, "cuda"), cu, 30, 0.1, portions=[(380, 20)])
+    ops.attention_prefill(q, k, v, table, ints(lens, "cuda"), cu, 30, 0.1, max_kv_len=400, portions=[(10, 20), (270, 30)])
+    with pytest.raises(RuntimeError, match="bad argument"):
+        ops.native.check_status(torch.device("cuda"))
+
+
 @pytest.mark.gpu
 def test_padded_rows_of_a_prefill_are_left_as_they_were():
     """As many rows as sequences times the longest portion, some of them behind the last sequence."""

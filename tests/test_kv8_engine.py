@@ -103,6 +103,23 @@ def test_drafts_are_verified_over_8_bits(device):
     assert len(other.generate([prompt(21)], GREEDY, max_new_tokens=24)[0]) == 24
 
 
+@pytest.mark.gpu
+def test_a_long_sequence_beside_short_ones_takes_the_memory_of_one():
+    """A pass over sequences of unequal lengths: keys and values in bf16 of what they see, 8 KB a page here, not as many times the longest as there are sequences."""
+    model = build("cuda", num_attention_heads=4, num_key_value_heads=2, head_dim=64)
+    eng = Engine(model, max_batch=16, max_seq_len=8192, num_pages=700, kv_bits=8)
+    seqs = [eng.new_sequence(prompt(n, seed=n), GREEDY, max_new_tokens=8) for n in (8000, *range(20, 35))]
+    eng.prefill(seqs[:1], limits=[7990])
+    eng.prefill(seqs, limits=[2] + [len(s.prompt) - 3 for s in seqs[1:]])      # (so that nothing is set up for the first time below)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    eng.prefill(seqs)
+    peak = torch.cuda.max_memory_allocated() - before
+    seen = sum(-(-len(s.prompt) // PAGE) for s in seqs)
+    assert 16 * 500 * 8192 > 60e6 and peak <= 2 * seen * 8192 + (8 << 20)
+
+
 def test_what_does_not_take_8_bit_pages_says_so(tmp_path):
     from eredu_b200.runtime.kv_residency import KVHostTier
     from eredu_b200.runtime.prompt_cache import load_prompt_cache, save_prompt_cache
