@@ -349,6 +349,7 @@ class LoadedModel:
                 slots=eng._t(pages[p // PAGE] * PAGE + (p % PAGE), torch.int64),
                 block_table=eng._block_table([seq]), seq_lens=eng._t(np.asarray([n], dtype=np.int32), torch.int32),
                 is_prefill=True, cu_q=eng._t(np.asarray([0, n], dtype=np.int32), torch.int32), max_q_len=n,
+                portions=[(0, n)] if eng.kv.kv_bits else None,
                 logit_rows=eng._t(np.asarray([n - 1], dtype=np.int64), torch.int64))
             return self.model.forward(batch, eng.kv)[0].float().cpu()
         finally:

@@ -94,8 +94,10 @@ class SpeculativeDecoder:
             splits = self._splits(eng, len(seqs), lens[0], int(kv_after.max()))
             batch = ForwardBatch(is_prefill=False, q_per_seq=lens[0], splits=splits, **common)
         else:
+            # 8-bit pages: without the portions a pass brings the whole table's width to bf16, in every layer
+            portions = [(s.kv_len, n) for s, n in zip(seqs, lens)] if getattr(eng.kv, "kv_bits", None) else None
             batch = ForwardBatch(is_prefill=True, cu_q=eng._t(cu.astype(np.int32), torch.int32), max_q_len=max(lens),
-                                 **common)
+                                 portions=portions, **common)
         if prepare is not None:
             prepare(batch)             # embedded heads: activations instead of token embeddings, hidden-state capture
         return eng.model.forward(batch, eng.kv)

@@ -103,6 +103,39 @@ def test_drafts_are_verified_over_8_bits(device):
     assert len(other.generate([prompt(21)], GREEDY, max_new_tokens=24)[0]) == 24
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_passes_of_a_speculative_round_state_their_portions(device, monkeypatch):
+    """Ragged passes, of which every round has one, and the logits of a prompt: of the memory that a table of 32768 tokens would take they need what is there."""
+    from eredu_b200.api import LoadedModel
+    from eredu_b200.runtime.speculative import SpeculativeDecoder
+
+    model = build(device)
+    stated = []
+    plain = ops.attention_prefill
+
+    def attention_prefill(*args, portions=None, **more):
+        lens, cu = args[4].tolist(), args[5].tolist()
+        stated.append(portions is not None and [tuple(p) for p in portions] == [(n - (b - a), b - a) for n, a, b in zip(lens, cu, cu[1:])])
+        return plain(*args, portions=portions, **more)
+
+    monkeypatch.setattr(ops, "attention_prefill", attention_prefill)
+    target, draft = (Engine(model, max_batch=2, max_seq_len=32768, num_pages=200, kv_bits=8) for _ in "td")
+    dec = SpeculativeDecoder(target, draft, k=3)
+    dec.generate([prompt(21), prompt(40, seed=1)], GREEDY, max_new_tokens=4)
+    if device == "cuda":
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+    assert [len(o) for o in dec.generate([prompt(21), prompt(40, seed=1)], GREEDY, max_new_tokens=12)] == [12, 12]
+    lm = LoadedModel.__new__(LoadedModel)
+    lm.engine, lm.model = target, model
+    assert torch.isfinite(lm.prefill_logits(prompt(33))).all()
+    assert stated and all(stated)
+    if device == "cuda":
+        # (2 sequences x 2048 pages x 8 KB would be 33 MB)
+        assert torch.cuda.max_memory_allocated() - before <= 8 << 20
+
+
 @pytest.mark.gpu
 def test_a_long_sequence_beside_short_ones_takes_the_memory_of_one():
     """A pass over sequences of unequal lengths: keys and values in bf16 of what they see, 8 KB a page here, not as many times the longest as there are sequences."""
