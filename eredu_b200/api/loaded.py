@@ -136,7 +136,7 @@ class LoadedModel:
         par = opt.parallel
         ranks = 1 if par is None else par.topology.tensor
         hw.device_count = max(1, ranks)                  # this process drives one device of `ranks`
-        prof = estimate_runtime_state(report.config, report.tensor_bytes)
+        prof = estimate_runtime_state(report.config, report.tensor_bytes, kv_bits=opt.kv_bits)
         plan = AutomaticPlanner(hw).plan(report.config, prof, context=context, batch=batch,
                                          allow_quantization=allow_quantization and opt.quantization is None and not on_cpu,
                                          prefer_devices=ranks if ranks > 1 else None)

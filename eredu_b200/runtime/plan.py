@@ -215,8 +215,10 @@ class ModelResourceProfile:
     #                                    (then ``kv_bytes_per_token`` counts what grows with the whole context and ``sliding_layers`` is 0)
 
 
-def estimate_runtime_state(cfg: ModelConfig, weight_bytes: Optional[int] = None, cache_dtype_bytes: int = 2) -> ModelResourceProfile:
-    """KV bytes per token and static weight bytes of a decoder (``estimate_runtime_state``, capability.rs)."""
+def estimate_runtime_state(cfg: ModelConfig, weight_bytes: Optional[int] = None, cache_dtype_bytes: int = 2,
+                           kv_bits: Optional[int] = None) -> ModelResourceProfile:
+    """KV bytes per token and static weight bytes of a decoder (``estimate_runtime_state``, capability.rs). ``kv_bits`` = 8: keys and values in 8 bits with
+    a 4-byte scale per page and head; recurrent states stay in ``cache_dtype_bytes``."""
     H, D = cfg.hidden_size, cfg.head_dim
     L = cfg.num_hidden_layers
     family = _family_profile(cfg, weight_bytes, cache_dtype_bytes)
@@ -226,6 +228,10 @@ def estimate_runtime_state(cfg: ModelConfig, weight_bytes: Optional[int] = None,
     stateful = [li for li in range(L) if cfg.layer_is_conv(li) or cfg.layer_has_recurrent_state(li)]
     attn_layers = sum(1 for li in range(L) if cfg.layer_has_kv(li))
     kv_tok = 2 * cfg.num_key_value_heads * D * cache_dtype_bytes * attn_layers
+    if kv_bits == 8:
+        from .kv_cache import PAGE
+
+        kv_tok = -(-2 * cfg.num_key_value_heads * (PAGE * D + 4) // PAGE) * attn_layers
     if cfg.is_mla:   # one compressed latent + rotary key per token and layer, shared by the heads
         kv_tok = (cfg.kv_lora_rank + cfg.qk_rope_head_dim) * cache_dtype_bytes * attn_layers
     state = 0
