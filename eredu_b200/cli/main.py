@@ -217,7 +217,7 @@ def benchmark_candidates(model_path: str, a, candidates: list, prompt: str) -> d
                 open(plan_path, "w").write(plan.to_json())
                 cmd = [sys.executable, "-m", "eredu_b200.cli", "--model", model_path, "--device", a.device, "--auto-trial-plan",
                        plan_path, "--telemetry-json", tel_path, "--max-tokens", str(a.auto_benchmark_tokens), "--raw",
-                       "--mapped-shards", str(a.mapped_shards), prompt]
+                       "--mapped-shards", str(a.mapped_shards), "--kv-bits", str(a.kv_bits), prompt]
                 trial = {"run": run}
                 try:
                     r = subprocess.run(cmd, stdin=subprocess.DEVNULL, stdout=subprocess.DEVNULL, stderr=subprocess.PIPE,

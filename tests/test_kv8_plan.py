@@ -1,6 +1,7 @@
-"""Plans count the bytes of a cache held in 8 bits."""
+"""Plans count the bytes of a cache held in 8 bits, and trials of a plan run with it."""
 import dataclasses
 import json
+import subprocess
 
 import pytest
 import torch
@@ -75,3 +76,21 @@ def test_plans_of_either_cache_are_kept_apart(checkpoint, capsys):
     for bits in ("16", "8", "16"):
         assert main(["-m", str(checkpoint), "hi", "--device", "cpu", "-n", "2", "--auto-cache", str(cache), "--kv-bits", bits]) == 0
     assert len(json.loads(cache.read_text())) == 2
+
+
+@pytest.mark.parametrize("bits", ["8", "16"])
+def test_trials_run_with_the_cache_that_was_asked_for(checkpoint, capsys, monkeypatch, bits):
+    from eredu_b200.cli.main import build_parser, main
+
+    asked = []
+
+    def run(cmd, **how):
+        asked.append(build_parser().parse_args(cmd[3:]).kv_bits)
+        return subprocess.CompletedProcess(cmd, 1, b"", b"not run")
+
+    monkeypatch.setattr(subprocess, "run", run)
+    try:
+        main(["-m", str(checkpoint), "--device", "cpu", "--auto", "benchmark", "--auto-benchmark-tokens", "2", "--kv-bits", bits, "hello"])
+    except (SystemExit, RuntimeError):
+        pass                                # (no candidate is left)
+    assert asked and set(asked) == {int(bits)}
