@@ -89,7 +89,8 @@ def check_pages8(k: Pages8, v: Pages8, n_kv: int, head_dim: int) -> None:
     if (kc.dtype is torch.int8 and vc.dtype is torch.int8 and ks.dtype is torch.float32 and vs.dtype is torch.float32 and vc.shape == shape and len(shape) == 4
             and shape[1] == n_kv and shape[2] == PAGE and shape[3] == head_dim and ks.shape == shape[:2] and vs.shape == shape[:2]
             and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
-            and kc.get_device() == vc.get_device() == ks.get_device() == vs.get_device() and (head_dim in KV8_HEAD_DIMS or not kc.is_cuda)):
+            and kc.get_device() == vc.get_device() == ks.get_device() == vs.get_device()
+            and (not kc.is_cuda or (head_dim in KV8_HEAD_DIMS and (kc.data_ptr() | vc.data_ptr()) % 16 == 0))):
         return
     for name, t in (("keys", k), ("values", v)):
         if t.codes.dtype != torch.int8 or t.scales.dtype != torch.float32 or tuple(t.codes.shape[1:]) != (n_kv, PAGE, head_dim) \
@@ -100,6 +101,8 @@ def check_pages8(k: Pages8, v: Pages8, n_kv: int, head_dim: int) -> None:
             raise ValueError(f"{name}: codes and scales have to be contiguous and on one device")
     if kc.shape[0] != vc.shape[0] or kc.device != vc.device:
         raise ValueError("keys and values have to have the same pages")
+    if (kc.data_ptr() | vc.data_ptr()) % 16:
+        raise ValueError("codes have to begin at a multiple of 16 bytes")
     raise NotImplementedError(f"the kernels of 8-bit pages are built for head sizes {KV8_HEAD_DIMS}, not {head_dim}")
 
 
@@ -108,9 +111,12 @@ def address(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _need(name, t, dtype, device) -> None:
+def _need(name, t, dtype, device, align=1) -> None:
+    """``align``: bytes of the widest access that a kernel makes."""
     if t is not None and (t.dtype is not dtype or not t.is_contiguous() or t.device != device):
         raise ValueError(f"{name}: a contiguous {dtype} tensor on {device} is expected, not {t.dtype} on {t.device}")
+    if align > 1 and t is not None and t.data_ptr() % align:
+        raise ValueError(f"{name} has to begin at a multiple of {align} bytes")
 
 
 # ------------------------------------------------------------------------------------------ writing
@@ -154,6 +160,14 @@ def _store(q, k, v, slots, k_cache, v_cache, q_out, positions, inv_freq, n_q, n_
     check(code, "eredu_kv8_store")
 
 
+def _aligned_rows(t, head_dim):
+    """Rows as the kernel reads them: bf16, four values at a time."""
+    if t.dtype == torch.bfloat16 and t.stride()[1:] == (head_dim, 1) and t.stride(0) % 4 == 0 and t.data_ptr() % 8 == 0:
+        return t
+    t = t.to(torch.bfloat16).contiguous()
+    return t if t.data_ptr() % 8 == 0 else t.clone()      # (what is bf16 and contiguous already has not moved)
+
+
 def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
     """Keys and values [M, heads, head size] (as they are: rotated where the model rotates them) into the blocks of ``slots`` [M] int64 (page * 16 +
     offset; negative: not stored). The rows of a page follow one another in the order of their offsets, and a page occurs once in a call."""
@@ -166,8 +180,7 @@ def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
         store_rows_ref(v, slots, v_cache)
         return
     _need("slots", slots, torch.int64, k_cache.device)
-    k, v = (t if t.dtype == torch.bfloat16 and t.stride()[1:] == (head_dim, 1) and t.stride(0) % 4 == 0 and t.data_ptr() % 8 == 0
-            else t.to(torch.bfloat16).contiguous() for t in (k, v))
+    k, v = _aligned_rows(k, head_dim), _aligned_rows(v, head_dim)
     _store(0, k.data_ptr(), v.data_ptr(), slots, k_cache, v_cache, None, None, None, 0, n_kv, head_dim, 0, False, 1.0, None, None, 0.0, 0.0,
            (0, k.stride(0), v.stride(0)))
 
@@ -201,7 +214,7 @@ def rope_kv8(qkv, positions, slots, inv_freq, k_cache: Pages8, v_cache: Pages8, 
     if q_out is None:
         q_out = qkv.new_empty((M, n_q, head_dim))
     else:
-        _need("q_out", q_out, qkv.dtype, dev)
+        _need("q_out", q_out, qkv.dtype, dev, 16)
         if q_out.numel() != M * n_q * head_dim:
             raise ValueError(f"q_out has {q_out.numel()} elements for {M} rows of {n_q} heads of {head_dim}")
     ld, at = qkv.stride(0), qkv.data_ptr()
@@ -249,8 +262,8 @@ def check_attention8(q, k_cache, v_cache, block_table, seq_lens, sinks, out, cu_
     n_kv, dev = k_cache.codes.shape[1], k_cache.codes.device
     check_pages8(k_cache, v_cache, n_kv, dim)
     _check_batch(n_q, n_kv, block_table, seq_lens, sinks, dev)
-    _need("q", q, torch.bfloat16, dev)
-    _need("out", out, torch.bfloat16, dev)
+    _need("q", q, torch.bfloat16, dev, 16)
+    _need("out", out, torch.bfloat16, dev, 16)
     _need("cu_q", cu_q, torch.int32, dev)
     if cu_q is not None and cu_q.shape[0] != seq_lens.shape[0] + 1:
         raise ValueError(f"{cu_q.shape[0]} query offsets for {seq_lens.shape[0]} sequences")

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from eredu_b200 import ops
+from eredu_b200.ops import kv8
 from eredu_b200.ops.kv8 import PAGE, Pages8
 from eredu_b200.runtime.engine import Engine
 from eredu_b200.runtime.speculative import SpeculativeDecoder
@@ -189,3 +190,61 @@ def test_portions_of_whole_pages_leave_the_same_scales(device):
         assert ((a - b).abs() <= torch.maximum(*scales)[..., None, None] + 2.0 ** -7 * a.abs()).all()
         if device == "cpu":
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------ refusals
+def beside(t, elements):
+    """The same contents, contiguous, ``elements`` behind where an allocation begins."""
+    room = torch.empty(t.numel() + 64, dtype=t.dtype, device=t.device)
+    at = room[elements:elements + t.numel()].view(t.shape)
+    at.copy_(t)
+    assert at.is_contiguous()
+    return at
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_rows_to_be_stored_are_brought_to_where_they_can_be_read(kind):
+    x = torch.randn((5, 3, 64)).to(kind)
+    for t in (x, beside(x, 1), beside(x, 2), x[1:], torch.randn((5, 4, 64)).to(kind)[:, 1:], x.expand(5, 3, 64), x[:1].expand(4, 3, 64), torch.randn((5, 194)).to(kind)[:, :192].view(5, 3, 64),
+              x.transpose(1, 2).contiguous().transpose(1, 2)):
+        got = kv8._aligned_rows(t, 64)
+        assert got.dtype == torch.bfloat16 and got.data_ptr() % 8 == 0 and got.stride()[1:] == (64, 1) and got.stride(0) % 4 == 0 and torch.equal(got, t.bfloat16())
+
+
+@pytest.mark.gpu
+def test_addresses_that_the_kernels_cannot_take_are_refused():
+    """Contiguous tensors that begin inside an allocation: an access that is wider than their alignment would end the process's use of the GPU."""
+    dev = torch.device("cuda")
+    n_q, n_kv, dim = 4, 2, 64
+    k, v = (filled(4, n_kv, dim, dev, seed=i) for i in range(2))
+    rows, slots = torch.zeros((3, n_kv, dim), dtype=torch.bfloat16, device=dev), torch.arange(16, 19, device=dev)
+    q, table, lens, cu = torch.zeros((2, n_q, dim), dtype=torch.bfloat16, device=dev), ints([[1], [2]], dev), ints([3, 4], dev), ints([0, 1, 2], dev)
+    qkv, pos, to, freq = torch.zeros((2, 8 * dim), dtype=torch.bfloat16, device=dev), ints([2, 3], dev), torch.tensor([18, 35], device=dev), torch.ones(32, device=dev)
+    calls = dict(
+        store=lambda k, v, q, out: ops.store_kv(rows, rows, slots, k, v),
+        rope=lambda k, v, q, out: ops.rope_kv(qkv, pos, to, freq, k, v, n_q, n_kv, dim, q_out=out),
+        values=lambda k, v, q, out: ops.page_values(k, v, ints([1, 2], dev)),
+        decode=lambda k, v, q, out: ops.attention_decode(q, k, v, table, lens, 1, 1.0, out=out),
+        prefill=lambda k, v, q, out: ops.attention_prefill(q, k, v, table, lens, cu, 1, 1.0, out=out),
+        equal=lambda k, v, q, out: ops.attention_prefill(q, k, v, table, lens, cu, 1, 1.0, out=out, max_kv_len=4, equal=True),
+        step=lambda k, v, q, out: ops.attention_decode_rope(qkv, k, v, table, lens, 1, 1.0, pos, to, freq, n_q, n_kv, dim))
+    for name, call in calls.items():
+        call(k, v, q, torch.empty_like(q))
+        for by in (1, 4, 8):
+            for pair in ((Pages8(beside(k.codes, by), k.scales), v), (k, Pages8(beside(v.codes, by), v.scales))):
+                with pytest.raises(ValueError, match="16 bytes"):
+                    call(*pair, q, torch.empty_like(q))
+        call(Pages8(beside(k.codes, 16), beside(k.scales, 1)), Pages8(beside(v.codes, 32), beside(v.scales, 3)), beside(q, 8), beside(q, 16))
+        for by in (1, 2, 4):
+            if name in ("decode", "prefill", "equal"):
+                with pytest.raises(ValueError, match="16 bytes"):
+                    call(k, v, beside(q, by), torch.empty_like(q))
+            if name in ("rope", "decode", "prefill", "equal"):
+                with pytest.raises(ValueError, match="16 bytes"):
+                    call(k, v, q, beside(q, by))
+    # rows to be stored, and the projection's, may begin anywhere that is said
+    ops.store_kv(beside(rows, 1), beside(rows, 3), slots, k, v)
+    with pytest.raises(ValueError, match="8-byte aligned"):
+        ops.rope_kv(beside(qkv, 2), pos, to, freq, k, v, n_q, n_kv, dim)
+    torch.cuda.synchronize()
+    ops.native.check_status(dev)
