@@ -180,6 +180,8 @@ def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
         store_rows_ref(v, slots, v_cache)
         return
     _need("slots", slots, torch.int64, k_cache.device)
+    if k.device != k_cache.device or v.device != k_cache.device:
+        raise ValueError(f"keys on {k.device} and values on {v.device} for pages on {k_cache.device}")
     k, v = _aligned_rows(k, head_dim), _aligned_rows(v, head_dim)
     _store(0, k.data_ptr(), v.data_ptr(), slots, k_cache, v_cache, None, None, None, 0, n_kv, head_dim, 0, False, 1.0, None, None, 0.0, 0.0,
            (0, k.stride(0), v.stride(0)))

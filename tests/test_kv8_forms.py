@@ -213,7 +213,7 @@ def test_rows_to_be_stored_are_brought_to_where_they_can_be_read(kind):
 
 @pytest.mark.gpu
 def test_addresses_that_the_kernels_cannot_take_are_refused():
-    """Contiguous tensors that begin inside an allocation: an access that is wider than their alignment would end the process's use of the GPU."""
+    """Contiguous tensors that begin inside an allocation: an access that is wider than their alignment would end the process's use of the GPU. And rows on the host."""
     dev = torch.device("cuda")
     n_q, n_kv, dim = 4, 2, 64
     k, v = (filled(4, n_kv, dim, dev, seed=i) for i in range(2))
@@ -242,6 +242,9 @@ def test_addresses_that_the_kernels_cannot_take_are_refused():
             if name in ("rope", "decode", "prefill", "equal"):
                 with pytest.raises(ValueError, match="16 bytes"):
                     call(k, v, q, beside(q, by))
+    for a, b in ((rows.cpu(), rows), (rows, rows.cpu())):
+        with pytest.raises(ValueError, match="pages on cuda"):
+            ops.store_kv(a, b, slots, k, v)
     # rows to be stored, and the projection's, may begin anywhere that is said
     ops.store_kv(beside(rows, 1), beside(rows, 3), slots, k, v)
     with pytest.raises(ValueError, match="8-byte aligned"):
