@@ -5,11 +5,13 @@ The cache of a layer is a pair of :class:`Pages8` in place of two bf16 tensors; 
 
 A block is the 16 rows of one key / value head in a page: int8 codes in [-127, 127] and one fp32 scale, a power of two, value = code * scale.
 ``code = round(x / scale)`` (ties to even) with the smallest scale that keeps all codes in range, 2^-100 at least: a value is off by at most
-half a scale, between 1/254 and 1/127 of the block's largest magnitude.
+half a scale, between 1/254 and 1/127 of the block's largest magnitude. (With positions of three axes a key is rotated by tensor operations, and on a GPU rounded to bf16
+in front of its code.)
 Rows are written in the order of their tokens. A row at offset 0 opens its block and sets the scale; rows behind others keep the scale or,
 where one of them needs a larger one, raise it, and the codes in front are rounded again (at least twofold each time, so that all roundings of a value
 together stay below one scale). What lies behind the last row written is left from earlier use and means nothing. A row with an infinity or a NaN
-makes the scale, and with it the whole block, no number until the block is opened again.
+makes the scale, and with it the whole block, no number until the block is opened again. Rows that are taken back and written again (a verification) leave the scale they
+have raised.
 """
 from __future__ import annotations
 
@@ -169,7 +171,7 @@ def _aligned_rows(t, head_dim):
 
 
 def store_kv(k, v, slots, k_cache: Pages8, v_cache: Pages8) -> None:
-    """Keys and values [M, heads, head size] (as they are: rotated where the model rotates them) into the blocks of ``slots`` [M] int64 (page * 16 +
+    """Keys and values [M, heads, head size] (as they are: rotated where the model rotates them; on a GPU in bf16, others are rounded to it first) into the blocks of ``slots`` [M] int64 (page * 16 +
     offset; negative: not stored). The rows of a page follow one another in the order of their offsets, and a page occurs once in a call."""
     if k.shape != v.shape or k.dim() != 3 or slots.shape != k.shape[:1]:
         raise ValueError(f"keys {tuple(k.shape)}, values {tuple(v.shape)} and slots {tuple(slots.shape)} do not go together")
