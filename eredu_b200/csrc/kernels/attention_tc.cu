@@ -61,6 +61,7 @@ struct AttnTcParams {
   // POOL form (window > 0): all whole blocks of `pool` tokens of a sequence as dense rows from pool_first[b] on
   const int* pool_first;
   int pool;
+  float* lse;                  // optional [tokens, n_q]: log2 of the sum of 2^(score log2 e) of every row, the sink's term included (-inf: it saw nothing)
   // SPLIT form: 2^gshift query heads of a key / value head share a tile, row = (token << gshift) + head
   int gshift;
 };
@@ -338,6 +339,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const bool next = jj + 1 < total;
         bool k_ready = false;
         ok = mbar_wait_warp(&v_full[VST == 2 ? jj & 1 : 0], (VST == 2 ? jj >> 1 : jj) & 1, p.status, kStatusTmaFullTimeout);
+        if (!ROWS && ok && jj >= pooled && (j0 + jj - pooled + 1) * kTcTile > kv_len) {
+          // value rows behind the last token are whatever their page was left with: a probability of zero does not make a number of what is none
+          const uint32_t va = smem_u32(v_s + (VST == 2 ? jj & 1 : 0) * NV * kTcHalf);
+          for (int i = max(0, kv_len - (j0 + jj - pooled) * kTcTile) * 8 + lane; i < kTcTile * 8; i += 32)
+#pragma unroll
+            for (int x = 0; x < NV; ++x) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(va + x * kTcHalf + i * 16), "r"(0) : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         for (int w = 0; w < 2 && ok; ++w) {
           if (active(w, jj)) {
             ok = mbar_wait_warp(&p_full[w], done[w] & 1, p.status, kStatusAccumTimeout);   // P_w(j) is in tensor memory, O_w is rescaled
@@ -473,6 +483,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const bool store = tile_row0 + row < q_len;
       if (p.sinks != nullptr) l += ex2_approx(p.sinks[head] * 1.4426950408889634f - m);
       const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (!ROWS && !POOL && p.lse != nullptr && store)
+        p.lse[static_cast<size_t>(q0 + tile_row0 + row) * p.n_q_heads + head] = m == -INFINITY && l == l ? -INFINITY : m + __log2f(l);
       uint4* dst = reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(q0 + tile_row0 + row) * p.n_q_heads + head) * p.dv);
 #pragma unroll 1
       for (int c = 0; c < o_steps; ++c) {
@@ -567,6 +579,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const int h = head + (r & ((1 << gs) - 1));
       if (p.sinks != nullptr) l += ex2_approx(p.sinks[h] * 1.4426950408889634f - top);
       const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (p.lse != nullptr && piece == 0)
+        p.lse[static_cast<size_t>(q0 + row0 + (r >> gs)) * p.n_q_heads + h] = top == -INFINITY && l == l ? -INFINITY : top + __log2f(l);
       uint2* dst = reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(q0 + row0 + (r >> gs)) * p.n_q_heads + h) * p.dv);
       dst[piece] = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
     }
@@ -622,7 +636,7 @@ static int attn_prefill_tc_impl(const void* q, const void* k_cache, const void* 
                                 const int* block_table, const int* seq_lens, const int* cu_q, const int* pool_first, const float* sinks, int batch,
                                 int total_q, int max_q_len, int max_pages, int num_pages, int rows, int n_q_heads, int n_kv_heads, int key_dim,
                                 int value_dim, int window, int chunk, int pool, int max_kv_len, int sm_count, float scale, int* status,
-                                cudaStream_t stream) {
+                                cudaStream_t stream, float* lse = nullptr) {
   if (key_dim <= 0 || key_dim > 128 || key_dim % 8 != 0 || value_dim <= 0 || value_dim > 128 || value_dim % 8 != 0 || batch <= 0 ||
       total_q <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || window < 0 || chunk < 0)
     return -2;
@@ -676,6 +690,7 @@ static int attn_prefill_tc_impl(const void* q, const void* k_cache, const void* 
   p.dv = value_dim;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status;
+  p.lse = lse;
   dim3 grid(n_q_heads, (max_q_len + kTcRows - 1) / kTcRows, batch);
   int e;
   if (pool > 0) {
@@ -719,6 +734,15 @@ extern "C" int eredu_attn_prefill_tc(const void* q, const void* k_cache, const v
                                      int chunk, int max_kv_len, int sm_count, float scale, int* status, cudaStream_t stream) {
   return attn_prefill_tc_impl(q, k_cache, v_cache, nullptr, nullptr, out, block_table, seq_lens, cu_q, nullptr, sinks, batch, total_q, max_q_len,
                               max_pages, num_pages, 0, n_q_heads, n_kv_heads, key_dim, value_dim, window, chunk, 0, max_kv_len, sm_count, scale, status, stream);
+}
+
+// The same, and the logarithm of every row's sum (see AttnTcParams): lse [total_q, n_q_heads].
+extern "C" int eredu_attn_prefill_tc_lse(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int* block_table,
+                                         const int* seq_lens, const int* cu_q, const float* sinks, int batch, int total_q, int max_q_len,
+                                         int max_pages, int num_pages, int n_q_heads, int n_kv_heads, int dim, int window, int max_kv_len, int sm_count,
+                                         float scale, int* status, cudaStream_t stream) {
+  return attn_prefill_tc_impl(q, k_cache, v_cache, nullptr, nullptr, out, block_table, seq_lens, cu_q, nullptr, sinks, batch, total_q, max_q_len,
+                              max_pages, num_pages, 0, n_q_heads, n_kv_heads, dim, dim, window, 0, 0, max_kv_len, sm_count, scale, status, stream, lse);
 }
 
 // The POOL form: over the `window` newest tokens and the means of the blocks of `pool` tokens that end before them. k_rows / v_rows [rows,

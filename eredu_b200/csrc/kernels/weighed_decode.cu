@@ -1,0 +1,534 @@
+// Decode attention that adds up the weight it gives: out = softmax(scale q k^T) v over the pages of a sequence, as attention.cu has it, and
+// for every cached token and key / value head the sum of the softmax weights over the query rows and the query heads that share the head,
+// added to what earlier calls gave the token (the tokens that the call brings begin with it).
+//
+// A weight is known when the sum of its row is, behind the last key, so the scores have to be kept until then: 4 bytes for every
+// row and token beside the 512 (head size 128) of its key and value, in memory that stays in L2, where reading the keys a second time would be half as much again.
+//
+// grid (splits, n_kv, batch), four warps. A warp walks every fourth page of the split's share through a ring of its own, filled by TMA (page blocks
+// [16][64] with the 128-byte swizzle that ldmatrix reads without conflicts). Scores come as S^T = K Q^T (mma.sync m16n8k16: the sixteen keys of a page by eight rows, so
+// that the four to eight rows of a group fill the narrow side), and so does O^T = V^T P^T: a lane has two rows in both, whose maxima rescale its own accumulators. The
+// row maximum is a bound that is moved when a score is above it by more than 2^8: most pages need no exchange between lanes.
+// The splits of a sequence and head (up to eight) are a cluster: maxima, sums and outputs meet in shared memory, and every CTA weighs its own tokens. More splits leave
+// their part in memory, and a second kernel does the same.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "../common/launch.h"
+#include "../common/launch_count.h"
+#include "../common/ptx.cuh"
+#include "../common/tma_host.h"
+#include "../common/weights_args.h"
+
+namespace eredu {
+
+constexpr int kWdPage = 16;
+constexpr int kWdWarps = 4;
+constexpr int kWdStages = 3;
+constexpr int kWdCluster = 8;            // splits of a cluster
+constexpr int kWdMaxSplits = 64;
+constexpr float kWdGrow = 8.f;           // log2 units a score may lie above the bound in use
+
+struct WdParams {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const int *block_table, *seq_lens;
+  const float* sinks;
+  float *weights, *scores, *part_o, *part_ml;
+  int* status;
+  int q_per_seq, pitch, max_tokens, room, num_pages, n_q, n_kv, group, rows, pad, splits, window;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void wd_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void wd_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t wd_transposed(uint32_t v) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+__device__ __forceinline__ void wd_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void wd_load_page(void* dst, const CUtensorMap* map, int x, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ float wd_remote(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// What a (sequence, split) walks.
+struct WdShare {
+  int kv_len, first_pos;     // tokens, position of the first query row
+  int low;                   // first token that some row sees
+  int page0, page1;
+};
+__device__ __forceinline__ WdShare wd_share(const WdParams& p, int b, int split) {
+  WdShare s;
+  const int n = p.seq_lens[b];
+  s.kv_len = min(n, min(p.max_tokens, p.room));
+  if (n > s.kv_len) report_status(p.status, kStatusBadArgument);
+  s.first_pos = s.kv_len - p.q_per_seq;
+  s.low = p.window > 0 ? max(0, s.first_pos - p.window + 1) : 0;
+  const int base = s.low / kWdPage, pages = (s.kv_len + kWdPage - 1) / kWdPage;
+  const int per = max(0, (pages - base + p.splits - 1) / p.splits);
+  s.page0 = min(pages, base + split * per);
+  s.page1 = min(pages, s.page0 + per);
+  return s;
+}
+
+// The weights of the tokens of pages [page0, page1), summed over rows: 2^(score - top) / sum.
+__device__ __forceinline__ void wd_weigh(const WdParams& p, const WdShare& s, int b, int h, const float* top, const float* inv, int threads) {
+  const float* scores = p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad;
+  for (int t = s.page0 * kWdPage + static_cast<int>(threadIdx.x); t < s.page1 * kWdPage; t += threads) {
+    if (t >= s.kv_len || t < s.low) continue;
+    const float* at = scores + static_cast<size_t>(t) * p.pad;
+    float sum = 0.f;
+    for (int r = 0; r < p.rows; r += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(at + r);
+      sum += ex2_approx(v.x - top[r]) * inv[r];
+      if (r + 1 < p.rows) sum += ex2_approx(v.y - top[r + 1]) * inv[r + 1];
+    }
+    const int page = p.block_table[static_cast<size_t>(b) * p.pitch + t / kWdPage];
+    if (page < 0 || page >= p.num_pages) continue;
+    float* w = p.weights + (static_cast<size_t>(page) * p.n_kv + h) * kWdPage + t % kWdPage;
+    *w = t >= s.first_pos ? sum : *w + sum;
+  }
+}
+
+// Shared memory: the ring [warps][stages][K, V]; behind the last page the warps' parts [warps][ROWS][D + 4], maxima and sums, then
+// the CTA's part [ROWS][D], maxima and sums.
+template <int D, int NT>
+constexpr int wd_smem() {
+  constexpr int ring = kWdWarps * kWdStages * 2 * kWdPage * D * 2;
+  constexpr int rows = 8 * NT;
+  constexpr int merge = (kWdWarps * rows * (D + 4) + 2 * kWdWarps * rows + rows * D + 2 * rows) * 4;
+  return 1024 + (ring > merge ? ring : merge);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WdParams p) {
+  constexpr int KS = D / 16, HALVES = D / 64, ROWS = 8 * NT, NTH = 32 * kWdWarps;
+  constexpr int BLOCK = kWdPage * D * 2, STAGE = 2 * BLOCK;
+  extern __shared__ __align__(1024) uint8_t wd_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wd_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ uint64_t full[kWdWarps][kWdStages];
+  __shared__ float s_top[ROWS], s_inv[ROWS], s_part[ROWS][kWdCluster];
+  const int warp = static_cast<int>(warp_uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  pdl_launch_early();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWdWarps * kWdStages; ++i) mbar_init(&full[0][0] + i, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  const WdShare s = wd_share(p, b, split);
+  const int* table = p.block_table + static_cast<size_t>(b) * p.pitch;
+  const bool one = elect_one();
+  uint8_t* ring = smem + warp * kWdStages * STAGE;
+  const int first = s.page0 + warp;
+  int ids = 0;                                                        // lane l: the page of this warp's iteration 32 i + l
+  auto next_ids = [&](int it) {
+    const int pg = first + (it + lane) * kWdWarps;
+    ids = pg < s.page1 ? table[pg] : 0;
+    if (ids < 0 || ids >= p.num_pages) {
+      report_status(p.status, kStatusBadArgument);
+      ids = 0;
+    }
+  };
+  auto fetch = [&](int it) {                                          // called with it = 0, 1, 2, ..
+    if ((it & 31) == 0) next_ids(it);
+    const int page = __shfl_sync(0xffffffffu, ids, it & 31);
+    if (first + it * kWdWarps >= s.page1) return;
+    const int st = it % kWdStages;
+    if (one) {
+      mbar_arrive_expect_tx(&full[warp][st], STAGE);
+#pragma unroll
+      for (int i = 0; i < HALVES; ++i) {
+        wd_load_page(ring + st * STAGE + i * 2048, &tmK, i * 64, h, page, &full[warp][st]);
+        wd_load_page(ring + st * STAGE + BLOCK + i * 2048, &tmV, i * 64, h, page, &full[warp][st]);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kWdStages; ++i) fetch(i);
+  // queries as B fragments: lane (g, t) has row g of every eight, dims 16 ks + 2 t and + 8
+  uint32_t qf[NT][KS][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g;
+    const int token = r / p.group, head = h * p.group + r % p.group;
+    const uint32_t* row = reinterpret_cast<const uint32_t*>(p.q + (static_cast<size_t>(b * p.q_per_seq + token) * p.n_q + head) * D);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[nt][ks][0] = r < p.rows ? row[ks * 8 + tig] : 0u;
+      qf[nt][ks][1] = r < p.rows ? row[ks * 8 + tig + 4] : 0u;
+    }
+  }
+  float o[NT][KS][4], top[NT][2], sum[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    top[nt][0] = top[nt][1] = -INFINITY;
+    sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+  }
+  float* scores = p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad;
+  const uint32_t ring_addr = smem_u32(ring);
+  const int a_row = lane & 15, v_row = (lane >> 4) * 8 + (lane & 7);
+  bool ok = true;
+  int it = 0;
+  for (int pg = first; pg < s.page1 && ok; pg += kWdWarps, ++it) {
+    const int st = it % kWdStages;
+    ok = mbar_wait_warp(&full[warp][st], (it / kWdStages) & 1, p.status, kStatusTmaFullTimeout);
+    if (!ok) break;
+    const uint32_t k_addr = ring_addr + st * STAGE, v_addr = k_addr + BLOCK;
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a[4];
+      const int chunk = ks * 2 + (lane >> 4);
+      wd_ldsm(k_addr + (chunk >> 3) * 2048 + a_row * 128 + (((chunk & 7) ^ (a_row & 7)) << 4), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) wd_mma(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+    }
+    const int key0 = pg * kWdPage;
+    const bool edge = key0 + kWdPage - 1 > s.first_pos || (p.window > 0 && key0 < s.kv_len - p.window);
+    uint32_t pf[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[nt][e] *= p.scale_log2;
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + g + (e >> 1) * 8, r = nt * 8 + 2 * tig + (e & 1), pos = s.first_pos + r / p.group;
+          if (key > pos || (p.window > 0 && key <= pos - p.window)) sc[nt][e] = -INFINITY;
+        }
+      }
+      if (nt * 8 + 2 * tig < p.pad) {
+        float* at = scores + static_cast<size_t>(key0 + g) * p.pad + nt * 8 + 2 * tig;
+        *reinterpret_cast<float2*>(at) = make_float2(sc[nt][0], sc[nt][1]);
+        *reinterpret_cast<float2*>(at + 8 * p.pad) = make_float2(sc[nt][2], sc[nt][3]);
+      }
+      float mx0 = fmaxf(sc[nt][0], sc[nt][2]), mx1 = fmaxf(sc[nt][1], sc[nt][3]);
+      const bool grow = (mx0 > top[nt][0] + kWdGrow) || (mx1 > top[nt][1] + kWdGrow);
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, m));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, m));
+        }
+        mx0 = fmaxf(mx0, top[nt][0]);
+        mx1 = fmaxf(mx1, top[nt][1]);
+        // (a row that has seen nothing has nothing to rescale)
+        const float c0 = top[nt][0] == -INFINITY ? 0.f : ex2_approx(top[nt][0] - mx0), c1 = top[nt][1] == -INFINITY ? 0.f : ex2_approx(top[nt][1] - mx1);
+        top[nt][0] = mx0;
+        top[nt][1] = mx1;
+        sum[nt][0] *= c0;
+        sum[nt][1] *= c1;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          o[nt][i][0] *= c0;
+          o[nt][i][1] *= c1;
+          o[nt][i][2] *= c0;
+          o[nt][i][3] *= c1;
+        }
+      }
+      const float m0 = top[nt][0] == -INFINITY ? 0.f : top[nt][0], m1 = top[nt][1] == -INFINITY ? 0.f : top[nt][1];
+      const float p0 = ex2_approx(sc[nt][0] - m0), p1 = ex2_approx(sc[nt][1] - m1), p2 = ex2_approx(sc[nt][2] - m0), p3 = ex2_approx(sc[nt][3] - m1);
+      sum[nt][0] += p0 + p2;
+      sum[nt][1] += p1 + p3;
+      pf[nt][0] = wd_transposed(pack_bf16x2(p0, p1));
+      pf[nt][1] = wd_transposed(pack_bf16x2(p2, p3));
+    }
+    // values of tokens that no row sees, in front of the window or behind the last one: a weight of zero does not make a number of what is none
+    if (key0 < s.low || key0 + kWdPage > s.kv_len) {
+      for (int i = lane; i < kWdPage * (D / 8); i += 32) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        if (key0 + r < s.low || key0 + r >= s.kv_len)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_addr + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4)), "r"(0) : "memory");
+      }
+      fence_proxy_async_smem();                                       // the stage is filled again by TMA
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      uint32_t a[4];
+      const int chunk = i * 2 + ((lane >> 3) & 1);
+      wd_ldsm_t(v_addr + (chunk >> 3) * 2048 + v_row * 128 + (((chunk & 7) ^ (v_row & 7)) << 4), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) wd_mma(o[nt][i], a, pf[nt][0], pf[nt][1]);
+    }
+    __syncwarp();
+    fetch(it + kWdStages);
+  }
+  // (a wait that ran out: what is on its way must have landed before the ring is used for anything else)
+  if (!ok)
+    for (int i = 0; i < kWdStages; ++i)
+      if (first + (it + i) * kWdWarps < s.page1) mbar_wait(&full[warp][(it + i) % kWdStages], ((it + i) / kWdStages) & 1, p.status, kStatusTmaFullTimeout);
+  __syncthreads();
+  // ---- the warps' parts
+  float* mo = reinterpret_cast<float*>(smem);                         // [warps][ROWS][D + 4]
+  float* mm = mo + kWdWarps * ROWS * (D + 4);                         // [warps][ROWS]
+  float* ml = mm + kWdWarps * ROWS;
+  float* po = ml + kWdWarps * ROWS;                                   // [ROWS][D]
+  float* pm = po + ROWS * D;
+  float* pl = pm + ROWS;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float l = sum[nt][j];
+#pragma unroll
+      for (int m = 4; m < 32; m <<= 1) l += __shfl_xor_sync(0xffffffffu, l, m);
+      const int r = nt * 8 + 2 * tig + j;
+      if (g == 0) {
+        mm[warp * ROWS + r] = top[nt][j];
+        ml[warp * ROWS + r] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        mo[(warp * ROWS + r) * (D + 4) + i * 16 + g] = o[nt][i][j];
+        mo[(warp * ROWS + r) * (D + 4) + i * 16 + g + 8] = o[nt][i][2 + j];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.rows * D; i += NTH) {
+    const int r = i / D, d = i % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWdWarps; ++w) M = fmaxf(M, mm[w * ROWS + r]);
+    float L = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWdWarps; ++w) {
+      const float m = mm[w * ROWS + r], c = m == -INFINITY ? (ml[w * ROWS + r] != 0.f ? 1.f : 0.f) : ex2_approx(m - M);   // (a sum without a maximum is no number, and stays)
+      L += ml[w * ROWS + r] * c;
+      acc += mo[(w * ROWS + r) * (D + 4) + d] * c;
+    }
+    po[r * D + d] = acc;
+    if (d == 0) {
+      pm[r] = M;
+      pl[r] = L;
+    }
+  }
+  if (p.part_o != nullptr) {
+    // a second kernel joins the splits
+    __syncthreads();
+    const size_t at = (static_cast<size_t>(b) * p.n_kv + h) * p.splits + split;
+    for (int i = threadIdx.x; i < p.rows * D; i += NTH) p.part_o[at * p.rows * D + i] = po[i];
+    for (int i = threadIdx.x; i < p.rows; i += NTH) {
+      p.part_ml[(at * p.rows + i) * 2] = pm[i];
+      p.part_ml[(at * p.rows + i) * 2 + 1] = pl[i];
+    }
+    return;
+  }
+  const bool many = p.splits > 1;
+  if (many) {
+    __syncwarp();
+    cluster_arrive_release();
+    cluster_wait_acquire();
+  } else {
+    __syncthreads();
+  }
+  const uint32_t a_o = smem_u32(po), a_m = smem_u32(pm), a_l = smem_u32(pl);
+  for (int r = threadIdx.x; r < p.rows; r += NTH) {
+    float ms[kWdCluster], ls[kWdCluster], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWdCluster; ++i) {
+      ms[i] = -INFINITY;
+      ls[i] = 0.f;
+      if (i < p.splits) {
+        ms[i] = many ? wd_remote(mapa_shared(a_m + r * 4, i)) : pm[r];
+        ls[i] = many ? wd_remote(mapa_shared(a_l + r * 4, i)) : pl[r];
+      }
+      M = fmaxf(M, ms[i]);
+    }
+    const float sink = p.sinks != nullptr ? p.sinks[h * p.group + r % p.group] * 1.4426950408889634f : -INFINITY;
+    if (M > -INFINITY && sink > M + 64.f) M = sink;                    // (a sink far above all scores: its own term stays finite)
+#pragma unroll
+    for (int i = 0; i < kWdCluster; ++i) {
+      const float c = ms[i] == -INFINITY ? (ls[i] != 0.f ? 1.f : 0.f) : ex2_approx(ms[i] - M);
+      s_part[r][i] = c;
+      L += ls[i] * c;
+    }
+    if (M > -INFINITY && p.sinks != nullptr) L += ex2_approx(sink - M);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    s_top[r] = M == -INFINITY ? 0.f : M;
+    s_inv[r] = inv;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x + split * NTH; i < p.rows * D; i += NTH * p.splits) {
+    const int r = i / D, d = i % D;
+    float acc = 0.f;
+    if (many) {
+#pragma unroll
+      for (int sp = 0; sp < kWdCluster; ++sp)
+        if (sp < p.splits) acc += wd_remote(mapa_shared(a_o + i * 4, sp)) * s_part[r][sp];
+    } else {
+      acc = po[i] * s_part[r][0];
+    }
+    p.out[(static_cast<size_t>(b * p.q_per_seq + r / p.group) * p.n_q + h * p.group + r % p.group) * D + d] = __float2bfloat16(acc * s_inv[r]);
+  }
+  if (many) {
+    __syncwarp();
+    cluster_arrive_release();                                         // done with the peers' shared memory
+  }
+  wd_weigh(p, s, b, h, s_top, s_inv, NTH);
+  if (many) {
+    __syncwarp();
+    cluster_wait_acquire();                                           // nobody leaves while a peer reads its part
+  }
+}
+
+// grid (splits, n_kv, batch): joins what the splits have left, a share of the output and of the tokens each.
+constexpr int kWdJoinThreads = 256;
+__global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdParams p, const int D) {
+  __shared__ float s_top[16], s_inv[16], s_part[16][kWdMaxSplits];
+  pdl_launch_early();
+  pdl_wait();
+  pdl_launch_dependents();
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const WdShare s = wd_share(p, b, split);
+  const size_t at = (static_cast<size_t>(b) * p.n_kv + h) * p.splits;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < p.rows; r += kWdJoinThreads / 32) {
+    float M = -INFINITY, L = 0.f;
+    float2 v[kWdMaxSplits / 32];
+#pragma unroll
+    for (int i = 0; i < kWdMaxSplits / 32; ++i) {
+      const int sp = i * 32 + lane;
+      v[i] = sp < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + ((at + sp) * p.rows + r) * 2) : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, v[i].x);
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, m));
+    const float sink = p.sinks != nullptr ? p.sinks[h * p.group + r % p.group] * 1.4426950408889634f : -INFINITY;
+    if (M > -INFINITY && sink > M + 64.f) M = sink;
+#pragma unroll
+    for (int i = 0; i < kWdMaxSplits / 32; ++i) {
+      const float c = v[i].x == -INFINITY ? (v[i].y != 0.f ? 1.f : 0.f) : ex2_approx(v[i].x - M);
+      s_part[r][i * 32 + lane] = c;
+      L += v[i].y * c;
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) L += __shfl_xor_sync(0xffffffffu, L, m);
+    if (M > -INFINITY && p.sinks != nullptr) L += ex2_approx(sink - M);
+    if (lane == 0) {
+      s_top[r] = M == -INFINITY ? 0.f : M;
+      s_inv[r] = L == 0.f ? 0.f : 1.f / L;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x + split * kWdJoinThreads; i < p.rows * D; i += kWdJoinThreads * p.splits) {
+    const int r = i / D, d = i % D;
+    float acc = 0.f;
+    for (int sp = 0; sp < p.splits; ++sp) acc += p.part_o[(at + sp) * p.rows * D + i] * s_part[r][sp];
+    p.out[(static_cast<size_t>(b * p.q_per_seq + r / p.group) * p.n_q + h * p.group + r % p.group) * D + d] = __float2bfloat16(acc * s_inv[r]);
+  }
+  wd_weigh(p, s, b, h, s_top, s_inv, kWdJoinThreads);
+}
+
+template <int D, int NT>
+static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdParams& p, int batch, cudaStream_t stream) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT>()) != cudaSuccess) return -1;
+    configured[dev] = true;
+  }
+  const bool cluster = p.part_o == nullptr && p.splits > 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.splits, p.n_kv, batch);
+  cfg.blockDim = dim3(32 * kWdWarps);
+  cfg.dynamicSmemBytes = wd_smem<D, NT>();
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = p.splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, weighed_decode_kernel<D, NT>, tmK, tmV, p);
+  eredu_count_launches(1);
+  if (e == cudaSuccess && p.part_o != nullptr) {
+    e = launch_pdl(weighed_join_kernel, dim3(p.splits, p.n_kv, batch), dim3(kWdJoinThreads), 0, stream, p, D);
+    eredu_count_launches(1);
+  }
+  return static_cast<int>(e);
+}
+
+}  // namespace eredu
+
+using namespace eredu;
+
+extern "C" int eredu_weighed_decode(const void* args, int bytes) {
+  WeighedDecodeArgs a;
+  if (!weights_args(a, args, bytes)) return -2;
+  if (a.batch <= 0 || a.q_per_seq <= 0) return 0;
+  if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.n_q % a.n_kv != 0 || a.num_pages <= 0 || a.batch > 65535 || a.n_kv > 65535 || a.splits < 1 ||
+      a.splits > kWdMaxSplits || a.window < 0 || a.room <= 0 || a.room % kWdPage != 0 || (a.splits > kWdCluster) != (a.part_o != nullptr))
+    return -2;
+  WdParams p = {};
+  p.group = a.n_q / a.n_kv;
+  if (static_cast<long long>(a.q_per_seq) * p.group > 16) return -2;
+  p.rows = a.q_per_seq * p.group;
+  p.pad = p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : p.rows <= 8 ? 8 : 16;
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.block_table = a.block_table;
+  p.seq_lens = a.seq_lens;
+  p.sinks = a.sinks;
+  p.weights = a.weights;
+  p.scores = a.scores;
+  p.part_o = a.part_o;
+  p.part_ml = a.part_ml;
+  p.status = a.status;
+  p.q_per_seq = a.q_per_seq;
+  p.pitch = a.pitch;
+  p.max_tokens = a.max_tokens;
+  p.room = a.room;
+  p.num_pages = a.num_pages;
+  p.n_q = a.n_q;
+  p.n_kv = a.n_kv;
+  p.splits = a.splits;
+  p.window = a.window;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  const uint64_t D = static_cast<uint64_t>(a.D), H = static_cast<uint64_t>(a.n_kv);
+  CUtensorMap tmK, tmV;
+  int r = make_tma_4d(&tmK, a.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, D, 16, H, static_cast<uint64_t>(a.num_pages), D * 2, 16 * D * 2, H * 16 * D * 2, 64, 16, 1, 1);
+  if (r != 0) return -100 + r;
+  r = make_tma_4d(&tmV, a.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, D, 16, H, static_cast<uint64_t>(a.num_pages), D * 2, 16 * D * 2, H * 16 * D * 2, 64, 16, 1, 1);
+  if (r != 0) return -200 + r;
+  if (a.D == 128) return p.rows <= 8 ? wd_launch<128, 1>(tmK, tmV, p, a.batch, a.stream) : wd_launch<128, 2>(tmK, tmV, p, a.batch, a.stream);
+  return p.rows <= 8 ? wd_launch<64, 1>(tmK, tmV, p, a.batch, a.stream) : wd_launch<64, 2>(tmK, tmV, p, a.batch, a.stream);
+}

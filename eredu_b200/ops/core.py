@@ -18,6 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import native
+from .eviction import weighed_decode, weighed_prefill
 from .kv8 import Pages8, attention_decode8, attention_prefill8, attention_step8, decode_splits8, rope_kv8, store_kv
 from .native import check, lib, ptr, status_word, stream_ptr
 
@@ -605,14 +606,18 @@ def _tensor_core_dims(q, k_cache, v_cache) -> bool:
 
 
 def attention_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window=0, sinks=None,
-                      out=None, chunk=0, max_kv_len=0, equal=False, portions=None):
+                      out=None, chunk=0, max_kv_len=0, equal=False, portions=None, weights=None, observed=0):
     """``window`` > 0: a query at position p sees keys in (p - window, p]; ``chunk`` > 0: the keys of its own chunk of
     positions. ``max_kv_len``: the largest of ``seq_lens`` where the host knows it (it chooses how the work is split, never what is
     computed; 0: unknown). Key and value widths are those of the caches. Returns [total_q, n_q, value width].
     Caches of :class:`Pages8`: the pages that some query sees are brought to bf16 first - once for all query tiles and heads that read them -, in memory
     that the call allocates: as many pages as sequences see in all where ``portions`` states (cached tokens, new tokens) of every sequence, as the device has
     them, else as many times the longest as there are sequences (``max_kv_len`` bounds it, and then has to be that of the longest sequence at least).
-    ``equal``: the caller knows that every sequence brings max_q_len rows and that ``q`` has no others; few rows behind 8-bit pages then go to the decode kernel."""
+    ``equal``: the caller knows that every sequence brings max_q_len rows and that ``q`` has no others; few rows behind 8-bit pages then go to the decode kernel.
+    ``weights`` (fp32 [pages, heads, 16]): the weight that every cached token gets is added up there (:mod:`.eviction`), over all rows or the last ``observed``
+    ones of every sequence."""
+    if weights is not None:
+        return weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, weights, out, chunk, max_kv_len, observed)
     if equal and q.shape[0] != seq_lens.shape[0] * max_q_len:
         raise ValueError(f"{q.shape[0]} query rows are not {max_q_len} for each of {seq_lens.shape[0]} sequences")
     if q.is_cuda and (isinstance(k_cache, Pages8) or isinstance(v_cache, Pages8)):
@@ -699,9 +704,13 @@ def _one_round_pays(ctas, pages, one_round, splits, sm_count, head_dim):
 
 
 def attention_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits=1, window=0, sinks=None,
-                     scratch=None, out=None, chunk=0):
+                     scratch=None, out=None, chunk=0, weights=None, max_kv_len=0):
     """q: [B * q_per_seq, n_q, D]; ``window`` / ``chunk`` as in :func:`attention_prefill`. ``scratch`` = (part_o, part_ml, counters) from :func:`decode_scratch` when
-    splits > 1 (fp32 partials and zeroed int32 arrival tickets). Caches of :class:`Pages8` need no ``scratch``; a query that sees no key gives zeros."""
+    splits > 1 (fp32 partials and zeroed int32 arrival tickets). Caches of :class:`Pages8` need no ``scratch``; a query that sees no key gives zeros.
+    ``weights`` (fp32 [pages, heads, 16]): the weight that every cached token gets is added up there (:mod:`.eviction`), by a kernel that chooses its own splits
+    and scratch; ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it."""
+    if weights is not None:
+        return weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len)
     if q.is_cuda and (isinstance(k_cache, Pages8) or isinstance(v_cache, Pages8)):
         return attention_decode8(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, splits, window, sinks, out, chunk)
     if q.is_cuda and (chunk > 0 or q.dtype == torch.float32 or v_cache.shape[3] != q.shape[2]):
