@@ -12,11 +12,10 @@ struct EvictArgs {
   float* weights;                         // [layers, pages, n_kv, 16]
   const int *block_table, *seq_lens;
   int* left;                              // [batch]: tokens that every sequence has left
-  int* list;                              // scratch [layers, batch, n_kv, keep]: the tokens that stay, in order
+  int* list;                              // scratch [layers, batch, n_kv, keep] of long sequences: the tokens that stay, in order
   int* status;
   cudaStream_t stream;
-  int layers, batch, n_kv, num_pages, pitch, max_tokens, keep, recent, first, k_row, v_row;
-  int unused;
+  int layers, batch, n_kv, num_pages, pitch, max_tokens, keep, recent, first, k_row, v_row, sm_count;
 };
 
 struct WeighedDecodeArgs {
@@ -33,14 +32,16 @@ struct WeighedDecodeArgs {
   float scale;
 };
 
-struct PromptWeightsArgs {
-  const void *q, *k;
-  const float* lse;                       // [total_q, n_q]: log2 of the sum of 2^(score log2 e)
+struct WeighedPrefillArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;                             // scratch [total_q, n_q]: log2 of the sum of 2^(score log2 e)
   const int *block_table, *seq_lens, *cu_q;
+  const float* sinks;
   float* weights;
   int* status;
   cudaStream_t stream;
-  int batch, total_q, max_q_len, max_kv_len, pitch, wide, num_pages, n_q, n_kv, D, window, observed, sm_count;
+  int batch, total_q, max_q_len, max_kv_len, wide, num_pages, n_q, n_kv, D, window, observed, ranks, sm_count;
   float scale;
 };
 

@@ -36,7 +36,7 @@ struct PwParams {
   const int *block_table, *seq_lens, *cu_q;
   float* weights;
   int* status;
-  int pitch, wide, num_pages, n_q, n_kv, group, gshift, window, observed;
+  int wide, num_pages, n_q, n_kv, group, gshift, window, observed;
   float scale_log2;
 };
 
@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
   pdl_wait();
   pdl_launch_dependents();
 
-  const int h = blockIdx.y, b = blockIdx.z, key0 = static_cast<int>(blockIdx.x) / ranks * kPwKeys;
+  // (blocks of keys vary slowest: the first ones are seen by the most rows)
+  const int h = static_cast<int>(blockIdx.x) / ranks, b = blockIdx.y, key0 = blockIdx.z * kPwKeys;
   const int q0 = static_cast<int>(warp_uniform(p.cu_q[b])), q_len = static_cast<int>(warp_uniform(p.cu_q[b + 1])) - q0;
   const int n = static_cast<int>(warp_uniform(p.seq_lens[b])), kv_len = min(n, p.wide * kPwPage);
   if (n > kv_len && threadIdx.x == 0) report_status(p.status, kStatusBadArgument);
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
     const bool one = elect_one();
     if (begin < end) {
       const int entry = key0 / kPwPage + (lane & 15);
-      int page = entry < p.wide && entry * kPwPage < kv_len ? p.block_table[static_cast<size_t>(b) * p.pitch + entry] : 0;
+      int page = entry < p.wide && entry * kPwPage < kv_len ? p.block_table[static_cast<size_t>(b) * p.wide + entry] : 0;
       if (page < 0 || page >= p.num_pages) {
         report_status(p.status, kStatusBadArgument);
         page = 0;
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
       total += v;
     }
     if (key < kv_len && q_len > 0 && (tiles > 0 || key >= before)) {
-      const int page = p.block_table[static_cast<size_t>(b) * p.pitch + key / kPwPage];
+      const int page = p.block_table[static_cast<size_t>(b) * p.wide + key / kPwPage];
       if (page >= 0 && page < p.num_pages) {
         float* at_w = p.weights + (static_cast<size_t>(page) * p.n_kv + h) * kPwPage + key % kPwPage;
         *at_w = key >= before ? total : *at_w + total;
@@ -280,7 +281,7 @@ static int pw_launch(const CUtensorMap& tmQ, const CUtensorMap& tmK, const PwPar
     configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks * ranks, p.n_kv, batch);
+  cfg.gridDim = dim3(p.n_kv * ranks, batch, blocks);
   cfg.blockDim = dim3(kPwThreads);
   cfg.dynamicSmemBytes = pw_smem(NK);
   cfg.stream = stream;
@@ -301,12 +302,23 @@ static int pw_launch(const CUtensorMap& tmQ, const CUtensorMap& tmK, const PwPar
 
 using namespace eredu;
 
-extern "C" int eredu_prompt_weights(const void* args, int bytes) {
-  PromptWeightsArgs a;
+extern "C" int eredu_attn_prefill_tc_lse(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int* block_table,
+                                         const int* seq_lens, const int* cu_q, const float* sinks, int batch, int total_q, int max_q_len,
+                                         int max_pages, int num_pages, int n_q_heads, int n_kv_heads, int dim, int window, int max_kv_len, int sm_count,
+                                         float scale, int* status, cudaStream_t stream);
+
+// Attention of prompts or portions of them (attention_tc.cu), and the weights behind it.
+extern "C" int eredu_weighed_prefill(const void* args, int bytes) {
+  WeighedPrefillArgs a;
   if (!weights_args(a, args, bytes)) return -2;
   if (a.batch <= 0 || a.total_q <= 0 || a.max_kv_len <= 0) return 0;
-  if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.n_q % a.n_kv != 0 || a.num_pages <= 0 || a.batch > 65535 || a.n_kv > 65535 || a.window < 0 || a.observed < 0)
+  const int blocks = (std::min(a.max_kv_len, a.wide * kPwPage) + kPwKeys - 1) / kPwKeys;
+  if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.n_q % a.n_kv != 0 || a.num_pages <= 0 || a.batch > 65535 || blocks > 65535 || a.window < 0 || a.observed < 0 ||
+      (a.ranks != 1 && a.ranks != 2 && a.ranks != 4 && a.ranks != kPwCluster))
     return -2;
+  const int e = eredu_attn_prefill_tc_lse(a.q, a.k, a.v, a.out, a.lse, a.block_table, a.seq_lens, a.cu_q, a.sinks, a.batch, a.total_q, a.max_q_len, a.wide, a.num_pages,
+                                          a.n_q, a.n_kv, a.D, a.window, a.max_kv_len, a.sm_count, a.scale, a.status, a.stream);
+  if (e != 0) return e;
   PwParams p = {};
   p.lse = a.lse;
   p.block_table = a.block_table;
@@ -314,7 +326,6 @@ extern "C" int eredu_prompt_weights(const void* args, int bytes) {
   p.cu_q = a.cu_q;
   p.weights = a.weights;
   p.status = a.status;
-  p.pitch = a.pitch;
   p.wide = a.wide;
   p.num_pages = a.num_pages;
   p.n_q = a.n_q;
@@ -330,10 +341,5 @@ extern "C" int eredu_prompt_weights(const void* args, int bytes) {
   if (r != 0) return -100 + r;
   r = make_tma_4d(&tmK, a.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, D, 16, H, static_cast<uint64_t>(a.num_pages), D * 2, 16 * D * 2, H * 16 * D * 2, 64, 16, 1, 1);
   if (r != 0) return -200 + r;
-  const int blocks = (std::min(a.max_kv_len, a.wide * kPwPage) + kPwKeys - 1) / kPwKeys;
-  const int rows = a.observed > 0 ? std::min(a.observed, a.max_q_len) : a.max_q_len;
-  const int tokens = kPwTile >> p.gshift, longest = (rows + tokens - 1) / tokens * (p.group >> p.gshift);
-  int ranks = 1;
-  while (ranks < kPwCluster && static_cast<long long>(blocks) * a.n_kv * a.batch * ranks * 2 <= a.sm_count && longest >= ranks * 4) ranks *= 2;
-  return a.D == 128 ? pw_launch<2>(tmQ, tmK, p, blocks, ranks, a.batch, a.stream) : pw_launch<1>(tmQ, tmK, p, blocks, ranks, a.batch, a.stream);
+  return a.D == 128 ? pw_launch<2>(tmQ, tmK, p, blocks, a.ranks, a.batch, a.stream) : pw_launch<1>(tmQ, tmK, p, blocks, a.ranks, a.batch, a.stream);
 }

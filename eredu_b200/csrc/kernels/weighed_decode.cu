@@ -25,8 +25,9 @@ namespace eredu {
 
 constexpr int kWdPage = 16;
 constexpr int kWdWarps = 4;
-constexpr int kWdStages = 3;
-constexpr int kWdCluster = 8;            // splits of a cluster
+constexpr int kWdPages = 8;              // of the rings of a CTA: 64 KB with heads of 128, three CTAs to an SM
+constexpr int kWdMaxRows = 64;
+constexpr int kWdCluster = 16;           // splits of a cluster (more than eight: where the device has room for it)
 constexpr int kWdMaxSplits = 64;
 constexpr float kWdGrow = 8.f;           // log2 units a score may lie above the bound in use
 
@@ -53,7 +54,7 @@ __device__ __forceinline__ uint32_t wd_transposed(uint32_t v) {
   return d;
 }
 __device__ __forceinline__ void wd_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -89,48 +90,93 @@ __device__ __forceinline__ WdShare wd_share(const WdParams& p, int b, int split)
   return s;
 }
 
-// The weights of the tokens of pages [page0, page1), summed over rows: 2^(score - top) / sum.
-__device__ __forceinline__ void wd_weigh(const WdParams& p, const WdShare& s, int b, int h, const float* top, const float* inv, int threads) {
+// Tokens of pages [page0, page1): thread i has i, i + threads, .. of them, kWdDeep at a time. Where their weights lie, and what they are, does not hang on the
+// attention and is asked for ahead; one token after the other, a thread waited for two reads for each (32768 tokens in one CTA: 400 us of 494).
+constexpr int kWdDeep = 4;
+struct WdCells {
+  float* at[kWdDeep];                      // null: none
+  float held[kWdDeep];
+  float4 score[kWdDeep][2];                // of the first eight rows
+};
+__device__ __forceinline__ void wd_scores(const WdParams& p, const float* scores, int t0, int r, int threads, WdCells& c) {
+#pragma unroll
+  for (int u = 0; u < kWdDeep; ++u)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      c.score[u][i] = c.at[u] != nullptr && r + 4 * i < p.pad ? *reinterpret_cast<const float4*>(scores + static_cast<size_t>(t0 + u * threads) * p.pad + r + 4 * i)
+                                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void wd_cells(const WdParams& p, const WdShare& s, int b, int h, int t0, int threads, WdCells& c) {
+  int page[kWdDeep];
+#pragma unroll
+  for (int u = 0; u < kWdDeep; ++u) {
+    const int t = t0 + u * threads;
+    page[u] = t < s.page1 * kWdPage && t < s.kv_len && t >= s.low ? p.block_table[static_cast<size_t>(b) * p.pitch + t / kWdPage] : -1;
+  }
+#pragma unroll
+  for (int u = 0; u < kWdDeep; ++u) {
+    const int t = t0 + u * threads;
+    c.at[u] = page[u] >= 0 && page[u] < p.num_pages ? p.weights + (static_cast<size_t>(page[u]) * p.n_kv + h) * kWdPage + t % kWdPage : nullptr;
+    c.held[u] = c.at[u] != nullptr && t < s.first_pos ? *c.at[u] : 0.f;
+  }
+  wd_scores(p, p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad, t0, 0, threads, c);
+}
+// Their weights, summed over rows: 2^(score - top) / sum. `c`: the first cells.
+__device__ __forceinline__ void wd_weigh(const WdParams& p, const WdShare& s, int b, int h, const float* top, const float* inv, int threads, WdCells& c) {
   const float* scores = p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad;
-  for (int t = s.page0 * kWdPage + static_cast<int>(threadIdx.x); t < s.page1 * kWdPage; t += threads) {
-    if (t >= s.kv_len || t < s.low) continue;
-    const float* at = scores + static_cast<size_t>(t) * p.pad;
-    float sum = 0.f;
-    for (int r = 0; r < p.rows; r += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(at + r);
-      sum += ex2_approx(v.x - top[r]) * inv[r];
-      if (r + 1 < p.rows) sum += ex2_approx(v.y - top[r + 1]) * inv[r + 1];
+  for (int t0 = s.page0 * kWdPage + static_cast<int>(threadIdx.x); t0 < s.page1 * kWdPage; t0 += kWdDeep * threads) {
+    if (t0 >= s.page0 * kWdPage + threads) wd_cells(p, s, b, h, t0, threads, c);
+    float sum[kWdDeep];
+#pragma unroll
+    for (int u = 0; u < kWdDeep; ++u) sum[u] = 0.f;
+    for (int r = 0; r < p.pad; r += 8) {
+      if (r > 0) wd_scores(p, scores, t0, r, threads, c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (r + 4 * i >= p.pad) break;
+        const float4 m = *reinterpret_cast<const float4*>(top + r + 4 * i), f = *reinterpret_cast<const float4*>(inv + r + 4 * i);   // (rows behind the last have f = 0)
+#pragma unroll
+        for (int u = 0; u < kWdDeep; ++u) {
+          const float4 v = c.score[u][i];
+          sum[u] += ex2_approx(v.x - m.x) * f.x + ex2_approx(v.y - m.y) * f.y + (ex2_approx(v.z - m.z) * f.z + ex2_approx(v.w - m.w) * f.w);
+        }
+      }
     }
-    const int page = p.block_table[static_cast<size_t>(b) * p.pitch + t / kWdPage];
-    if (page < 0 || page >= p.num_pages) continue;
-    float* w = p.weights + (static_cast<size_t>(page) * p.n_kv + h) * kWdPage + t % kWdPage;
-    *w = t >= s.first_pos ? sum : *w + sum;
+#pragma unroll
+    for (int u = 0; u < kWdDeep; ++u)
+      if (c.at[u] != nullptr) *c.at[u] = c.held[u] + sum[u];
   }
 }
 
-// Shared memory: the ring [warps][stages][K, V]; behind the last page the warps' parts [warps][ROWS][D + 4], maxima and sums, then
-// the CTA's part [ROWS][D], maxima and sums.
-template <int D, int NT>
+// Shared memory: the rings [page groups][stages][K, V]; behind the last page the warps' parts [warps][ROWS][D + 4], maxima and sums, then
+// the CTA's part [RG * ROWS][D], maxima and sums.
+template <int D, int NT, int RG>
 constexpr int wd_smem() {
-  constexpr int ring = kWdWarps * kWdStages * 2 * kWdPage * D * 2;
+  constexpr int ring = kWdPages * 2 * kWdPage * D * 2;
   constexpr int rows = 8 * NT;
-  constexpr int merge = (kWdWarps * rows * (D + 4) + 2 * kWdWarps * rows + rows * D + 2 * rows) * 4;
+  constexpr int merge = (kWdWarps * rows * (D + 4) + 2 * kWdWarps * rows + RG * rows * D + 2 * RG * rows) * 4;
   return 1024 + (ring > merge ? ring : merge);
 }
 
-template <int D, int NT>
+// RG: warps that share the pages of a ring, with 8 NT query rows each.
+template <int D, int NT, int RG>
 __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WdParams p) {
-  constexpr int KS = D / 16, HALVES = D / 64, ROWS = 8 * NT, NTH = 32 * kWdWarps;
+  constexpr int KS = D / 16, HALVES = D / 64, ROWS = 8 * NT, ALL = RG * ROWS, NTH = 32 * kWdWarps;
+  constexpr int PG = kWdWarps / RG, STAGES = kWdPages / PG;            // page groups, pages of a ring
   constexpr int BLOCK = kWdPage * D * 2, STAGE = 2 * BLOCK;
   extern __shared__ __align__(1024) uint8_t wd_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wd_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  __shared__ uint64_t full[kWdWarps][kWdStages];
-  __shared__ float s_top[ROWS], s_inv[ROWS], s_part[ROWS][kWdCluster];
+  __shared__ uint64_t full[PG][STAGES], empty[PG][STAGES];
+  __shared__ __align__(16) float s_top[ALL], s_inv[ALL];
+  __shared__ float s_part[ALL][kWdCluster];
   const int warp = static_cast<int>(warp_uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z, pgroup = warp / RG, rgroup = warp % RG, row0 = rgroup * ROWS;
   pdl_launch_early();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kWdWarps * kWdStages; ++i) mbar_init(&full[0][0] + i, 1);
+    for (int i = 0; i < PG * STAGES; ++i) {
+      mbar_init(&full[0][0] + i, 1);
+      mbar_init(&empty[0][0] + i, RG);
+    }
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -141,38 +187,42 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
   const WdShare s = wd_share(p, b, split);
   const int* table = p.block_table + static_cast<size_t>(b) * p.pitch;
   const bool one = elect_one();
-  uint8_t* ring = smem + warp * kWdStages * STAGE;
-  const int first = s.page0 + warp;
-  int ids = 0;                                                        // lane l: the page of this warp's iteration 32 i + l
+  uint8_t* ring = smem + pgroup * STAGES * STAGE;
+  const int first = s.page0 + pgroup;
+  bool ok = true;
+  int ids = 0;                                                        // lane l: the page of this ring's iteration 32 i + l
   auto next_ids = [&](int it) {
-    const int pg = first + (it + lane) * kWdWarps;
+    const int pg = first + (it + lane) * PG;
     ids = pg < s.page1 ? table[pg] : 0;
     if (ids < 0 || ids >= p.num_pages) {
       report_status(p.status, kStatusBadArgument);
       ids = 0;
     }
   };
-  auto fetch = [&](int it) {                                          // called with it = 0, 1, 2, ..
+  // called with it = 0, 1, 2, ..; one warp of those that share a ring fills it, when all of them have read the page
+  auto fetch = [&](int it) {
+    if (RG > 1 && rgroup != 0) return;
     if ((it & 31) == 0) next_ids(it);
     const int page = __shfl_sync(0xffffffffu, ids, it & 31);
-    if (first + it * kWdWarps >= s.page1) return;
-    const int st = it % kWdStages;
-    if (one) {
-      mbar_arrive_expect_tx(&full[warp][st], STAGE);
+    if (first + it * PG >= s.page1) return;
+    const int st = it % STAGES;
+    if (RG > 1 && it >= STAGES && ok) ok = mbar_wait_warp(&empty[pgroup][st], (it / STAGES - 1) & 1, p.status, kStatusSmemEmptyTimeout);
+    if (one && ok) {
+      mbar_arrive_expect_tx(&full[pgroup][st], STAGE);
 #pragma unroll
       for (int i = 0; i < HALVES; ++i) {
-        wd_load_page(ring + st * STAGE + i * 2048, &tmK, i * 64, h, page, &full[warp][st]);
-        wd_load_page(ring + st * STAGE + BLOCK + i * 2048, &tmV, i * 64, h, page, &full[warp][st]);
+        wd_load_page(ring + st * STAGE + i * 2048, &tmK, i * 64, h, page, &full[pgroup][st]);
+        wd_load_page(ring + st * STAGE + BLOCK + i * 2048, &tmV, i * 64, h, page, &full[pgroup][st]);
       }
     }
   };
 #pragma unroll
-  for (int i = 0; i < kWdStages; ++i) fetch(i);
+  for (int i = 0; i < STAGES; ++i) fetch(i);
   // queries as B fragments: lane (g, t) has row g of every eight, dims 16 ks + 2 t and + 8
   uint32_t qf[NT][KS][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 8 + g;
+    const int r = row0 + nt * 8 + g;
     const int token = r / p.group, head = h * p.group + r % p.group;
     const uint32_t* row = reinterpret_cast<const uint32_t*>(p.q + (static_cast<size_t>(b * p.q_per_seq + token) * p.n_q + head) * D);
 #pragma unroll
@@ -192,40 +242,64 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
   float* scores = p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad;
   const uint32_t ring_addr = smem_u32(ring);
   const int a_row = lane & 15, v_row = (lane >> 4) * 8 + (lane & 7);
-  bool ok = true;
   int it = 0;
-  for (int pg = first; pg < s.page1 && ok; pg += kWdWarps, ++it) {
-    const int st = it % kWdStages;
-    ok = mbar_wait_warp(&full[warp][st], (it / kWdStages) & 1, p.status, kStatusTmaFullTimeout);
+  for (int pg = first; pg < s.page1 && ok; pg += PG, ++it) {
+    const int st = it % STAGES;
+    ok = mbar_wait_warp(&full[pgroup][st], (it / STAGES) & 1, p.status, kStatusTmaFullTimeout);
     if (!ok) break;
     const uint32_t k_addr = ring_addr + st * STAGE, v_addr = k_addr + BLOCK;
-    float sc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    // all fragments of the keys are on their way ahead of the first product, which run in two chains; those of the values during the softmax
+    uint32_t a[KS][4];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      uint32_t a[4];
       const int chunk = ks * 2 + (lane >> 4);
-      wd_ldsm(k_addr + (chunk >> 3) * 2048 + a_row * 128 + (((chunk & 7) ^ (a_row & 7)) << 4), a);
+      wd_ldsm(k_addr + (chunk >> 3) * 2048 + a_row * 128 + (((chunk & 7) ^ (a_row & 7)) << 4), a[ks]);
+    }
+    float sc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) wd_mma(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+    for (int nt = 0; nt < NT; ++nt) {
+      float odd[4] = {0.f, 0.f, 0.f, 0.f};
+      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks += 2) {
+        wd_mma(sc[nt], a[ks], qf[nt][ks][0], qf[nt][ks][1]);
+        wd_mma(odd, a[ks + 1], qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[nt][e] = (sc[nt][e] + odd[e]) * p.scale_log2;
     }
     const int key0 = pg * kWdPage;
     const bool edge = key0 + kWdPage - 1 > s.first_pos || (p.window > 0 && key0 < s.kv_len - p.window);
+    // values of tokens that no row sees, in front of the window or behind the last one: a weight of zero does not make a number of what is none
+    if (key0 < s.low || key0 + kWdPage > s.kv_len) {
+      for (int i = lane; i < kWdPage * (D / 8); i += 32) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        if (key0 + r < s.low || key0 + r >= s.kv_len)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_addr + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4)), "r"(0) : "memory");
+      }
+      fence_proxy_async_smem();                                       // the stage is filled again by TMA
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const int chunk = i * 2 + ((lane >> 3) & 1);
+      wd_ldsm_t(v_addr + (chunk >> 3) * 2048 + v_row * 128 + (((chunk & 7) ^ (v_row & 7)) << 4), a[i]);
+    }
+    __syncwarp();
+    if (RG > 1 && lane == 0) mbar_arrive(&empty[pgroup][st]);
+    fetch(it + STAGES);
     uint32_t pf[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sc[nt][e] *= p.scale_log2;
       if (edge) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = key0 + g + (e >> 1) * 8, r = nt * 8 + 2 * tig + (e & 1), pos = s.first_pos + r / p.group;
+          const int key = key0 + g + (e >> 1) * 8, r = row0 + nt * 8 + 2 * tig + (e & 1), pos = s.first_pos + r / p.group;
           if (key > pos || (p.window > 0 && key <= pos - p.window)) sc[nt][e] = -INFINITY;
         }
       }
-      if (nt * 8 + 2 * tig < p.pad) {
-        float* at = scores + static_cast<size_t>(key0 + g) * p.pad + nt * 8 + 2 * tig;
+      if (row0 + nt * 8 + 2 * tig < p.pad) {
+        float* at = scores + static_cast<size_t>(key0 + g) * p.pad + row0 + nt * 8 + 2 * tig;
         *reinterpret_cast<float2*>(at) = make_float2(sc[nt][0], sc[nt][1]);
         *reinterpret_cast<float2*>(at + 8 * p.pad) = make_float2(sc[nt][2], sc[nt][3]);
       }
@@ -260,39 +334,23 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
       pf[nt][0] = wd_transposed(pack_bf16x2(p0, p1));
       pf[nt][1] = wd_transposed(pack_bf16x2(p2, p3));
     }
-    // values of tokens that no row sees, in front of the window or behind the last one: a weight of zero does not make a number of what is none
-    if (key0 < s.low || key0 + kWdPage > s.kv_len) {
-      for (int i = lane; i < kWdPage * (D / 8); i += 32) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        if (key0 + r < s.low || key0 + r >= s.kv_len)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_addr + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4)), "r"(0) : "memory");
-      }
-      fence_proxy_async_smem();                                       // the stage is filled again by TMA
-      __syncwarp();
-    }
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      uint32_t a[4];
-      const int chunk = i * 2 + ((lane >> 3) & 1);
-      wd_ldsm_t(v_addr + (chunk >> 3) * 2048 + v_row * 128 + (((chunk & 7) ^ (v_row & 7)) << 4), a);
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) wd_mma(o[nt][i], a, pf[nt][0], pf[nt][1]);
-    }
-    __syncwarp();
-    fetch(it + kWdStages);
+      for (int nt = 0; nt < NT; ++nt) wd_mma(o[nt][i], a[i], pf[nt][0], pf[nt][1]);
   }
-  // (a wait that ran out: what is on its way must have landed before the ring is used for anything else)
+  // (a wait that ran out: what is on its way must have landed before the rings are used for anything else)
   if (!ok)
-    for (int i = 0; i < kWdStages; ++i)
-      if (first + (it + i) * kWdWarps < s.page1) mbar_wait(&full[warp][(it + i) % kWdStages], ((it + i) / kWdStages) & 1, p.status, kStatusTmaFullTimeout);
+    for (int i = 0; i < STAGES; ++i)
+      if (first + (it + i) * PG < s.page1) mbar_wait(&full[pgroup][(it + i) % STAGES], ((it + i) / STAGES) & 1, p.status, kStatusTmaFullTimeout);
   __syncthreads();
   // ---- the warps' parts
   float* mo = reinterpret_cast<float*>(smem);                         // [warps][ROWS][D + 4]
   float* mm = mo + kWdWarps * ROWS * (D + 4);                         // [warps][ROWS]
   float* ml = mm + kWdWarps * ROWS;
-  float* po = ml + kWdWarps * ROWS;                                   // [ROWS][D]
-  float* pm = po + ROWS * D;
-  float* pl = pm + ROWS;
+  float* po = ml + kWdWarps * ROWS;                                   // [ALL][D]
+  float* pm = po + ALL * D;
+  float* pl = pm + ALL;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -316,14 +374,16 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
   for (int i = threadIdx.x; i < p.rows * D; i += NTH) {
     const int r = i / D, d = i % D;
     float M = -INFINITY;
+    const int w0 = r / ROWS, own = r % ROWS;                          // the first of the warps that have this row (every RG-th), and its place there
 #pragma unroll
-    for (int w = 0; w < kWdWarps; ++w) M = fmaxf(M, mm[w * ROWS + r]);
+    for (int w = 0; w < PG; ++w) M = fmaxf(M, mm[(w0 + w * RG) * ROWS + own]);
     float L = 0.f, acc = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWdWarps; ++w) {
-      const float m = mm[w * ROWS + r], c = m == -INFINITY ? (ml[w * ROWS + r] != 0.f ? 1.f : 0.f) : ex2_approx(m - M);   // (a sum without a maximum is no number, and stays)
-      L += ml[w * ROWS + r] * c;
-      acc += mo[(w * ROWS + r) * (D + 4) + d] * c;
+    for (int w = 0; w < PG; ++w) {
+      const int at = (w0 + w * RG) * ROWS + own;
+      const float m = mm[at], c = m == -INFINITY ? (ml[at] != 0.f ? 1.f : 0.f) : ex2_approx(m - M);   // (a sum without a maximum is no number, and stays)
+      L += ml[at] * c;
+      acc += mo[at * (D + 4) + d] * c;
     }
     po[r * D + d] = acc;
     if (d == 0) {
@@ -343,15 +403,23 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
     return;
   }
   const bool many = p.splits > 1;
+  WdCells cells;
   if (many) {
     __syncwarp();
     cluster_arrive_release();
+    wd_cells(p, s, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), NTH, cells);
+    __syncwarp();
     cluster_wait_acquire();
   } else {
+    wd_cells(p, s, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), NTH, cells);
     __syncthreads();
   }
   const uint32_t a_o = smem_u32(po), a_m = smem_u32(pm), a_l = smem_u32(pl);
-  for (int r = threadIdx.x; r < p.rows; r += NTH) {
+  for (int r = threadIdx.x; r < ALL; r += NTH) {
+    if (r >= p.rows) {
+      s_top[r] = s_inv[r] = 0.f;
+      continue;
+    }
     float ms[kWdCluster], ls[kWdCluster], M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int i = 0; i < kWdCluster; ++i) {
@@ -393,7 +461,7 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
     __syncwarp();
     cluster_arrive_release();                                         // done with the peers' shared memory
   }
-  wd_weigh(p, s, b, h, s_top, s_inv, NTH);
+  wd_weigh(p, s, b, h, s_top, s_inv, NTH, cells);
   if (many) {
     __syncwarp();
     cluster_wait_acquire();                                           // nobody leaves while a peer reads its part
@@ -403,7 +471,8 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
 // grid (splits, n_kv, batch): joins what the splits have left, a share of the output and of the tokens each.
 constexpr int kWdJoinThreads = 256;
 __global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdParams p, const int D) {
-  __shared__ float s_top[16], s_inv[16], s_part[16][kWdMaxSplits];
+  __shared__ __align__(16) float s_top[kWdMaxRows], s_inv[kWdMaxRows];
+  __shared__ float s_part[kWdMaxRows][kWdMaxSplits];
   pdl_launch_early();
   pdl_wait();
   pdl_launch_dependents();
@@ -411,6 +480,7 @@ __global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdPa
   const WdShare s = wd_share(p, b, split);
   const size_t at = (static_cast<size_t>(b) * p.n_kv + h) * p.splits;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < kWdMaxRows && static_cast<int>(threadIdx.x) >= p.rows) s_top[threadIdx.x] = s_inv[threadIdx.x] = 0.f;
   for (int r = warp; r < p.rows; r += kWdJoinThreads / 32) {
     float M = -INFINITY, L = 0.f;
     float2 v[kWdMaxSplits / 32];
@@ -438,30 +508,34 @@ __global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdPa
       s_inv[r] = L == 0.f ? 0.f : 1.f / L;
     }
   }
+  WdCells cells;
+  wd_cells(p, s, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), kWdJoinThreads, cells);
   __syncthreads();
   for (int i = threadIdx.x + split * kWdJoinThreads; i < p.rows * D; i += kWdJoinThreads * p.splits) {
     const int r = i / D, d = i % D;
     float acc = 0.f;
+#pragma unroll 8
     for (int sp = 0; sp < p.splits; ++sp) acc += p.part_o[(at + sp) * p.rows * D + i] * s_part[r][sp];
     p.out[(static_cast<size_t>(b * p.q_per_seq + r / p.group) * p.n_q + h * p.group + r % p.group) * D + d] = __float2bfloat16(acc * s_inv[r]);
   }
-  wd_weigh(p, s, b, h, s_top, s_inv, kWdJoinThreads);
+  wd_weigh(p, s, b, h, s_top, s_inv, kWdJoinThreads, cells);
 }
 
-template <int D, int NT>
+template <int D, int NT, int RG>
 static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdParams& p, int batch, cudaStream_t stream) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT>()) != cudaSuccess) return -1;
+    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT, RG>()) != cudaSuccess) return -1;
+    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -1;
     configured[dev] = true;
   }
   const bool cluster = p.part_o == nullptr && p.splits > 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.splits, p.n_kv, batch);
   cfg.blockDim = dim3(32 * kWdWarps);
-  cfg.dynamicSmemBytes = wd_smem<D, NT>();
+  cfg.dynamicSmemBytes = wd_smem<D, NT, RG>();
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -478,7 +552,7 @@ static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdPar
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, weighed_decode_kernel<D, NT>, tmK, tmV, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, weighed_decode_kernel<D, NT, RG>, tmK, tmV, p);
   eredu_count_launches(1);
   if (e == cudaSuccess && p.part_o != nullptr) {
     e = launch_pdl(weighed_join_kernel, dim3(p.splits, p.n_kv, batch), dim3(kWdJoinThreads), 0, stream, p, D);
@@ -500,9 +574,9 @@ extern "C" int eredu_weighed_decode(const void* args, int bytes) {
     return -2;
   WdParams p = {};
   p.group = a.n_q / a.n_kv;
-  if (static_cast<long long>(a.q_per_seq) * p.group > 16) return -2;
+  if (static_cast<long long>(a.q_per_seq) * p.group > kWdMaxRows) return -2;
   p.rows = a.q_per_seq * p.group;
-  p.pad = p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : p.rows <= 8 ? 8 : 16;
+  p.pad = (p.rows + 3) / 4 * 4;
   p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.block_table = a.block_table;
@@ -529,6 +603,34 @@ extern "C" int eredu_weighed_decode(const void* args, int bytes) {
   if (r != 0) return -100 + r;
   r = make_tma_4d(&tmV, a.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, D, 16, H, static_cast<uint64_t>(a.num_pages), D * 2, 16 * D * 2, H * 16 * D * 2, 64, 16, 1, 1);
   if (r != 0) return -200 + r;
-  if (a.D == 128) return p.rows <= 8 ? wd_launch<128, 1>(tmK, tmV, p, a.batch, a.stream) : wd_launch<128, 2>(tmK, tmV, p, a.batch, a.stream);
-  return p.rows <= 8 ? wd_launch<64, 1>(tmK, tmV, p, a.batch, a.stream) : wd_launch<64, 2>(tmK, tmV, p, a.batch, a.stream);
+#define ER_WD(D_)                                                                                                          \
+  return p.rows <= 8    ? wd_launch<D_, 1, 1>(tmK, tmV, p, a.batch, a.stream)                                                  \
+         : p.rows <= 16 ? wd_launch<D_, 2, 1>(tmK, tmV, p, a.batch, a.stream)                                                  \
+         : p.rows <= 32 ? wd_launch<D_, 2, 2>(tmK, tmV, p, a.batch, a.stream)                                                  \
+                        : wd_launch<D_, 2, 4>(tmK, tmV, p, a.batch, a.stream)
+  if (a.D == 128) ER_WD(128);
+  ER_WD(64);
+#undef ER_WD
+}
+
+// Whether clusters of sixteen find room on the current device (1, or 0).
+extern "C" int eredu_weighed_clusters() {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kWdCluster);
+  cfg.blockDim = dim3(32 * kWdWarps);
+  cfg.dynamicSmemBytes = wd_smem<128, 2, 1>();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kWdCluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(weighed_decode_kernel<128, 2, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<128, 2, 1>()) != cudaSuccess ||
+      cudaFuncSetAttribute(weighed_decode_kernel<128, 2, 1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, weighed_decode_kernel<128, 2, 1>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n > 0 ? 1 : 0;
 }

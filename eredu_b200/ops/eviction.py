@@ -25,32 +25,52 @@ from .native import check, lib, status_word, stream_ptr
 
 PAGE = 16
 HEAD_DIMS = (64, 128)        # head sizes of the kernels
-DECODE_ROWS = 16             # query rows that share a head in the decode kernel; more go to the prefill kernels
-CLUSTER = 8                  # splits of a sequence and head that meet in a cluster
+DECODE_ROWS = 64             # query rows that share a head in the decode kernel; more go to the prefill kernels
+CLUSTER = 16                 # splits of a sequence and head that meet in a cluster
 MAX_SPLITS = 64
-LIST_BYTES = 64 << 20        # scratch that a call of evict_tokens takes for the lists of what stays: layers go in portions of it
+HELD_TOKENS = 48 * 1024      # longest sequence whose weights the eviction kernel holds in shared memory
+LIST_BYTES = 64 << 20        # scratch that a call takes for the lists of what stays where they are longer: layers go in portions of it
 
-_sms: dict = {}
-
-
-def _sm_count(device) -> int:
-    n = _sms.get(device)
-    if n is None:
-        n = _sms[device] = torch.cuda.get_device_properties(device).multi_processor_count
-    return n
+_devices: dict = {}
 
 
-P, I, F = native.P, native.I, native.F
+def _device(device) -> tuple:
+    """(SMs, largest cluster of the decode kernel) of a device, asked once."""
+    known = _devices.get(device)
+    if known is None:
+        with torch.cuda.device(device):
+            known = torch.cuda.get_device_properties(device).multi_processor_count, CLUSTER if lib().eredu_weighed_clusters() else 8
+        _devices[device] = known
+    return known
+
+
+P, I = native.P, native.I
 # the arguments of a call in one block, laid out as csrc/common/weights_args.h has them
-_EVICT, _DECODE, _PROMPT = struct.Struct("9Q12i"), struct.Struct("13Q11if"), struct.Struct("9Q13if")
+_EVICT, _DECODE, _PROMPT = struct.Struct("9Q12i"), struct.Struct("13Q11if"), struct.Struct("12Q13if")
 native.register("eredu_evict_tokens", I, [P, I])
 native.register("eredu_weighed_decode", I, [P, I])
-native.register("eredu_prompt_weights", I, [P, I])
-native.register("eredu_attn_prefill_tc_lse", I, [P] * 9 + [I] * 11 + [F, P, P])
+native.register("eredu_weighed_clusters", I, [])
+native.register("eredu_weighed_prefill", I, [P, I])
 
 
 # ------------------------------------------------------------------------------------------ attention
-def _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, rows, chunk, splits=1):
+def _kernels_take(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, rows, chunk) -> bool:
+    """Whether the call is one for the kernels; CPU tensors and other head sizes take tensor operations, and what neither can take is refused.
+    (One condition for the common case: these checks are a good part of what a short call costs.)"""
+    if type(k_cache) is not Pages8 and type(v_cache) is not Pages8 and not chunk and q.dim() == 3 and k_cache.dim() == 4:
+        shape, (m, n_q, dim), at = k_cache.shape, q.shape, k_cache.get_device()
+        if (at >= 0 and dim in HEAD_DIMS and shape[3] == dim and v_cache.shape == shape and shape[2] == PAGE and weights.shape == shape[:3] and n_q % shape[1] == 0
+                and (rows is None or m == rows) and at == q.get_device() == v_cache.get_device() == weights.get_device() == seq_lens.get_device() == block_table.get_device()
+                and q.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16 and weights.dtype is torch.float32
+                and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32 and seq_lens.dim() == 1 and block_table.dim() == 2
+                and block_table.shape[0] == seq_lens.shape[0] and block_table.stride(1) == 1 and q.is_contiguous() and k_cache.is_contiguous()
+                and v_cache.is_contiguous() and weights.is_contiguous() and seq_lens.is_contiguous()
+                and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0 and sinks is None and out is None):
+            return True
+    return _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, rows, chunk)
+
+
+def _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, rows, chunk) -> bool:
     if isinstance(k_cache, Pages8) or isinstance(v_cache, Pages8):
         raise NotImplementedError("weights are added up over pages of the model's type, not over 8-bit ones")
     if chunk:
@@ -69,22 +89,22 @@ def _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights,
     _need("sinks", sinks, torch.float32, dev)
     if sinks is not None and sinks.numel() != n_q:
         raise ValueError(f"{sinks.numel()} sinks for {n_q} query heads")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0] \
-            or block_table.device != dev:
-        raise ValueError("block_table: int32 rows, one per sequence")
+    _check_table(block_table, seq_lens, dev)
     if q.device != dev or v_cache.device != dev:
         raise ValueError(f"queries on {q.device} and values on {v_cache.device} for keys on {dev}")
     if out is not None and (out.shape != (*q.shape[:2], v_cache.shape[3]) or out.dtype != q.dtype or out.device != dev):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} for queries {tuple(q.shape)} {q.dtype}")
-
-
-def _kernels_take(q, k_cache, v_cache, out) -> bool:
-    """Whether the call is one for the kernels; other head sizes take tensor operations, and what the kernels cannot read is refused."""
     if not q.is_cuda or q.shape[2] not in HEAD_DIMS or v_cache.shape[3] != q.shape[2]:
         return False
     for name, t in (("q", q), ("keys", k_cache), ("values", v_cache), ("out", out)):
-        _need(name, t, torch.bfloat16, k_cache.device, 16)
+        _need(name, t, torch.bfloat16, dev, 16)
     return True
+
+
+def _check_table(block_table, seq_lens, dev) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.stride(1) != 1 \
+            or block_table.shape[0] != seq_lens.shape[0] or block_table.device != dev:
+        raise ValueError("block_table: int32 rows, one per sequence")
 
 
 def weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, scale, window=0, sinks=None, weights=None, observed=0, out=None):
@@ -118,61 +138,88 @@ def weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, sc
     return out
 
 
-def weighed_splits(batch, n_kv, max_kv_len, sm_count=148):
-    """CTAs that share a sequence and head of the decode kernel: as many as there is room for (two to an SM), with two pages for each of the four warps
-    at least. Up to eight meet in a cluster; more leave their parts to a second kernel, which pays where eight have long shares."""
+def weighed_splits(batch, n_kv, max_kv_len, sm_count=148, cluster=CLUSTER):
+    """CTAs that share a sequence and head of the decode kernel, each with eight pages at least. Three CTAs fit an SM, clusters not quite: as many splits as find room on
+    nine tenths of that, up to eight. Where sequences and heads fill most of the room by themselves, three, four or eight splits even out what sequences differ by
+    (us with 1 / 2 / 3 / 4 / 8: 32 x 8 heads of 1088 to 2175 tokens 51 / 54 / 50 / 52 / 64; 64 x 8 of 2048 to 4096 159 / 150 / 151 / 148 / 161; 16 x 8 of 8192 to 16384
+    234 / 178 / 170 / 169 / 159). Few sequences and heads have sixteen (``cluster``: what the device has room for; 16 heads of 32768 with 8 / 16: 64 / 57), and very few
+    with long contexts more, whose parts a second kernel joins (8 heads with 8 / 16 / 24 / 40: 16384 tokens 29 / 23 / 21 / 23, 32768 55 / 40 / 38 / 39, 131072
+    213 / 132 / 107 / 106)."""
     heads, pages = max(1, batch * n_kv), max(1, -(-max_kv_len // PAGE))
-    want = max(1, 2 * sm_count // heads)
-    if want > CLUSTER and pages > 64 * CLUSTER:
-        return min(want, pages // 32, MAX_SPLITS)
-    return max(1, min(want, pages // 8, CLUSTER))
+    most = max(1, pages // 8)
+    if heads * cluster <= 2 * sm_count:
+        if heads * cluster <= sm_count and pages >= 1024:
+            return min(max(cluster + 1, 27 * sm_count // (20 * heads)), MAX_SPLITS)
+        return min(cluster, most)
+    fit = 27 * sm_count // (10 * heads)
+    if fit > 3:
+        return min(8 if fit > 6 else fit, most)
+    return max(1, min(8 if pages >= 768 else 4 if pages >= 192 else 3, pages // 32))
 
 
 def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len):
     """The form of :func:`.core.attention_decode` that keeps ``weights``. ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it (0: what
     a row of the table holds); the call takes memory for the scores of so many tokens of every sequence."""
     B = seq_lens.shape[0]
-    _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, B * q_per_seq, chunk)
-    if not _kernels_take(q, k_cache, v_cache, out):
+    if not _kernels_take(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, B * q_per_seq, chunk):
         return weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, [q_per_seq] * B, scale, window, sinks, weights, 0, out)
-    n_q, dim = q.shape[1:]
+    total, n_q, dim = q.shape
     pages, n_kv = k_cache.shape[:2]
-    dev, wide = k_cache.device, block_table.shape[1]
+    dev, most = q.device, block_table.shape[1] * PAGE
     rows = q_per_seq * (n_q // n_kv)
-    longest = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE
+    longest = max_kv_len if 0 < max_kv_len < most else most
     if rows > DECODE_ROWS:
         cu_q = torch.arange(0, (B + 1) * q_per_seq, q_per_seq, dtype=torch.int32, device=dev)
         return weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, q_per_seq, scale, window, sinks, weights, out, 0, longest, 0)
     if out is None:
         out = torch.empty_like(q)
-    if q.shape[0] == 0 or wide == 0:
-        return out.zero_() if wide == 0 else out
-    splits = weighed_splits(B, n_kv, min(longest, window + q_per_seq + PAGE) if window > 0 else longest, _sm_count(dev))
-    room, pad = -(-longest // PAGE) * PAGE, 2 if rows <= 2 else 4 if rows <= 4 else 8 if rows <= 8 else 16
+    if total == 0 or most == 0:
+        return out.zero_() if most == 0 else out
+    splits = weighed_splits(B, n_kv, min(longest, window + q_per_seq + PAGE) if window > 0 else longest, *_device(dev))
+    room, pad = -(-longest // PAGE) * PAGE, (rows + 3) // 4 * 4
     scored = B * n_kv * room * pad
-    parts = B * n_kv * splits * rows if splits > CLUSTER else 0
-    scratch = torch.empty(scored + parts * (dim + 2), dtype=torch.float32, device=dev)
-    at = scratch.data_ptr()
+    if splits <= CLUSTER:
+        scratch = torch.empty(scored, dtype=torch.float32, device=dev)
+        at, part_o, part_ml = scratch.data_ptr(), 0, 0
+    else:
+        parts = B * n_kv * splits * rows
+        scratch = torch.empty(scored + parts * (dim + 2), dtype=torch.float32, device=dev)
+        at = scratch.data_ptr()
+        part_o, part_ml = at + 4 * scored, at + 4 * (scored + parts * dim)
     code = lib().eredu_weighed_decode(_DECODE.pack(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), address(sinks), weights.data_ptr(),
-        at, at + 4 * scored if parts else 0, at + 4 * (scored + parts * dim) if parts else 0, status_word(dev).data_ptr(), stream_ptr(dev),
-        B, q_per_seq, block_table.stride(0), wide * PAGE, room, pages, n_q, n_kv, dim, splits, int(window), scale), _DECODE.size)
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if sinks is None else sinks.data_ptr(),
+        weights.data_ptr(), at, part_o, part_ml, status_word(dev).data_ptr(), stream_ptr(dev), B, q_per_seq, block_table.stride(0), most, room, pages, n_q, n_kv, dim, splits,
+        window, scale), _DECODE.size)
     check(code, "eredu_weighed_decode")
     return out
 
 
+def prompt_ranks(batch, n_q, n_kv, max_q_len, max_kv_len, observed, sm_count=148):
+    """CTAs that share the rows of a block of 256 keys in the kernel of prompts' weights, one to an SM: 1, 2, 4 or 8. Early blocks are seen by more rows than late ones, and
+    a CTA costs what 14 of its tiles of 128 rows take beside them; the choice is the one with the least of the longest CTA or the mean over SMs, and that cost for every
+    round (us of the whole call with 1 / 2 / 4 / 8, 32 heads over 8: 4096 tokens 366 / 257 / 283 / 325, 2048 161 / 109 / 91 / 112, 512 48 / 37 / 29 / 32, eight of 512
+    82 / 82 / 94 / 127; 8192 tokens over 4 heads, the last 64 rows 490 / 497 / 510 / 550)."""
+    group, blocks = n_q // n_kv, -(-max_kv_len // 256)
+    shared = min(group & -group, 32)                                          # query heads of a tile
+    rows = min(observed, max_q_len) if observed > 0 else max_q_len
+    longest = -(-rows * shared // 128) * (group // shared)
+    ctas = blocks * n_kv * batch
+    mean = ctas * longest * (1 - 0.5 * min(1.0, rows / max_kv_len)) / sm_count
+    return min((1, 2, 4, 8), key=lambda r: (max(longest / r, mean) + 14 * -(-ctas * r // sm_count) + r / 2, r))
+
+
 def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, weights, out, chunk, max_kv_len, observed):
     """The form of :func:`.core.attention_prefill` that keeps ``weights``; ``observed`` > 0: the last so many rows of every sequence count, 0: all of them."""
-    _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, None, chunk)
-    _need("cu_q", cu_q, torch.int32, k_cache.device)
-    B, total, dev = seq_lens.shape[0], q.shape[0], k_cache.device
+    kernels = _kernels_take(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, None, chunk)
+    B, dev = seq_lens.shape[0], k_cache.device
+    _need("cu_q", cu_q, torch.int32, dev)
     if cu_q.shape != (B + 1,):
         raise ValueError(f"{cu_q.numel()} query offsets for {B} sequences")
     if observed < 0:
         raise ValueError(f"the last {observed} rows")
-    if not _kernels_take(q, k_cache, v_cache, out):
+    if not kernels:
         return weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, (cu_q[1:] - cu_q[:-1]).tolist(), scale, window, sinks, weights, observed, out)
-    n_q, dim = q.shape[1:]
+    total, n_q, dim = q.shape
     pages, n_kv = k_cache.shape[:2]
     block_table = block_table.contiguous()
     wide = block_table.shape[1]
@@ -180,17 +227,13 @@ def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len,
         out = torch.empty_like(q)
     if total == 0 or B == 0 or wide == 0:
         return out
-    sms, status, stream = _sm_count(dev), status_word(dev).data_ptr(), stream_ptr(dev)
-    lse = torch.empty((total, n_q), dtype=torch.float32, device=dev)
-    code = lib().eredu_attn_prefill_tc_lse(
+    longest, sms = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE, _device(dev)[0]
+    lse = torch.empty(total * n_q, dtype=torch.float32, device=dev)
+    code = lib().eredu_weighed_prefill(_PROMPT.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(),
-        address(sinks) or None, B, total, max_q_len, wide, pages, n_q, n_kv, dim, int(window), int(max_kv_len), sms, scale, status, stream)
-    check(code, "eredu_attn_prefill_tc_lse")
-    longest = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE
-    code = lib().eredu_prompt_weights(_PROMPT.pack(
-        q.data_ptr(), k_cache.data_ptr(), lse.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(), weights.data_ptr(), status, stream,
-        B, total, max_q_len, longest, wide, wide, pages, n_q, n_kv, dim, int(window), int(observed), sms, scale), _PROMPT.size)
-    check(code, "eredu_prompt_weights")
+        address(sinks), weights.data_ptr(), status_word(dev).data_ptr(), stream_ptr(dev), B, total, max_q_len, longest, wide, pages, n_q, n_kv, dim,
+        window, observed, prompt_ranks(B, n_q, n_kv, max_q_len, longest, observed, sms), sms, scale), _PROMPT.size)
+    check(code, "eredu_weighed_prefill")
     return out
 
 
@@ -232,9 +275,7 @@ def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, 
     _need("values", v, k.dtype, dev)
     _need("weights", weights, torch.float32, dev)
     _need("seq_lens", seq_lens, torch.int32, dev)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0] \
-            or block_table.device != dev:
-        raise ValueError("block_table: int32 rows, one per sequence")
+    _check_table(block_table, seq_lens, dev)
     if keep < 1 or recent < 0 or first < 0 or recent + first > keep:
         raise ValueError(f"of {keep} tokens the first {first} and the last {recent} cannot stay")
     layers, pages, n_kv = k.shape[:3]
@@ -242,18 +283,25 @@ def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, 
     if not k.is_cuda:
         return evict_tokens_ref(k, v, weights, block_table, seq_lens, keep, recent, first)
     k_row, v_row = k.shape[4] * k.element_size(), v.shape[4] * v.element_size()
-    if (k_row | v_row) % 16 or (k.data_ptr() | v.data_ptr()) % 16:
+    if (k_row | v_row) % 16:
         raise NotImplementedError(f"rows of {k_row} and {v_row} bytes: the kernel moves whole pieces of 16 bytes")
+    if (k.data_ptr() | v.data_ptr() | weights.data_ptr()) % 16:
+        raise ValueError("keys, values and weights have to begin at multiples of 16 bytes")
     left = torch.empty_like(seq_lens)
     longest = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE
     if B == 0 or layers == 0 or longest <= keep:
         return torch.clamp(seq_lens, max=keep, out=left)
-    step = max(1, min(layers, LIST_BYTES // (4 * B * n_kv * keep)))
-    lists = torch.empty(step * B * n_kv * keep, dtype=torch.int32, device=dev)
-    for at in range(0, layers, step):
+    step, lists, at = layers, None, 0
+    if longest > HELD_TOKENS:
+        step = max(1, min(layers, LIST_BYTES // (4 * B * n_kv * keep)))
+        lists = torch.empty(step * B * n_kv * keep, dtype=torch.int32, device=dev)
+    page = pages * n_kv * PAGE                                                                           # tokens and heads of a layer
+    ka, va, wa, status, stream = k.data_ptr(), v.data_ptr(), weights.data_ptr(), status_word(dev).data_ptr(), stream_ptr(dev)
+    while at < layers:
         some = min(step, layers - at)
         code = lib().eredu_evict_tokens(_EVICT.pack(
-            k[at].data_ptr(), v[at].data_ptr(), weights[at].data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), left.data_ptr(), lists.data_ptr(),
-            status_word(dev).data_ptr(), stream_ptr(dev), some, B, n_kv, pages, block_table.stride(0), longest, keep, recent, first, k_row, v_row, 0), _EVICT.size)
+            ka + at * page * k_row, va + at * page * v_row, wa + at * page * 4, block_table.data_ptr(), seq_lens.data_ptr(), left.data_ptr(), address(lists),
+            status, stream, some, B, n_kv, pages, block_table.stride(0), longest, keep, recent, first, k_row, v_row, _device(dev)[0]), _EVICT.size)
         check(code, "eredu_evict_tokens")
+        at += some
     return left

@@ -1,5 +1,7 @@
 """Caches that give up tokens: attention that adds up the weight every cached token gets, and eviction by it, against the definition in 64 bits."""
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -131,6 +133,10 @@ STEPS = [
     ((16, 1, 128), [222], 1, 1, False),
     ((8, 1, 128), [140, 35], 5, 0, True),
     ((12, 2, 64), [300, 17, 65], 7, 40, False),
+    ((16, 2, 64), [200, 31, 8], 8, 50, False),
+    ((8, 2, 128), [600], 8, 0, False),
+    ((16, 1, 128), [100, 6], 5, 0, True),
+    ((33, 1, 64), [70], 1, 0, False),
 ]
 
 
@@ -154,8 +160,9 @@ def test_step(device, heads, lens, new, window, sinks):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8, 9, 31, 64])
-@pytest.mark.parametrize("heads, lens, new, window", [((8, 2, 128), [1000, 17, 3], 1, 0), ((8, 1, 64), [777, 300], 2, 400)])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8, 12, 16, 17, 64])
+@pytest.mark.parametrize("heads, lens, new, window", [((8, 2, 128), [1000, 17, 3], 1, 0), ((8, 1, 64), [777, 300], 2, 400),
+                                                      ((8, 2, 64), [700, 90], 5, 0), ((16, 2, 128), [600, 33], 7, 300)])
 def test_step_in_any_number_of_splits(monkeypatch, splits, heads, lens, new, window):
     monkeypatch.setattr(eviction, "weighed_splits", lambda *a: splits)
     test_step("cuda", heads, lens, new, window, True)
@@ -339,6 +346,18 @@ def arguments(device="cpu", dim=64):
     k, v, w = cache(num, 2, dim, device)
     q = torch.zeros((2, 4, dim), dtype=torch.bfloat16, device=device)
     return q, k, v, w, table, torch.tensor([20, 5], dtype=torch.int32, device=device)
+
+
+def test_formats_and_header_agree():
+    """The argument blocks as Python packs them and as the header has them: as many pointers, whole and real numbers, in whole multiples of eight bytes."""
+    header = (Path(ops.__file__).resolve().parent.parent / "csrc/common/weights_args.h").read_text()
+    for name, block in (("EvictArgs", eviction._EVICT), ("WeighedDecodeArgs", eviction._DECODE), ("WeighedPrefillArgs", eviction._PROMPT)):
+        body = re.sub(r"//.*", "", header.partition(f"struct {name} {{")[2].partition("};")[0])
+        kinds = ""
+        for line in body.split(";"):
+            names = line.count(",") + 1
+            kinds += "" if not line.strip() else ("Q" if "*" in line or "cudaStream_t" in line else "f" if "float" in line else "i") * names
+        assert kinds == "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Qif])", block.format)) and block.size % 8 == 0
 
 
 def test_refusals_of_attention():
