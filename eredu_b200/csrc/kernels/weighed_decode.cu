@@ -27,6 +27,7 @@ constexpr int kWdPage = 16;
 constexpr int kWdWarps = 4;
 constexpr int kWdPages = 8;              // of the rings of a CTA: 64 KB with heads of 128, three CTAs to an SM
 constexpr int kWdMaxRows = 64;
+constexpr int kWdHeld = 16 * 1024;       // bytes of scores that a CTA may hold in shared memory
 constexpr int kWdCluster = 16;           // splits of a cluster (more than eight: where the device has room for it)
 constexpr int kWdMaxSplits = 64;
 constexpr float kWdGrow = 8.f;           // log2 units a score may lie above the bound in use
@@ -98,15 +99,21 @@ struct WdCells {
   float held[kWdDeep];
   float4 score[kWdDeep][2];                // of the first eight rows
 };
-__device__ __forceinline__ void wd_scores(const WdParams& p, const float* scores, int t0, int r, int threads, WdCells& c) {
+// Where a CTA finds its scores: memory, or shared memory behind everything else where they are few.
+struct WdScores {
+  float* at;
+  int first;                               // token that lies there
+  __device__ __forceinline__ float* row(int t, int pad) const { return at + static_cast<size_t>(t - first) * pad; }
+};
+__device__ __forceinline__ void wd_scores(const WdParams& p, const WdScores& scores, int t0, int r, int threads, WdCells& c) {
 #pragma unroll
   for (int u = 0; u < kWdDeep; ++u)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      c.score[u][i] = c.at[u] != nullptr && r + 4 * i < p.pad ? *reinterpret_cast<const float4*>(scores + static_cast<size_t>(t0 + u * threads) * p.pad + r + 4 * i)
+      c.score[u][i] = c.at[u] != nullptr && r + 4 * i < p.pad ? *reinterpret_cast<const float4*>(scores.row(t0 + u * threads, p.pad) + r + 4 * i)
                                                               : make_float4(0.f, 0.f, 0.f, 0.f);
 }
-__device__ __forceinline__ void wd_cells(const WdParams& p, const WdShare& s, int b, int h, int t0, int threads, WdCells& c) {
+__device__ __forceinline__ void wd_cells(const WdParams& p, const WdShare& s, const WdScores& scores, int b, int h, int t0, int threads, WdCells& c) {
   int page[kWdDeep];
 #pragma unroll
   for (int u = 0; u < kWdDeep; ++u) {
@@ -119,13 +126,13 @@ __device__ __forceinline__ void wd_cells(const WdParams& p, const WdShare& s, in
     c.at[u] = page[u] >= 0 && page[u] < p.num_pages ? p.weights + (static_cast<size_t>(page[u]) * p.n_kv + h) * kWdPage + t % kWdPage : nullptr;
     c.held[u] = c.at[u] != nullptr && t < s.first_pos ? *c.at[u] : 0.f;
   }
-  wd_scores(p, p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad, t0, 0, threads, c);
+  wd_scores(p, scores, t0, 0, threads, c);
 }
 // Their weights, summed over rows: 2^(score - top) / sum. `c`: the first cells.
-__device__ __forceinline__ void wd_weigh(const WdParams& p, const WdShare& s, int b, int h, const float* top, const float* inv, int threads, WdCells& c) {
-  const float* scores = p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad;
+__device__ __forceinline__ void wd_weigh(const WdParams& p, const WdShare& s, const WdScores& scores, int b, int h, const float* top, const float* inv, int threads,
+                                         WdCells& c) {
   for (int t0 = s.page0 * kWdPage + static_cast<int>(threadIdx.x); t0 < s.page1 * kWdPage; t0 += kWdDeep * threads) {
-    if (t0 >= s.page0 * kWdPage + threads) wd_cells(p, s, b, h, t0, threads, c);
+    if (t0 >= s.page0 * kWdPage + threads) wd_cells(p, s, scores, b, h, t0, threads, c);
     float sum[kWdDeep];
 #pragma unroll
     for (int u = 0; u < kWdDeep; ++u) sum[u] = 0.f;
@@ -239,7 +246,9 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
 #pragma unroll
     for (int i = 0; i < KS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
   }
-  float* scores = p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad;
+  const bool held = p.scores == nullptr;
+  const WdScores scores{held ? reinterpret_cast<float*>(smem + wd_smem<D, NT, RG>() - 1024) : p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad,
+                        held ? s.page0 * kWdPage : 0};
   const uint32_t ring_addr = smem_u32(ring);
   const int a_row = lane & 15, v_row = (lane >> 4) * 8 + (lane & 7);
   int it = 0;
@@ -299,7 +308,7 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
         }
       }
       if (row0 + nt * 8 + 2 * tig < p.pad) {
-        float* at = scores + static_cast<size_t>(key0 + g) * p.pad + row0 + nt * 8 + 2 * tig;
+        float* at = scores.row(key0 + g, p.pad) + row0 + nt * 8 + 2 * tig;
         *reinterpret_cast<float2*>(at) = make_float2(sc[nt][0], sc[nt][1]);
         *reinterpret_cast<float2*>(at + 8 * p.pad) = make_float2(sc[nt][2], sc[nt][3]);
       }
@@ -407,11 +416,11 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
   if (many) {
     __syncwarp();
     cluster_arrive_release();
-    wd_cells(p, s, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), NTH, cells);
+    wd_cells(p, s, scores, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), NTH, cells);
     __syncwarp();
     cluster_wait_acquire();
   } else {
-    wd_cells(p, s, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), NTH, cells);
+    wd_cells(p, s, scores, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), NTH, cells);
     __syncthreads();
   }
   const uint32_t a_o = smem_u32(po), a_m = smem_u32(pm), a_l = smem_u32(pl);
@@ -461,7 +470,7 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
     __syncwarp();
     cluster_arrive_release();                                         // done with the peers' shared memory
   }
-  wd_weigh(p, s, b, h, s_top, s_inv, NTH, cells);
+  wd_weigh(p, s, scores, b, h, s_top, s_inv, NTH, cells);
   if (many) {
     __syncwarp();
     cluster_wait_acquire();                                           // nobody leaves while a peer reads its part
@@ -508,8 +517,9 @@ __global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdPa
       s_inv[r] = L == 0.f ? 0.f : 1.f / L;
     }
   }
+  const WdScores scores{p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad, 0};
   WdCells cells;
-  wd_cells(p, s, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), kWdJoinThreads, cells);
+  wd_cells(p, s, scores, b, h, s.page0 * kWdPage + static_cast<int>(threadIdx.x), kWdJoinThreads, cells);
   __syncthreads();
   for (int i = threadIdx.x + split * kWdJoinThreads; i < p.rows * D; i += kWdJoinThreads * p.splits) {
     const int r = i / D, d = i % D;
@@ -518,16 +528,16 @@ __global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdPa
     for (int sp = 0; sp < p.splits; ++sp) acc += p.part_o[(at + sp) * p.rows * D + i] * s_part[r][sp];
     p.out[(static_cast<size_t>(b * p.q_per_seq + r / p.group) * p.n_q + h * p.group + r % p.group) * D + d] = __float2bfloat16(acc * s_inv[r]);
   }
-  wd_weigh(p, s, b, h, s_top, s_inv, kWdJoinThreads, cells);
+  wd_weigh(p, s, scores, b, h, s_top, s_inv, kWdJoinThreads, cells);
 }
 
 template <int D, int NT, int RG>
-static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdParams& p, int batch, cudaStream_t stream) {
+static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdParams& p, int batch, int held, cudaStream_t stream) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT, RG>()) != cudaSuccess) return -1;
+    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT, RG>() + kWdHeld) != cudaSuccess) return -1;
     if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -1;
     configured[dev] = true;
   }
@@ -535,7 +545,7 @@ static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdPar
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.splits, p.n_kv, batch);
   cfg.blockDim = dim3(32 * kWdWarps);
-  cfg.dynamicSmemBytes = wd_smem<D, NT, RG>();
+  cfg.dynamicSmemBytes = wd_smem<D, NT, RG>() + held;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -597,6 +607,10 @@ extern "C" int eredu_weighed_decode(const void* args, int bytes) {
   p.splits = a.splits;
   p.window = a.window;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  // (the pages of a split, however short the others are)
+  const long long few = static_cast<long long>((a.room / kWdPage + a.splits - 1) / a.splits) * kWdPage * p.pad * 4;
+  if (a.scores == nullptr && (few > kWdHeld || a.part_o != nullptr)) return -2;
+  const int held = a.scores == nullptr ? static_cast<int>(few) : 0;
   const uint64_t D = static_cast<uint64_t>(a.D), H = static_cast<uint64_t>(a.n_kv);
   CUtensorMap tmK, tmV;
   int r = make_tma_4d(&tmK, a.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, D, 16, H, static_cast<uint64_t>(a.num_pages), D * 2, 16 * D * 2, H * 16 * D * 2, 64, 16, 1, 1);
@@ -604,10 +618,10 @@ extern "C" int eredu_weighed_decode(const void* args, int bytes) {
   r = make_tma_4d(&tmV, a.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, D, 16, H, static_cast<uint64_t>(a.num_pages), D * 2, 16 * D * 2, H * 16 * D * 2, 64, 16, 1, 1);
   if (r != 0) return -200 + r;
 #define ER_WD(D_)                                                                                                          \
-  return p.rows <= 8    ? wd_launch<D_, 1, 1>(tmK, tmV, p, a.batch, a.stream)                                                  \
-         : p.rows <= 16 ? wd_launch<D_, 2, 1>(tmK, tmV, p, a.batch, a.stream)                                                  \
-         : p.rows <= 32 ? wd_launch<D_, 2, 2>(tmK, tmV, p, a.batch, a.stream)                                                  \
-                        : wd_launch<D_, 2, 4>(tmK, tmV, p, a.batch, a.stream)
+  return p.rows <= 8    ? wd_launch<D_, 1, 1>(tmK, tmV, p, a.batch, held, a.stream)                                                  \
+         : p.rows <= 16 ? wd_launch<D_, 2, 1>(tmK, tmV, p, a.batch, held, a.stream)                                                  \
+         : p.rows <= 32 ? wd_launch<D_, 2, 2>(tmK, tmV, p, a.batch, held, a.stream)                                                  \
+                        : wd_launch<D_, 2, 4>(tmK, tmV, p, a.batch, held, a.stream)
   if (a.D == 128) ER_WD(128);
   ER_WD(64);
 #undef ER_WD

@@ -28,6 +28,7 @@ HEAD_DIMS = (64, 128)        # head sizes of the kernels
 DECODE_ROWS = 64             # query rows that share a head in the decode kernel; more go to the prefill kernels
 CLUSTER = 16                 # splits of a sequence and head that meet in a cluster
 MAX_SPLITS = 64
+HELD_SCORES = 16 << 10       # bytes of scores that a CTA of the decode kernel may hold in shared memory
 HELD_TOKENS = 48 * 1024      # longest sequence whose weights the eviction kernel holds in shared memory
 LIST_BYTES = 64 << 20        # scratch that a call takes for the lists of what stays where they are longer: layers go in portions of it
 
@@ -175,17 +176,17 @@ def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale,
         out = torch.empty_like(q)
     if total == 0 or most == 0:
         return out.zero_() if most == 0 else out
-    splits = weighed_splits(B, n_kv, min(longest, window + q_per_seq + PAGE) if window > 0 else longest, *_device(dev))
+    sms, cluster = _device(dev)
+    splits = weighed_splits(B, n_kv, min(longest, window + q_per_seq + PAGE) if window > 0 else longest, sms, cluster)
     room, pad = -(-longest // PAGE) * PAGE, (rows + 3) // 4 * 4
-    scored = B * n_kv * room * pad
-    if splits <= CLUSTER:
-        scratch = torch.empty(scored, dtype=torch.float32, device=dev)
-        at, part_o, part_ml = scratch.data_ptr(), 0, 0
-    else:
-        parts = B * n_kv * splits * rows
+    # few scores stay in shared memory, where a third CTA of an SM would have nothing to do in any case: no scratch to allocate (1.7 us of the host's)
+    at = part_o = part_ml = 0
+    if splits > CLUSTER or B * n_kv * splits > 2 * sms or -(-room // (PAGE * splits)) * PAGE * pad * 4 > HELD_SCORES:
+        scored, parts = B * n_kv * room * pad, B * n_kv * splits * rows if splits > CLUSTER else 0
         scratch = torch.empty(scored + parts * (dim + 2), dtype=torch.float32, device=dev)
         at = scratch.data_ptr()
-        part_o, part_ml = at + 4 * scored, at + 4 * (scored + parts * dim)
+        if parts:
+            part_o, part_ml = at + 4 * scored, at + 4 * (scored + parts * dim)
     code = lib().eredu_weighed_decode(_DECODE.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if sinks is None else sinks.data_ptr(),
         weights.data_ptr(), at, part_o, part_ml, status_word(dev).data_ptr(), stream_ptr(dev), B, q_per_seq, block_table.stride(0), most, room, pages, n_q, n_kv, dim, splits,
