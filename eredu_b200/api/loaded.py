@@ -37,6 +37,7 @@ class ModelLoadOptions:
     max_seq_len: int = 4096
     kv_pages: Optional[int] = None
     kv_bits: Optional[int] = None        # 8: keys and values are cached in 8 bits with a scale per page and head
+    kv_keep: object = None               # tokens (or KeptTokens) that a sequence's cache is brought down to, by the weight that attention gives them
     state_slots: Optional[int] = None    # recurrent-state slots of hybrid models (None: twice the decode batch)
     prefix_cache: bool = False           # later requests lease the published KV pages of an equal prompt prefix
     kv_host_tier_bytes: int = 0          # with prefix_cache: evicted published pages are kept in pinned host memory ...
@@ -227,7 +228,7 @@ class LoadedModel:
         engine = Engine(model, max_batch=opt.max_batch, max_seq_len=opt.max_seq_len, num_pages=opt.kv_pages,
                         use_cuda_graph=opt.use_cuda_graph, prefix_cache=opt.prefix_cache,
                         kv_host_tier_bytes=opt.kv_host_tier_bytes, kv_disk_tier_dir=opt.kv_disk_tier_dir,
-                        kv_disk_tier_bytes=opt.kv_disk_tier_bytes, state_slots=opt.state_slots, kv_bits=opt.kv_bits)
+                        kv_disk_tier_bytes=opt.kv_disk_tier_bytes, state_slots=opt.state_slots, kv_bits=opt.kv_bits, kv_keep=opt.kv_keep)
         tokenizer = None
         try:
             from ..text.tokenizer import load_tokenizer
@@ -663,6 +664,8 @@ class LoadedModel:
             raise NotImplementedError(f"{src.cfg.model_type}: tensor / pipeline / expert parallelism is not built for this family")
         if opt.kv_bits == 8:
             raise NotImplementedError(f"{src.cfg.model_type}: this family's attention does not take 8-bit pages")
+        if opt.kv_keep is not None:
+            raise NotImplementedError(f"{src.cfg.model_type}: this family's cache gives up no tokens")
         if opt.weight_residency != "device" or opt.expert_cache or opt.prefix_cache:
             raise NotImplementedError(f"{src.cfg.model_type}: weight residency tiers, expert caches and prefix reuse are not built for this family")
         if src.cfg.model_type == "inkling_mm_model":

@@ -68,6 +68,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--expert-cache-eviction", choices=["lru", "lfu"], default="lru")
     p.add_argument("--expert-cache-benchmark", action="store_true")
     p.add_argument("--kv-bits", type=int, choices=[8, 16], default=16, help="8: keys and values cached in 8 bits with a scale per page and head")
+    p.add_argument("--kv-keep", type=int, default=None, metavar="TOKENS", help="bound of the cache: tokens that attention gives the least weight are given up")
     p.add_argument("--mapped-shards", type=int, default=4)
     p.add_argument("--raw", action="store_true", help="no chat template: the prompt is fed verbatim")
     p.add_argument("--image", action="append", default=[], metavar="PATH", help="image part of the prompt (vision-language models)")
@@ -217,7 +218,7 @@ def benchmark_candidates(model_path: str, a, candidates: list, prompt: str) -> d
                 open(plan_path, "w").write(plan.to_json())
                 cmd = [sys.executable, "-m", "eredu_b200.cli", "--model", model_path, "--device", a.device, "--auto-trial-plan",
                        plan_path, "--telemetry-json", tel_path, "--max-tokens", str(a.auto_benchmark_tokens), "--raw",
-                       "--mapped-shards", str(a.mapped_shards), "--kv-bits", str(a.kv_bits), prompt]
+                       "--mapped-shards", str(a.mapped_shards), "--kv-bits", str(a.kv_bits), *(["--kv-keep", str(a.kv_keep)] if a.kv_keep is not None else []), prompt]
                 trial = {"run": run}
                 try:
                     r = subprocess.run(cmd, stdin=subprocess.DEVNULL, stdout=subprocess.DEVNULL, stderr=subprocess.PIPE,
@@ -376,7 +377,7 @@ def main(argv=None) -> int:
             ec_budget = ec_budget or plan.expert_cache.get("device_budget_bytes")
             ec_eviction = plan.expert_cache.get("eviction", ec_eviction)
     t0 = time.perf_counter()
-    lm = LoadedModel.load(model_path, ModelLoadOptions(device=device, quantization=quant, mapped_shards=a.mapped_shards, kv_bits=a.kv_bits,
+    lm = LoadedModel.load(model_path, ModelLoadOptions(device=device, quantization=quant, mapped_shards=a.mapped_shards, kv_bits=a.kv_bits, kv_keep=a.kv_keep,
                                                        max_batch=1, max_seq_len=max(4096, a.max_tokens + 2048),
                                                        weight_residency=("dense_disk_stream" if dense_disk else
                                                                          "layerwise_host" if layerwise else "device"),

@@ -415,11 +415,11 @@ __global__ void decode_advance_kernel(const int* __restrict__ sampled, int* __re
   }
   const int tok = sampled[b];
   token_ids[b] = tok;
-  const int pos = positions[b] + 1;
-  positions[b] = pos;
-  seq_lens[b] = pos + 1;
-  const int page = block_table[static_cast<size_t>(b) * max_pages + (pos >> 4)];
-  slots[b] = static_cast<long long>(page) * 16 + (pos & 15);
+  positions[b] += 1;
+  const int at = seq_lens[b];                     // the next token's place: its position, less the tokens that the cache has given up
+  seq_lens[b] = at + 1;
+  const int page = block_table[static_cast<size_t>(b) * max_pages + (at >> 4)];
+  slots[b] = static_cast<long long>(page) * 16 + (at & 15);
   if (sampler_rows != nullptr) {
     int* row = sampler_rows + static_cast<size_t>(b) * row_ints;
     if (history != nullptr) {

@@ -66,6 +66,7 @@ class ForwardBatch:
     # prefill: (first new position, new tokens) of every sequence, known on the host (operators that size scratch by context)
     portions: Optional[list] = None
     pool_rows: dict = field(default_factory=dict)   # prefill: where pooled blocks of each size lie as dense rows (ops.pooling)
+    observed: int = 0                  # prefill into a cache that keeps weights: the last so many rows of every sequence count (0: all)
     max_kv_len: int = 0                # decode: the longest context the step (or every replay of its graph) can see
     sm_count: int = 1
 
@@ -292,10 +293,11 @@ class CausalLM:
             width = (self.n_q_local + 2 * self.n_kv_local) * cfg.head_dim
             gate, qkv = qkv[:, width:], qkv[:, :width]
         k_cache, v_cache = kv.layer(li)
+        weights = kv.layer_weights(li)
         rope_pos = batch.positions if batch.rope_positions is None else batch.rope_positions
         window = cfg.layer_window(li)
         if (not batch.is_prefill and rope_pos.dim() == 1 and qkv.is_cuda and cfg.head_dim in ops.KERNEL_HEAD_DIMS
-                and FUSED_DECODE_ROPE):
+                and FUSED_DECODE_ROPE and weights is None):
             # decode / verify steps: q/k norm, RoPE and the KV append happen inside the attention kernel
             attn = ops.attention_decode_rope(qkv, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.q_per_seq,
                                              self.scale, rope_pos, batch.slots, self.inv_freq, self.n_q_local,
@@ -313,11 +315,11 @@ class CausalLM:
             attn = ops.attention_prefill(q, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.cu_q,
                                          batch.max_q_len, self.scale, window=window, sinks=lw.sinks,
                                          max_kv_len=max((a + n for a, n in batch.portions), default=0) if batch.portions else 0,
-                                         portions=batch.portions)
+                                         portions=batch.portions, weights=weights, observed=batch.observed)
         else:
             attn = ops.attention_decode(q, k_cache, v_cache, batch.block_table, batch.seq_lens, batch.q_per_seq,
                                         self.scale, splits=batch.splits, window=window, sinks=lw.sinks,
-                                        scratch=batch.scratch)
+                                        scratch=batch.scratch, weights=weights, max_kv_len=batch.max_kv_len)
         return self._attn_out(lw, attn, gate, h, next_folded)
 
     def _attn_out(self, lw: LayerWeights, attn, gate, h, next_folded):

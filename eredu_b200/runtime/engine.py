@@ -24,7 +24,7 @@ from ..models.llama import CausalLM, ForwardBatch
 from ..ops.sampling import ROW_DTYPE, SamplingParams, pack_rows
 from ..utils import nvtx
 from ..utils.capture import captured
-from .kv_cache import PAGE, PagedKVCache
+from .kv_cache import PAGE, KeptTokens, PagedKVCache
 
 
 @dataclass
@@ -41,6 +41,12 @@ class Sequence:
     finish_reason: Optional[str] = None
     slot: int = -1             # row in the decode batch
     cached_tokens: int = 0     # prompt tokens whose K/V came from published pages of earlier requests
+    evicted: int = 0           # of the kv_len tokens, those that a bounded cache has given up
+
+    @property
+    def cached(self) -> int:
+        """Tokens that the cache holds: the place of the next one, whose position is kv_len."""
+        return self.kv_len - self.evicted
 
     @property
     def total_len(self) -> int:
@@ -51,8 +57,11 @@ class Engine:
     def __init__(self, model: CausalLM, max_batch: int = 32, max_seq_len: int = 4096, num_pages: Optional[int] = None,
                  use_cuda_graph: Optional[bool] = None, prefill_chunk: int = 8192, hist_cap: int = 1024,
                  prefix_cache: bool = False, kv_host_tier_bytes: int = 0, kv_disk_tier_dir=None, kv_disk_tier_bytes: int = 0,
-                 state_slots: Optional[int] = None, kv_bits: Optional[int] = None):
-        """``kv_bits`` = 8: keys and values are cached in 8 bits (:mod:`eredu_b200.ops.kv8`)."""
+                 state_slots: Optional[int] = None, kv_bits: Optional[int] = None, kv_keep=None):
+        """``kv_bits`` = 8: keys and values are cached in 8 bits (:mod:`eredu_b200.ops.kv8`).
+        ``kv_keep`` (a number of tokens, or :class:`KeptTokens`): the cache of a sequence is bounded; every layer and head gives up the tokens that attention has given
+        the least weight, behind the prompt and while decoding."""
+        self.keep = KeptTokens(kv_keep) if isinstance(kv_keep, int) else kv_keep
         self.model = model
         self.cfg = model.cfg
         self.device = model.device
@@ -72,13 +81,15 @@ class Engine:
             layer_pools = {li: self.cfg.layer_kv_pool(li) for li in kv_layers if self.cfg.layer_kv_pool(li)}
         if kv_bits == 8:
             self._check_8bit_pages()
+        if self.keep is not None:
+            self._check_kept_tokens(prefix_cache or kv_bits == 8 or conv_layers)
         self.kv = PagedKVCache(model.num_local_layers(), model.n_kv_local, key_dim, num_pages, model.dtype,
                                self.device, first_layer=model.first_layer, value_dim=value_dim,
                                attention_layers=kv_layers,
                                conv_layers=conv_layers,
                                conv_channels=self.cfg.hidden_size // model.par.tp_size if conv_layers else 0,
                                conv_hist=self.cfg.conv_l_cache - 1, layer_dims=layer_dims, donors=donors,
-                               layer_pools=layer_pools, kv_bits=kv_bits)
+                               layer_pools=layer_pools, kv_bits=kv_bits, weighed=self.keep is not None)
         # recurrent-state slots: by default twice the decode batch, so that prompts can be prefilled while a batch decodes
         slots = max(2 * max_batch, 8) if state_slots is None else state_slots
         shapes = {li: self.cfg.layer_state_shape(li) for li in local if self.cfg.layer_state_shape(li) is not None}
@@ -148,6 +159,36 @@ class Engine:
         if self.device.type == "cuda" and cfg.head_dim not in ops.KV8_HEAD_DIMS:
             raise NotImplementedError(f"8-bit pages are built for head sizes {ops.KV8_HEAD_DIMS}, not {cfg.head_dim}")
 
+    def _check_kept_tokens(self, other) -> None:
+        """The families whose attention layers keep weights, and see all that stands in front of a token."""
+        cfg = self.cfg
+        own = (cfg.mixers is not None or cfg.is_mla or getattr(self.model, "family", None) is not None
+               or any(getattr(self.model, name, None) is not None for name in ("g4", "mg")))
+        layers = range(self.model.first_layer, self.model.last_layer)
+        hybrid = any(cfg.layer_is_mamba(li) or cfg.layer_is_kda(li) or cfg.layer_is_linear_attention(li) for li in layers)
+        if own or hybrid or any(cfg.layer_window(li) for li in layers):
+            raise NotImplementedError(f"{cfg.model_type}: caches that give up tokens are for layers of plain attention over the whole context")
+        if other:
+            raise NotImplementedError("a cache that gives up tokens goes without prefix reuse, 8-bit pages and convolution states")
+
+    def _shrink(self, seqs, new: int = 1) -> list:
+        """Brings those of ``seqs`` down to ``keep.keep`` tokens that ``new`` more would take behind their bound; pages that a sequence cannot need any more go back to
+        the pool. Returns them."""
+        rule = self.keep
+        some = [s for s in seqs if s.cached > rule.keep and s.cached + new > rule.limit] if rule is not None else []
+        if some:
+            held = [s.cached for s in some]
+            table, lens = self._block_table(some), self._t(np.asarray(held, dtype=np.int32), torch.int32)
+            for (k, v), (w,) in zip(self.kv.pools, self.kv.weights):
+                ops.evict_tokens(k, v, w, table, lens, rule.keep, recent=rule.recent, first=rule.first, max_kv_len=max(held))
+            need = PagedKVCache.pages_for(rule.limit)
+            for s in some:
+                s.evicted += s.cached - rule.keep
+                if len(s.pages) > need:
+                    self.kv.allocator.release(s.pages[need:])
+                    s.pages = s.pages[:need]
+        return some
+
     # ------------------------------------------------------------------------------------------ requests
     def new_sequence(self, prompt, sampling=None, max_new_tokens=256, eos_ids=()) -> Sequence:
         seq = Sequence(self._next_id, list(prompt), sampling or SamplingParams(), max_new_tokens, tuple(eos_ids))
@@ -157,7 +198,8 @@ class Engine:
                              f"max_seq_len {self.max_seq_len}")
         # Reserve every page the request can need up front: the block table is then static for the
         # whole decode and the captured graph never needs a host update.
-        need = PagedKVCache.pages_for(len(seq.prompt) + max_new_tokens)
+        total = len(seq.prompt) + max_new_tokens
+        need = PagedKVCache.pages_for(total if self.keep is None else max(len(seq.prompt), min(total, self.keep.limit)))
         if self.prefix_cache:
             # at least one prompt token is always prefilled: its logits choose the first output token
             usable = (len(seq.prompt) - 1) // PAGE * PAGE
@@ -190,6 +232,8 @@ class Engine:
 
     def open_sequence(self, sampling=None, eos_ids=()) -> Sequence:
         """A sequence without a reservation: it gets pages as its tokens arrive (:meth:`forward_tokens`)."""
+        if self.keep is not None:
+            raise NotImplementedError("sequences without a reservation go without a bound for their cache")
         seq = Sequence(self._next_id, [], sampling or SamplingParams(), 0, tuple(eos_ids))
         self._next_id += 1
         return seq
@@ -260,14 +304,14 @@ class Engine:
         """A second sequence at the same point: same prompt, output and cached tokens. Full pages are shared, which nobody writes to any more; the page that is
         being filled is copied (in all layers, one launch). It draws random numbers of its own."""
         other = Sequence(self._next_id, list(seq.prompt), seq.sampling, seq.max_new_tokens, seq.eos_ids, list(seq.output), kv_len=seq.kv_len,
-                         cached_tokens=seq.cached_tokens)
+                         cached_tokens=seq.cached_tokens, evicted=seq.evicted)
         if seq.kv_len and not seq.pages:
             raise RuntimeError("a sequence whose pages are parked is not forked")
         if getattr(seq, "rope_delta", 0):
             other.rope_delta = seq.rope_delta
         self._next_id += 1
         if seq.pages:
-            other.pages = self.kv.fork(seq.pages, seq.kv_len)
+            other.pages = self.kv.fork(seq.pages, seq.cached)
             try:
                 if self.kv.page_to_slot is not None:
                     self.kv.bind_state(other.pages[0])
@@ -423,6 +467,8 @@ class Engine:
             s.kv_len = n
             if self.prefix_cache and n == len(s.prompt):
                 self.publish_pages(s)           # concurrent requests with the same system prompt hit from here on
+        if self.keep is not None:
+            self._shrink([s for s in seqs if s.kv_len == len(s.prompt)])
         tokens = None
         if logits is not None:
             tokens = self._sample(logits, seqs, [len(s.prompt) for s in seqs])
@@ -436,9 +482,11 @@ class Engine:
         B = len(seqs)
         assert B <= self.max_batch
         dev = self.device
+        self._shrink(seqs)
         pos = np.asarray([s.kv_len for s in seqs], dtype=np.int32)
+        at = np.asarray([s.cached for s in seqs], dtype=np.int32)
         pages = [np.asarray(s.pages, dtype=np.int64) for s in seqs]
-        slots = np.asarray([pg[p // PAGE] * PAGE + (p % PAGE) for pg, p in zip(pages, pos)], dtype=np.int64)
+        slots = np.asarray([pg[p // PAGE] * PAGE + (p % PAGE) for pg, p in zip(pages, at)], dtype=np.int64)
         rows = pack_rows([s.sampling for s in seqs], [int(p) + 1 for p in pos],
                          hist_lens=[min(len(s.output), self.hist_cap) for s in seqs],
                          stream_ids=[s.seq_id for s in seqs])
@@ -451,14 +499,16 @@ class Engine:
                 tail = s.output[-self.hist_cap:]
                 h[i, :len(tail)] = tail
             hist = self._t(h, torch.int32)
-        max_len = int(pos.max()) + 1 + max(s.max_new_tokens for s in seqs)
+        max_len = int(at.max()) + 1 + max(s.max_new_tokens for s in seqs)
+        if self.keep is not None:
+            max_len = min(max_len, self.keep.limit)
         splits = self.decode_splits(B, max_len)
         st = {
             "B": B,
             "seqs": list(seqs),
             "token_ids": first_tokens.to(dev, torch.int32).clone(),
             "positions": self._t(pos, torch.int32),
-            "seq_lens": self._t(pos + 1, torch.int32),
+            "seq_lens": self._t(at + 1, torch.int32),
             "slots": self._t(slots, torch.int64),
             "block_table": self._block_table(seqs),
             "active": self._t(np.ones(B, dtype=np.int32), torch.int32),
@@ -487,11 +537,11 @@ class Engine:
         counts = [len(t) for _, t in entries]
         pos = [np.arange(s.kv_len, s.kv_len + n) for s, n in zip(seqs, counts)]
         pages = [np.asarray(s.pages, dtype=np.int64) for s in seqs]
-        lens = np.asarray([s.kv_len + n for s, n in zip(seqs, counts)], dtype=np.int32)
+        lens = np.asarray([s.cached + n for s, n in zip(seqs, counts)], dtype=np.int32)
         arrays = dict(
             token_ids=np.concatenate([np.asarray(t, dtype=np.int32) for _, t in entries]),
             positions=np.concatenate(pos).astype(np.int32),
-            slots=np.concatenate([pg[p // PAGE] * PAGE + p % PAGE for pg, p in zip(pages, pos)]).astype(np.int64, copy=False),
+            slots=np.concatenate([pg[p // PAGE] * PAGE + p % PAGE for pg, p in zip(pages, [q - s.evicted for q, s in zip(pos, seqs)])]).astype(np.int64, copy=False),
             block_table=self._pages_of(seqs), seq_lens=lens, logit_rows=np.asarray(logit_rows, dtype=np.int64))
         if decode_form and max(counts) == 1:
             common = dict(self._upload(**arrays), sm_count=self.sm_count)
@@ -499,8 +549,8 @@ class Engine:
             splits = self.decode_splits(len(seqs), longest)
             return ForwardBatch(**common, is_prefill=False, q_per_seq=1, max_kv_len=longest, splits=splits)
         arrays["cu_q"] = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
-        return ForwardBatch(**self._upload(**arrays), sm_count=self.sm_count, is_prefill=True, max_q_len=max(counts),
-                            portions=[(s.kv_len, n) for s, n in zip(seqs, counts)])
+        return ForwardBatch(**self._upload(**arrays), sm_count=self.sm_count, is_prefill=True, max_q_len=max(counts), observed=self.keep.observed if self.keep else 0,
+                            portions=[(s.cached, n) for s, n in zip(seqs, counts)])
 
     @torch.no_grad()
     def forward_tokens(self, entries) -> torch.Tensor:
@@ -527,7 +577,11 @@ class Engine:
         token, -1 for text: tokens of a group attend to each other in both directions) for prompts with images; it sets
         ``seq.rope_delta`` so that later text tokens continue after the largest position the images used."""
         n = len(tokens)
+        self._shrink([seq], n)
+        if self.keep is not None and seq.cached + n > len(seq.pages) * PAGE:
+            raise ValueError(f"{n} tokens behind {seq.cached} are more than the cache's bound of {self.keep.limit} has room for")
         p = np.arange(seq.kv_len, seq.kv_len + n)
+        at = p - seq.evicted
         pages = np.asarray(seq.pages, dtype=np.int64)
         extra = {}
         delta = getattr(seq, "rope_delta", 0)
@@ -549,9 +603,10 @@ class Engine:
         batch = ForwardBatch(**extra, 
             token_ids=self._t(np.asarray(tokens, dtype=np.int32), torch.int32),
             positions=self._t(p.astype(np.int32), torch.int32),
-            slots=self._t(pages[p // PAGE] * PAGE + (p % PAGE), torch.int64),
-            block_table=self._block_table([seq]), seq_lens=self._t(np.asarray([seq.kv_len + n], dtype=np.int32), torch.int32),
-            is_prefill=True, cu_q=self._t(np.asarray([0, n], dtype=np.int32), torch.int32), max_q_len=n, portions=[(seq.kv_len, n)],
+            slots=self._t(pages[at // PAGE] * PAGE + (at % PAGE), torch.int64),
+            block_table=self._block_table([seq]), seq_lens=self._t(np.asarray([seq.cached + n], dtype=np.int32), torch.int32),
+            is_prefill=True, cu_q=self._t(np.asarray([0, n], dtype=np.int32), torch.int32), max_q_len=n, portions=[(seq.cached, n)],
+            observed=self.keep.observed if self.keep else 0,
             logit_rows=self._t(np.asarray([n - 1], dtype=np.int64), torch.int64))
         logits = self.model.forward(batch, self.kv)
         seq.kv_len += n
@@ -573,6 +628,8 @@ class Engine:
         dev = self.device
         rows = pack_rows([SamplingParams(temperature=0.0)] * B, [1] * B, hist_lens=[0] * B, stream_ids=[0] * B)
         max_len = max_context or self.max_seq_len
+        if self.keep is not None:
+            max_len = min(max_len, self.keep.limit)
         splits = self.decode_splits(B, max_len)
         st = {
             "B": B, "seqs": [None] * B, "slotted": True,
@@ -604,15 +661,16 @@ class Engine:
         if not free:
             raise RuntimeError("no free decode slot")
         i = free[0]
-        pos = seq.kv_len
+        self._shrink([seq])
+        pos, at = seq.kv_len, seq.cached
         pages = np.asarray(seq.pages, dtype=np.int64)
         bt = np.zeros(self.max_pages, dtype=np.int32)
         bt[:len(seq.pages)] = seq.pages
         row = pack_rows([seq.sampling], [pos + 1], hist_lens=[min(len(seq.output), self.hist_cap)], stream_ids=[seq.seq_id])
         st["token_ids"][i] = int(first_token)
         st["positions"][i] = pos
-        st["seq_lens"][i] = pos + 1
-        st["slots"][i] = int(pages[pos // PAGE] * PAGE + pos % PAGE)
+        st["seq_lens"][i] = at + 1
+        st["slots"][i] = int(pages[at // PAGE] * PAGE + at % PAGE)
         st["block_table"][i].copy_(self._t(bt, torch.int32))
         st["rows"][i].copy_(self._t(row.view(np.uint8).reshape(ROW_DTYPE.itemsize), torch.uint8))
         st["active"][i] = 1
@@ -654,8 +712,8 @@ class Engine:
         else:
             st["active"] = torch.as_tensor(act)
         # a row that is held back has no cache slot in this step (recurrent layers then keep its state) and gets the slot of
-        # its position back when it steps again
-        pos = st["positions"].long()
+        # its place back when it steps again
+        pos = st["seq_lens"].long() - 1
         page = st["block_table"].long().gather(1, (pos // PAGE).clamp_max(self.max_pages - 1)[:, None]).squeeze(1)
         slots = torch.where(st["active"] > 0, page * PAGE + pos % PAGE, torch.full_like(page, -1))
         if self.cuda:
@@ -714,6 +772,8 @@ class Engine:
         the host->device copy of its inputs. With ``sync`` the sampled ids are copied back and returned.
         """
         st = self._decode_state
+        if self.keep is not None:
+            self._shrink_decoding(st)
         if not self.cuda:
             with nvtx.annotate("decode_step"):
                 return self._decode_step_cpu(st)
@@ -732,7 +792,8 @@ class Engine:
                 # warm-up run outside capture (lazy kernel attribute setup), then restore the state it advanced
                 saved = {k: st[k].clone() for k in ("token_ids", "positions", "seq_lens", "slots", "rows")}
                 saved_h = st["history"].clone() if st["history"] is not None else None
-                saved_rec = [(t, t.clone()) for t in self.kv.recurrent_tensors()]   # hybrid layers: not idempotent
+                # hybrid layers, and weights of tokens: not idempotent
+                saved_rec = [(t, t.clone()) for t in (*self.kv.recurrent_tensors(), *(w for w, in self.kv.weights))]
                 s = torch.cuda.Stream(device=self.device)
                 s.wait_stream(torch.cuda.current_stream(self.device))
                 with torch.cuda.stream(s):
@@ -762,6 +823,17 @@ class Engine:
         torch.cuda.current_stream(self.device).synchronize()
         return st["host_tokens"]
 
+    def _shrink_decoding(self, st) -> None:
+        """Sequences of the decode state that have reached their bound, and what the state says of them. Goes by what :meth:`commit` has recorded."""
+        some = {id(s) for s in self._shrink([s for s in st["seqs"] if s is not None and not s.finished])}
+        rows = [i for i, s in enumerate(st["seqs"]) if id(s) in some]
+        if rows:
+            at = self._t(np.asarray(rows, dtype=np.int64), torch.int64)
+            keep = self.keep.keep
+            slots = self._t(np.asarray([st["seqs"][i].pages[keep // PAGE] * PAGE + keep % PAGE for i in rows], dtype=np.int64), torch.int64)
+            st["seq_lens"][at] = keep + 1
+            st["slots"][at] = torch.where(st["active"][at] > 0, slots, torch.full_like(slots, -1))
+
     def _decode_step_cpu(self, st):
         idle = Sequence(0, [0], SamplingParams(temperature=0.0))
         seqs = [s if s is not None else idle for s in st["seqs"]]
@@ -778,11 +850,12 @@ class Engine:
         st["sampled"] = toks
         newpos = st["positions"] + 1
         bt = st["block_table"].long()
-        page = bt.gather(1, (newpos.long() // PAGE)[:, None]).squeeze(1)
+        at = st["seq_lens"].long()                          # the next token's place
+        page = bt.gather(1, (at // PAGE)[:, None]).squeeze(1)
         st["token_ids"] = torch.where(active, toks, st["token_ids"])
         st["positions"] = torch.where(active, newpos, st["positions"])
-        st["seq_lens"] = torch.where(active, newpos + 1, st["seq_lens"])
-        st["slots"] = torch.where(active, page * PAGE + (newpos.long() % PAGE), torch.full_like(page, -1))
+        st["seq_lens"] = torch.where(active, st["seq_lens"] + 1, st["seq_lens"])
+        st["slots"] = torch.where(active, page * PAGE + (at % PAGE), torch.full_like(page, -1))
         return toks
 
     def commit(self, tokens) -> list[bool]:

@@ -8,6 +8,7 @@ Page 0 is never handed out: padded block-table entries point at it.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -15,6 +16,30 @@ import torch
 from ..ops.kv8 import FLOOR, Pages8, copy_pages
 
 PAGE = 16
+
+
+@dataclass(frozen=True)
+class KeptTokens:
+    """A bound for the cached tokens of a sequence (:mod:`eredu_b200.ops.eviction`): one that has grown to ``keep`` + ``slack`` tokens is brought down to ``keep`` -
+    the ``first`` ones, the ``recent`` last ones (half of all by default), and those that attention has given the most weight. ``observed`` > 0: of a prompt's portion
+    the last so many rows count, else all of them. ``slack``: a sixteenth of ``keep`` by default, a page at least."""
+    keep: int
+    recent: Optional[int] = None
+    first: int = 4
+    slack: Optional[int] = None
+    observed: int = 0
+
+    def __post_init__(self):
+        if self.recent is None:
+            object.__setattr__(self, "recent", self.keep // 2)
+        if self.slack is None:
+            object.__setattr__(self, "slack", max(PAGE, self.keep // 16))
+        if self.keep < 1 or self.recent < 0 or self.first < 0 or self.recent + self.first > self.keep or self.slack < 1 or self.observed < 0:
+            raise ValueError(f"a cache cannot be bounded like this: {self}")
+
+    @property
+    def limit(self) -> int:
+        return self.keep + self.slack
 
 
 class PageAllocator:
@@ -60,8 +85,9 @@ class PagedKVCache:
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, num_pages: int, dtype, device,
                  first_layer: int = 0, attention_layers=None, conv_layers=None, conv_channels: int = 0, conv_hist: int = 0,
                  value_dim: Optional[int] = None, layer_dims: Optional[dict] = None, donors: Optional[dict] = None,
-                 layer_pools: Optional[dict] = None, kv_bits: Optional[int] = None):
-        """``kv_bits`` = 8: keys and values are held as int8 codes with a scale per page and head (:mod:`eredu_b200.ops.kv8`), about half the memory of bf16;
+                 layer_pools: Optional[dict] = None, kv_bits: Optional[int] = None, weighed: bool = False):
+        """``weighed``: beside the pages of every layer the weight that attention has given their tokens is kept (:meth:`layer_weights`).
+        ``kv_bits`` = 8: keys and values are held as int8 codes with a scale per page and head (:mod:`eredu_b200.ops.kv8`), about half the memory of bf16;
         :meth:`layer` then gives a pair of ``Pages8``. ``layer_dims``: layer -> (kv heads, key width, value width) for families whose layers differ; layers of one
         geometry share a pool tensor, so a page id is valid in every layer. ``donors``: layer -> the earlier layer whose
         keys and values it reads (it keeps none of its own). ``layer_pools``: layer -> tokens of a block whose mean key and
@@ -99,6 +125,10 @@ class PagedKVCache:
                                                                  device=device)
             self.pools.append((k, v))
             self._kv_index.update({li: (g, i) for i, li in enumerate(members)})
+        # per pool fp32 [layers, pages, heads, 16], or nothing
+        self.weights: list = [(torch.zeros(k.shape[:4], dtype=torch.float32, device=device),) for k, _ in self.pools] if weighed else []
+        if weighed and (self.kv_bits or layer_pools or donors):
+            raise NotImplementedError("weights of tokens go with pages of the model's type, without means of blocks or shared layers")
         for li, donor in (donors or {}).items():
             self._kv_index[li] = self._kv_index[donor]
         self.pooled: dict = {}               # layer -> mean keys and values [pages, heads, blocks ending in a page, width]
@@ -241,11 +271,18 @@ class PagedKVCache:
             return Pages8(k[i], ks[i]), Pages8(v[i], vs[i])
         return k[i], v[i]
 
+    def layer_weights(self, li: int):
+        """What attention adds its weights to in a layer (None: the cache does not keep them)."""
+        if not self.weights:
+            return None
+        g, i = self._kv_index[li]
+        return self.weights[g][0][i]
+
     # ---- whole pages
     def page_tensors(self) -> list:
         """Everything that belongs to a page, as tensors [layers, pages, ...]."""
         pooled = [t[None] for pair in self.pooled.values() for t in pair]
-        return [t for pair in (*self.pools, *self.scales) for t in pair if t.shape[0]] + pooled
+        return [t for pair in (*self.pools, *self.scales, *self.weights) for t in pair if t.shape[0]] + pooled
 
     def copy_pages(self, src, dst) -> None:
         """Page ``src[i]`` to page ``dst[i]`` in every layer (:func:`eredu_b200.ops.copy_pages`, with its checks); page 0 is nobody's."""
@@ -255,10 +292,11 @@ class PagedKVCache:
 
     def fork(self, pages, kv_len: int) -> list:
         """Pages of a second sequence with the same ``kv_len`` cached tokens and as many pages: full ones are shared (leased once more), the others are new,
-        with a copy of what they hold. Sequences with a recurrent state, which is found by their first page, share none."""
+        with a copy of what they hold. Sequences with a recurrent state, which is found by their first page, share none, nor do those whose tokens are
+        given up one by one, which changes full pages too."""
         al = self.allocator
         held = self.pages_for(kv_len)
-        shared = kv_len // PAGE if hasattr(al, "retain") and not self.has_recurrent_state() else 0
+        shared = kv_len // PAGE if hasattr(al, "retain") and not self.has_recurrent_state() and not self.weights else 0
         fresh = self.alloc(len(pages) - shared)
         if shared:
             al.retain(list(pages[:shared]))
@@ -282,6 +320,7 @@ class PagedKVCache:
         """Every tensor with an entry per page: (what holds it, its place there, the dimension of the pages, what a new page holds)."""
         places = [(self.pools, g, j, 1, 0) for g in range(len(self.pools)) for j in range(2)]
         places += [(self.scales, g, j, 1, FLOOR) for g in range(len(self.scales)) for j in range(2)]
+        places += [(self.weights, g, 0, 1, 0) for g in range(len(self.weights))]
         places += [(self.pooled, li, j, 0, 0) for li in self.pooled for j in range(2)]
         places += [(vars(self), name, None, dim, 0) for name, dim in (("conv_state", 1), ("page_to_slot", 0)) if getattr(self, name) is not None]
         return places
@@ -324,6 +363,8 @@ class PagedKVCache:
         """Raised by the features that move pages of one geometry (lower tiers, parking, prompt caches)."""
         if self.kv_bits:
             raise NotImplementedError(f"{what} does not take 8-bit pages")
+        if self.weights:
+            raise NotImplementedError(f"{what} does not take caches that give up tokens")
         if len(self.pools) > 1:
             raise NotImplementedError(f"{what} needs one key / value geometry for all layers; this model has {len(self.pools)}")
         if self.pooled:
@@ -338,7 +379,7 @@ class PagedKVCache:
             extra += self.la_rec_state.numel() * 4 + self.la_conv_state.numel() * self.la_conv_state.element_size()
         extra += sum(t.numel() * 4 for t in self.layer_state.values())
         pools = (*self.pools, *self.pooled.values())
-        extra += sum(4 * (k.numel() + v.numel()) for k, v in self.scales)
+        extra += sum(4 * (k.numel() + v.numel()) for k, v in self.scales) + sum(4 * w.numel() for w, in self.weights)
         return sum((k.numel() + v.numel()) * k.element_size() for k, v in pools) + extra
 
     @staticmethod

@@ -269,7 +269,7 @@ def save_prompt_cache(engine, seq, directory, checkpoint_fingerprint: str, prefi
     from ..formats.checkpoint import _np
     from ..lib import _eredu_host as H
 
-    if engine.kv.kv_bits:
+    if engine.kv.kv_bits or engine.kv.weights:
         engine.kv.require_uniform("a prompt cache")
     ident = model_identity(engine, checkpoint_fingerprint)
     topo: PromptCacheTopology = ident["topology"]
@@ -379,7 +379,7 @@ def load_prompt_cache(engine, directory, tokens, checkpoint_fingerprint: str, sa
     of ``tokens`` (checked by hash); at least the last token is left to prefill so that logits exist."""
     from ..lib import _eredu_host as H
 
-    if engine.kv.kv_bits:
+    if engine.kv.kv_bits or engine.kv.weights:
         engine.kv.require_uniform("a prompt cache")
     ident = model_identity(engine, checkpoint_fingerprint)
     man = open_prompt_cache(directory, ident["topology"])

@@ -53,6 +53,8 @@ class SpeculativeDecoder:
 
     def __init__(self, target: Engine, draft: Engine, k: int = 4):
         assert target.cfg.vocab_size == draft.cfg.vocab_size, "draft and target must share the vocabulary"
+        if any(getattr(eng, "keep", None) is not None for eng in (target, draft)):
+            raise NotImplementedError("drafted tokens are taken back by length: not behind a cache that gives up tokens")
         self.t, self.d, self.k = target, draft, k
         # Hybrid models: rejected proposals also have to leave the recurrent states. The draft keeps a snapshot after every
         # draft step and goes back to the one that matches the accepted prefix; the target keeps one snapshot per round
