@@ -9,8 +9,14 @@
 // [16][64] with the 128-byte swizzle that ldmatrix reads without conflicts). Scores come as S^T = K Q^T (mma.sync m16n8k16: the sixteen keys of a page by eight rows, so
 // that the four to eight rows of a group fill the narrow side), and so does O^T = V^T P^T: a lane has two rows in both, whose maxima rescale its own accumulators. The
 // row maximum is a bound that is moved when a score is above it by more than 2^8: most pages need no exchange between lanes.
-// The splits of a sequence and head (up to eight) are a cluster: maxima, sums and outputs meet in shared memory, and every CTA weighs its own tokens. More splits leave
-// their part in memory, and a second kernel does the same.
+// The splits of a sequence and head (up to sixteen) are a cluster: maxima, sums and outputs meet in shared memory, and every CTA weighs its own tokens. More splits leave
+// their part in memory, and a second kernel does the same. Up to sixteen rows that share a head are a warp's; with more, two or four warps walk the same pages with
+// sixteen rows each.
+//
+// Measured (floor: K, V and weights at 6.54 TB/s): 64 sequences of 2048 to 4096 tokens, 32 heads of 128 over 8, 144 us (floor 124, 5.6 TB/s); 32 of 1088 to 2175 48 us
+// (33: what is left is the start and the end of the CTAs, about 8 us, and the raggedness of the last ones); one of 32768, 64 heads over 8, 38 us (21: 24 splits to a head and the second
+// kernel); one of 512, 32 heads of 64 over 8, 8.4 us between launches of a graph, a chain of latencies. A page costs a warp some 300 instructions at five cycles each while
+// it is alone on its scheduler, so that twelve warps to an SM (two stages to a ring) move more than eight with three stages: 64 x 4096 156 -> 148 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -167,7 +173,7 @@ constexpr int wd_smem() {
 
 // RG: warps that share the pages of a ring, with 8 NT query rows each.
 template <int D, int NT, int RG>
-__global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WdParams p) {
+__global__ void __launch_bounds__(32 * kWdWarps, 3) weighed_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WdParams p) {
   constexpr int KS = D / 16, HALVES = D / 64, ROWS = 8 * NT, ALL = RG * ROWS, NTH = 32 * kWdWarps;
   constexpr int PG = kWdWarps / RG, STAGES = kWdPages / PG;            // page groups, pages of a ring
   constexpr int BLOCK = kWdPage * D * 2, STAGE = 2 * BLOCK;
@@ -308,9 +314,12 @@ __global__ void __launch_bounds__(32 * kWdWarps) weighed_decode_kernel(const __g
         }
       }
       if (row0 + nt * 8 + 2 * tig < p.pad) {
-        float* at = scores.row(key0 + g, p.pad) + row0 + nt * 8 + 2 * tig;
-        *reinterpret_cast<float2*>(at) = make_float2(sc[nt][0], sc[nt][1]);
-        *reinterpret_cast<float2*>(at + 8 * p.pad) = make_float2(sc[nt][2], sc[nt][3]);
+        // (rows behind the last are nothing, whatever zeros make of a key that is no number)
+        const int r = row0 + nt * 8 + 2 * tig;
+        const bool r0 = r < p.rows, r1 = r + 1 < p.rows;
+        float* at = scores.row(key0 + g, p.pad) + r;
+        *reinterpret_cast<float2*>(at) = make_float2(r0 ? sc[nt][0] : -INFINITY, r1 ? sc[nt][1] : -INFINITY);
+        *reinterpret_cast<float2*>(at + 8 * p.pad) = make_float2(r0 ? sc[nt][2] : -INFINITY, r1 ? sc[nt][3] : -INFINITY);
       }
       float mx0 = fmaxf(sc[nt][0], sc[nt][2]), mx1 = fmaxf(sc[nt][1], sc[nt][3]);
       const bool grow = (mx0 > top[nt][0] + kWdGrow) || (mx1 > top[nt][1] + kWdGrow);

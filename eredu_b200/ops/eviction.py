@@ -10,8 +10,9 @@ What a page holds behind its sequence's last token means nothing.
 different tokens at the same place, in their order. A key keeps the rotation of the position that it had; new tokens come behind what is left, with positions that
 go on counting. Masks go by places in the cache: a row sees all that stands in front of it, and a window counts tokens that are left.
 
-The kernels take bf16 pages with heads of 64 or 128 (:func:`evict_tokens`: keys and values of any type whose rows are multiples of 16 bytes). Values of tokens that
-a row does not see have to be finite where they belong to the same call.
+The kernels take bf16 pages with heads of 64 or 128 (:func:`evict_tokens`: keys and values of any type whose rows are multiples of 16 bytes). What lies behind a sequence's
+last token may be anything; a value that is no number may reach rows that do not see its token where these see its neighbours (later tokens of the same call, the edge of
+a window). A page is one sequence's: sequences that share pages would add to the same sums at once.
 """
 from __future__ import annotations
 
@@ -52,6 +53,11 @@ native.register("eredu_evict_tokens", I, [P, I])
 native.register("eredu_weighed_decode", I, [P, I])
 native.register("eredu_weighed_clusters", I, [])
 native.register("eredu_weighed_prefill", I, [P, I])
+
+
+def _elsewhere(t) -> bool:
+    """Whether a tensor lies on another GPU than the current one, whose stream a launch would take."""
+    return t.is_cuda and t.device.index != torch.cuda.current_device()
 
 
 # ------------------------------------------------------------------------------------------ attention
@@ -161,6 +167,9 @@ def weighed_splits(batch, n_kv, max_kv_len, sm_count=148, cluster=CLUSTER):
 def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len):
     """The form of :func:`.core.attention_decode` that keeps ``weights``. ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it (0: what
     a row of the table holds); the call takes memory for the scores of so many tokens of every sequence."""
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len)
     B = seq_lens.shape[0]
     if not _kernels_take(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, B * q_per_seq, chunk):
         return weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, [q_per_seq] * B, scale, window, sinks, weights, 0, out)
@@ -211,6 +220,9 @@ def prompt_ranks(batch, n_q, n_kv, max_q_len, max_kv_len, observed, sm_count=148
 
 def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, weights, out, chunk, max_kv_len, observed):
     """The form of :func:`.core.attention_prefill` that keeps ``weights``; ``observed`` > 0: the last so many rows of every sequence count, 0: all of them."""
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len, scale, window, sinks, weights, out, chunk, max_kv_len, observed)
     kernels = _kernels_take(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, None, chunk)
     B, dev = seq_lens.shape[0], k_cache.device
     _need("cu_q", cu_q, torch.int32, dev)
@@ -288,6 +300,9 @@ def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, 
         raise NotImplementedError(f"rows of {k_row} and {v_row} bytes: the kernel moves whole pieces of 16 bytes")
     if (k.data_ptr() | v.data_ptr() | weights.data_ptr()) % 16:
         raise ValueError("keys, values and weights have to begin at multiples of 16 bytes")
+    if _elsewhere(k):
+        with torch.cuda.device(dev):
+            return evict_tokens(k, v, weights, block_table, seq_lens, keep, recent, first, max_kv_len)
     left = torch.empty_like(seq_lens)
     longest = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE
     if B == 0 or layers == 0 or longest <= keep:

@@ -773,7 +773,10 @@ class Engine:
         """
         st = self._decode_state
         if self.keep is not None:
+            if st.get("uncommitted"):
+                raise RuntimeError("a bounded cache goes by what commit() has recorded: every step is committed ahead of the next one")
             self._shrink_decoding(st)
+            st["uncommitted"] = True
         if not self.cuda:
             with nvtx.annotate("decode_step"):
                 return self._decode_step_cpu(st)
@@ -861,6 +864,7 @@ class Engine:
     def commit(self, tokens) -> list[bool]:
         """Record one sampled token per running sequence (host side); returns per-sequence 'just finished'."""
         st = self._decode_state
+        st["uncommitted"] = False
         done = []
         changed = False
         stepped = st.get("stepped")

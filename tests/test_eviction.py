@@ -425,6 +425,86 @@ def test_lengths_and_pages_that_the_table_does_not_have_are_reported():
         del cu
 
 
+def test_calls_for_another_device_are_made_there(monkeypatch):
+    """A launch takes the stream of the current device: tensors of another one make it the current one first."""
+    current, made = [0], []
+
+    class On:
+        is_cuda, device = True, torch.device("cuda", 1)
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[-1])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(eviction, "_kernels_take", lambda *a: made.append(current[-1]) or 1 / 0)
+    for call in (lambda: eviction.weighed_decode(On, On, On, None, torch.zeros(1), 1, 1.0, 0, None, None, None, 0, 0),
+                 lambda: eviction.weighed_prefill(On, On, On, None, torch.zeros(1), None, 1, 1.0, 0, None, None, None, 0, 0, 0)):
+        with pytest.raises(ZeroDivisionError):
+            call()
+    assert made == [1, 1] and current == [0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_keys_that_are_infinite(device):
+    """A key that is minus infinity in the direction of every query gets no weight, and no other token notices (three rows: one of a kernel's four is empty)."""
+    k, v, w = cache(4, 1, 64, device, 30)
+    k[:] = k.abs()
+    k[2, 0, 5] = float("-inf")
+    q = torch.rand((1, 3, 64), generator=torch.Generator().manual_seed(31)).bfloat16().to(device) + 0.1
+    table, lens, before = torch.tensor([[2, 3]], dtype=torch.int32, device=device), torch.tensor([20], dtype=torch.int32, device=device), w.clone()
+    out = ops.attention_decode(q, k, v, table, lens, 1, 0.125, weights=w)
+    at = ops.attention_prefill(q, k, v, table, lens, torch.tensor([0, 1], dtype=torch.int32, device=device), 1, 0.125, weights=before.clone())
+    assert torch.isfinite(out).all() and torch.isfinite(at).all() and torch.isfinite(w[2:]).all() and w[2, 0, 5] == before[2, 0, 5]
+    given = torch.cat((w[2, 0] - before[2, 0], w[3, 0, :3] - before[3, 0, :3], w[3, 0, 3:4]))
+    assert abs(float(given.double().sum()) - 3) <= 3 * 2.0 ** -12
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    """Calls on two streams have nothing in common but their inputs."""
+    cases = []
+    for seed in (40, 41):
+        num, table = layout([1500, 700], "cuda", seed)
+        k, v, w = cache(num, 2, 128, "cuda", seed)
+        q = torch.randn((2, 8, 128), generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+        cases.append((q, k, v, table, torch.tensor([1500, 700], dtype=torch.int32, device="cuda"), w))
+    alone = []
+    for q, k, v, table, lens, w in cases:
+        own = w.clone()
+        alone.append((ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=own), own))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        got = []
+        for stream, (q, k, v, table, lens, w) in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                own = w.clone()
+                got.append((ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=own), own))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for pair, other in zip(got, alone) for a, b in zip(pair, other))
+
+
+@pytest.mark.gpu
+def test_a_longest_length_that_is_none_is_reported():
+    q, k, v, w, table, lens = arguments("cuda", 128)
+    num, table = layout([600], "cuda")
+    k, v, w = cache(num, 2, 128, "cuda")
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([600], dtype=torch.int32, device="cuda")
+    ops.attention_prefill(q[:1], k, v, table, lens, cu, 1, 0.1, weights=w, max_kv_len=100)
+    with pytest.raises(RuntimeError, match="bad argument"):
+        ops.native.check_status(torch.device("cuda", 0))
+
+
 @pytest.mark.gpu
 def test_other_head_sizes_take_tensor_operations():
     test_step("cuda", (4, 2, 80), [33, 7], 1, 0, False)

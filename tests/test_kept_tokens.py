@@ -197,6 +197,17 @@ def test_what_does_not_go_with_a_bound_is_refused():
         eng.feed_logits(seq, prompt(60, 2))
 
 
+def test_steps_are_committed_one_by_one():
+    eng = Engine(build(), max_batch=1, max_seq_len=128, kv_keep=64)
+    s = eng.new_sequence(prompt(10), GREEDY, max_new_tokens=8)
+    eng.start_decode([s], eng.prefill([s]))
+    eng.decode_step()
+    with pytest.raises(RuntimeError):
+        eng.decode_step()
+    eng.commit([1])
+    eng.decode_step()
+
+
 def test_pools_that_move_and_grow_keep_the_weights():
     model = build()
     eng = Engine(model, max_batch=2, max_seq_len=128, kv_keep=64)
