@@ -255,10 +255,13 @@ __global__ void __launch_bounds__(32 * kWdWarps, 3) weighed_decode_kernel(const 
   const bool held = p.scores == nullptr;
   const WdScores scores{held ? reinterpret_cast<float*>(smem + wd_smem<D, NT, RG>() - 1024) : p.scores + (static_cast<size_t>(b) * p.n_kv + h) * p.room * p.pad,
                         held ? s.page0 * kWdPage : 0};
+  // A row of 128 bytes has its 16-byte pieces permuted by the row's number: piece 2 i + half of a lane's row is the half's place with bits 5 and 6 flipped by i
   const uint32_t ring_addr = smem_u32(ring);
-  const int a_row = lane & 15, v_row = (lane >> 4) * 8 + (lane & 7);
+  const uint32_t a_off = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_off = ((lane >> 4) * 8 + (lane & 7)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  float* score_at = scores.row(first * kWdPage + g, p.pad) + row0 + 2 * tig;
   int it = 0;
-  for (int pg = first; pg < s.page1 && ok; pg += PG, ++it) {
+  for (int pg = first; pg < s.page1 && ok; pg += PG, ++it, score_at += PG * kWdPage * p.pad) {
     const int st = it % STAGES;
     ok = mbar_wait_warp(&full[pgroup][st], (it / STAGES) & 1, p.status, kStatusTmaFullTimeout);
     if (!ok) break;
@@ -267,8 +270,7 @@ __global__ void __launch_bounds__(32 * kWdWarps, 3) weighed_decode_kernel(const 
     uint32_t a[KS][4];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const int chunk = ks * 2 + (lane >> 4);
-      wd_ldsm(k_addr + (chunk >> 3) * 2048 + a_row * 128 + (((chunk & 7) ^ (a_row & 7)) << 4), a[ks]);
+      wd_ldsm(((k_addr + a_off) ^ ((ks & 3) << 5)) + (ks >> 2) * 2048, a[ks]);
     }
     float sc[NT][4];
 #pragma unroll
@@ -297,8 +299,7 @@ __global__ void __launch_bounds__(32 * kWdWarps, 3) weighed_decode_kernel(const 
     }
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      const int chunk = i * 2 + ((lane >> 3) & 1);
-      wd_ldsm_t(v_addr + (chunk >> 3) * 2048 + v_row * 128 + (((chunk & 7) ^ (v_row & 7)) << 4), a[i]);
+      wd_ldsm_t(((v_addr + v_off) ^ ((i & 3) << 5)) + (i >> 2) * 2048, a[i]);
     }
     __syncwarp();
     if (RG > 1 && lane == 0) mbar_arrive(&empty[pgroup][st]);
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(32 * kWdWarps, 3) weighed_decode_kernel(const 
         // (rows behind the last are nothing, whatever zeros make of a key that is no number)
         const int r = row0 + nt * 8 + 2 * tig;
         const bool r0 = r < p.rows, r1 = r + 1 < p.rows;
-        float* at = scores.row(key0 + g, p.pad) + r;
+        float* at = score_at + nt * 8;
         *reinterpret_cast<float2*>(at) = make_float2(r0 ? sc[nt][0] : -INFINITY, r1 ? sc[nt][1] : -INFINITY);
         *reinterpret_cast<float2*>(at + 8 * p.pad) = make_float2(r0 ? sc[nt][2] : -INFINITY, r1 ? sc[nt][3] : -INFINITY);
       }
