@@ -5,16 +5,18 @@
 // The sum runs over the rows of a column, so the scores are taken as S^T = K Q^T: a tensor-memory lane is a key, and a thread adds up what lies in its
 // lane without any exchange. A CTA has 256 keys of one head (two tiles of 128, resident), and the rows that see them come by in tiles of 128:
 // 128 / 2^gshift tokens of 2^gshift query heads, so that few tokens of many heads fill a tile as well.
-//   warp 0      : TMA producer - both key tiles once (sixteen pages), then tiles of query rows through a ring; it also brings the rows' lse to shared memory, negated
-//                 and with -inf where a row does not count
-//   warp 1      : MMA issuer - two accumulators for each key tile, so that the tensor core runs ahead
-//   warps 2..5  : sums of key tile a, warps 6..9 of tile b: a score row comes to registers, the accumulator is released, then one FMA for two scores, one
-//                 exponential each, one addition for two
+//   warp 0      : TMA producer - both key tiles once (sixteen pages), then tiles of query rows through a ring, and beside them the rows' -lse (-inf where a row
+//                 does not count) as three bf16 pieces of 24 bits in all
+//   warp 1      : MMA issuer - two accumulators for each key tile, so that the tensor core runs ahead. One step more along K, ones by those pieces, takes lse off the scores:
+//                 read from shared memory it cost every thread 512 bytes a tile
+//   warps 2..5  : sums of key tile a, warps 6..9 of tile b: a score row comes to registers in halves, the next one asked for while one is added up: a product and an
+//                 exponential for each score (products of two at once were slower: 4096 tokens 254 -> 244 us), one addition for two
 // The CTAs of a cluster share the rows of the same keys; their sums are added up in the order of their ranks.
 //
-// Bound by exponentials: 32768 of a pair of tiles take the special-function unit 2048 cycles, the tensor core 1050. 4096 tokens, 32 heads of 128 over 8: 100 us of the 257
-// that the call takes (61 us at the unit's rate; counters at that size: the unit 60 % of active cycles, issue 29 %, tensor 29 %, the rest is the start and the end of CTAs
-// of one to an SM). Two CTAs to an SM with tiles of 64 rows measured the same (257 -> 263 us; 2048 tokens 91 -> 94).
+// Bound by exponentials, 2048 cycles of the special-function unit for a pair of tiles (the tensor core needs 1050), and by what each tile costs beside them: 4096 tokens, 32 heads
+// of 128 over 8, 105 us of the 244 that the call takes, 61 at the unit's rate. Left out in a copy for the time's sake, the exponentials take 32 us of it, the products of the tensor core 6;
+// 60 are tiles without arithmetic - accumulators read, barriers - and 12 the start and the end of a CTA (one to an SM). Tiles of 64 rows with two CTAs to an SM measured
+// the same (257 -> 263 us before the steps above; 2048 tokens 91 -> 94), an issuer for each key tile 243 for 244.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -41,12 +43,31 @@ struct PwParams {
   float* weights;
   int* status;
   int wide, num_pages, n_q, n_kv, group, gshift, window, observed;
-  float scale_log2;
+  float scale_log2, unscale;   // and 1 / scale_log2
 };
 
-// shared memory: key tiles a, b (NK halves each) | query ring | lse ring | sums of the keys | barriers
+// shared memory: key tiles a, b (NK halves each) | query ring | ones | lse ring | sums of the keys | barriers
+constexpr int kPwExtra = kPwTile * 16 * 2;   // a tile [128][16] of the step that brings the rows' lse
 // (more than half of an SM's in any case: a CTA has all of its tensor memory, and one that waited for a neighbour's while its own cluster waits for it would never get it)
-constexpr int pw_smem(int nk) { return std::max(120 * 1024, 1024 + (2 * nk + kPwStages * nk) * kPwHalf + kPwStages * kPwTile * 4 + kPwKeys * 4 + 256); }
+constexpr int pw_smem(int nk) { return std::max(120 * 1024, 1024 + (2 * nk + kPwStages * nk) * kPwHalf + (1 + kPwStages) * kPwExtra + kPwKeys * 4 + 256); }
+
+// Operand [rows][16] without swizzle: blocks of eight rows of 16 bytes (128 bytes each), the two of a row side by side along K.
+__device__ __forceinline__ uint64_t pw_desc_plain(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;            // along K: 128 bytes
+  d |= static_cast<uint64_t>(256 >> 4) << 32;            // eight rows on: 256 bytes
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+__device__ __forceinline__ int pw_plain(int row, int col) { return (row >> 3) * 256 + (col >> 3) * 128 + (row & 7) * 16 + (col & 7) * 2; }
+// Uses of the registers stay behind the wait in front of this.
+__device__ __forceinline__ void pw_settled(uint32_t (&r)[4][16]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    asm volatile("" : "+r"(r[c][0]), "+r"(r[c][1]), "+r"(r[c][2]), "+r"(r[c][3]), "+r"(r[c][4]), "+r"(r[c][5]), "+r"(r[c][6]), "+r"(r[c][7]), "+r"(r[c][8]),
+                 "+r"(r[c][9]), "+r"(r[c][10]), "+r"(r[c][11]), "+r"(r[c][12]), "+r"(r[c][13]), "+r"(r[c][14]), "+r"(r[c][15]));
+}
 
 __device__ __forceinline__ void pw_load_page(void* dst, const CUtensorMap* map, int x, int head, int page, uint64_t* bar) {
   asm volatile(
@@ -61,12 +82,13 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pw_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* k_s = smem;
   uint8_t* q_s = k_s + 2 * NK * kPwHalf;
-  float* lse_s = reinterpret_cast<float*>(q_s + kPwStages * NK * kPwHalf);
-  float* sum_s = lse_s + kPwStages * kPwTile;
+  uint8_t* one_s = q_s + kPwStages * NK * kPwHalf;
+  uint8_t* lse_s = one_s + kPwExtra;
+  float* sum_s = reinterpret_cast<float*>(lse_s + kPwStages * kPwExtra);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sum_s + kPwKeys);
   uint64_t* k_full = bars;                               // 1
   uint64_t* q_full = bars + 1;                           // [stages]: bytes, and the 32 lanes that wrote lse
-  uint64_t* q_empty = q_full + kPwStages;                // [stages]: the MMA's commit, and a lane of each warp that sums
+  uint64_t* q_empty = q_full + kPwStages;                // [stages]: the MMA's commit
   uint64_t* s_full = q_empty + kPwStages;                // [tile][2]
   uint64_t* s_empty = s_full + 4;                        // [tile][2], 128 arrivals
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_empty + 4);
@@ -82,7 +104,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
     mbar_init(k_full, 1);
     for (int s = 0; s < kPwStages; ++s) {
       mbar_init(&q_full[s], 1 + 32);
-      mbar_init(&q_empty[s], 1 + 8);
+      mbar_init(&q_empty[s], 1);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
@@ -92,6 +114,11 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
   }
+  // the step's A operand is three ones a key, its B operand what is left in three pieces; columns behind them are zero on both sides
+  for (int i = threadIdx.x; i < (1 + kPwStages) * kPwExtra / 16; i += kPwThreads) reinterpret_cast<uint4*>(one_s)[i] = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kPwTile; i += kPwThreads) *reinterpret_cast<uint2*>(one_s + pw_plain(i, 0)) = make_uint2(0x3F803F80u, 0x3F80u);
+  fence_proxy_async_smem();
   if (warp == 0) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -147,7 +174,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = lane + 32 * j, t = token + (c >> p.gshift);
-          v[j] = t < q_len ? -p.lse[static_cast<size_t>(q0 + t) * p.n_q + head + (c & ((1 << p.gshift) - 1))] : -INFINITY;
+          v[j] = t < q_len ? -p.lse[static_cast<size_t>(q0 + t) * p.n_q + head + (c & ((1 << p.gshift) - 1))] * p.unscale : -INFINITY;
           if (v[j] == INFINITY) v[j] = -INFINITY;                       // a row that saw nothing gives nothing
         }
         if (it >= kPwStages) ok = mbar_wait_warp(&q_empty[s], (it / kPwStages - 1) & 1, p.status, kStatusSmemEmptyTimeout);
@@ -157,7 +184,13 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
           for (int x = 0; x < NK; ++x) tma_load_3d(q_s + (s * NK + x) * kPwHalf, &tmQ, x * 64, head, q0 + token, &q_full[s]);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) lse_s[s * kPwTile + lane + 32 * j] = v[j];
+        for (int j = 0; j < 4; ++j) {
+          // 24 bits in three pieces of eight
+          const float high = __bfloat162float(__float2bfloat16(v[j])), rest = high == -INFINITY ? 0.f : v[j] - high;
+          const float mid = __bfloat162float(__float2bfloat16(rest));
+          *reinterpret_cast<uint2*>(lse_s + s * kPwExtra + pw_plain(lane + 32 * j, 0)) = make_uint2(pack_bf16x2(high, mid), pack_bf16x2(rest - mid, 0.f));
+        }
+        fence_proxy_async_smem();
         mbar_arrive(&q_full[s]);
       }
     }
@@ -180,6 +213,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
             const uint32_t off = (kk >> 2) * kPwHalf + (kk & 3) * 32;
             umma_f16(d, umma_desc_k_sw128(ka + off), umma_desc_k_sw128(qa + off), idesc, kk > 0 ? 1u : 0u);
           }
+          umma_f16(d, pw_desc_plain(smem_u32(one_s)), pw_desc_plain(smem_u32(lse_s + s * kPwExtra)), idesc, 1u);
           umma_commit(&s_full[w * 2 + buf]);
           if (w == 1) umma_commit(&q_empty[s]);
         }
@@ -191,58 +225,73 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
     const int key = key0 + w * kPwTile + quarter * 32 + lane;
     const int tile_first = key0 + w * kPwTile, tile_last = min(kv_len, tile_first + kPwTile) - 1;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
-    for (int i = begin; i < end && ok; ++i) {
-      const int it = i - begin, s = it % kPwStages, buf = it & 1;
-      ok = mbar_wait(&s_full[w * 2 + buf], (it >> 1) & 1, p.status, kStatusAccumTimeout);
-      if (ok) ok = mbar_wait(&q_full[s], (it / kPwStages) & 1, p.status, kStatusTmaFullTimeout);   // (it has passed: the lse is there)
-      if (!ok) break;
-      tc_fence_after_sync();
-      uint32_t sc[8][16];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) tmem_ld16(tmem + lanes + (w * 2 + buf) * kPwTile + c * 16, sc[c]);
-      tmem_wait_ld();
-      tc_fence_before_sync();
-      mbar_arrive(&s_empty[w * 2 + buf]);
-      const float* lse = lse_s + s * kPwTile;
-      const int token = t0 + i / head_tiles * tile_tokens;
-      // positions of the tile's rows: [pos, pos + tile_tokens)
-      const int pos = before + token;
+    uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
+    // the first column and the one behind the last of a tile that see this thread's key; all of them where no row or key of the tile is at an edge
+    auto seen = [&](int i, int& low, int& high) {
+      const int token = t0 + i / head_tiles * tile_tokens, pos = before + token;     // positions of the tile's rows: [pos, pos + tile_tokens)
+      low = 0;
+      high = kPwTile;
       const bool edge = pos < tile_last || token + tile_tokens > q_len || (p.window > 0 && pos + tile_tokens - 1 >= tile_first + p.window);
       if (edge) {
-        // columns [low, high) are rows that see this key
         const int high_t = p.window > 0 ? min(q_len, key - before + p.window) : q_len;
-        const int low = (key - pos) * (1 << p.gshift), high = (high_t - token) * (1 << p.gshift);
+        low = (key - pos) * (1 << p.gshift);
+        high = (high_t - token) * (1 << p.gshift);
+      }
+      return edge;
+    };
+    auto add = [&](const uint32_t (&sc)[4][16], int first, bool edge, int low, int high) {
+      if (edge) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int col = c * 16 + e;
-            const float v = ex2_approx(fmaf(__uint_as_float(sc[c][e]), p.scale_log2, lse[col]));
+            const int col = first + c * 16 + e;
+            const float v = ex2_approx(__uint_as_float(sc[c][e]) * p.scale_log2);
             total += col >= low && col < high ? v : 0.f;
           }
         }
       } else {
-        uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float4 l = *reinterpret_cast<const float4*>(lse + c * 16 + e);
-            float x0, x1, x2, x3;
-            unpack_f32x2(fma_f32x2(pack_b32x2(sc[c][e], sc[c][e + 1]), scale2, pack_f32x2(l.x, l.y)), x0, x1);
-            unpack_f32x2(fma_f32x2(pack_b32x2(sc[c][e + 2], sc[c][e + 3]), scale2, pack_f32x2(l.z, l.w)), x2, x3);
-            acc[(e >> 2) & 1] = add_f32x2(acc[(e >> 2) & 1], pack_f32x2(ex2_approx(x0), ex2_approx(x1)));
-            acc[2 + ((e >> 2) & 1)] = add_f32x2(acc[2 + ((e >> 2) & 1)], pack_f32x2(ex2_approx(x2), ex2_approx(x3)));
+          for (int e = 0; e < 16; e += 2) {
+            const float x0 = __uint_as_float(sc[c][e]) * p.scale_log2, x1 = __uint_as_float(sc[c][e + 1]) * p.scale_log2;
+            acc[(e >> 1) & 3] = add_f32x2(acc[(e >> 1) & 3], pack_f32x2(ex2_approx(x0), ex2_approx(x1)));
           }
         }
-        float s0, s1;
-        unpack_f32x2(add_f32x2(add_f32x2(acc[0], acc[1]), add_f32x2(acc[2], acc[3])), s0, s1);
-        total += s0 + s1;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[s]);
+    };
+    // A score row comes in two halves; while one is added up the next is on its way, the next tile's first half as well.
+    uint32_t left[4][16], right[4][16];
+    auto ask = [&](uint32_t (&sc)[4][16], int i, int first) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld16(tmem + lanes + (w * 2 + ((i - begin) & 1)) * kPwTile + first + c * 16, sc[c]);
+    };
+    auto ready = [&](int i) {
+      ok = mbar_wait_warp(&s_full[w * 2 + ((i - begin) & 1)], ((i - begin) >> 1) & 1, p.status, kStatusAccumTimeout);
+      if (ok) {
+        tc_fence_after_sync();
+        ask(left, i, 0);
+      }
+    };
+    if (begin < end) ready(begin);
+    for (int i = begin; i < end && ok; ++i) {
+      int low, high;
+      const bool edge = seen(i, low, high);
+      tmem_wait_ld();
+      pw_settled(left);
+      ask(right, i, 64);
+      add(left, 0, edge, low, high);
+      tmem_wait_ld();
+      pw_settled(right);
+      tc_fence_before_sync();
+      mbar_arrive(&s_empty[w * 2 + ((i - begin) & 1)]);
+      if (i + 1 < end) ready(i + 1);
+      add(right, 64, edge, low, high);
     }
+    float s0, s1;
+    unpack_f32x2(add_f32x2(add_f32x2(acc[0], acc[1]), add_f32x2(acc[2], acc[3])), s0, s1);
+    total += s0 + s1;
     if (ranks > 1) sum_s[w * kPwTile + quarter * 32 + lane] = total;
   }
   if (ranks > 1) {
@@ -339,6 +388,7 @@ extern "C" int eredu_weighed_prefill(const void* args, int bytes) {
   p.window = a.window;
   p.observed = a.observed;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.unscale = 1.f / p.scale_log2;
   const uint64_t D = static_cast<uint64_t>(a.D), H = static_cast<uint64_t>(a.n_kv), Q = static_cast<uint64_t>(a.n_q);
   CUtensorMap tmQ, tmK;
   int r = make_tma_3d(&tmQ, a.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, Q, static_cast<uint64_t>(a.total_q), D * 2, Q * D * 2, 64, 1 << p.gshift, kPwTile >> p.gshift);

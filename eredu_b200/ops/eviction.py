@@ -207,8 +207,8 @@ def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale,
 def prompt_ranks(batch, n_q, n_kv, max_q_len, max_kv_len, observed, sm_count=148):
     """CTAs that share the rows of a block of 256 keys in the kernel of prompts' weights, one to an SM: 1, 2, 4 or 8. Early blocks are seen by more rows than late ones, and
     a CTA costs what 14 of its tiles of 128 rows take beside them; the choice is the one with the least of the longest CTA or the mean over SMs, and that cost for every
-    round (us of the whole call with 1 / 2 / 4 / 8, 32 heads over 8: 4096 tokens 366 / 257 / 283 / 325, 2048 161 / 109 / 91 / 112, 512 48 / 37 / 29 / 32, eight of 512
-    82 / 82 / 94 / 127; 8192 tokens over 4 heads, the last 64 rows 490 / 497 / 510 / 550)."""
+    round (us of the whole call with 1 / 2 / 4 / 8, 32 heads over 8: 4096 tokens 346 / 244 / 267 / 311, 2048 149 / 102 / 88 / 109, 512 45 / 35 / 29 / 32, eight of 512
+    80 / 80 / 92 / 127; 8192 tokens over 4 heads, the last 64 rows 490 / 497 / 509 / 566)."""
     group, blocks = n_q // n_kv, -(-max_kv_len // 256)
     shared = min(group & -group, 32)                                          # query heads of a tile
     rows = min(observed, max_q_len) if observed > 0 else max_q_len
@@ -232,6 +232,8 @@ def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len,
         raise ValueError(f"the last {observed} rows")
     if not kernels:
         return weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, (cu_q[1:] - cu_q[:-1]).tolist(), scale, window, sinks, weights, observed, out)
+    if not scale > 0:
+        raise ValueError(f"the kernels of prompts take scales above zero, not {scale}")
     total, n_q, dim = q.shape
     pages, n_kv = k_cache.shape[:2]
     block_table = block_table.contiguous()
