@@ -126,10 +126,11 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs p,
   float* w = p.weights + static_cast<size_t>(layer) * p.num_pages * p.n_kv * kEvictPage;
   int* pages = reinterpret_cast<int*>(kept + (p.max_tokens + 3) / 4 * 4);
   const EvictTable<HELD> table{p, pages, b};
-  if (HELD) {
+  if (HELD)
     for (int i = tid; i * kEvictPage < n; i += threads) pages[i] = evict_page(p, b, i);
-    __syncthreads();
-  }
+  for (int i = tid; i < kEvictBins; i += threads) hist[i] = 0;
+  if (tid == 0) s_first = n;
+  __syncthreads();
   auto page_cell = [&](int t) -> float* {
     const int page = table[t / kEvictPage];
     return page < 0 ? nullptr : w + (static_cast<size_t>(page) * p.n_kv + h) * kEvictPage + t % kEvictPage;
@@ -139,58 +140,69 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs p,
     const float* at = t < n ? page_cell(t) : nullptr;
     return at == nullptr ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(at);
   };
-  if (HELD) {
-#pragma unroll 4
-    for (int t = 4 * tid; t < n; t += 4 * threads) *reinterpret_cast<float4*>(kept + t) = quad(t);
-  }
-  if (ranks > 1) {
-    __syncwarp();
-    cluster_arrive_release();                        // this CTA has read the weights, which the first one moves
-  }
   // ---- the border: the quota-th largest of the tokens [first, last)
   const int first = p.first, last = n - p.recent, quota = p.keep - p.first - p.recent;
   uint32_t border = 0;
   int left = quota;                                  // of those that agree with the border so far, how many stay
-  if (tid == 0) s_first = n;
+  int shift = 21, bins = kEvictBins;                 // the digit that is counted
+  uint32_t above = 0;                                // bits in front of it
+  // Lanes that all have the same digit (weights that are equal) count as one. Behind the first round few weights agree with the border.
+  auto count = [&](int t, const float4& q) {
+    const float x[4] = {q.x, q.y, q.z, q.w};
+    uint32_t u[4];
+    bool in[4], any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] = weight_order(x[i]);
+      in[i] = t + i >= first && t + i < last && (u[i] & above) == border;
+      any = any || in[i];
+    }
+    if (above != 0 && !__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int digit = in[i] ? static_cast<int>(u[i] >> shift) & (bins - 1) : -1;
+      if (__all_sync(0xffffffffu, digit == __shfl_sync(0xffffffffu, digit, 0))) {
+        if (lane == 0 && digit >= 0) atomicAdd(&hist[digit], 32);
+      } else if (digit >= 0) {
+        atomicAdd(&hist[digit], 1);
+      }
+    }
+  };
+  // (HELD: the first digits are counted as the weights come in)
+  auto from_memory = [&](bool counted) {
+    for (int t0 = 0; t0 < n; t0 += 16 * threads) {
+      float4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = quad(t0 + 4 * (i * threads + tid));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (t0 + 4 * i * threads >= n) break;
+        const int t = t0 + 4 * (i * threads + tid);
+        if (HELD && t < n) *reinterpret_cast<float4*>(kept + t) = x[i];
+        __syncwarp();
+        if (counted) count(t, x[i]);
+      }
+    }
+  };
+  if (HELD) from_memory(quota > 0);
+  if (ranks > 1) {
+    __syncwarp();
+    cluster_arrive_release();                        // this CTA has read the weights, which the first one moves
+  }
   for (int round = 0; round < 3 && quota > 0; ++round) {
-    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round == 2 ? 1024 : 2048;
-    for (int i = tid; i < bins; i += threads) hist[i] = 0;
-    __syncthreads();
-    const uint32_t above = round == 0 ? 0u : ~0u << (round == 1 ? 21 : 10);
-    // Lanes that all have the same digit (weights that are equal) count as one. Behind the first round few weights agree with the border.
-    auto count = [&](int t, const float4& q) {
-      const float x[4] = {q.x, q.y, q.z, q.w};
-      uint32_t u[4];
-      bool in[4], any = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u[i] = weight_order(x[i]);
-        in[i] = t + i >= first && t + i < last && (u[i] & above) == border;
-        any = any || in[i];
-      }
-      if (round > 0 && !__any_sync(0xffffffffu, any)) return;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int digit = in[i] ? static_cast<int>(u[i] >> shift) & (bins - 1) : -1;
-        if (__all_sync(0xffffffffu, digit == __shfl_sync(0xffffffffu, digit, 0))) {
-          if (lane == 0 && digit >= 0) atomicAdd(&hist[digit], 32);
-        } else if (digit >= 0) {
-          atomicAdd(&hist[digit], 1);
-        }
-      }
-    };
-    if (HELD) {
+    if (round > 0) {
+      shift = round == 1 ? 10 : 0;
+      bins = round == 1 ? 2048 : 1024;
+      above = ~0u << (shift + (round == 1 ? 11 : 10));
+      for (int i = tid; i < bins; i += threads) hist[i] = 0;
+      __syncthreads();
+    }
+    if (!HELD) {
+      from_memory(true);
+    } else if (round > 0) {
       for (int t0 = 0; t0 < n; t0 += 4 * threads) {
         const int t = t0 + 4 * tid;
         count(t, t < n ? *reinterpret_cast<const float4*>(kept + t) : make_float4(0.f, 0.f, 0.f, 0.f));
-      }
-    } else {
-      for (int t0 = 0; t0 < n; t0 += 16 * threads) {
-        float4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = quad(t0 + 4 * (i * threads + tid));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) count(t0 + 4 * (i * threads + tid), x[i]);
       }
     }
     __syncthreads();
