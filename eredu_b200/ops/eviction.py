@@ -55,24 +55,29 @@ native.register("eredu_weighed_clusters", I, [])
 native.register("eredu_weighed_prefill", I, [P, I])
 
 
+_current = getattr(torch._C, "_cuda_getDevice", lambda: -1)       # the current device, without the checks around it
+
+
 def _elsewhere(t) -> bool:
     """Whether a tensor lies on another GPU than the current one, whose stream a launch would take."""
-    return t.is_cuda and t.device.index != torch.cuda.current_device()
+    at = t.get_device()
+    return at >= 0 and at != _current()
 
 
 # ------------------------------------------------------------------------------------------ attention
 def _kernels_take(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, rows, chunk) -> bool:
     """Whether the call is one for the kernels; CPU tensors and other head sizes take tensor operations, and what neither can take is refused.
     (One condition for the common case: these checks are a good part of what a short call costs.)"""
-    if type(k_cache) is not Pages8 and type(v_cache) is not Pages8 and not chunk and q.dim() == 3 and k_cache.dim() == 4:
-        shape, (m, n_q, dim), at = k_cache.shape, q.shape, k_cache.get_device()
-        if (at >= 0 and dim in HEAD_DIMS and shape[3] == dim and v_cache.shape == shape and shape[2] == PAGE and weights.shape == shape[:3] and n_q % shape[1] == 0
-                and (rows is None or m == rows) and at == q.get_device() == v_cache.get_device() == weights.get_device() == seq_lens.get_device() == block_table.get_device()
+    at, shape, row = q.get_device(), k_cache.shape, q.shape
+    if at >= 0 and sinks is None and out is None and not chunk and type(k_cache) is not Pages8 and type(v_cache) is not Pages8 and len(row) == 3 and len(shape) == 4:
+        m, n_q, dim = row
+        if (dim in HEAD_DIMS and shape[3] == dim and v_cache.shape == shape and shape[2] == PAGE and weights.shape == shape[:3] and n_q % shape[1] == 0
+                and (rows is None or m == rows) and at == k_cache.get_device() == v_cache.get_device() == weights.get_device() == seq_lens.get_device() == block_table.get_device()
                 and q.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16 and weights.dtype is torch.float32
                 and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32 and seq_lens.dim() == 1 and block_table.dim() == 2
                 and block_table.shape[0] == seq_lens.shape[0] and block_table.stride(1) == 1 and q.is_contiguous() and k_cache.is_contiguous()
                 and v_cache.is_contiguous() and weights.is_contiguous() and seq_lens.is_contiguous()
-                and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0 and sinks is None and out is None):
+                and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0):
             return True
     return _check_attention(q, k_cache, v_cache, block_table, seq_lens, sinks, weights, out, rows, chunk)
 
@@ -274,13 +279,7 @@ def evict_tokens_ref(k, v, weights, block_table, seq_lens, keep, recent=0, first
     return seq_lens.clamp_max(keep)
 
 
-def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, max_kv_len=0):
-    """Brings every sequence of more than ``keep`` tokens down to ``keep``, in place, and returns the tokens that each has left (int32 [B]). ``k``, ``v``: pages
-    of all layers [layers, pages, heads, 16, width], ``weights`` [layers, pages, heads, 16] fp32 (see above). For every layer and head by itself
-    the ``first`` tokens of a sequence and its ``recent`` last ones stay, and of those between them the ones with the largest weights; of equal weights the
-    earlier token, and what is no number goes first. What stays moves to the front in its order - keys, values and weights, bit by bit -, and the rows
-    behind it are left as they were. A page belongs to one sequence of the call only (shared pages are copied first, :func:`.kv8.copy_pages`).
-    ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it."""
+def _check_eviction(k, v, weights, block_table, seq_lens) -> None:
     if isinstance(k, Pages8) or isinstance(v, Pages8) or k.dtype == torch.int8:
         raise NotImplementedError("tokens of 8-bit pages share the scale of their block: they are not evicted one by one")
     if k.dim() != 5 or v.dim() != 5 or k.shape[3] != PAGE or v.shape[:4] != k.shape[:4] or weights.shape != k.shape[:4]:
@@ -291,35 +290,55 @@ def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, 
     _need("weights", weights, torch.float32, dev)
     _need("seq_lens", seq_lens, torch.int32, dev)
     _check_table(block_table, seq_lens, dev)
+
+
+def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, max_kv_len=0):
+    """Brings every sequence of more than ``keep`` tokens down to ``keep``, in place, and returns the tokens that each has left (int32 [B]). ``k``, ``v``: pages
+    of all layers [layers, pages, heads, 16, width], ``weights`` [layers, pages, heads, 16] fp32 (see above). For every layer and head by itself
+    the ``first`` tokens of a sequence and its ``recent`` last ones stay, and of those between them the ones with the largest weights; of equal weights the
+    earlier token, and what is no number goes first. What stays moves to the front in its order - keys, values and weights, bit by bit -, and the rows
+    behind it are left as they were. A page belongs to one sequence of the call only (shared pages are copied first, :func:`.kv8.copy_pages`).
+    ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it."""
     if keep < 1 or recent < 0 or first < 0 or recent + first > keep:
         raise ValueError(f"of {keep} tokens the first {first} and the last {recent} cannot stay")
-    layers, pages, n_kv = k.shape[:3]
+    shape, at = k.shape, -1 if type(k) is Pages8 else k.get_device()
+    # (one condition for the common case, as above)
+    if not (at >= 0 and type(v) is not Pages8 and len(shape) == 5 and shape[3] == PAGE and v.shape == shape and weights.shape == shape[:4] and k.dtype is v.dtype
+            and k.dtype is not torch.int8 and weights.dtype is torch.float32 and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32
+            and seq_lens.dim() == 1 and block_table.dim() == 2 and block_table.shape[0] == seq_lens.shape[0] and block_table.stride(1) == 1
+            and at == v.get_device() == weights.get_device() == seq_lens.get_device() == block_table.get_device() and k.is_contiguous() and v.is_contiguous()
+            and weights.is_contiguous() and seq_lens.is_contiguous()):
+        _check_eviction(k, v, weights, block_table, seq_lens)
+    dev = k.device
+    layers, pages, n_kv = shape[:3]
     B, wide = block_table.shape
-    if not k.is_cuda:
+    if at < 0:
         return evict_tokens_ref(k, v, weights, block_table, seq_lens, keep, recent, first)
-    k_row, v_row = k.shape[4] * k.element_size(), v.shape[4] * v.element_size()
+    size = k.element_size()
+    k_row, v_row = shape[4] * size, v.shape[4] * size
+    ka, va, wa = k.data_ptr(), v.data_ptr(), weights.data_ptr()
     if (k_row | v_row) % 16:
         raise NotImplementedError(f"rows of {k_row} and {v_row} bytes: the kernel moves whole pieces of 16 bytes")
-    if (k.data_ptr() | v.data_ptr() | weights.data_ptr()) % 16:
+    if (ka | va | wa) % 16:
         raise ValueError("keys, values and weights have to begin at multiples of 16 bytes")
-    if _elsewhere(k):
+    if at != _current():
         with torch.cuda.device(dev):
             return evict_tokens(k, v, weights, block_table, seq_lens, keep, recent, first, max_kv_len)
     left = torch.empty_like(seq_lens)
     longest = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE
     if B == 0 or layers == 0 or longest <= keep:
-        return torch.clamp(seq_lens, max=keep, out=left)
-    step, lists, at = layers, None, 0
+        return left.copy_(seq_lens)
+    step, lists, done = layers, None, 0
     if longest > HELD_TOKENS:
         step = max(1, min(layers, LIST_BYTES // (4 * B * n_kv * keep)))
         lists = torch.empty(step * B * n_kv * keep, dtype=torch.int32, device=dev)
     page = pages * n_kv * PAGE                                                                           # tokens and heads of a layer
-    ka, va, wa, status, stream = k.data_ptr(), v.data_ptr(), weights.data_ptr(), status_word(dev).data_ptr(), stream_ptr(dev)
-    while at < layers:
-        some = min(step, layers - at)
+    status, stream = status_word(dev).data_ptr(), stream_ptr(dev)
+    while done < layers:
+        some = min(step, layers - done)
         code = lib().eredu_evict_tokens(_EVICT.pack(
-            ka + at * page * k_row, va + at * page * v_row, wa + at * page * 4, block_table.data_ptr(), seq_lens.data_ptr(), left.data_ptr(), address(lists),
+            ka + done * page * k_row, va + done * page * v_row, wa + done * page * 4, block_table.data_ptr(), seq_lens.data_ptr(), left.data_ptr(), address(lists),
             status, stream, some, B, n_kv, pages, block_table.stride(0), longest, keep, recent, first, k_row, v_row, _device(dev)[0]), _EVICT.size)
         check(code, "eredu_evict_tokens")
-        at += some
+        done += some
     return left

@@ -430,7 +430,11 @@ def test_calls_for_another_device_are_made_there(monkeypatch):
     current, made = [0], []
 
     class On:
-        is_cuda, device = True, torch.device("cuda", 1)
+        device = torch.device("cuda", 1)
+
+        @staticmethod
+        def get_device():
+            return 1
 
     class Device:
         def __init__(self, device):
@@ -442,7 +446,7 @@ def test_calls_for_another_device_are_made_there(monkeypatch):
         def __exit__(self, *_):
             current.pop()
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[-1])
+    monkeypatch.setattr(eviction, "_current", lambda: current[-1])
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(eviction, "_kernels_take", lambda *a: made.append(current[-1]) or 1 / 0)
     for call in (lambda: eviction.weighed_decode(On, On, On, None, torch.zeros(1), 1, 1.0, 0, None, None, None, 0, 0),
