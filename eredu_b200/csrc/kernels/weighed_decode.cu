@@ -13,9 +13,10 @@
 // their part in memory, and a second kernel does the same. Up to sixteen rows that share a head are a warp's; with more, two or four warps walk the same pages with
 // sixteen rows each.
 //
-// Measured (floor: K, V and weights at 6.54 TB/s): 64 sequences of 2048 to 4096 tokens, 32 heads of 128 over 8, 144 us (floor 124, 5.6 TB/s); 32 of 1088 to 2175 48 us
-// (33: what is left is the start and the end of the CTAs, about 8 us, and the raggedness of the last ones); one of 32768, 64 heads over 8, 38 us (21: 24 splits to a head and the second
-// kernel); one of 512, 32 heads of 64 over 8, 8.4 us between launches of a graph, a chain of latencies. A page costs a warp some 300 instructions at five cycles each while
+// Measured (floor: K, V and weights at 6.54 TB/s): 64 sequences of 2048 to 4096 tokens, 32 heads of 128 over 8, 134 us (floor 124, 6.1 TB/s); 32 of 1088 to 2175 42 us
+// (33: what is left is the start and the end of the CTAs, about 8 us); one of 32768, 64 heads over 8, 31 us (21: 24 splits to a head and the second
+// kernel); one of 512, 32 heads of 64 over 8, 8.4 us between launches of a graph, a chain of latencies. Storing the scores and adding up the weights took 18 us of 144 in the first of these
+// before keys and values were kept from pushing the scores out of the second-level cache. A page costs a warp some 300 instructions at five cycles each while
 // it is alone on its scheduler, so that twelve warps to an SM (two stages to a ring) move more than eight with three stages: 64 x 4096 156 -> 148 us.
 #include <cuda_bf16.h>
 

@@ -150,13 +150,14 @@ def weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, sc
     return out
 
 
-def weighed_splits(batch, n_kv, max_kv_len, sm_count=148, cluster=CLUSTER):
+def weighed_splits(batch, n_kv, max_kv_len, sm_count=148, cluster=CLUSTER, rows=1):
     """CTAs that share a sequence and head of the decode kernel, each with eight pages at least. Three CTAs fit an SM, clusters not quite: as many splits as find room on
-    nine tenths of that, up to eight. Where sequences and heads fill most of the room by themselves, three, four or eight splits even out what sequences differ by
-    (us with 1 / 2 / 3 / 4 / 8: 32 x 8 heads of 1088 to 2175 tokens 51 / 54 / 50 / 52 / 64; 64 x 8 of 2048 to 4096 159 / 150 / 151 / 148 / 161; 16 x 8 of 8192 to 16384
-    234 / 178 / 170 / 169 / 159). Few sequences and heads have sixteen (``cluster``: what the device has room for; 16 heads of 32768 with 8 / 16: 64 / 57), and very few
-    with long contexts more, whose parts a second kernel joins (8 heads with 8 / 16 / 24 / 40: 16384 tokens 29 / 23 / 21 / 23, 32768 55 / 40 / 38 / 39, 131072
-    213 / 132 / 107 / 106)."""
+    nine tenths of that, up to eight (us with 4 / 6 / 8: 8 x 8 heads of 1024 to 2048 tokens 17.2 / 15.4 / 20.8; 4 x 8 of 2048 to 4096 18.6 / 17.0 / 17.4). Where sequences and
+    heads fill most of the room by themselves, three even out what they differ by while all run at once, as does one where they do not and contexts are short; two or eight where they are long
+    (1 / 2 / 3 / 4 / 8: 32 x 8 heads of 1088 to 2175 tokens 49 / 48 / 44 / 46 / 59; 64 x 8 of 500 to 1000 43 / 47 / 51 / 55 / 85, of 2048 to 4096 142 / 138 / 139 / 139 / 152;
+    16 x 8 of 8192 to 16384 184 / 182 / 153 / 150 / 144; with 20 ``rows`` a head 32 x 8 of 1000 to 2000 86 / 84 / 75 / 80 / 105). Few sequences and heads have sixteen
+    (``cluster``: what the device has room for; 16 heads of 32768 with 8 / 16: 57 / 53), and very few with long contexts more, whose parts a second kernel joins (8 heads with
+    8 / 16 / 24 / 40: 16384 tokens 28 / 21 / 19 / 19, 32768 50 / 37 / 33 / 33, 131072 167 / 108 / 92 / 94)."""
     heads, pages = max(1, batch * n_kv), max(1, -(-max_kv_len // PAGE))
     most = max(1, pages // 8)
     if heads * cluster <= 2 * sm_count:
@@ -166,7 +167,9 @@ def weighed_splits(batch, n_kv, max_kv_len, sm_count=148, cluster=CLUSTER):
     fit = 27 * sm_count // (10 * heads)
     if fit > 3:
         return min(8 if fit > 6 else fit, most)
-    return max(1, min(8 if pages >= 768 else 4 if pages >= 192 else 3, pages // 32))
+    if pages >= 192:
+        return 8 if pages >= 768 else 2
+    return 3 if pages >= 96 and (heads <= 3 * sm_count or rows > 16) else 1
 
 
 def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len):
@@ -191,7 +194,7 @@ def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale,
     if total == 0 or most == 0:
         return out.zero_() if most == 0 else out
     sms, cluster = _device(dev)
-    splits = weighed_splits(B, n_kv, min(longest, window + q_per_seq + PAGE) if window > 0 else longest, sms, cluster)
+    splits = weighed_splits(B, n_kv, min(longest, window + q_per_seq + PAGE) if window > 0 else longest, sms, cluster, rows)
     room, pad = -(-longest // PAGE) * PAGE, (rows + 3) // 4 * 4
     # few scores stay in shared memory, where a third CTA of an SM would have nothing to do in any case: no scratch to allocate (1.7 us of the host's)
     at = part_o = part_ml = 0
