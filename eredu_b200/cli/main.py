@@ -91,6 +91,8 @@ def build_parser() -> argparse.ArgumentParser:
 def validate_args(a) -> None:
     if a.max_tokens <= 0:
         raise SystemExit("--max-tokens must be positive")
+    if a.kv_keep is not None and (a.kv_keep < 1 or a.kv_bits == 8):
+        raise SystemExit("--kv-keep is a number of tokens, of a cache that is not held in 8 bits")
     if a.dense_disk_stream and a.layerwise_host:
         raise SystemExit("--dense-disk-stream conflicts with --layerwise-host")
     if a.dense_disk_stream and (a.dense_host_lookahead < 1 or a.dense_background_queue < 1):

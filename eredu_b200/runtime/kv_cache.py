@@ -21,17 +21,19 @@ PAGE = 16
 @dataclass(frozen=True)
 class KeptTokens:
     """A bound for the cached tokens of a sequence (:mod:`eredu_b200.ops.eviction`): one that has grown to ``keep`` + ``slack`` tokens is brought down to ``keep`` -
-    the ``first`` ones, the ``recent`` last ones (half of all by default), and those that attention has given the most weight. ``observed`` > 0: of a prompt's portion
+    the ``first`` ones (four by default), the ``recent`` last ones (half of all by default), and those that attention has given the most weight. ``observed`` > 0: of a prompt's portion
     the last so many rows count, else all of them. ``slack``: a sixteenth of ``keep`` by default, a page at least."""
     keep: int
     recent: Optional[int] = None
-    first: int = 4
+    first: Optional[int] = None
     slack: Optional[int] = None
     observed: int = 0
 
     def __post_init__(self):
         if self.recent is None:
             object.__setattr__(self, "recent", self.keep // 2)
+        if self.first is None:
+            object.__setattr__(self, "first", max(0, min(4, self.keep - self.recent)))
         if self.slack is None:
             object.__setattr__(self, "slack", max(PAGE, self.keep // 16))
         if self.keep < 1 or self.recent < 0 or self.first < 0 or self.recent + self.first > self.keep or self.slack < 1 or self.observed < 0:

@@ -10,6 +10,7 @@ from eredu_b200.models.llama import build_from_tensors, random_state
 from eredu_b200.ops import SamplingParams
 from eredu_b200.runtime.engine import Engine
 from eredu_b200.runtime.kv_cache import PAGE, KeptTokens
+from eredu_b200.runtime.server import Server
 from eredu_b200.runtime.speculative import SpeculativeDecoder
 
 GREEDY = SamplingParams(temperature=0.0)
@@ -168,11 +169,38 @@ def test_continuations_of_a_prompt_have_pages_of_their_own():
     assert out[0] == out[1] == out[2] and len(out[0]) == 24
 
 
+def test_a_server_gives_what_a_batch_gives():
+    """Prompts in portions between other requests' steps, each with its own evictions."""
+    model = build()
+    rule = KeptTokens(keep=32, recent=12, slack=6)
+    prompts = [prompt(n, i) for i, n in enumerate((70, 9, 45))]
+    alone = [Engine(model, max_batch=1, max_seq_len=256, kv_keep=rule).generate([p], GREEDY, max_new_tokens=30)[0] for p in prompts]
+    server = Server(Engine(model, max_batch=2, max_seq_len=256, kv_keep=rule), prefill_chunk=16, max_step_tokens=40)
+    ids = [server.submit(p, GREEDY, 30) for p in prompts]
+    server.run_until_idle(max_steps=400)
+    assert [server.result(i).tokens for i in ids] == alone
+
+
+def test_command_line(tmp_path, capsys):
+    from eredu_b200.cli.main import build_parser, main, validate_args
+    from eredu_b200.formats import checkpoint
+    from test_text_streaming import make_bundle
+
+    for bad in (["--kv-keep", "0"], ["--kv-keep", "64", "--kv-bits", "8"]):
+        with pytest.raises(SystemExit):
+            validate_args(build_parser().parse_args(["-m", "x", "hi", *bad]))
+    bundle = make_bundle(tmp_path)
+    cfg = dataclasses.replace(C.tiny_llama(), vocab_size=bundle.vocab_size(), eos_token_id=bundle.eos_ids[0])
+    checkpoint.save_safetensors_checkpoint(tmp_path, cfg, random_state(cfg, seed=0, std=0.05), torch.float32)
+    assert main(["-m", str(tmp_path), "hello", "--device", "cpu", "-n", "40", "--kv-keep", "6"]) == 0
+    assert capsys.readouterr().out
+
+
 def test_bounds_are_checked():
     for wrong in (dict(keep=0), dict(keep=8, recent=6, first=4), dict(keep=8, slack=0), dict(keep=8, recent=-1), dict(keep=20, observed=-1)):
         with pytest.raises(ValueError):
             KeptTokens(**wrong)
-    assert KeptTokens(64).recent == 32 and KeptTokens(64).limit == 80 and KeptTokens(1024).slack == 64
+    assert KeptTokens(1).first == 1 and KeptTokens(6).first == 3 and KeptTokens(64).recent == 32 and KeptTokens(64).limit == 80 and KeptTokens(1024).slack == 64
 
 
 def test_what_does_not_go_with_a_bound_is_refused():
