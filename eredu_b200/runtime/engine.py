@@ -168,6 +168,8 @@ class Engine:
         hybrid = any(cfg.layer_is_mamba(li) or cfg.layer_is_kda(li) or cfg.layer_is_linear_attention(li) for li in layers)
         if own or hybrid or any(cfg.layer_window(li) for li in layers):
             raise NotImplementedError(f"{cfg.model_type}: caches that give up tokens are for layers of plain attention over the whole context")
+        if self.device.type == "cuda" and cfg.head_dim in ops.KERNEL_HEAD_DIMS and self.model.dtype != torch.bfloat16:
+            raise NotImplementedError(f"caches that give up tokens hold bf16 on a GPU, not {self.model.dtype}")
         if other:
             raise NotImplementedError("a cache that gives up tokens goes without prefix reuse, 8-bit pages and convolution states")
 

@@ -137,6 +137,8 @@ STEPS = [
     ((8, 2, 128), [600], 8, 0, False),
     ((16, 1, 128), [100, 6], 5, 0, True),
     ((33, 1, 64), [70], 1, 0, False),
+    ((8, 2, 128), [0, 30, 1], 1, 0, False),
+    ((16, 2, 64), [3, 0, 20], 5, 8, True),
 ]
 
 
