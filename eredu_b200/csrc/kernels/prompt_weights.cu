@@ -119,16 +119,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
   __syncthreads();
   for (int i = threadIdx.x; i < kPwTile; i += kPwThreads) *reinterpret_cast<uint2*>(one_s + pw_plain(i, 0)) = make_uint2(0x3F803F80u, 0x3F80u);
   fence_proxy_async_smem();
-  if (warp == 0) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = warp_uniform(*tmem_slot);
   pdl_wait();
-  pdl_launch_dependents();
 
   // (blocks of keys vary slowest: the first ones are seen by the most rows)
   const int h = static_cast<int>(blockIdx.x) / ranks, b = blockIdx.y, key0 = blockIdx.z * kPwKeys;
@@ -143,6 +134,17 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
   const int tile_tokens = kPwTile >> p.gshift, per_head = max(0, t1 - t0 + tile_tokens - 1) / tile_tokens;
   const int tiles = key0 < kv_len ? per_head * (p.group >> p.gshift) : 0;
   const int begin = static_cast<int>(static_cast<long long>(tiles) * rank / ranks), end = static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / ranks);
+  // nothing to do (the same for all CTAs of a cluster): behind the sequence's last token, or older tokens that no row sees
+  if (key0 >= kv_len || q_len <= 0 || (tiles == 0 && key0 + kPwKeys <= before)) return;
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = warp_uniform(*tmem_slot);
+  pdl_launch_dependents();                               // (behind the allocation: what comes next may want tensor memory too)
   // (tile i of the CTA: tokens from t0 + i / heads on, heads varying fastest, so that CTAs of one head read the same rows at about the same time)
   const int head_tiles = p.group >> p.gshift;
 
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kPwThreads, 1) prompt_weights_kernel(const __g
       asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(sum_s + at), r)) : "memory");
       total += v;
     }
-    if (key < kv_len && q_len > 0 && (tiles > 0 || key >= before)) {
+    if (key < kv_len && (tiles > 0 || key >= before)) {
       const int page = p.block_table[static_cast<size_t>(b) * p.wide + key / kPwPage];
       if (page >= 0 && page < p.num_pages) {
         float* at_w = p.weights + (static_cast<size_t>(page) * p.n_kv + h) * kPwPage + key % kPwPage;
