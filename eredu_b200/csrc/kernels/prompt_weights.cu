@@ -14,9 +14,9 @@
 // The CTAs of a cluster share the rows of the same keys; their sums are added up in the order of their ranks.
 //
 // Bound by exponentials, 2048 cycles of the special-function unit for a pair of tiles (the tensor core needs 1050), and by what each tile costs beside them: 4096 tokens, 32 heads
-// of 128 over 8, 105 us of the 244 that the call takes, 61 at the unit's rate. Left out in a copy for the time's sake, the exponentials take 32 us of it, the products of the tensor core 6;
+// of 128 over 8, 101 us of the 240 that the call takes, 61 at the unit's rate. Left out in a copy for the time's sake, the exponentials take 32 us of it, the products of the tensor core 6;
 // 60 are tiles without arithmetic - accumulators read, barriers - and 12 the start and the end of a CTA (one to an SM). Tiles of 64 rows with two CTAs to an SM measured
-// the same (257 -> 263 us before the steps above; 2048 tokens 91 -> 94), an issuer for each key tile 243 for 244.
+// the same (257 -> 263 us before the steps above; 2048 tokens 91 -> 94), an issuer for each key tile 243 for 244, old sums asked for by the producer 240 for 240.
 #include <cuda_bf16.h>
 
 #include <algorithm>
