@@ -174,7 +174,8 @@ def weighed_splits(batch, n_kv, max_kv_len, sm_count=148, cluster=CLUSTER, rows=
 
 def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len):
     """The form of :func:`.core.attention_decode` that keeps ``weights``. ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it (0: what
-    a row of the table holds); the call takes memory for the scores of so many tokens of every sequence."""
+    a row of the table holds); the call takes memory for the scores of so many tokens of every sequence. A sequence of length 0 - one that does not step - gives rows of
+    zeros and leaves all sums as they are."""
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale, window, sinks, weights, out, chunk, max_kv_len)

@@ -729,9 +729,14 @@ class Engine:
             st["all_greedy"] = greedy
             st["graph"] = st["graphs"].get(greedy)  # graphs are captured per sampler path
 
+    def _attended(self, st) -> torch.Tensor:
+        """Tokens that every row of the decode state attends to. Where weights are added up, a row that does not step - held back, finished, a free slot - has
+        none: it asks nothing, and must give its tokens no weight."""
+        return st["seq_lens"] if self.keep is None else st["seq_lens"] * st["active"]
+
     def _decode_body(self, st):
         batch = ForwardBatch(token_ids=st["token_ids"], positions=st["positions"], slots=st["slots"],
-                             block_table=st["block_table"], seq_lens=st["seq_lens"], is_prefill=False, q_per_seq=1,
+                             block_table=st["block_table"], seq_lens=self._attended(st), is_prefill=False, q_per_seq=1,
                              splits=st["splits"], scratch=st["scratch"], max_kv_len=st["max_len"], sm_count=self.sm_count)
         logits = self.model.forward(batch, self.kv)
         if logits is not None:
@@ -843,7 +848,7 @@ class Engine:
         idle = Sequence(0, [0], SamplingParams(temperature=0.0))
         seqs = [s if s is not None else idle for s in st["seqs"]]
         batch = ForwardBatch(token_ids=st["token_ids"], positions=st["positions"], slots=st["slots"],
-                             block_table=st["block_table"], seq_lens=st["seq_lens"], is_prefill=False, q_per_seq=1)
+                             block_table=st["block_table"], seq_lens=self._attended(st), is_prefill=False, q_per_seq=1)
         logits = self.model.forward(batch, self.kv)
         pos = st["positions"].tolist()
         toks = None
