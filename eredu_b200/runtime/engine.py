@@ -779,11 +779,16 @@ class Engine:
         the host->device copy of its inputs. With ``sync`` the sampled ids are copied back and returned.
         """
         st = self._decode_state
-        if self.keep is not None:
-            if st.get("uncommitted"):
-                raise RuntimeError("a bounded cache goes by what commit() has recorded: every step is committed ahead of the next one")
-            self._shrink_decoding(st)
-            st["uncommitted"] = True
+        if self.keep is None:
+            return self._run_step(st, host_tokens, sync)
+        if st.get("uncommitted"):
+            raise RuntimeError("a bounded cache goes by what commit() has recorded: every step is committed ahead of the next one")
+        self._shrink_decoding(st)
+        tokens = self._run_step(st, host_tokens, sync)
+        st["uncommitted"] = True             # (a step that raises leaves nothing to commit)
+        return tokens
+
+    def _run_step(self, st, host_tokens, sync):
         if not self.cuda:
             with nvtx.annotate("decode_step"):
                 return self._decode_step_cpu(st)

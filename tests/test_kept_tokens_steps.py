@@ -92,3 +92,42 @@ def test_a_budget_that_holds_rows_back_changes_no_answer(budget, chunk, seed):
     ids = [server.submit(p, GREEDY, 60) for p in prompts]
     server.run_until_idle(max_steps=2000)
     assert [server.result(i).tokens for i in ids] == alone
+
+
+def failing(eng, monkeypatch, at):
+    """The ``at``-th forward pass from now on raises."""
+    forward, count = eng.model.forward, [0]
+
+    def once(*a, **k):
+        count[0] += 1
+        if count[0] == at:
+            raise RuntimeError("a step that fails")
+        return forward(*a, **k)
+
+    monkeypatch.setattr(eng.model, "forward", once)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_that_fails_is_not_one_to_commit(device, monkeypatch):
+    eng = Engine(build(device), max_batch=1, max_seq_len=128, kv_keep=64, use_cuda_graph=False)
+    joined(eng, prompt(10))
+    failing(eng, monkeypatch, 2)
+    step(eng, [True])
+    with pytest.raises(RuntimeError, match="fails"):
+        eng.decode_step()
+    step(eng, [True])
+    eng.decode_step()
+    with pytest.raises(RuntimeError, match="committed"):
+        eng.decode_step()
+
+
+def test_a_server_goes_on_after_a_step_that_fails(monkeypatch):
+    model = build()
+    alone = Engine(model, max_batch=1, max_seq_len=128, kv_keep=64).generate([prompt(12, 1)], GREEDY, max_new_tokens=10)[0]
+    server = Server(Engine(model, max_batch=2, max_seq_len=128, kv_keep=64))
+    failing(server.engine, monkeypatch, 3)
+    first = server.submit(prompt(10), GREEDY, 10)
+    server.run_until_idle(max_steps=100)
+    second = server.submit(prompt(12, 1), GREEDY, 10)
+    server.run_until_idle(max_steps=100)
+    assert server.result(first).failed and not server.result(second).failed and server.result(second).tokens == alone
