@@ -173,11 +173,16 @@ class Engine:
         if other:
             raise NotImplementedError("a cache that gives up tokens goes without prefix reuse, 8-bit pages and convolution states")
 
+    def _over(self, seq: Sequence, new: int) -> bool:
+        """Whether a sequence is brought down ahead of ``new`` more tokens."""
+        rule = self.keep
+        return rule is not None and seq.cached > rule.keep and seq.cached + new > rule.limit
+
     def _shrink(self, seqs, new: int = 1) -> list:
         """Brings those of ``seqs`` down to ``keep.keep`` tokens that ``new`` more would take behind their bound; pages that a sequence cannot need any more go back to
         the pool. Returns them."""
         rule = self.keep
-        some = [s for s in seqs if s.cached > rule.keep and s.cached + new > rule.limit] if rule is not None else []
+        some = [s for s in seqs if self._over(s, new)]
         if some:
             held = [s.cached for s in some]
             table, lens = self._block_table(some), self._t(np.asarray(held, dtype=np.int32), torch.int32)
@@ -579,9 +584,13 @@ class Engine:
         token, -1 for text: tokens of a group attend to each other in both directions) for prompts with images; it sets
         ``seq.rope_delta`` so that later text tokens continue after the largest position the images used."""
         n = len(tokens)
-        self._shrink([seq], n)
-        if self.keep is not None and seq.cached + n > len(seq.pages) * PAGE:
-            raise ValueError(f"{n} tokens behind {seq.cached} are more than the cache's bound of {self.keep.limit} has room for")
+        if self.keep is not None:
+            held, room = seq.cached, len(seq.pages)
+            if self._over(seq, n):
+                held, room = self.keep.keep, min(room, PagedKVCache.pages_for(self.keep.limit))
+            if held + n > room * PAGE:
+                raise ValueError(f"{n} tokens behind {held} are more than the cache's bound of {self.keep.limit} has room for")
+            self._shrink([seq], n)
         p = np.arange(seq.kv_len, seq.kv_len + n)
         at = p - seq.evicted
         pages = np.asarray(seq.pages, dtype=np.int64)

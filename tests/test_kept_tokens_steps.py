@@ -131,3 +131,16 @@ def test_a_server_goes_on_after_a_step_that_fails(monkeypatch):
     second = server.submit(prompt(12, 1), GREEDY, 10)
     server.run_until_idle(max_steps=100)
     assert server.result(first).failed and not server.result(second).failed and server.result(second).tokens == alone
+
+
+def test_a_continuation_that_is_refused_changes_nothing():
+    """No token is given up for a call that then raises."""
+    eng = Engine(build(), max_batch=1, max_seq_len=256, kv_keep=KeptTokens(keep=32, recent=8, slack=16))
+    seq = eng.new_sequence(prompt(40), GREEDY, max_new_tokens=100)
+    eng.feed_logits(seq, prompt(40))
+    before, pages = sums(eng, seq), list(seq.pages)
+    with pytest.raises(ValueError):
+        eng.feed_logits(seq, prompt(60, 2))
+    assert seq.cached == seq.kv_len == 40 and seq.evicted == 0 and seq.pages == pages and torch.equal(sums(eng, seq), before)
+    eng.feed_logits(seq, prompt(12, 3))                      # 32 + 12 find room
+    assert seq.kv_len == 52 and seq.cached == 44
