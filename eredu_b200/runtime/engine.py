@@ -246,10 +246,11 @@ class Engine:
         return seq
 
     def _reserve(self, seq: Sequence, total: int) -> None:
-        """Pages (and, with the first one, a recurrent-state slot) for ``total`` tokens."""
+        """Pages (and, with the first one, a recurrent-state slot) for ``total`` tokens, less those that a bounded cache gives up ahead of them."""
         if total > self.max_seq_len:
             raise ValueError(f"{total} tokens exceed max_seq_len {self.max_seq_len}")
-        need = PagedKVCache.pages_for(total) - len(seq.pages)
+        self._shrink([seq], total - seq.kv_len)
+        need = PagedKVCache.pages_for(total - seq.evicted) - len(seq.pages)
         if need <= 0:
             return
         fresh = self.kv.alloc(need)

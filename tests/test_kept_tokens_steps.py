@@ -144,3 +144,25 @@ def test_a_continuation_that_is_refused_changes_nothing():
     assert seq.cached == seq.kv_len == 40 and seq.evicted == 0 and seq.pages == pages and torch.equal(sums(eng, seq), before)
     eng.feed_logits(seq, prompt(12, 3))                      # 32 + 12 find room
     assert seq.kv_len == 52 and seq.cached == 44
+
+
+def test_single_tokens_of_many_sequences_stay_within_the_bound():
+    """``forward_tokens`` of sequences with a reservation: the same logits as one by one, and no more pages than the bound has."""
+    rule = KeptTokens(keep=32, recent=8, slack=8)
+    logits, pages = [], []
+    for together in (False, True):
+        eng = Engine(build(), max_batch=2, max_seq_len=256, kv_keep=rule)
+        seqs = [eng.new_sequence(prompt(n, n), GREEDY, max_new_tokens=100) for n in (50, 36)]
+        for s in seqs:
+            eng.feed_logits(s, s.prompt)
+        rows = []
+        for t in range(30):
+            if together:
+                rows.append(eng.forward_tokens([(s, [t + i], [0]) for i, s in enumerate(seqs)]))
+            else:
+                rows.append(torch.stack([eng.feed_logits(s, [t + i]) for i, s in enumerate(seqs)]))
+        assert [s.kv_len for s in seqs] == [80, 66] and all(s.cached <= rule.limit for s in seqs)
+        logits.append(torch.stack(rows))
+        pages.append([len(s.pages) for s in seqs])
+    assert pages == [[3, 3], [3, 3]]
+    assert torch.allclose(*logits, rtol=1e-4, atol=1e-4)
