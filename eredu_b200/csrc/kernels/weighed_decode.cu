@@ -9,8 +9,8 @@
 // [16][64] with the 128-byte swizzle that ldmatrix reads without conflicts). Scores come as S^T = K Q^T (mma.sync m16n8k16: the sixteen keys of a page by eight rows, so
 // that the four to eight rows of a group fill the narrow side), and so does O^T = V^T P^T: a lane has two rows in both, whose maxima rescale its own accumulators. The
 // row maximum is a bound that is moved when a score is above it by more than 2^8: most pages need no exchange between lanes.
-// The splits of a sequence and head (up to sixteen) are a cluster: maxima, sums and outputs meet in shared memory, and every CTA weighs its own tokens. More splits leave
-// their part in memory, and a second kernel does the same. Up to sixteen rows that share a head are a warp's; with more, two or four warps walk the same pages with
+// The splits of a sequence and head (up to sixteen, or to the largest cluster that the device has room for) are a cluster: maxima, sums and outputs meet in shared memory, and
+// every CTA weighs its own tokens. More splits leave their part in memory, and a second kernel does the same. Up to sixteen rows that share a head are a warp's; with more, two or four warps walk the same pages with
 // sixteen rows each.
 //
 // Measured (floor: K, V and weights at 6.54 TB/s): 64 sequences of 2048 to 4096 tokens, 32 heads of 128 over 8, 134 us (floor 124, 6.1 TB/s); 32 of 1088 to 2175 42 us
@@ -600,7 +600,7 @@ extern "C" int eredu_weighed_decode(const void* args, int bytes) {
   if (!weights_args(a, args, bytes)) return -2;
   if (a.batch <= 0 || a.q_per_seq <= 0) return 0;
   if ((a.D != 64 && a.D != 128) || a.n_kv <= 0 || a.n_q % a.n_kv != 0 || a.num_pages <= 0 || a.batch > 65535 || a.n_kv > 65535 || a.splits < 1 ||
-      a.splits > kWdMaxSplits || a.window < 0 || a.room <= 0 || a.room % kWdPage != 0 || (a.splits > kWdCluster) != (a.part_o != nullptr))
+      a.splits > kWdMaxSplits || a.window < 0 || a.room <= 0 || a.room % kWdPage != 0 || (a.part_o != nullptr ? a.splits < 2 || a.part_ml == nullptr : a.splits > kWdCluster))
     return -2;
   WdParams p = {};
   p.group = a.n_q / a.n_kv;

@@ -27,7 +27,7 @@ from .native import check, lib, status_word, stream_ptr
 PAGE = 16
 HEAD_DIMS = (64, 128)        # head sizes of the kernels
 DECODE_ROWS = 64             # query rows that share a head in the decode kernel; more go to the prefill kernels
-CLUSTER = 16                 # splits of a sequence and head that meet in a cluster
+CLUSTER = 16                 # splits of a sequence and head that meet in a cluster, where the device has room for one of so many
 MAX_SPLITS = 64
 HELD_SCORES = 16 << 10       # bytes of scores that a CTA of the decode kernel may hold in shared memory
 HELD_TOKENS = 48 * 1024      # longest sequence whose weights the eviction kernel holds in shared memory
@@ -199,8 +199,9 @@ def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale,
     room, pad = -(-longest // PAGE) * PAGE, (rows + 3) // 4 * 4
     # few scores stay in shared memory, where a third CTA of an SM would have nothing to do in any case: no scratch to allocate (1.7 us of the host's)
     at = part_o = part_ml = 0
-    if splits > CLUSTER or B * n_kv * splits > 2 * sms or -(-room // (PAGE * splits)) * PAGE * pad * 4 > HELD_SCORES:
-        scored, parts = B * n_kv * room * pad, B * n_kv * splits * rows if splits > CLUSTER else 0
+    joined = splits > cluster                # a second kernel joins what so many splits leave in memory
+    if joined or B * n_kv * splits > 2 * sms or -(-room // (PAGE * splits)) * PAGE * pad * 4 > HELD_SCORES:
+        scored, parts = B * n_kv * room * pad, B * n_kv * splits * rows if joined else 0
         scratch = torch.empty(scored + parts * (dim + 2), dtype=torch.float32, device=dev)
         at = scratch.data_ptr()
         if parts:

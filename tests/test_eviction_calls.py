@@ -1,0 +1,63 @@
+"""Calls of attention with weights that are rare: other devices' limits, odd windows, scales and lengths, and what must not be touched."""
+import pytest
+import torch
+
+from eredu_b200 import ops
+from eredu_b200.ops import eviction
+from test_eviction import arguments, attended, cache, compare, layout
+
+PAGE = eviction.PAGE
+
+
+def packed(monkeypatch, cluster, sms=148):
+    """Arguments of the decode kernel as the host packs them, on a device whose largest cluster is ``cluster``; nothing is launched."""
+    calls = []
+
+    class Lib:
+        @staticmethod
+        def eredu_weighed_decode(block, size):
+            names = ("q", "k", "v", "out", "table", "lens", "sinks", "weights", "scores", "part_o", "part_ml", "status", "stream", "batch", "q_per_seq", "pitch",
+                     "max_tokens", "room", "pages", "n_q", "n_kv", "D", "splits", "window", "scale")
+            calls.append(dict(zip(names, eviction._DECODE.unpack(block))))
+            return 0
+
+    monkeypatch.setattr(eviction, "lib", Lib)
+    monkeypatch.setattr(eviction, "_device", lambda device: (sms, cluster))
+    monkeypatch.setattr(eviction, "_kernels_take", lambda *a: True)
+    monkeypatch.setattr(eviction, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(eviction, "stream_ptr", lambda device: 0)
+    return calls
+
+
+# ------------------------------------------------------------------------------------------ clusters
+@pytest.mark.parametrize("cluster", [8, 16])
+def test_splits_are_a_cluster_that_the_device_has_room_for_or_leave_parts(monkeypatch, cluster):
+    """More splits than the device's largest cluster leave their parts in memory, whatever their number."""
+    calls = packed(monkeypatch, cluster)
+    seen = set()
+    for heads in range(1, 41):
+        for pages in (64, 1024, 4096):
+            k = torch.empty((1, heads, PAGE, 64), dtype=torch.bfloat16)
+            table = torch.zeros((1, pages), dtype=torch.int32)
+            q = torch.empty((1, heads, 64), dtype=torch.bfloat16)
+            ops.attention_decode(q, k, k, table, torch.tensor([pages * PAGE], dtype=torch.int32), 1, 0.1, weights=torch.empty((1, heads, PAGE)))
+            call = calls.pop()
+            joined = call["splits"] > cluster
+            assert (call["part_o"] != 0) == (call["part_ml"] != 0) == joined and (call["scores"] != 0 or not joined)
+            seen.add(call["splits"])
+    assert any(s > cluster for s in seen) and any(1 < s <= cluster for s in seen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, lens, new", [((14, 14, 64), [16500], 1), ((24, 12, 128), [16400], 3), ((16, 8, 128), [700, 40], 1)])
+def test_step_on_a_device_without_large_clusters(monkeypatch, heads, lens, new):
+    monkeypatch.setattr(eviction, "_device", lambda device: (148, 8))
+    n_q, n_kv, dim = heads
+    num, table = layout(lens, "cuda", wider=2)
+    k, v, w = cache(num, n_kv, dim, "cuda")
+    q = torch.randn((len(lens) * new, n_q, dim), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    before, scale = w.clone(), dim ** -0.5
+    out = ops.attention_decode(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), new, scale, weights=w, max_kv_len=max(lens))
+    expect = attended(q, k, v, table, lens, [new] * len(lens), scale)
+    compare(out, w, before, expect, dim, new * n_q // n_kv, True)
+    ops.native.check_status(torch.device("cuda", 0))
