@@ -551,16 +551,23 @@ __global__ void __launch_bounds__(kWdJoinThreads) weighed_join_kernel(const WdPa
   wd_weigh(p, s, scores, b, h, s_top, s_inv, kWdJoinThreads, cells);
 }
 
+// What every launch of a kernel may want, whoever asks first.
 template <int D, int NT, int RG>
-static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdParams& p, int batch, int held, cudaStream_t stream) {
+static bool wd_configure() {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT, RG>() + kWdHeld) != cudaSuccess) return -1;
-    if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -1;
-    configured[dev] = true;
-  }
+  if (dev >= 0 && dev < 64 && configured[dev]) return true;
+  if (cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<D, NT, RG>() + kWdHeld) != cudaSuccess ||
+      cudaFuncSetAttribute(weighed_decode_kernel<D, NT, RG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return false;
+  if (dev >= 0 && dev < 64) configured[dev] = true;
+  return true;
+}
+
+template <int D, int NT, int RG>
+static int wd_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const WdParams& p, int batch, int held, cudaStream_t stream) {
+  if (!wd_configure<D, NT, RG>()) return -1;
   const bool cluster = p.part_o == nullptr && p.splits > 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.splits, p.n_kv, batch);
@@ -652,7 +659,7 @@ extern "C" int eredu_weighed_clusters() {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kWdCluster);
   cfg.blockDim = dim3(32 * kWdWarps);
-  cfg.dynamicSmemBytes = wd_smem<128, 2, 1>();
+  cfg.dynamicSmemBytes = wd_smem<128, 2, 1>() + kWdHeld;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kWdCluster;
@@ -660,9 +667,7 @@ extern "C" int eredu_weighed_clusters() {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaFuncSetAttribute(weighed_decode_kernel<128, 2, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, wd_smem<128, 2, 1>()) != cudaSuccess ||
-      cudaFuncSetAttribute(weighed_decode_kernel<128, 2, 1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, weighed_decode_kernel<128, 2, 1>, &cfg) != cudaSuccess) {
+  if (!wd_configure<128, 2, 1>() || cudaOccupancyMaxActiveClusters(&n, weighed_decode_kernel<128, 2, 1>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }

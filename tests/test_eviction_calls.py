@@ -61,3 +61,18 @@ def test_step_on_a_device_without_large_clusters(monkeypatch, heads, lens, new):
     expect = attended(q, k, v, table, lens, [new] * len(lens), scale)
     compare(out, w, before, expect, dim, new * n_q // n_kv, True)
     ops.native.check_status(torch.device("cuda", 0))
+
+
+@pytest.mark.gpu
+def test_asking_for_clusters_leaves_the_kernels_as_they_are():
+    """The question may come behind launches (two threads' first calls): those with scores in shared memory, which take the most of it, go on."""
+    num, table = layout([500], "cuda")
+    k, v, w = cache(num, 1, 128, "cuda")
+    q = torch.randn((1, 16, 128), generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    lens = torch.tensor([500], dtype=torch.int32, device="cuda")
+    outs = []
+    for _ in range(2):
+        own = w.clone()
+        outs.append((ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=own, max_kv_len=500), own))
+        assert ops.native.lib().eredu_weighed_clusters() in (0, 1)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
