@@ -640,6 +640,7 @@ static int attn_prefill_tc_impl(const void* q, const void* k_cache, const void* 
   if (key_dim <= 0 || key_dim > 128 || key_dim % 8 != 0 || value_dim <= 0 || value_dim > 128 || value_dim % 8 != 0 || batch <= 0 ||
       total_q <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || window < 0 || chunk < 0)
     return -2;
+  if (pool == 0 && window / 16 >= max_pages) window = 0;                // wider than any sequence: hides nothing, and sums with it stay within 32 bits
   const uint64_t D = static_cast<uint64_t>(key_dim), V = static_cast<uint64_t>(value_dim);
   CUtensorMap tmQ, tmK, tmV;
   // Short portions (see SPLIT above the kernel): heads of 64 or 128, no chunks or pooled blocks, a context that the host has stated.

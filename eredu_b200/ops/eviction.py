@@ -119,6 +119,11 @@ def _check_table(block_table, seq_lens, dev) -> None:
         raise ValueError("block_table: int32 rows, one per sequence")
 
 
+def _narrow(window, tokens) -> int:
+    """A window that no sequence of ``tokens`` fills hides nothing (0): what the kernels add to one stays within 32 bits."""
+    return window if window < tokens else 0
+
+
 def weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, scale, window=0, sinks=None, weights=None, observed=0, out=None):
     """Attention of the last ``q_lens[b]`` tokens of every sequence, by tensor operations, with ``weights`` kept as above. ``observed`` > 0: the last so many
     rows of a sequence count. A row that sees nothing gives zeros."""
@@ -187,6 +192,7 @@ def weighed_decode(q, k_cache, v_cache, block_table, seq_lens, q_per_seq, scale,
     dev, most = q.device, block_table.shape[1] * PAGE
     rows = q_per_seq * (n_q // n_kv)
     longest = max_kv_len if 0 < max_kv_len < most else most
+    window = _narrow(window, most)
     if rows > DECODE_ROWS:
         cu_q = torch.arange(0, (B + 1) * q_per_seq, q_per_seq, dtype=torch.int32, device=dev)
         return weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, q_per_seq, scale, window, sinks, weights, out, 0, longest, 0)
@@ -252,6 +258,7 @@ def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len,
         out = torch.empty_like(q)
     if total == 0 or B == 0 or wide == 0:
         return out
+    window = _narrow(window, wide * PAGE)
     longest, sms = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE, _device(dev)[0]
     lse = torch.empty(total * n_q, dtype=torch.float32, device=dev)
     code = lib().eredu_weighed_prefill(_PROMPT.pack(

@@ -76,3 +76,41 @@ def test_asking_for_clusters_leaves_the_kernels_as_they_are():
         outs.append((ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=own, max_kv_len=500), own))
         assert ops.native.lib().eredu_weighed_clusters() in (0, 1)
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+# ------------------------------------------------------------------------------------------ windows
+WIDE = [2 ** 31 - 1, 2 ** 31 - 200, 2 ** 31, 2 ** 40]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("window", WIDE)
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_window_wider_than_any_sequence_hides_nothing(device, window, new):
+    """Some configurations write "none" so. Steps, steps of so many rows that they go to the prompt's kernels, and prompts: bit by bit what no window gives."""
+    lens = [300, 50]
+    num, table = layout(lens, device)
+    k, v, w = cache(num, 2, 64, device)
+    q = torch.randn((2 * new, 8, 64), generator=torch.Generator().manual_seed(3)).bfloat16().to(device)
+    at = torch.tensor(lens, dtype=torch.int32, device=device)
+    cu = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=device)
+    for call in (lambda w, window: ops.attention_decode(q, k, v, table, at, new, 0.125, window=window, weights=w, max_kv_len=300),
+                 lambda w, window: ops.attention_prefill(q, k, v, table, at, cu, new, 0.125, window=window, weights=w, max_kv_len=300),
+                 lambda w, window: ops.attention_prefill(q, k, v, table, at, cu, new, 0.125, window=window, weights=w, observed=3)):
+        got = []
+        for hide in (0, window):
+            own = w.clone()
+            got.append((call(own, hide), own))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_windows_that_the_kernels_are_given_are_narrower_than_the_table(monkeypatch):
+    """Sums of a position and a window then stay within 32 bits."""
+    calls = packed(monkeypatch, 16)
+    prompts = []
+    monkeypatch.setattr(eviction.lib, "eredu_weighed_prefill", staticmethod(lambda block, size: prompts.append(eviction._PROMPT.unpack(block)) or 0), raising=False)
+    q, k, v, w, table, lens = arguments()
+    for window in (0, 5, 31, 32, 33, *WIDE):
+        ops.attention_decode(q, k, v, table, lens, 1, 0.1, window=window, weights=w)
+        ops.attention_prefill(q, k, v, table, lens, torch.tensor([0, 1, 2], dtype=torch.int32), 1, 0.1, window=window, weights=w)
+        want = window if window < 32 else 0
+        assert calls.pop()["window"] == want and prompts.pop()[12 + 9] == want
