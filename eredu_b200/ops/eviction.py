@@ -249,7 +249,10 @@ def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len,
     if not kernels:
         return weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, (cu_q[1:] - cu_q[:-1]).tolist(), scale, window, sinks, weights, observed, out)
     if not scale > 0:
-        raise ValueError(f"the kernels of prompts take scales above zero, not {scale}")
+        if scale != scale:
+            raise ValueError(f"a scale of {scale}")
+        # the kernels take scales above zero: the sign goes to the queries, or they are nothing (bf16 holds both without rounding)
+        q, scale = (-q, -scale) if scale < 0 else (q * 0, 1.0)
     total, n_q, dim = q.shape
     pages, n_kv = k_cache.shape[:2]
     block_table = block_table.contiguous()

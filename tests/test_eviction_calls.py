@@ -114,3 +114,28 @@ def test_windows_that_the_kernels_are_given_are_narrower_than_the_table(monkeypa
         ops.attention_prefill(q, k, v, table, lens, torch.tensor([0, 1, 2], dtype=torch.int32), 1, 0.1, window=window, weights=w)
         want = window if window < 32 else 0
         assert calls.pop()["window"] == want and prompts.pop()[12 + 9] == want
+
+
+# ------------------------------------------------------------------------------------------ scales
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, -0.0])
+@pytest.mark.parametrize("new", [3, 40])
+def test_scales_of_zero_and_below(device, scale, new):
+    """What the decode form takes is taken with any number of rows, and by the prompt form."""
+    lens, dim = [200, 41], 64
+    num, table = layout(lens, device)
+    k, v, w = cache(num, 2, dim, device)
+    q = torch.randn((2 * new, 8, dim), generator=torch.Generator().manual_seed(4)).bfloat16().to(device)
+    at = torch.tensor(lens, dtype=torch.int32, device=device)
+    cu = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=device)
+    expect = attended(q, k, v, table, lens, [new, new], scale)
+    for call in (lambda w: ops.attention_decode(q, k, v, table, at, new, scale, weights=w), lambda w: ops.attention_prefill(q, k, v, table, at, cu, new, scale, weights=w)):
+        own = w.clone()
+        compare(call(own), own, w, expect, dim, new * 4, device == "cuda")
+
+
+def test_a_scale_that_is_no_number_is_refused(monkeypatch):
+    packed(monkeypatch, 16)
+    q, k, v, w, table, lens = arguments()
+    with pytest.raises(ValueError):
+        ops.attention_prefill(q, k, v, table, lens, torch.tensor([0, 1, 2], dtype=torch.int32), 1, float("nan"), weights=w)
