@@ -260,7 +260,7 @@ def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len,
     if out is None:
         out = torch.empty_like(q)
     if total == 0 or B == 0 or wide == 0:
-        return out
+        return out.zero_() if wide == 0 else out
     window = _narrow(window, wide * PAGE)
     longest, sms = min(max_kv_len, wide * PAGE) if max_kv_len > 0 else wide * PAGE, _device(dev)[0]
     lse = torch.empty(total * n_q, dtype=torch.float32, device=dev)

@@ -139,3 +139,21 @@ def test_a_scale_that_is_no_number_is_refused(monkeypatch):
     q, k, v, w, table, lens = arguments()
     with pytest.raises(ValueError):
         ops.attention_prefill(q, k, v, table, lens, torch.tensor([0, 1, 2], dtype=torch.int32), 1, float("nan"), weights=w)
+
+
+# ------------------------------------------------------------------------------------------ rows that see nothing
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_tables_without_pages_give_zeros(monkeypatch, device):
+    """Steps and prompts over no pages at all: no row sees a token."""
+    k, v, w = cache(3, 2, 64, device)
+    if device == "cpu":
+        packed(monkeypatch, 16)                              # the checks and the allocation in front of the kernels
+        real = torch.empty_like
+        monkeypatch.setattr(torch, "empty_like", lambda t: real(t).fill_(float("nan")))
+    before = w.clone()
+    q = torch.ones((2, 4, 64), dtype=torch.bfloat16, device=device)
+    table, lens, cu = (torch.zeros(s, dtype=torch.int32, device=device) for s in ((2, 0), (2,), (3,)))
+    cu[1:] = torch.tensor([1, 2])
+    for out in (None, torch.full_like(q, 3)):
+        for got in (ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=w, out=out), ops.attention_prefill(q, k, v, table, lens, cu, 1, 0.1, weights=w, out=out)):
+            assert bool((got == 0).all()) and torch.equal(w, before)
