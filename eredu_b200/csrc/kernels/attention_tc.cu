@@ -175,9 +175,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   if (row0 >= q_len) return;                                            // uniform: before any barrier or allocation
   const int kv_head = head / (p.n_q_heads / p.n_kv_heads);
   const int pos0 = kv_len - q_len + row0;                               // position of the CTA's first query row
-  // causal: nothing beyond the position of a tile's last row
-  int n_a = min(kv_len - 1, pos0 + tile_tokens - 1) / kTcTile + 1;
-  int n_b = row0 + tile_tokens < q_len ? min(kv_len - 1, pos0 + 2 * tile_tokens - 1) / kTcTile + 1 : 0;
+  // causal: nothing beyond the position of a tile's last row (rows in front of the first token, of a sequence shorter than its rows, walk a
+  // tile that is masked for them, and give zeros: without one, waits would have nothing to wait for)
+  int n_a = max(0, min(kv_len - 1, pos0 + tile_tokens - 1)) / kTcTile + 1;
+  int n_b = row0 + tile_tokens < q_len ? max(0, min(kv_len - 1, pos0 + 2 * tile_tokens - 1)) / kTcTile + 1 : 0;
   int n_tiles = max(n_a, n_b);
   // window / chunk: key tiles that lie wholly before what a tile's FIRST row sees are skipped
   int j0_a = tc_lowest_key(p, pos0) / kTcTile;

@@ -157,3 +157,21 @@ def test_tables_without_pages_give_zeros(monkeypatch, device):
     for out in (None, torch.full_like(q, 3)):
         for got in (ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=w, out=out), ops.attention_prefill(q, k, v, table, lens, cu, 1, 0.1, weights=w, out=out)):
             assert bool((got == 0).all()) and torch.equal(w, before)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("lens, new", [([0, 5, 310], 300), ([0], 600), ([45, 256, 0], 300), ([44, 700], 300), ([1, 128], 129)])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_sequences_shorter_than_their_rows(device, lens, new, sinks):
+    """Many rows a head, the first of which stand in front of a sequence's first token: they see nothing and give zeros, the others are as ever."""
+    num, table = layout(lens, device, wider=1)
+    k, v, w = cache(num, 2, 64, device)
+    q = torch.randn((len(lens) * new, 4, 64), generator=torch.Generator().manual_seed(5)).bfloat16().to(device)
+    sink = torch.randn(4, generator=torch.Generator().manual_seed(6)).to(device) if sinks else None
+    expect = attended(q, k, v, table, lens, [new] * len(lens), 0.125, sinks=sink)
+    for known in (0, max(lens)):
+        own = w.clone()
+        out = ops.attention_decode(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=device), new, 0.125, sinks=sink, weights=own, max_kv_len=known)
+        compare(out, own, w, expect, 64, new * 2, device == "cuda")
+    if device == "cuda":
+        ops.native.check_status(torch.device("cuda", 0))
