@@ -170,7 +170,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   const int b = blockIdx.z, head = SPLIT ? static_cast<int>(blockIdx.x) / nsplit << gs : blockIdx.x, qt = tc_query_tile(p, gridDim.y, blockIdx.y);
   const int4 seq = ROWS ? p.table[b] : make_int4(p.cu_q[b], p.cu_q[b + 1] - p.cu_q[b], 0, p.seq_lens[b]);
   // (the same in all lanes for the compiler too: loops of the issuing warps hang on them)
-  const int q0 = static_cast<int>(warp_uniform(seq.x)), q_len = static_cast<int>(warp_uniform(seq.y)), kv_len = static_cast<int>(warp_uniform(seq.w));
+  const int q0 = static_cast<int>(warp_uniform(seq.x)), q_len = static_cast<int>(warp_uniform(seq.y));
+  const int kv_len = min(static_cast<int>(warp_uniform(seq.w)), ROWS ? 0x7fffffff : p.max_pages * 16);     // no more than the sequence's row of the table holds
   const int row0 = qt * 2 * tile_tokens;
   if (row0 >= q_len) return;                                            // uniform: before any barrier or allocation
   const int kv_head = head / (p.n_q_heads / p.n_kv_heads);

@@ -175,3 +175,53 @@ def test_sequences_shorter_than_their_rows(device, lens, new, sinks):
         compare(out, own, w, expect, 64, new * 2, device == "cuda")
     if device == "cuda":
         ops.native.check_status(torch.device("cuda", 0))
+
+
+# ------------------------------------------------------------------------------------------ what must not be touched
+CALLS = {
+    "step": lambda q, k, v, w, table, lens, cu: ops.attention_decode(q, k, v, table, lens, 1, 0.1, weights=w),
+    "prompt": lambda q, k, v, w, table, lens, cu: ops.attention_prefill(q, k, v, table, lens, cu, 1, 0.1, weights=w),
+    "evict": lambda q, k, v, w, table, lens, cu: ops.evict_tokens(k[None], v[None], w[None], table, lens, 8),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", CALLS)
+@pytest.mark.parametrize("fault", ["length", "page behind the pool", "page before it"])
+def test_what_the_table_does_not_name_stays_as_it_is(what, fault):
+    """A length beyond the table's row, or a page that is none, is reported; pages that the sequences do not have are what they were, bit by bit."""
+    q, k, v, w, table, lens = arguments("cuda", 128)
+    table = table.clone()
+    if fault == "length":
+        lens = lens + torch.tensor([100, 0], dtype=torch.int32, device="cuda")
+    else:
+        table[0, 1] = 1 << 20 if "behind" in fault else -3
+    mine = [int(p) for p in table.flatten().tolist() if 0 < p < k.shape[0]]
+    others = [p for p in range(k.shape[0]) if p not in mine]
+    assert others
+    before = [x[others].clone() for x in (k, v, w)]
+    CALLS[what](q, k, v, w, table, lens, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="bad argument"):
+        ops.native.check_status(torch.device("cuda", 0))
+    assert all(torch.equal(x[others], old) for x, old in zip((k, v, w), before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["step", "prompt"])
+@pytest.mark.parametrize("beyond", [1, 100, 1 << 24])
+def test_lengths_beyond_the_table_are_taken_as_what_it_holds(what, beyond):
+    """Attention and weights go by the same length."""
+    q, k, v, w, table, lens = arguments("cuda", 128)
+    q = torch.randn(q.shape, generator=torch.Generator().manual_seed(7)).bfloat16().cuda()
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    most = table.shape[1] * PAGE
+    got = []
+    for length in (most, most + beyond):
+        own, at = w.clone(), lens.clone()
+        at[0] = length
+        got.append((CALLS[what](q, k, v, own, table, at, cu), own))
+        if length > most:
+            with pytest.raises(RuntimeError, match="bad argument"):
+                ops.native.check_status(torch.device("cuda", 0))
+        ops.native.check_status(torch.device("cuda", 0))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
