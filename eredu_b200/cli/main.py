@@ -316,10 +316,10 @@ def main(argv=None) -> int:
         context = max(4096, a.max_tokens + 2048)
         hw = HardwareProfile.discover() if device != "cpu" else HardwareProfile(device_count=1, device_memory_bytes=1 << 62, name="cpu")
         hw.device_count = 1     # the command-line front end drives one device; multi-GPU runs use the library API
-        prof = estimate_runtime_state(report.config, report.tensor_bytes, kv_bits=a.kv_bits)
+        prof = estimate_runtime_state(report.config, report.tensor_bytes, kv_bits=a.kv_bits, weighed=a.kv_keep is not None)
         feedback = read_feedback(a.auto_feedback)
         cache_path = a.auto_cache
-        key = f"{report.model_type}:{report.tensor_bytes}:{device}:{a.max_tokens}" + (":kv8" if a.kv_bits == 8 else "")   # (a plan counts the cache's bytes)
+        key = f"{report.model_type}:{report.tensor_bytes}:{device}:{a.max_tokens}" + (":kv8" if a.kv_bits == 8 else ":kept" if a.kv_keep is not None else "")   # (a plan counts the cache's bytes)
         cached = None
         if cache_path and a.auto != "benchmark":
             try:

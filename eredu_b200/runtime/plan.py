@@ -216,9 +216,10 @@ class ModelResourceProfile:
 
 
 def estimate_runtime_state(cfg: ModelConfig, weight_bytes: Optional[int] = None, cache_dtype_bytes: int = 2,
-                           kv_bits: Optional[int] = None) -> ModelResourceProfile:
+                           kv_bits: Optional[int] = None, weighed: bool = False) -> ModelResourceProfile:
     """KV bytes per token and static weight bytes of a decoder (``estimate_runtime_state``, capability.rs). ``kv_bits`` = 8: keys and values in 8 bits with
-    a 4-byte scale per page and head; recurrent states stay in ``cache_dtype_bytes``."""
+    a 4-byte scale per page and head; recurrent states stay in ``cache_dtype_bytes``. ``weighed``: a cache of bounded size, which has a 4-byte sum beside every token and
+    head (a prompt is cached whole before it is brought down to the bound, and pools are as large as without one: the bound takes nothing off)."""
     H, D = cfg.hidden_size, cfg.head_dim
     L = cfg.num_hidden_layers
     family = _family_profile(cfg, weight_bytes, cache_dtype_bytes)
@@ -232,6 +233,8 @@ def estimate_runtime_state(cfg: ModelConfig, weight_bytes: Optional[int] = None,
         from .kv_cache import PAGE
 
         kv_tok = -(-2 * cfg.num_key_value_heads * (PAGE * D + 4) // PAGE) * attn_layers
+    if weighed:
+        kv_tok += 4 * cfg.num_key_value_heads * attn_layers
     if cfg.is_mla:   # one compressed latent + rotary key per token and layer, shared by the heads
         kv_tok = (cfg.kv_lora_rank + cfg.qk_rope_head_dim) * cache_dtype_bytes * attn_layers
     state = 0
