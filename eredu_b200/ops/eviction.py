@@ -124,6 +124,16 @@ def _narrow(window, tokens) -> int:
     return window if window < tokens else 0
 
 
+def _named(block_table, seq_lens, pages) -> list:
+    """The lengths, behind a look at them and at the pages that they reach: tensor operations follow whatever they are given."""
+    wide = block_table.shape[1]
+    held = torch.arange(wide, device=block_table.device) * PAGE < seq_lens[:, None]
+    wrong = (seq_lens > wide * PAGE).any() | (held & ((block_table < 0) | (block_table >= pages))).any()
+    if bool(wrong):
+        raise ValueError(f"lengths beyond {wide * PAGE} tokens of a table's row, or pages in it that are none of {pages}")
+    return seq_lens.tolist()
+
+
 def weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, scale, window=0, sinks=None, weights=None, observed=0, out=None):
     """Attention of the last ``q_lens[b]`` tokens of every sequence, by tensor operations, with ``weights`` kept as above. ``observed`` > 0: the last so many
     rows of a sequence count. A row that sees nothing gives zeros."""
@@ -132,7 +142,7 @@ def weighed_attention_ref(q, k_cache, v_cache, block_table, seq_lens, q_lens, sc
     n_q, n_kv = q.shape[1], k_cache.shape[1]
     out = q.new_empty((*q.shape[:2], v_cache.shape[3])) if out is None else out
     start = 0
-    for b, (n, m) in enumerate(zip(seq_lens.tolist(), q_lens)):
+    for b, (n, m) in enumerate(zip(_named(block_table, seq_lens, k_cache.shape[0]), q_lens)):
         if m == 0:
             continue
         k, v = (_gather_kv(c, block_table[b], n).float() for c in (k_cache, v_cache))
@@ -274,7 +284,7 @@ def weighed_prefill(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q_len,
 
 # ------------------------------------------------------------------------------------------ eviction
 def evict_tokens_ref(k, v, weights, block_table, seq_lens, keep, recent=0, first=0):
-    for b, n in enumerate(seq_lens.tolist()):
+    for b, n in enumerate(_named(block_table, seq_lens, k.shape[1])):
         if n <= keep:
             continue
         t = torch.arange(n, device=k.device)

@@ -225,3 +225,21 @@ def test_lengths_beyond_the_table_are_taken_as_what_it_holds(what, beyond):
                 ops.native.check_status(torch.device("cuda", 0))
         ops.native.check_status(torch.device("cuda", 0))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("what", CALLS)
+@pytest.mark.parametrize("fault", ["length", "page behind the pool", "page before it"])
+def test_tensor_operations_refuse_what_the_table_does_not_name(what, fault):
+    """The plain forms - on the CPU, and for heads that have no kernel - look at lengths and pages first: on a GPU an index out of range would end the process."""
+    q, k, v, w, table, lens = arguments(dim=80)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32)
+    table[1, 1] = 99                                         # (nobody's: the second sequence has one page)
+    CALLS[what](q, k, v, w.clone(), table, torch.tensor([20, 5], dtype=torch.int32), cu)
+    if fault == "length":
+        lens = lens + torch.tensor([100, 0], dtype=torch.int32)
+    else:
+        table[0, 1] = 1 << 20 if "behind" in fault else -3
+    before = [x.clone() for x in (k, v, w)]
+    with pytest.raises(ValueError):
+        CALLS[what](q, k, v, w, table, lens, cu)
+    assert all(torch.equal(x, old) for x, old in zip((k, v, w), before))
