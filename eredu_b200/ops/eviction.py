@@ -317,13 +317,19 @@ def _check_eviction(k, v, weights, block_table, seq_lens) -> None:
     _check_table(block_table, seq_lens, dev)
 
 
+def _apart(*pools) -> bool:
+    """Whether the layers of some pool, each contiguous, do not lie one behind the other (a part of a larger pool's pages)."""
+    return (all(torch.is_tensor(t) and t.dim() > 1 and t.shape[0] == pools[0].shape[0] > 1 and t[0].is_contiguous() for t in pools)
+            and not all(t.is_contiguous() for t in pools))
+
+
 def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, max_kv_len=0):
     """Brings every sequence of more than ``keep`` tokens down to ``keep``, in place, and returns the tokens that each has left (int32 [B]). ``k``, ``v``: pages
     of all layers [layers, pages, heads, 16, width], ``weights`` [layers, pages, heads, 16] fp32 (see above). For every layer and head by itself
     the ``first`` tokens of a sequence and its ``recent`` last ones stay, and of those between them the ones with the largest weights; of equal weights the
     earlier token, and what is no number goes first. What stays moves to the front in its order - keys, values and weights, bit by bit -, and the rows
     behind it are left as they were. A page belongs to one sequence of the call only (shared pages are copied first, :func:`.kv8.copy_pages`).
-    ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it."""
+    ``max_kv_len``: the largest of ``seq_lens`` at least, where the host knows it. Layers that do not lie one behind the other are brought down one by one."""
     if keep < 1 or recent < 0 or first < 0 or recent + first > keep:
         raise ValueError(f"of {keep} tokens the first {first} and the last {recent} cannot stay")
     shape, at = k.shape, -1 if type(k) is Pages8 else k.get_device()
@@ -333,6 +339,10 @@ def evict_tokens(k, v, weights, block_table, seq_lens, keep, recent=0, first=0, 
             and seq_lens.dim() == 1 and block_table.dim() == 2 and block_table.shape[0] == seq_lens.shape[0] and block_table.stride(1) == 1
             and at == v.get_device() == weights.get_device() == seq_lens.get_device() == block_table.get_device() and k.is_contiguous() and v.is_contiguous()
             and weights.is_contiguous() and seq_lens.is_contiguous()):
+        if _apart(k, v, weights):
+            for i in range(shape[0]):
+                left = evict_tokens(k[i:i + 1], v[i:i + 1], weights[i:i + 1], block_table, seq_lens, keep, recent, first, max_kv_len)
+            return left
         _check_eviction(k, v, weights, block_table, seq_lens)
     dev = k.device
     layers, pages, n_kv = shape[:3]

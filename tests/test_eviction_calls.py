@@ -243,3 +243,48 @@ def test_tensor_operations_refuse_what_the_table_does_not_name(what, fault):
     with pytest.raises(ValueError):
         CALLS[what](q, k, v, w, table, lens, cu)
     assert all(torch.equal(x, old) for x, old in zip((k, v, w), before))
+
+
+# ------------------------------------------------------------------------------------------ layers that lie apart
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("apart", ["kvw", "k", "w"])
+def test_layers_may_lie_apart(device, apart):
+    """A part of the pages of every layer, as a pool has them that could not change its size."""
+    num, table = layout([100, 20], device, seed=3)
+    pools = dict(zip("kvw", cache(num, 2, 64, device, 4, layers=(3,))))
+    lens = torch.tensor([100, 20], dtype=torch.int32, device=device)
+    want = {x: t.clone() for x, t in pools.items()}
+    ops.evict_tokens(want["k"], want["v"], want["w"], table, lens, 32, recent=4, first=1)
+    for x in apart:
+        room = pools[x].new_full((3, num + 5, *pools[x].shape[2:]), 7)
+        room[:, :num] = pools[x]
+        pools[x] = room[:, :num]
+    left = ops.evict_tokens(pools["k"], pools["v"], pools["w"], table, lens, 32, recent=4, first=1)
+    assert left.tolist() == [32, 20] and all(torch.equal(pools[x], want[x]) for x in "kvw")
+    assert all(bool((pools[x]._base[:, num:] == 7).all()) for x in apart)
+
+
+@pytest.mark.parametrize("pages", [9, 41])
+def test_a_bounded_cache_goes_on_in_a_pool_that_could_not_change_its_size(pages):
+    from eredu_b200.runtime.engine import Engine
+    from test_kept_tokens_steps import GREEDY, build, prompt
+    from test_kv8_engine import Failing
+
+    model = build()
+    outs = []
+    for n in (None, 0, 1, 2):
+        eng = Engine(model, max_batch=2, max_seq_len=128, kv_keep=eviction_rule())
+        seq = eng.new_sequence(prompt(40), GREEDY, max_new_tokens=60)
+        eng.feed_logits(seq, seq.prompt)
+        if n is not None:
+            with pytest.raises(torch.OutOfMemoryError), Failing(n, pages):
+                eng.resize_cache(pages, [seq])
+        outs.append(torch.stack([eng.feed_logits(seq, [5 + t]) for t in range(30)]))
+        assert seq.cached < 40
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
+
+
+def eviction_rule():
+    from eredu_b200.runtime.kv_cache import KeptTokens
+
+    return KeptTokens(keep=24, recent=6, slack=8)
