@@ -10,13 +10,16 @@
 // that the four to eight rows of a group fill the narrow side), and so does O^T = V^T P^T: a lane has two rows in both, whose maxima rescale its own accumulators. The
 // row maximum is a bound that is moved when a score is above it by more than 2^8: most pages need no exchange between lanes.
 // The splits of a sequence and head (up to sixteen, or to the largest cluster that the device has room for) are a cluster: maxima, sums and outputs meet in shared memory, and
-// every CTA weighs its own tokens. More splits leave their part in memory, and a second kernel does the same. Up to sixteen rows that share a head are a warp's; with more, two or four warps walk the same pages with
-// sixteen rows each.
+// every CTA weighs its own tokens. More splits leave their part in memory, and a second kernel does the same. Up to sixteen rows that share a head are a warp's; with more, two
+// or four warps walk the same pages with sixteen rows each.
 //
-// Measured (floor: K, V and weights at 6.54 TB/s): 64 sequences of 2048 to 4096 tokens, 32 heads of 128 over 8, 134 us (floor 124, 6.1 TB/s); 32 of 1088 to 2175 42 us
-// (33: what is left is the start and the end of the CTAs, about 8 us); one of 32768, 64 heads over 8, 31 us (21: 24 splits to a head and the second
-// kernel); one of 512, 32 heads of 64 over 8, 8.4 us between launches of a graph, a chain of latencies. Storing the scores and adding up the weights took 18 us of 144 in the first of these
-// before keys and values were kept from pushing the scores out of the second-level cache. A page costs a warp some 300 instructions at five cycles each while
+// Probabilities are rounded to bf16 in front of the product with the values, the type of its other operand: outputs are 0.0018 to 0.0023 off 64 bits, where bf16 outputs alone
+// make it 0.0017; the weights are made of unrounded ones, and all sums are held in 32 bits.
+//
+// Measured (floor: K, V and weights at 6.54 TB/s; launches of a graph on inputs that together exceed the second-level cache): 64 sequences of 2048 to 4096 tokens, 32 heads of
+// 128 over 8, 135 us (floor 124, 6.0 TB/s); 32 of 1088 to 2175 45 us (33: what is left is the start and the end of the CTAs, about 8 us); one of 32768, 64 heads over 8, 32 us (21:
+// 24 splits to a head and the second kernel); one of 512, 32 heads of 64 over 8, 6.0 us, a chain of latencies. Storing the scores and adding up the weights took 18 us of 144 in the
+// first of these before keys and values were kept from pushing the scores out of the second-level cache. A page costs a warp some 300 instructions at five cycles each while
 // it is alone on its scheduler, so that twelve warps to an SM (two stages to a ring) move more than eight with three stages: 64 x 4096 156 -> 148 us.
 #include <cuda_bf16.h>
 
